@@ -181,7 +181,7 @@ def prepare(case, seed):
             s["index"] = pick.sort(-1).values.to(torch.int32)
         return s
     s["lengths"] = torch.tensor(_lengths(case), dtype=torch.int32, device="cuda")
-    s["k_codes"], s["k_scales"] = _encode(_keys(gen, B, H, N, D, torch.float32))
+    s["k_codes"], s["k_scales"] = _encode(_keys(gen, B, H, N, D, torch.float32).contiguous())
     s["v_codes"], s["v_scales"] = _encode(_draw_rows(gen, B, H, N, D))
     # accumulated weights: a few heavy rows, a long tail, exact ties among the rows without any
     mass = torch.exp(3.0 * torch.randn(B, H, N, generator=gen, device="cuda") - 6.0)
