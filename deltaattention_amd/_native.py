@@ -23,7 +23,7 @@ DA_SELECT_COSINE = 1
 DA_SELECT_ARITH16 = 2
 DA_NUM_STRIDES = 24
 
-# (name, restype, argtypes) for every symbol of include/deltaattn.h
+# (name, restype, argtypes) for every symbol of include/deltaattn.h and deltaattn_cache.h
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 SIGNATURES = {
     "da_last_error": (ctypes.c_char_p, []),
@@ -54,6 +54,18 @@ SIGNATURES = {
                                          _L, _P, _L, _P, _P, _L, _L, _L, _L, _L, _F, _P, _L, _L,
                                          _P]),
     "da_decode_step": (_I, [_P, _P]),
+    # include/deltaattn_cache.h
+    "da_kv4_quantize": (_I, [_P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _P, _P]),
+    "da_kv4_dequantize": (_I, [_P, _L, _L, _L, _L, _P, _P, _I, _P]),
+    "da_kv4_evict_workspace_size": (_L, [_L, _L, _L, _L]),
+    "da_kv4_evict": (_I, [_P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _P]),
+    "da_heavy_rows": (_I, [_P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _P]),
+    "da_kv4_attention_workspace_size": (_L, [_L, _L, _L, _L, _I]),
+    "da_kv4_attention": (_I, [_P, _I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _L, _L, _L, _F, _I, _P, _L, _L, _P, _L,
+                              _P]),
+    "da_attention_mass_workspace_size": (_L, [_L, _L, _L, _L, _L]),
+    "da_attention_mass": (_I, [_P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _F, _P, _P,
+                               _L, _P]),
 }
 
 
@@ -72,6 +84,13 @@ class DecodeStep(ctypes.Structure):
         ("B", _L), ("Hq", _L), ("Hkv", _L), ("D", _L),
         ("workspace", _P), ("workspace_bytes", _L),
     ]
+
+
+class Kv4Block(ctypes.Structure):
+    """struct DaKv4 of include/deltaattn_cache.h (field for field)."""
+    _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("counts", _P),
+                ("timestamps", _P), ("lengths", _P), ("mass", _P), ("capacity", _L)]
+
 
 DA_DECODE_SCRATCH_BYTES = 32 << 20
 
@@ -160,3 +179,25 @@ def _raw_stream(index: int) -> int:
     if get is None:  # pragma: no cover - older torch
         return torch.cuda.current_stream(index).cuda_stream
     return get(index)
+
+
+class on_device:
+    """``with on_device(device) as stream``: ``device`` is the current one inside, whichever was
+    before, and ``stream`` the handle of its current stream."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.index is None:
+            self.index = self.before
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)

@@ -177,6 +177,16 @@ __device__ __forceinline__ float wave_tree_sum_all(float t) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+// x is 0 or -0 / is -inf, by its bits: the build takes comparisons to see no NaN, so these hide
+// the float from the compiler and a NaN is neither.
+__device__ __forceinline__ uint32_t opaque_bits(float x) {
+  uint32_t u = __float_as_uint(x);
+  asm("" : "+v"(u));
+  return u;
+}
+__device__ __forceinline__ bool zero_bits(float x) { return (opaque_bits(x) << 1) == 0; }
+__device__ __forceinline__ bool is_neg_inf(float x) { return opaque_bits(x) == 0xff800000u; }
+
 // Correctly rounded fp32 square root (round to nearest even), as the CPU restatement's
 // sqrtf.  HIP's __fsqrt_rn is the hardware approximation unless OCML's rounded
 // operations are enabled, and differs from it in the last place often enough to flip a

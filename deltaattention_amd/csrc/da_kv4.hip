@@ -1,0 +1,557 @@
+// Key and value rows in 4 bits on gfx950: conversion into the cache and back, and eviction
+// by accumulated attention weight.
+//
+// Format (include/deltaattn_cache.h): groups of 32 dims, elements E2M1 (sign, two exponent
+// bits, one mantissa bit) times one power of two a group.  A power of two makes every value
+// exact in bf16 and lets v_cvt_scalef32_pk_* convert a byte of two codes, scale included, in
+// one instruction.
+#include "da_common.hpp"
+#include "../../include/deltaattn_cache.h"
+
+namespace da {
+
+// ------------------------------------------------------------------------------------
+// rows -> 4 bits
+// ------------------------------------------------------------------------------------
+struct Quant4Args {
+  const void* x[2];  // k, v
+  int64_t s_b[2], s_h[2], s_n[2];
+  uint8_t* codes[2];
+  uint8_t* scales[2];
+  const int32_t* counts;
+  const int32_t* ts;
+  const float* mass;
+  const int32_t* lengths;
+  const int32_t* index;
+  int32_t* o_counts;
+  int32_t* o_ts;
+  float* o_mass;
+  int32_t* o_lengths;
+  int64_t N, M, capacity;
+  int H, D;
+};
+
+// Eight consecutive elements of a row, as fp32.
+template <int DT>
+__device__ __forceinline__ void load8(const void* row, int64_t at, float (&x)[8]) {
+  if constexpr (DT == DA_F32) {
+    const f32x4 a = *(const f32x4*)((const float*)row + at), b = *(const f32x4*)((const float*)row + at + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = a[i];
+      x[4 + i] = b[i];
+    }
+  } else {
+    const u32x4 w = *(const u32x4*)((const uint16_t*)row + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = E16<DT>::lo(w[i]);
+      x[2 * i + 1] = E16<DT>::hi(w[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t quad_umax(uint32_t v) {
+  const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppXor1, 0xF, 0xF, false);
+  v = v > a ? v : a;
+  const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppXor2, 0xF, 0xF, false);
+  return v > b ? v : b;
+}
+
+// The exponent byte of a group whose largest magnitude has fp32 bits `top`: with top = 1.f x
+// 2^(E - 127), 4 x 1.f <= 6 exactly where the fraction is at most one half.  Magnitudes are
+// compared as integers, so a NaN is the largest.
+__device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
+  const int E = (int)(top >> 23);
+  if (E == 255) return 255u;
+  int x = E - 2 + ((top & 0x7fffffu) > 0x400000u ? 1 : 0);
+  x = x < 2 ? 2 : x;
+  return (uint32_t)(x > 252 ? 252 : x);
+}
+
+// A lane takes 8 dims: 16 bytes of a 16-bit row (32 of an fp32 one), 4 bytes of codes; the
+// four lanes of a quad are one group, whose largest magnitude is two quad permutes away.
+// Lanes per row: 4 NG.  Each thread takes kQuantItems of them, a block's width apart, with
+// all of its loads in flight.  blockIdx.y = (sequence, head), z = key or value.
+constexpr int kQuantItems = 4;
+template <int DT, int NG>
+__global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
+  constexpr int kLpr = 4 * NG;
+  const int bh = blockIdx.y, z = blockIdx.z;
+  const int b = bh / a.H, h = bh - b * a.H;
+  int64_t len = a.lengths ? a.lengths[bh] : a.M;
+  len = len < 0 ? 0 : (len > a.M ? a.M : len);
+  const char* base = (const char*)a.x[z] + (b * a.s_b[z] + h * a.s_h[z]) * (DT == DA_F32 ? 4 : 2);
+  const int64_t first = (int64_t)blockIdx.x * 256 * kQuantItems + threadIdx.x;
+  float x[kQuantItems][8];
+  int64_t src[kQuantItems];
+#pragma unroll
+  for (int u = 0; u < kQuantItems; ++u) {
+    const int64_t it = first + u * 256, m = it / kLpr;
+    int64_t s = -1;
+    if (m < len) {
+      s = m;
+      if (a.index) {
+        s = a.index[bh * a.M + m];
+        if (s >= a.N) s = -1;
+      }
+    }
+    src[u] = s;
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantItems; ++u) {
+    const int64_t it = first + u * 256;
+    const int d = 8 * (int)(it - it / kLpr * kLpr);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[u][i] = 0.0f;
+    if (src[u] >= 0 && d < a.D) load8<DT>(base, src[u] * a.s_n[z] + d, x[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantItems; ++u) {
+    const int64_t it = first + u * 256, m = it / kLpr;
+    const int c = (int)(it - m * kLpr);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = __float_as_uint(x[u][i]) & 0x7fffffffu;
+      top = top > w ? top : w;
+    }
+    top = quad_umax(top);
+    const uint32_t e = group_exponent(top);
+    uint32_t codes = 0;
+    if (e != 255u) {
+      // multiplying by a power of two is exact (results below the smallest normal are far
+      // below the first rounding border, 0.25); the conversion rounds to nearest even and
+      // saturates, which only the largest exponent reaches
+      const float inv = __uint_as_float((254u - e) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[u][i] *= inv;
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][0], x[u][1], 1.0f, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][2], x[u][3], 1.0f, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][4], x[u][5], 1.0f, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][6], x[u][7], 1.0f, 3);
+    }
+    if (m < a.M) {
+      const int64_t row = bh * a.capacity + m;
+      ((uint32_t*)a.codes[z])[row * kLpr + c] = codes;
+      if ((c & 3) == 0) a.scales[z][row * NG + (c >> 2)] = (uint8_t)(src[u] < 0 ? 0u : e);
+      if (z == 0 && c == 0) {
+        const int64_t s = bh * a.N + src[u];
+        const bool real = src[u] >= 0;
+        a.o_counts[row] = real ? (a.counts ? a.counts[s] : 1) : 0;
+        a.o_ts[row] = real ? (a.ts ? a.ts[s] : (int32_t)src[u]) : 0;
+        if (a.o_mass) a.o_mass[row] = real && a.mass ? a.mass[s] : 0.0f;
+        if (m == 0) a.o_lengths[bh] = (int32_t)len;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// 4 bits -> rows
+// ------------------------------------------------------------------------------------
+struct Dequant4Args {
+  const uint8_t* codes[2];
+  const uint8_t* scales[2];
+  void* x[2];
+  const int32_t* lengths;
+  int64_t N, capacity;
+  int D;
+};
+
+// A lane turns 4 bytes of codes into 8 elements; kQuantItems of them in flight a thread.
+template <int DT, int NG>
+__global__ __launch_bounds__(256) void dequantize4_kernel(Dequant4Args a) {
+  constexpr int kLpr = 4 * NG;
+  const int bh = blockIdx.y, z = blockIdx.z;
+  int64_t len = a.lengths[bh];
+  len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
+  const int64_t first = (int64_t)blockIdx.x * 256 * kQuantItems + threadIdx.x;
+  uint32_t w[kQuantItems], e[kQuantItems];
+#pragma unroll
+  for (int u = 0; u < kQuantItems; ++u) {
+    const int64_t it = first + u * 256, m = it / kLpr;
+    const int c = (int)(it - m * kLpr);
+    const int64_t row = bh * a.capacity + m;
+    w[u] = e[u] = 0;
+    if (m < a.N && m < len) {
+      w[u] = ((const uint32_t*)a.codes[z])[row * kLpr + c];
+      e[u] = a.scales[z][row * NG + (c >> 2)];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantItems; ++u) {
+    const int64_t it = first + u * 256, m = it / kLpr;
+    const int d = 8 * (int)(it - m * kLpr);
+    if (m >= a.N || d >= a.D) continue;
+    const float s = __uint_as_float(e[u] << 23);
+    const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], s, 0);
+    const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], s, 1);
+    const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], s, 2);
+    const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], s, 3);
+    const int64_t at = (bh * a.N + m) * a.D + d;
+    if constexpr (DT == DA_F32) {
+      float* o = (float*)a.x[z] + at;
+      *(f32x4*)o = f32x4{p0[0], p0[1], p1[0], p1[1]};
+      *(f32x4*)(o + 4) = f32x4{p2[0], p2[1], p3[0], p3[1]};
+    } else {
+      *(u32x4*)((uint16_t*)a.x[z] + at) = u32x4{E16<DT>::pack(p0[0], p0[1]), E16<DT>::pack(p1[0], p1[1]),
+                                                E16<DT>::pack(p2[0], p2[1]), E16<DT>::pack(p3[0], p3[1])};
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// eviction: the rows kept
+// ------------------------------------------------------------------------------------
+struct HeavyArgs {
+  const float* mass;
+  const int32_t* lengths;
+  int64_t capacity;  // rows a head's mass array holds
+  int budget, sinks, recent;
+  int32_t* index;  // [bh][budget]
+  int32_t* kept;   // [bh]
+};
+
+// Masses in an order of unsigned integers (-0 as 0).
+__device__ __forceinline__ uint32_t mass_order(float m) {
+  const uint32_t u = __float_as_uint(m);
+  if ((u << 1) == 0) return 0x80000000u;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kHeavyThreads = 1024, kHeavyWaves = kHeavyThreads / 64, kHeavyBins = 2048;
+
+// One workgroup per (sequence, head).  The border (the need-th largest mass between the
+// protected ends) comes from three histogram passes over 11, 11 and 10 bits of the order;
+// a last pass writes the rows above it, and as many of its equals as still fit, lowest row
+// first, in row order.
+__global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) {
+  __shared__ uint32_t s_hist[kHeavyBins];
+  __shared__ uint32_t s_wave[2][kHeavyWaves];
+  __shared__ uint32_t s_pick[2];  // the chosen bin, the rows still needed from it
+  const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  int64_t n64 = a.lengths ? a.lengths[bh] : a.capacity;
+  n64 = n64 < 0 ? 0 : (n64 > a.capacity ? a.capacity : n64);
+  const int n = (int)n64;
+  int32_t* const out = a.index + (int64_t)bh * a.budget;
+  const int kept = n < a.budget ? n : a.budget;
+  if (tid == 0) a.kept[bh] = kept;
+  if (n <= a.budget) {
+    for (int i = tid; i < a.budget; i += kHeavyThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float* const mass = a.mass + (int64_t)bh * a.capacity;
+  const int lo = a.sinks, hi = n - a.recent;  // the rows that compete
+  uint32_t need = (uint32_t)(a.budget - a.sinks - a.recent);
+  uint32_t prefix = 0, mask = 0;  // bits of the border found so far
+  for (int pass = 0; pass < 3 && need > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t bits = pass == 2 ? 1023u : 2047u;
+    for (int i = tid; i < kHeavyBins; i += kHeavyThreads) s_hist[i] = 0;
+    __syncthreads();
+    for (int i0 = lo; i0 < hi; i0 += kHeavyThreads) {
+      const int i = i0 + tid;
+      const uint32_t u = i < hi ? mass_order(mass[i]) : 0;
+      const bool in = i < hi && (u & mask) == prefix;
+      const uint32_t bin = (u >> shift) & bits;
+      // lanes that share the first active lane's bin (rows of no weight at all, often most
+      // of them) add together; the others one by one
+      const uint64_t act = __ballot(in);
+      if (act) {
+        const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
+        const uint64_t same = __ballot(in && bin == lead);
+        if (lane == 0) atomicAdd(&s_hist[lead], (uint32_t)__popcll(same));
+        if (in && bin != lead) atomicAdd(&s_hist[bin], 1u);
+      }
+    }
+    __syncthreads();
+    // the highest bin such that it and those above hold at least `need` rows: thread t owns
+    // bins 2 t and 2 t + 1, suffix sums over the threads
+    const uint32_t c0 = s_hist[2 * tid], c1 = s_hist[2 * tid + 1];
+    uint32_t suf = c0 + c1;  // becomes the sum over this thread's bins and those above
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t up = (uint32_t)__shfl_down((int)suf, d, 64);
+      suf += lane + d < 64 ? up : 0;
+    }
+    if (lane == 0) s_wave[0][wid] = suf;
+    __syncthreads();
+    uint32_t above = 0;
+    for (int w = wid + 1; w < kHeavyWaves; ++w) above += s_wave[0][w];
+    suf += above;
+    const uint32_t after1 = suf - c0 - c1;  // rows in bins above 2 t + 1
+    if (after1 < need && after1 + c1 >= need) {
+      s_pick[0] = 2 * tid + 1;
+      s_pick[1] = need - after1;
+    } else if (after1 + c1 < need && suf >= need) {
+      s_pick[0] = 2 * tid;
+      s_pick[1] = need - after1 - c1;
+    }
+    __syncthreads();
+    prefix |= s_pick[0] << shift;
+    mask |= bits << shift;
+    need = s_pick[1];
+    __syncthreads();
+  }
+  // rows above the border, and the first `need` of its equals, in order
+  const bool any = a.budget > a.sinks + a.recent;
+  for (int i = tid; i < a.sinks; i += kHeavyThreads) out[i] = i;
+  for (int i = tid; i < a.recent; i += kHeavyThreads) out[a.budget - a.recent + i] = hi + i;
+  uint32_t gt_before = 0, eq_before = 0;
+  if (any) {
+    for (int i0 = lo; i0 < hi; i0 += kHeavyThreads) {
+      const int i = i0 + tid;
+      const uint32_t u = i < hi ? mass_order(mass[i]) : 0;
+      const bool gt = i < hi && u > prefix, eq = i < hi && u == prefix;
+      const uint64_t bg = __ballot(gt), be = __ballot(eq);
+      if (lane == 0) {
+        s_wave[0][wid] = (uint32_t)__popcll(bg);
+        s_wave[1][wid] = (uint32_t)__popcll(be);
+      }
+      __syncthreads();
+      uint32_t g = gt_before, e = eq_before, gall = 0, eall = 0;
+#pragma unroll
+      for (int w = 0; w < kHeavyWaves; ++w) {
+        const uint32_t cg = s_wave[0][w], ce = s_wave[1][w];
+        if (w < wid) {
+          g += cg;
+          e += ce;
+        }
+        gall += cg;
+        eall += ce;
+      }
+      const uint64_t below = (1ull << lane) - 1;
+      g += (uint32_t)__popcll(bg & below);
+      e += (uint32_t)__popcll(be & below);
+      if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = i;
+      gt_before += gall;
+      eq_before += eall;
+      __syncthreads();
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// eviction: the rows moved
+// ------------------------------------------------------------------------------------
+struct Move4Args {
+  const uint8_t* codes[2];
+  const uint8_t* scales[2];
+  uint8_t* o_codes[2];
+  uint8_t* o_scales[2];
+  const int32_t* counts;
+  const int32_t* ts;
+  const float* mass;
+  int32_t* o_counts;
+  int32_t* o_ts;
+  float* o_mass;
+  const int32_t* index;
+  int64_t capacity, o_capacity;
+  int budget;
+};
+
+// A lane moves 16 bytes of codes (2 NG lanes a row, keys then values) and the first lanes of
+// a row its small fields.
+constexpr int kMoveItems = 2;
+template <int NG>
+__global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
+  constexpr int kLpr = 2 * NG;
+  const int bh = blockIdx.y;
+  const int64_t first = (int64_t)blockIdx.x * 256 * kMoveItems + threadIdx.x;
+  u32x4 w[kMoveItems];
+  int src[kMoveItems];
+#pragma unroll
+  for (int u = 0; u < kMoveItems; ++u) {
+    const int64_t m = (first + u * 256) / kLpr;
+    src[u] = m < a.budget ? a.index[(int64_t)bh * a.budget + m] : -1;
+  }
+#pragma unroll
+  for (int u = 0; u < kMoveItems; ++u) {
+    const int64_t it = first + u * 256;
+    const int c = (int)(it % kLpr), z = c >= NG ? 1 : 0;
+    w[u] = u32x4{0, 0, 0, 0};
+    if (src[u] >= 0) w[u] = *(const u32x4*)(a.codes[z] + ((bh * a.capacity + src[u]) * NG + (c - z * NG)) * 16);
+  }
+#pragma unroll
+  for (int u = 0; u < kMoveItems; ++u) {
+    const int64_t it = first + u * 256, m = it / kLpr;
+    if (m >= a.budget) continue;
+    const int c = (int)(it - m * kLpr), z = c >= NG ? 1 : 0, cc = c - z * NG;
+    const int64_t to = bh * a.o_capacity + m, from = bh * a.capacity + src[u];
+    const bool real = src[u] >= 0;
+    *(u32x4*)(a.o_codes[z] + (to * NG + cc) * 16) = w[u];
+    a.o_scales[z][to * NG + cc] = real ? a.scales[z][from * NG + cc] : (uint8_t)0;
+    if (c == 0) {
+      a.o_counts[to] = real ? a.counts[from] : 0;
+      a.o_ts[to] = real ? a.ts[from] : 0;
+      a.o_mass[to] = real ? a.mass[from] : 0.0f;
+    }
+  }
+}
+
+static int check_kv4(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, bool mass, const char* who) {
+  DA_REQUIRE(kv, "%s: null cache", who);
+  DA_REQUIRE(kv->k_codes && kv->k_scales && kv->v_codes && kv->v_scales && kv->counts && kv->timestamps &&
+                 kv->lengths && (!mass || kv->mass),
+             "%s: null pointer in the cache", who);
+  if (D <= 0 || D > 128 || (D & 7))
+    return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128]", who);
+  DA_REQUIRE(B > 0 && Hkv > 0 && kv->capacity > 0, "%s: empty shape", who);
+  DA_REQUIRE(B * Hkv <= 65535, "%s: at most 65535 (sequence, head) pairs", who);
+  DA_REQUIRE(kv->capacity < (1ll << 31) - 65536, "%s: capacity must be below 2^31 - 65536", who);
+  DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
+  return DA_OK;
+}
+
+template <int DT>
+static void launch_quantize(const Quant4Args& a, int groups, dim3 grid, hipStream_t st) {
+  switch (groups) {
+    case 1: hipLaunchKernelGGL((quantize4_kernel<DT, 1>), grid, dim3(256), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((quantize4_kernel<DT, 2>), grid, dim3(256), 0, st, a); break;
+    case 3: hipLaunchKernelGGL((quantize4_kernel<DT, 3>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((quantize4_kernel<DT, 4>), grid, dim3(256), 0, st, a); break;
+  }
+}
+template <int DT>
+static void launch_dequantize(const Dequant4Args& a, int groups, dim3 grid, hipStream_t st) {
+  switch (groups) {
+    case 1: hipLaunchKernelGGL((dequantize4_kernel<DT, 1>), grid, dim3(256), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((dequantize4_kernel<DT, 2>), grid, dim3(256), 0, st, a); break;
+    case 3: hipLaunchKernelGGL((dequantize4_kernel<DT, 3>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((dequantize4_kernel<DT, 4>), grid, dim3(256), 0, st, a); break;
+  }
+}
+
+static int check_budget(int64_t budget, int64_t sinks, int64_t recent, const char* who) {
+  DA_REQUIRE(budget > 0 && budget < (1ll << 31) - 65536 && sinks >= 0 && recent >= 0 && sinks <= budget &&
+                 recent <= budget - sinks,
+             "%s: needs sinks + recent <= budget, budget positive", who);
+  return DA_OK;
+}
+
+static int launch_heavy(const float* mass, const int32_t* lengths, int64_t BH, int64_t capacity, int64_t budget,
+                        int64_t sinks, int64_t recent, int32_t* index, int32_t* kept, hipStream_t st,
+                        const char* who) {
+  HeavyArgs a = {};
+  a.mass = mass; a.lengths = lengths; a.capacity = capacity;
+  a.budget = (int)budget; a.sinks = (int)sinks; a.recent = (int)recent;
+  a.index = index; a.kept = kept;
+  hipLaunchKernelGGL(heavy_rows_kernel, dim3((unsigned)BH), dim3(kHeavyThreads), 0, st, a);
+  return check_launch(who);
+}
+
+}  // namespace da
+
+using namespace da;
+
+extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t B, int64_t Hkv, int64_t N, int64_t D,
+                               int64_t sk_b, int64_t sk_h, int64_t sk_n, int64_t sv_b, int64_t sv_h, int64_t sv_n,
+                               const int32_t* counts, const int32_t* timestamps, const float* mass,
+                               const int32_t* lengths, const int32_t* index, int64_t M, const DaKv4* out,
+                               void* stream) {
+  const char* who = "da_kv4_quantize";
+  DA_REQUIRE(k && v, "%s: null pointer", who);
+  if (int rc = check_kv4(out, B, Hkv, D, false, who)) return rc;
+  if (dtype != DA_BF16 && dtype != DA_F16 && dtype != DA_F32)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: rows must be bf16, fp16 or fp32", who);
+  DA_REQUIRE(N > 0 && N < (1ll << 31) && M > 0 && M <= out->capacity && (index || M == N),
+             "%s: needs 0 < M <= capacity, and M = N without an index", who);
+  const int64_t align = dtype == DA_F32 ? 3 : 7;
+  DA_REQUIRE(((sk_b | sk_h | sk_n | sv_b | sv_h | sv_n) & align) == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
+             "%s: rows must be 16-byte aligned", who);
+  Quant4Args a = {};
+  a.x[0] = k; a.s_b[0] = sk_b; a.s_h[0] = sk_h; a.s_n[0] = sk_n;
+  a.x[1] = v; a.s_b[1] = sv_b; a.s_h[1] = sv_h; a.s_n[1] = sv_n;
+  a.codes[0] = out->k_codes; a.codes[1] = out->v_codes;
+  a.scales[0] = out->k_scales; a.scales[1] = out->v_scales;
+  a.counts = counts; a.ts = timestamps; a.mass = mass; a.lengths = lengths; a.index = index;
+  a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass; a.o_lengths = out->lengths;
+  a.N = N; a.M = M; a.capacity = out->capacity; a.H = (int)Hkv; a.D = (int)D;
+  const int groups = (int)((D + 31) / 32);
+  const int64_t blocks = (M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems);
+  const dim3 grid((unsigned)blocks, (unsigned)(B * Hkv), 2);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DA_F32) launch_quantize<DA_F32>(a, groups, grid, st);
+  else if (dtype == DA_F16) launch_quantize<DA_F16>(a, groups, grid, st);
+  else launch_quantize<DA_BF16>(a, groups, grid, st);
+  return check_launch(who);
+}
+
+extern "C" int da_kv4_dequantize(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t N, int64_t D, void* k, void* v,
+                                 int dtype, void* stream) {
+  const char* who = "da_kv4_dequantize";
+  if (int rc = check_kv4(kv, B, Hkv, D, false, who)) return rc;
+  if (dtype != DA_BF16 && dtype != DA_F16 && dtype != DA_F32)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: rows must be bf16, fp16 or fp32", who);
+  DA_REQUIRE(k && v && (((uintptr_t)k | (uintptr_t)v) & 15) == 0, "%s: rows must be 16-byte aligned", who);
+  DA_REQUIRE(N > 0 && N <= kv->capacity, "%s: needs 0 < N <= capacity", who);
+  Dequant4Args a = {};
+  a.codes[0] = kv->k_codes; a.codes[1] = kv->v_codes;
+  a.scales[0] = kv->k_scales; a.scales[1] = kv->v_scales;
+  a.x[0] = k; a.x[1] = v; a.lengths = kv->lengths; a.N = N; a.capacity = kv->capacity; a.D = (int)D;
+  const int groups = (int)((D + 31) / 32);
+  const int64_t blocks = (N * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems);
+  const dim3 grid((unsigned)blocks, (unsigned)(B * Hkv), 2);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DA_F32) launch_dequantize<DA_F32>(a, groups, grid, st);
+  else if (dtype == DA_F16) launch_dequantize<DA_F16>(a, groups, grid, st);
+  else launch_dequantize<DA_BF16>(a, groups, grid, st);
+  return check_launch(who);
+}
+
+// The rows kept, [B, Hkv, budget].
+extern "C" int64_t da_kv4_evict_workspace_size(int64_t B, int64_t Hkv, int64_t capacity, int64_t budget) {
+  (void)capacity;
+  return B * Hkv * budget * (int64_t)sizeof(int32_t);
+}
+
+extern "C" int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, int64_t budget, int64_t sinks,
+                            int64_t recent, const DaKv4* out, int32_t* index, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  const char* who = "da_kv4_evict";
+  if (int rc = check_kv4(kv, B, Hkv, D, true, who)) return rc;
+  if (int rc = check_kv4(out, B, Hkv, D, true, who)) return rc;
+  if (int rc = check_budget(budget, sinks, recent, who)) return rc;
+  DA_REQUIRE(budget <= out->capacity, "%s: the budget exceeds the new cache's capacity", who);
+  DA_REQUIRE(kv->k_codes != out->k_codes && kv->v_codes != out->v_codes && kv->mass != out->mass &&
+                 kv->counts != out->counts && kv->lengths != out->lengths,
+             "%s: the rows move to other memory", who);
+  const int64_t need = da_kv4_evict_workspace_size(B, Hkv, kv->capacity, budget);
+  if (!index && (!workspace || workspace_bytes < need))
+    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
+  int32_t* rows = index ? index : (int32_t*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  if (int rc = launch_heavy(kv->mass, kv->lengths, B * Hkv, kv->capacity, budget, sinks, recent, rows, out->lengths,
+                            st, who))
+    return rc;
+  Move4Args a = {};
+  a.codes[0] = kv->k_codes; a.codes[1] = kv->v_codes;
+  a.scales[0] = kv->k_scales; a.scales[1] = kv->v_scales;
+  a.o_codes[0] = out->k_codes; a.o_codes[1] = out->v_codes;
+  a.o_scales[0] = out->k_scales; a.o_scales[1] = out->v_scales;
+  a.counts = kv->counts; a.ts = kv->timestamps; a.mass = kv->mass;
+  a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass;
+  a.index = rows; a.capacity = kv->capacity; a.o_capacity = out->capacity; a.budget = (int)budget;
+  const int groups = (int)((D + 31) / 32);
+  const dim3 grid((unsigned)((budget * 2 * groups + 256 * kMoveItems - 1) / (256 * kMoveItems)), (unsigned)(B * Hkv));
+  switch (groups) {
+    case 1: hipLaunchKernelGGL((move4_kernel<1>), grid, dim3(256), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((move4_kernel<2>), grid, dim3(256), 0, st, a); break;
+    case 3: hipLaunchKernelGGL((move4_kernel<3>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((move4_kernel<4>), grid, dim3(256), 0, st, a); break;
+  }
+  return check_launch(who);
+}
+
+extern "C" int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t B, int64_t Hkv, int64_t N,
+                             int64_t budget, int64_t sinks, int64_t recent, int32_t* index, int32_t* kept,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "da_heavy_rows";
+  (void)workspace;
+  (void)workspace_bytes;
+  DA_REQUIRE(mass && index && kept, "%s: null pointer", who);
+  DA_REQUIRE(B > 0 && Hkv > 0 && N > 0 && N < (1ll << 31) - 65536 && B * Hkv <= 65535, "%s: bad shape", who);
+  if (int rc = check_budget(budget, sinks, recent, who)) return rc;
+  return launch_heavy(mass, lengths, B * Hkv, N, budget, sinks, recent, index, kept, (hipStream_t)stream, who);
+}

@@ -1,0 +1,528 @@
+// Decode attention over key and value rows held in 4 bits (format: deltaattn_cache.h), with a
+// ring of exact rows, on gfx950.
+//
+// For a query head: s_j = scale q . k_j + log c_j over the rows, s_j = scale q . k_j over the
+// ring; out = sum_j softmax(s)_j v_j, and row j's weight, summed over the heads of its KV
+// head's group, is added to its accumulated weight.
+//
+// The rows are what a call has to read: 34 ceil(D / 32) + 4 bytes each.  All heads of a group
+// (up to 16, the columns of a 16 x 16 MFMA) share one reading of a row.  A row's values are
+// E2M1 codes times a power of two, exact in bf16, and v_cvt_scalef32_pk_bf16_fp4 makes two of
+// them in one instruction, so both products run on bf16 MFMA with K and V as they are; what has
+// more bits is cut into bf16 parts whose sum is exact or near fp32: q into 1 (bf16), 2 (fp16)
+// or 3 (fp32), the weights p into 2 (16-bit outputs) or 3.  Sums, maxima and partials are fp32.
+//
+// S = K Q^T, tile by tile of 16 keys: lane (r = lane % 16, t = lane / 16) of a K fragment holds
+// 16 bytes of key r, which are group t of its row; MFMA m takes dims 32 t + 8 m .. + 7 of every
+// lane, so four MFMAs cover 128 dims in the order that memory has them.  The accumulator of a
+// lane is query head r and keys 4 t .. 4 t + 3.  O^T += V^T P^T over 32 keys: the B operand is p
+// as it comes from S (slot e of lane t is key 4 t + e of the first 16, then of the second), and
+// V^T comes from a bf16 copy of the tile in LDS through ds_read_b64_tr_b16 in the same order.
+//
+// Ring rows (bf16, fp16 or fp32, at most a few hundred) run on fp32 MFMA with values converted
+// exactly; it needs no transposed operand, so they go from memory to the matrix unit directly.
+//
+// The keys of a (sequence, KV head) are split over `nsplit` workgroups of four waves, tiles dealt
+// out by the device's own length, so that a short cache leaves no workgroup more than a tile;
+// a second launch joins the splits and adds the weights, which need the whole softmax.
+#include "da_common.hpp"
+#include "../../include/deltaattn_cache.h"
+
+namespace da {
+
+typedef short i16x4v __attribute__((ext_vector_type(4)));
+
+constexpr int kA4Waves = 4;
+constexpr int kA4Tile = 32;                 // keys a wave takes at once
+constexpr int kA4VRow = 128 * 2 + 16;       // bytes of a bf16 V row in LDS, padded off the banks
+constexpr int kA4Cols = 16;                 // query heads of one workgroup
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Attn4Args {
+  const void* q;
+  int64_t sq_b, sq_h;
+  const uint8_t* kc;
+  const uint8_t* ks;
+  const uint8_t* vc;
+  const uint8_t* vs;
+  const int32_t* counts;
+  const int32_t* lengths;
+  int64_t capacity;
+  const void* kx;
+  const void* vx;
+  int64_t sx_b, sx_h, sx_s;
+  int exact_len;
+  float scale_log2;
+  void* out;
+  int64_t so_b, so_h;
+  float* mass;
+  float* part;   // [bh][G][nsplit][2 + 128]: max and sum (log2 units), P.V
+  float* score;  // [bh][G][score_cap]: scores (log2 units), where the weights are wanted
+  int64_t score_cap;
+  int nsplit;
+  int B, Hkv, G, D;
+};
+
+constexpr int kA4Part = 2 + 128;
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+
+// x = sum of N bf16 parts, largest first (exact for bf16 with 1, for fp16 with 2).
+template <int N>
+__device__ __forceinline__ void split_bf16(float x, uint16_t (&p)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    p[i] = E16<DA_BF16>::bits(x);
+    x -= E16<DA_BF16>::one(p[i]);
+  }
+}
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                 0, 0);
+}
+
+template <int SEL>
+__device__ __forceinline__ uint32_t fp4_to_bf16x2(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+}
+// eight codes (4 bytes) -> eight bf16 values
+__device__ __forceinline__ u32x4 fp4_to_bf16x8(uint32_t w, float scale) {
+  return u32x4{fp4_to_bf16x2<0>(w, scale), fp4_to_bf16x2<1>(w, scale), fp4_to_bf16x2<2>(w, scale),
+               fp4_to_bf16x2<3>(w, scale)};
+}
+
+// max / sum over the four lanes l % 16 + 16 t
+__device__ __forceinline__ float cols_max(float v) {
+  v = __builtin_fmaxf(v, __shfl_xor(v, 16, 64));
+  return __builtin_fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float cols_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+template <int DT>
+__device__ __forceinline__ float load_elem(const void* p, int64_t at) {
+  if constexpr (DT == DA_F32) return ((const float*)p)[at];
+  else return E16<DT>::one(((const uint16_t*)p)[at]);
+}
+
+// One workgroup: (sequence, KV head) blockIdx.x, split blockIdx.y, heads 16 z .. of the group.
+template <int DT, int NG, bool MASS>
+__global__ __launch_bounds__(256) void kv4_attn_kernel(Attn4Args a) {
+  constexpr int QP = DT == DA_BF16 ? 1 : DT == DA_F16 ? 2 : 3;
+  constexpr int PP = DT == DA_F32 ? 3 : 2;
+  constexpr int NJ = 2 * NG;  // output tiles of 16 dims
+  constexpr int kTileBytes = kA4Tile * kA4VRow;
+  __shared__ __attribute__((aligned(16))) char s_v[kA4Waves][kTileBytes];
+  __shared__ float s_ml[kA4Waves][2][kA4Cols];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int r = lane & 15, t = lane >> 4;
+  const int bh = blockIdx.x, split = blockIdx.y;
+  const int b = bh / a.Hkv, g = bh - b * a.Hkv;
+  const int h0 = blockIdx.z * kA4Cols;
+  const int cols = min(a.G - h0, kA4Cols);
+  int n = a.lengths[bh];
+  n = n < 0 ? 0 : (n > a.capacity ? (int)a.capacity : n);
+  const int tiles = (n + kA4Tile - 1) / kA4Tile;
+  const int rtiles = (a.exact_len + 15) / 16;
+  // tiles of the rows: split s takes [s * per, (s + 1) * per); ring tiles go to the waves from
+  // the last one on
+  const int per = (tiles + a.nsplit - 1) / a.nsplit;
+  const int t_begin = min(split * per, tiles), t_end = min(t_begin + per, tiles);
+  const int nwave = a.nsplit * kA4Waves;
+  const int rfirst = nwave - 1 - (split * kA4Waves + wid);
+  float* const part = a.part + (((int64_t)bh * a.G + h0) * a.nsplit + split) * kA4Part;
+  const int64_t pstride = (int64_t)a.nsplit * kA4Part;
+  if (t_begin >= t_end && nwave - 1 - (split * kA4Waves + kA4Waves - 1) >= rtiles) {  // nothing to do
+    if (tid < cols) {
+      part[tid * pstride] = -INFINITY;
+      part[tid * pstride + 1] = 0.0f;
+    }
+    return;
+  }
+
+  // ---- q in bf16 parts, the B operand: lane (head r, t), slot e of MFMA m: dim 32 t + 8 m + e
+  const bool have = r < cols;
+  const int64_t q_at = b * a.sq_b + (int64_t)(g * a.G + h0 + (have ? r : 0)) * a.sq_h;
+  u32x4 qf[QP][4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    uint16_t p[8][QP];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = 32 * t + 8 * m + e;
+      split_bf16<QP>(have && d < a.D ? load_elem<DT>(a.q, q_at + d) : 0.0f, p[e]);
+    }
+#pragma unroll
+    for (int i = 0; i < QP; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) qf[i][m][w] = p[2 * w][i] | ((uint32_t)p[2 * w + 1][i] << 16);
+  }
+
+  f32x4 acc[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  const int64_t row0 = (int64_t)bh * a.capacity;
+  const bool grp = t < NG;
+  const int tg = grp ? t : 0;
+  char* const vt = s_v[wid];
+  float* const score = MASS ? a.score + ((int64_t)bh * a.G + h0 + (have ? r : 0)) * a.score_cap : nullptr;
+
+  // ---- the rows, 32 at a time ----
+  for (int tile = t_begin + wid; tile < t_end; tile += kA4Waves) {
+    const int j0 = tile * kA4Tile;
+    u32x4 kc[2], vc[2];
+    uint32_t ksc[2], vsc[2];
+    int cnt[2][4], vcnt[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // rows past the length read the last one and carry no weight
+      const int64_t row = row0 + min(j0 + 16 * u + r, n - 1);
+      kc[u] = *(const u32x4*)(a.kc + (row * NG + tg) * 16);
+      vc[u] = *(const u32x4*)(a.vc + (row * NG + tg) * 16);
+      ksc[u] = a.ks[row * NG + tg];
+      vsc[u] = a.vs[row * NG + tg];
+      vcnt[u] = a.counts[row];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cnt[u][i] = a.counts[row0 + min(j0 + 16 * u + 4 * t + i, n - 1)];
+    }
+    // ---- scores ----
+    f32x4 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float sc = __uint_as_float(ksc[u] << 23);
+      s[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        u32x4 kf = fp4_to_bf16x8(kc[u][m], sc);
+        if (NG < 4 && !grp) kf = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = QP - 1; i >= 0; --i) s[u] = mfma16(kf, qf[i][m], s[u]);
+      }
+    }
+    // ---- V to LDS as bf16; a row without weight as zeros, whatever it holds ----
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool live = vcnt[u] > 0 && j0 + 16 * u + r < n;
+      const float sc = __uint_as_float(vsc[u] << 23);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        u32x4 v = fp4_to_bf16x8(vc[u][m], sc);
+        if (!live) v = u32x4{0, 0, 0, 0};
+        if (grp) *(u32x4*)(vt + (16 * u + r) * kA4VRow + 64 * t + 16 * m) = v;
+      }
+    }
+    // ---- softmax: lane (head r), keys 4 t + i of both halves ----
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = j0 + 16 * u + 4 * t + i;
+        const bool live = cnt[u][i] > 0 && key < n;
+        s[u][i] = live ? s[u][i] * a.scale_log2 + __builtin_amdgcn_logf((float)cnt[u][i]) : -INFINITY;
+        mx = __builtin_fmaxf(mx, s[u][i]);
+      }
+    if (MASS) {
+      if (have)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) *(f32x4*)(score + j0 + 16 * u + 4 * t) = s[u];
+    }
+    mx = cols_max(mx);
+    if (__ballot(mx > m_run)) {
+      const float m_new = __builtin_fmaxf(mx, m_run);
+      const float f = m_run == -INFINITY ? 0.0f : exp2_hw(m_run - m_new);
+      l_run *= f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
+      m_run = m_new;
+    }
+    const float base = m_run == -INFINITY ? 0.0f : m_run;
+    uint16_t pp[8][PP];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = exp2_hw(s[u][i] - base);
+        l_run += p;
+        split_bf16<PP>(p, pp[4 * u + i]);
+      }
+    u32x4 pf[PP];
+#pragma unroll
+    for (int i = 0; i < PP; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) pf[i][w] = pp[2 * w][i] | ((uint32_t)pp[2 * w + 1][i] << 16);
+    // ---- O^T += V^T P^T ----
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      // in each group of 16 lanes, lane i receives element i % 4 of the 8 bytes that lanes
+      // 4 e + i / 4 address, e = 0 .. 3: dim 16 j + i of keys 4 t + e
+      typedef __attribute__((address_space(3))) i16x4v lds4;
+      char* const at = vt + (4 * t + (r >> 2)) * kA4VRow + 32 * j + 8 * (r & 3);
+      const i16x4v v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(uint32_t)(uintptr_t)(
+          const __attribute__((address_space(3))) char*)at);
+      const i16x4v v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(uint32_t)(uintptr_t)(
+          const __attribute__((address_space(3))) char*)(at + 16 * kA4VRow));
+      const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+      const u32x4 vf = u32x4{w0[0], w0[1], w1[0], w1[1]};
+#pragma unroll
+      for (int i = PP - 1; i >= 0; --i) acc[j] = mfma16(vf, pf[i], acc[j]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  }
+
+  // ---- the ring, 16 slots at a time, in fp32 ----
+  const int64_t x_at = b * a.sx_b + g * a.sx_h;
+  for (int rt = rfirst; rt < rtiles; rt += nwave) {
+    const int j0 = rt * 16;
+    const int64_t krow = x_at + (int64_t)min(j0 + r, a.exact_len - 1) * a.sx_s;
+    f32x4 s = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < 2 * NG; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * u + 4 * t + i;
+        const float kf = d < a.D ? load_elem<DT>(a.kx, krow + d) : 0.0f;
+        const float qv = have && d < a.D ? load_elem<DT>(a.q, q_at + d) : 0.0f;
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, qv, s, 0, 0, 0);
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = j0 + 4 * t + i < a.exact_len ? s[i] * a.scale_log2 : -INFINITY;
+      mx = __builtin_fmaxf(mx, s[i]);
+    }
+    mx = cols_max(mx);
+    const float m_new = __builtin_fmaxf(mx, m_run);
+    const float f = m_run == -INFINITY ? 0.0f : exp2_hw(m_run - m_new);
+    l_run *= f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[j] *= f;
+    m_run = m_new;
+    const float base = m_run == -INFINITY ? 0.0f : m_run;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = exp2_hw(s[i] - base);
+      l_run += p;
+      const int slot = j0 + 4 * t + i;
+      const int64_t vrow = x_at + (int64_t)min(slot, a.exact_len - 1) * a.sx_s;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int d = 16 * j + r;
+        const float v = d < a.D && slot < a.exact_len ? load_elem<DT>(a.vx, vrow + d) : 0.0f;
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p, acc[j], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- join the four waves; the V tiles' LDS holds their sums ----
+  l_run = cols_sum(l_run);
+  if (t == 0) {
+    s_ml[wid][0][r] = m_run;
+    s_ml[wid][1][r] = l_run;
+  }
+  float* const so = (float*)(void*)vt;  // [16 heads][16 NJ + 4] of this wave
+  constexpr int kRow = 16 * NJ + 4;
+  static_assert(kA4Cols * kRow * 4 <= kTileBytes, "a wave's sums must fit its tile");
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) *(f32x4*)(so + r * kRow + 16 * j + 4 * t) = acc[j];
+  __syncthreads();
+  for (int i = tid; i < cols * 16 * NJ; i += 256) {
+    const int c = i / (16 * NJ), d = i - c * (16 * NJ);
+    float M = s_ml[0][0][c];
+#pragma unroll
+    for (int w = 1; w < kA4Waves; ++w) M = __builtin_fmaxf(M, s_ml[w][0][c]);
+    const float base = M == -INFINITY ? 0.0f : M;
+    float o = 0.0f, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kA4Waves; ++w) {
+      const float f = exp2_hw(s_ml[w][0][c] - base);
+      o += f * ((const float*)(const void*)s_v[w])[c * kRow + d];
+      L += f * s_ml[w][1][c];
+    }
+    part[c * pstride + 2 + d] = o;
+    if (d == 0) {
+      part[c * pstride] = M;
+      part[c * pstride + 1] = L;
+    }
+  }
+}
+
+// Blocks [0, B Hq): one query head's splits joined (a thread a dim).  Blocks from there on add
+// the weights: kMassKeys keys of one (sequence, KV head) each, after the group's maxima and
+// sums over the splits.
+constexpr int kMassKeys = 1024;
+template <int DT, bool MASS>
+__global__ __launch_bounds__(128) void kv4_join_kernel(Attn4Args a) {
+  __shared__ float s_m[64], s_l[64];
+  const int Hq = a.Hkv * a.G;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int heads = a.B * Hq;
+  if (!MASS || (int)blockIdx.x < heads) {
+    const int bhq = blockIdx.x, b = bhq / Hq, hq = bhq - b * Hq;
+    const float* part = a.part + (int64_t)bhq * a.nsplit * kA4Part;
+    float M = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) M = __builtin_fmaxf(M, part[s * kA4Part]);
+    const float base = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f, o = 0.0f;
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float m = part[s * kA4Part];
+      if (m == -INFINITY) continue;  // an empty split wrote no sums
+      const float f = exp2_hw(m - base);
+      L += f * part[s * kA4Part + 1];
+      if (tid < a.D) o += f * part[s * kA4Part + 2 + tid];
+    }
+    if (tid < a.D) {
+      const float v = zero_bits(L) ? 0.0f : o / L;
+      const int64_t at = b * a.so_b + hq * a.so_h + tid;
+      if constexpr (DT == DA_F32) ((float*)a.out)[at] = v;
+      else ((uint16_t*)a.out)[at] = E16<DT>::bits(v);
+    }
+    return;
+  }
+  if constexpr (MASS) {
+    const int chunks = (int)((a.capacity + kMassKeys - 1) / kMassKeys);
+    const int id = blockIdx.x - heads, bh = id / chunks, chunk = id - bh * chunks;
+    int n = a.lengths[bh];
+    n = n < 0 ? 0 : (n > a.capacity ? (int)a.capacity : n);
+    const int first = chunk * kMassKeys;
+    if (first >= n) return;
+    for (int h = wid; h < a.G; h += 2) {
+      const float* part = a.part + ((int64_t)bh * a.G + h) * a.nsplit * kA4Part;
+      float m = -INFINITY, l = 0.0f;
+      for (int s = lane; s < a.nsplit; s += 64) {
+        const float ms = part[s * kA4Part];
+        if (ms == -INFINITY) continue;
+        const float mm = __builtin_fmaxf(m, ms);
+        l = (m == -INFINITY ? 0.0f : l * exp2_hw(m - mm)) + part[s * kA4Part + 1] * exp2_hw(ms - mm);
+        m = mm;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const float m2 = __shfl_xor(m, d, 64), l2 = __shfl_xor(l, d, 64);
+        const float mm = __builtin_fmaxf(m, m2);
+        const float base = mm == -INFINITY ? 0.0f : mm;
+        l = l * exp2_hw(m - base) + l2 * exp2_hw(m2 - base);
+        m = mm;
+      }
+      if (lane == 0) {
+        s_m[h] = m == -INFINITY ? 0.0f : m;
+        s_l[h] = zero_bits(l) ? 0.0f : 1.0f / l;
+      }
+    }
+    __syncthreads();
+    const int end = min(first + kMassKeys, n);
+    const float* score = a.score + (int64_t)bh * a.G * a.score_cap;
+    float* const mass = a.mass + (int64_t)bh * a.capacity;
+    for (int j = first + tid; j < end; j += 128) {
+      float w = 0.0f;
+      for (int h = 0; h < a.G; ++h) w += exp2_hw(score[h * a.score_cap + j] - s_m[h]) * s_l[h];
+      mass[j] += w;
+    }
+  }
+}
+
+// Workgroups of the attention launch: enough to fill the chip's 256 CUs a few times over, and
+// no split shorter than one tile a wave.
+static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
+  const int64_t units = B * Hkv * ((G + kA4Cols - 1) / kA4Cols);
+  const int64_t most = (capacity + kA4Tile * kA4Waves - 1) / (kA4Tile * kA4Waves);
+  int64_t want = (1024 + units - 1) / units;
+  if (want > 128) want = 128;
+  if (want > most) want = most;
+  return (int)(want < 1 ? 1 : want);
+}
+static int64_t kv4_score_cap(int64_t capacity) { return (capacity + kA4Tile - 1) / kA4Tile * kA4Tile; }
+
+template <int DT, int NG>
+static void launch_attn4_ng(const Attn4Args& a, dim3 grid, bool mass, hipStream_t st) {
+  if (mass) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, false>), grid, dim3(256), 0, st, a);
+}
+template <int DT>
+static int launch_attn4(const Attn4Args& a, bool mass, hipStream_t st, const char* who) {
+  const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)a.nsplit, (unsigned)((a.G + kA4Cols - 1) / kA4Cols));
+  switch ((a.D + 31) / 32) {
+    case 1: launch_attn4_ng<DT, 1>(a, grid, mass, st); break;
+    case 2: launch_attn4_ng<DT, 2>(a, grid, mass, st); break;
+    case 3: launch_attn4_ng<DT, 3>(a, grid, mass, st); break;
+    default: launch_attn4_ng<DT, 4>(a, grid, mass, st); break;
+  }
+  if (int rc = check_launch(who)) return rc;
+  const unsigned heads = (unsigned)(a.B * a.Hkv * a.G);
+  if (mass) {
+    const unsigned chunks = (unsigned)((a.capacity + kMassKeys - 1) / kMassKeys);
+    hipLaunchKernelGGL((kv4_join_kernel<DT, true>), dim3(heads + (unsigned)(a.B * a.Hkv) * chunks), dim3(128), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((kv4_join_kernel<DT, false>), dim3(heads), dim3(128), 0, st, a);
+  }
+  return check_launch(who);
+}
+
+}  // namespace da
+
+using namespace da;
+
+// The splits' partials, then (accumulate) the scores.
+extern "C" int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t capacity,
+                                                   int accumulate) {
+  if (B <= 0 || Hkv <= 0 || Hq <= 0 || capacity <= 0) return 0;
+  const int64_t parts = B * Hq * kv4_splits(B, Hkv, Hq / Hkv, capacity) * kA4Part;
+  const int64_t scores = accumulate ? B * Hq * kv4_score_cap(capacity) : 0;
+  return ((parts + 3) / 4 * 4 + scores) * (int64_t)sizeof(float);
+}
+
+extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t sq_b,
+                                int64_t sq_h, const DaKv4* kv, const void* k_exact, const void* v_exact, int64_t sx_b,
+                                int64_t sx_h, int64_t sx_s, int64_t exact_len, float scale, int accumulate, void* out,
+                                int64_t so_b, int64_t so_h, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "da_kv4_attention";
+  DA_REQUIRE(kv && q && out, "%s: null pointer", who);
+  DA_REQUIRE(kv->k_codes && kv->k_scales && kv->v_codes && kv->v_scales && kv->counts && kv->lengths &&
+                 (!accumulate || kv->mass),
+             "%s: null pointer in the cache", who);
+  if (dtype != DA_BF16 && dtype != DA_F16 && dtype != DA_F32)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: q must be bf16, fp16 or fp32", who);
+  if (D <= 0 || D > 128 || (D & 7))
+    return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128]", who);
+  DA_REQUIRE(B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "%s: bad head counts", who);
+  if (Hq / Hkv > 64) return set_error(DA_ERR_UNSUPPORTED, "%s: GQA group above 64", who);
+  DA_REQUIRE(kv->capacity > 0 && exact_len >= 0 && exact_len < (1 << 24), "%s: bad cache lengths", who);
+  if (kv->capacity > (1 << 24)) return set_error(DA_ERR_UNSUPPORTED, "%s: capacity above 2^24 rows", who);
+  DA_REQUIRE(exact_len == 0 || (k_exact && v_exact), "%s: null ring", who);
+  DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
+  DA_REQUIRE(scale > 0.0f, "%s: scale must be positive", who);
+  const int64_t need = da_kv4_attention_workspace_size(B, Hq, Hkv, kv->capacity, accumulate);
+  if (!workspace || workspace_bytes < need)
+    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
+  DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
+  Attn4Args a = {};
+  a.q = q; a.sq_b = sq_b; a.sq_h = sq_h;
+  a.kc = kv->k_codes; a.ks = kv->k_scales; a.vc = kv->v_codes; a.vs = kv->v_scales;
+  a.counts = kv->counts; a.lengths = kv->lengths; a.capacity = kv->capacity;
+  a.kx = k_exact; a.vx = v_exact; a.sx_b = sx_b; a.sx_h = sx_h; a.sx_s = sx_s; a.exact_len = (int)exact_len;
+  a.scale_log2 = scale * kLog2e;
+  a.out = out; a.so_b = so_b; a.so_h = so_h; a.mass = kv->mass;
+  a.B = (int)B; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.D = (int)D;
+  a.nsplit = kv4_splits(B, Hkv, a.G, kv->capacity);
+  a.part = (float*)workspace;
+  a.score_cap = kv4_score_cap(kv->capacity);
+  a.score = a.part + (B * Hq * a.nsplit * (int64_t)kA4Part + 3) / 4 * 4;
+  const unsigned long long blocks = (unsigned long long)(B * Hq) + (unsigned long long)(B * Hkv) * ((kv->capacity + kMassKeys - 1) / kMassKeys);
+  DA_REQUIRE(B * Hkv < (1ll << 31) && blocks < (1ull << 31), "%s: too many heads", who);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DA_F32) return launch_attn4<DA_F32>(a, accumulate != 0, st, who);
+  if (dtype == DA_F16) return launch_attn4<DA_F16>(a, accumulate != 0, st, who);
+  return launch_attn4<DA_BF16>(a, accumulate != 0, st, who);
+}

@@ -1,0 +1,527 @@
+// The attention weight every key receives from a run of queries, on gfx950.
+//
+// mass_j = sum over the queries (i, h) of a KV head's group of c_j 2^(s_ij - lse_i), with
+// s_ij = scale log2(e) q_i . k_j and lse_i = log2 sum_j c_j 2^(s_ij) over the keys that query
+// sees.  The weights need the whole row's sum before the first of them is known, and storing
+// the scores (4 bytes for 256 flops) costs more than computing them twice, so there are two
+// passes over the score matrix on MFMA:
+//
+//   rows     S^T = K Q^T, queries as columns: running maximum and sum in the lane that owns the
+//            query (16 of a tile's 32 keys a lane), no exchange until the end;
+//   columns  S = Q K^T, keys as columns: sum of 2^(s - lse) over the queries, in the lane that
+//            owns the key.
+//
+// They are one kernel with the operands swapped: a wave holds its 64 columns' operand in
+// registers for the whole run and the rows stream through LDS, 32 at a time, shared by the four
+// waves of a workgroup, so that each fragment read from LDS feeds two MFMAs.  Per score there is
+// one fused multiply-add, one exp2 and one addition; the maximum is looked at only where a sum
+// leaves fp32's comfortable range.  Queries of a group are interleaved (row = query G + head),
+// so a tile's positions are close together and whole tiles are either visible or not.
+//
+// Both passes split their streamed axis where there are too few columns to fill the chip; the
+// parts are joined by small launches in a fixed order.
+//
+// fp32 tensors: each operand is cut into three bf16 parts, and the six products of weight
+// 2^-16 and above are kept (error about 2^-24 of |q||k|, as an fp32 product's own rounding).
+#include "da_common.hpp"
+#include "../../include/deltaattn_cache.h"
+
+namespace da {
+
+constexpr int kMTile = 32;             // streamed rows a tile
+constexpr int kMRow = 256;             // bytes of a row in LDS (128 16-bit dims)
+constexpr float kMLog2e = 1.4426950408889634f;
+constexpr float kMLarge = 1.2676506e30f;  // 2^100: a tile's sum above it moves the maximum
+
+struct MassArgs {
+  const void* q;
+  const void* k;
+  int64_t sq_b, sq_h, sq_n, sk_b, sk_h, sk_n;
+  const int32_t* counts;
+  const int32_t* ts;
+  const int32_t* lengths;
+  int64_t q_start;
+  float scale_log2;
+  float* part;    // rows pass: [bh][R][split] (max, sum); columns pass: [split][bh][Nk] sums
+  float* rowadd;  // [bh][R]: -lse, or -inf where a query sees nothing
+  float* mass;
+  int B, Hkv, G, Nq, Nk, D;
+  int split;
+};
+
+__device__ __forceinline__ float mexp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ int mass_pos(const MassArgs& a, int i) {
+  const int64_t p = a.q_start + i;
+  return p < -0x7ffffffe ? -0x7ffffffe : (p > 0x7fffffff ? 0x7fffffff : (int)p);
+}
+
+// Eight fp32 elements as NP bf16 operands of eight, largest part first.
+template <int NP>
+__device__ __forceinline__ void cut_chunk(f32x4 x0, f32x4 x1, u32x4 (&w)[NP]) {
+  float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t lo = E16<DA_BF16>::bits(x[2 * i]), hi = E16<DA_BF16>::bits(x[2 * i + 1]);
+      x[2 * i] -= E16<DA_BF16>::one(lo);
+      x[2 * i + 1] -= E16<DA_BF16>::one(hi);
+      w[p][i] = lo | ((uint32_t)hi << 16);
+    }
+}
+
+// PASS 0: rows (stream keys, columns are queries); PASS 1: columns (stream queries, columns are
+// keys).  blockIdx: x = column block, y = split, z = (sequence, KV head).
+template <int DT, int PASS>
+__global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
+  constexpr int NP = DT == DA_F32 ? 3 : 1;
+  constexpr int NW = DT == DA_F32 ? 2 : 1;    // 16-byte loads of a chunk of 8 elements
+  constexpr int NCB = DT == DA_F32 ? 1 : 2;   // column blocks of 32 a wave holds
+  constexpr int MT = DT == DA_F32 ? DA_BF16 : DT;
+  constexpr int kCols = 4 * NCB * 32;
+  __shared__ __attribute__((aligned(16))) char s_y[2][NP * kMTile * kMRow];
+  __shared__ __attribute__((aligned(16))) float s_add[2][kMTile];
+  __shared__ __attribute__((aligned(16))) int s_t[2][kMTile];
+  __shared__ int s_flag[2], s_ext[2];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int cl = lane & 31, hl = lane >> 5;
+  const int bh = blockIdx.z, b = bh / a.Hkv, g = bh - b * a.Hkv;
+  const int G = a.G;
+  const int R = G * a.Nq;
+  int n = a.lengths ? a.lengths[bh] : a.Nk;
+  n = n < 0 ? 0 : (n > a.Nk ? a.Nk : n);
+  const int ncol = PASS == 0 ? R : n;
+  // rows pass: later queries see more keys, so the last blocks go first
+  const int block = PASS == 0 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+  const int c0 = block * kCols;
+  const int KK = (a.D + 15) / 16;
+  constexpr int es = DT == DA_F32 ? 4 : 2;
+  const char* const qb = (const char*)a.q + (b * a.sq_b + (int64_t)g * G * a.sq_h) * es;
+  const char* const kb = (const char*)a.k + (b * a.sk_b + g * a.sk_h) * es;
+  const int32_t* const cnt = a.counts ? a.counts + (int64_t)bh * a.Nk : nullptr;
+  const int32_t* const ts = a.ts ? a.ts + (int64_t)bh * a.Nk : nullptr;
+  float* const rowadd = a.rowadd + (int64_t)bh * R;
+
+  // ---- this workgroup's share of the streamed rows, in tiles ----
+  const int c_last = min(c0 + kCols, ncol) - 1;  // below c0 where there is no column
+  int row_lo = 0, row_hi = PASS == 0 ? n : R;
+  if (!ts && c_last >= c0) {
+    if (PASS == 0) {  // keys up to the last query's own place
+      const int p = mass_pos(a, c_last / G);
+      row_hi = p < row_hi ? p + 1 : row_hi;
+    } else {  // from the first query that sees key c0
+      const int64_t first = (int64_t)c0 - a.q_start;
+      row_lo = first <= 0 ? 0 : (first >= a.Nq ? R : (int)first * G);
+    }
+  }
+  const int tile_lo = row_lo / kMTile, tile_hi = (row_hi + kMTile - 1) / kMTile;
+  const int ntile = c_last >= c0 && tile_hi > tile_lo ? tile_hi - tile_lo : 0;
+  const int per = (ntile + a.split - 1) / a.split;
+  const int t_begin = tile_lo + min((int)blockIdx.y * per, ntile);
+  const int t_end = min(t_begin + per, tile_lo + ntile);
+
+  // ---- the columns' operand and times ----
+  u32x4 x[NP][NCB][8];
+  int ct[NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int c = c0 + (wid * NCB + cb) * 32 + cl;
+    const bool have = c < ncol;
+    const char* src = kb;
+    ct[cb] = 0;
+    if (have) {
+      if (PASS == 0) {
+        const int i = c / G, h = c - i * G;
+        src = qb + (h * a.sq_h + i * a.sq_n) * es;
+        ct[cb] = mass_pos(a, i);
+      } else {
+        src = kb + c * a.sk_n * es;
+        ct[cb] = ts ? ts[c] : c;
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      const int d = 16 * kk + 8 * hl;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) x[p][cb][kk] = u32x4{0, 0, 0, 0};
+      if (have && d < a.D) {
+        if constexpr (DT == DA_F32) {
+          u32x4 w[NP];
+          cut_chunk<NP>(*(const f32x4*)(src + 4 * d), *(const f32x4*)(src + 4 * d + 16), w);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) x[p][cb][kk] = w[p];
+        } else {
+          x[0][cb][kk] = *(const u32x4*)(src + 2 * d);
+        }
+      }
+    }
+  }
+  // an extreme time of the columns, to decide for whole tiles: rows pass, the earliest query (keys
+  // at or before it need no mask); columns pass, the wave's latest key
+  int ext = PASS == 0 ? mass_pos(a, c0 / G) : c_last;
+  if (PASS == 1 && ts) {
+    ext = -0x7fffffff;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+      if (c0 + (wid * NCB + cb) * 32 + cl < ncol) ext = max(ext, ct[cb]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) ext = max(ext, __shfl_xor(ext, d, 64));
+  }
+  ext = __builtin_amdgcn_readfirstlane(ext);
+
+  // ---- staging: 16 chunks of 8 elements a row, thread: rows tid / 16 + 16 u, chunk tid % 16 ----
+  const int sr = tid >> 4, sc = tid & 15;
+  u32x4 y[2][NW];
+  bool y_live[2];
+  float m_add = 0.0f;
+  int m_t = 0;
+  auto load_tile = [&](int tile) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = tile * kMTile + sr + 16 * u;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) y[u][w] = u32x4{0, 0, 0, 0};
+      y_live[u] = false;
+      if (row < (PASS == 0 ? n : R)) {
+        const char* src;
+        if (PASS == 0) {
+          src = kb + row * a.sk_n * es;
+          y_live[u] = !cnt || cnt[row] > 0;
+        } else {
+          const int i = row / G, h = row - i * G;
+          src = qb + (h * a.sq_h + i * a.sq_n) * es;
+          y_live[u] = !is_neg_inf(rowadd[row]);
+        }
+        if (8 * sc < a.D) {
+#pragma unroll
+          for (int w = 0; w < NW; ++w) y[u][w] = *(const u32x4*)(src + 8 * es * sc + 16 * w);
+        }
+      }
+    }
+    if (tid < kMTile) {
+      const int row = tile * kMTile + tid;
+      m_add = -INFINITY;
+      m_t = PASS == 0 ? -0x7fffffff : 0x7fffffff;  // past the end: no weight, a time that asks for no mask
+      if (PASS == 0) {
+        if (row < n) {
+          const int c = cnt ? cnt[row] : 1;
+          m_add = c <= 0 ? -INFINITY : (cnt ? __builtin_amdgcn_logf((float)c) : 0.0f);
+          m_t = ts ? ts[row] : row;
+        }
+      } else if (row < R) {
+        m_add = rowadd[row];
+        m_t = mass_pos(a, row / G);
+      }
+    }
+  };
+  auto store_tile = [&](int st) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = sr + 16 * u;
+      char* const at = s_y[st] + row * kMRow + ((sc ^ (row & 15)) << 4);
+      if (!y_live[u]) {  // a row without weight counts as zeros, whatever it holds
+#pragma unroll
+        for (int w = 0; w < NW; ++w) y[u][w] = u32x4{0, 0, 0, 0};
+      }
+      if constexpr (DT == DA_F32) {
+        u32x4 w[NP];
+        cut_chunk<NP>(__builtin_bit_cast(f32x4, y[u][0]), __builtin_bit_cast(f32x4, y[u][1]), w);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *(u32x4*)(at + p * kMTile * kMRow) = w[p];
+      } else {
+        *(u32x4*)at = y[u][0];
+      }
+    }
+    if (wid == 0) {
+      // rows pass: whether any key has a weight other than 1; both: the extreme time of the rows
+      const bool mine = lane < kMTile;
+      if (mine) {
+        s_add[st][lane] = m_add;
+        s_t[st][lane] = m_t;
+      }
+      int e = mine ? m_t : (PASS == 0 ? -0x7fffffff : 0x7fffffff);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_xor(e, d, 64);
+        e = PASS == 0 ? max(e, o) : min(e, o);
+      }
+      const uint64_t odd = __ballot(mine && !zero_bits(m_add));
+      if (lane == 0) {
+        s_flag[st] = odd != 0;
+        s_ext[st] = e;
+      }
+    }
+  };
+
+  float m_run[NCB], sum[NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    m_run[cb] = -INFINITY;
+    sum[cb] = 0.0f;
+  }
+  const float c2 = a.scale_log2;
+
+  if (t_begin < t_end) {
+    load_tile(t_begin);
+    store_tile(0);
+  }
+  __syncthreads();
+  for (int tile = t_begin; tile < t_end; ++tile) {
+    const int st = (tile - t_begin) & 1;
+    const bool next = tile + 1 < t_end;
+    if (next) load_tile(tile + 1);
+    f32x16 s[NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[cb][r] = 0.0f;
+    const char* const yb = s_y[st] + cl * kMRow;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      if (kk < KK) {
+        u32x4 f[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          f[p] = *(const u32x4*)(yb + p * kMTile * kMRow + (((2 * kk + hl) ^ (cl & 15)) << 4));
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+          if constexpr (NP == 1) {
+            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
+          } else {  // the smallest products first
+            s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
+          }
+        }
+      }
+    }
+    const int e = __builtin_amdgcn_readfirstlane(s_ext[st]);
+    const bool weights = __builtin_amdgcn_readfirstlane(s_flag[st]) != 0;
+    const bool mask = PASS == 0 ? e > ext : e < ext;
+    // register r of a block is row 8 (r / 4) + 4 hl + r % 4 of the tile
+    if (PASS == 0) {
+      const bool plain = !weights && !mask;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        float p = 0.0f;
+        if (plain) {
+          const float base = is_neg_inf(m_run[cb]) ? 0.0f : m_run[cb];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p += mexp2(__builtin_fmaf(s[cb][r], c2, -base));
+        } else {
+          const float base = is_neg_inf(m_run[cb]) ? 0.0f : m_run[cb];
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 add = *(const f32x4*)&s_add[st][8 * r4 + 4 * hl];
+            const int4 t4 = *(const int4*)&s_t[st][8 * r4 + 4 * hl];
+            const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v = __builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]);
+              if (mask && tt[i] > ct[cb]) v = -INFINITY;
+              s[cb][4 * r4 + i] = v;
+              p += mexp2(v - base);
+            }
+          }
+        }
+        if (__ballot(is_neg_inf(m_run[cb]) || p > kMLarge)) {
+          float mx = m_run[cb];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            if (plain) s[cb][r] *= c2;
+            mx = __builtin_fmaxf(mx, s[cb][r]);
+          }
+          const float base = is_neg_inf(mx) ? 0.0f : mx;
+          sum[cb] *= mexp2(m_run[cb] - base);
+          p = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p += mexp2(s[cb][r] - base);
+          m_run[cb] = mx;
+        }
+        sum[cb] += p;
+      }
+    } else {
+      if (!mask) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 add = *(const f32x4*)&s_add[st][8 * r4 + 4 * hl];
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[cb] += mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]));
+        }
+      } else {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 add = *(const f32x4*)&s_add[st][8 * r4 + 4 * hl];
+          const int4 t4 = *(const int4*)&s_t[st][8 * r4 + 4 * hl];
+          const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]));
+              sum[cb] += tt[i] < ct[cb] ? 0.0f : p;
+            }
+        }
+      }
+    }
+    if (next) store_tile(st ^ 1);
+    __syncthreads();
+  }
+
+  // ---- the two halves of a column, then out ----
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int c = c0 + (wid * NCB + cb) * 32 + cl;
+    if (PASS == 0) {
+      const float m2 = __shfl_xor(m_run[cb], 32, 64), l2 = __shfl_xor(sum[cb], 32, 64);
+      const float M = __builtin_fmaxf(m_run[cb], m2), base = is_neg_inf(M) ? 0.0f : M;
+      const float L = sum[cb] * mexp2(m_run[cb] - base) + l2 * mexp2(m2 - base);
+      if (hl == 0 && c < R) {
+        if (a.split == 1) {
+          rowadd[c] = zero_bits(L) ? -INFINITY : -(M + __builtin_amdgcn_logf(L));
+        } else {
+          float* const p = a.part + (((int64_t)bh * R + c) * a.split + blockIdx.y) * 2;
+          p[0] = M;
+          p[1] = L;
+        }
+      }
+    } else {
+      const float t = sum[cb] + __shfl_xor(sum[cb], 32, 64);
+      if (hl == 0 && c < a.Nk) {
+        float v = c < n ? t : 0.0f;
+        if (cnt && c < n) v = cnt[c] > 0 ? t * (float)cnt[c] : 0.0f;
+        if (a.split == 1) a.mass[(int64_t)bh * a.Nk + c] = v;
+        else a.part[((int64_t)blockIdx.y * gridDim.z + bh) * a.Nk + c] = v;
+      }
+    }
+  }
+}
+
+// A query's (max, sum) parts -> -lse, or -inf where it saw nothing.
+__global__ __launch_bounds__(256) void mass_join_rows_kernel(const float* part, float* rowadd, int64_t rows, int split) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows) return;
+  const f32x2* p = (const f32x2*)part + i * split;
+  float M = -INFINITY;
+  for (int s = 0; s < split; ++s) M = __builtin_fmaxf(M, p[s][0]);
+  const float base = is_neg_inf(M) ? 0.0f : M;
+  float L = 0.0f;
+  for (int s = 0; s < split; ++s) L += p[s][1] * mexp2(p[s][0] - base);
+  rowadd[i] = zero_bits(L) ? -INFINITY : -(M + __builtin_amdgcn_logf(L));
+}
+
+// The splits' column sums, added in order.
+__global__ __launch_bounds__(256) void mass_join_cols_kernel(const float* part, float* mass, int64_t cols, int split) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= cols) return;
+  float v = 0.0f;
+  for (int s = 0; s < split; ++s) v += part[(int64_t)s * cols + i];
+  mass[i] = v;
+}
+
+// Splits of the streamed rows: workgroups for every CU a few times over, and at least
+// kMinTiles tiles each.
+static int mass_split(int64_t blocks, int64_t streamed) {
+  constexpr int64_t kMinTiles = 4;
+  int64_t want = (1024 + blocks - 1) / blocks;
+  const int64_t most = (streamed + kMTile * kMinTiles - 1) / (kMTile * kMinTiles);
+  if (want > most) want = most;
+  if (want > 64) want = 64;
+  return (int)(want < 1 ? 1 : want);
+}
+struct MassPlan {
+  int cols, split0, split1;
+  int64_t blocks0, blocks1, rows, part;
+};
+static MassPlan mass_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq, int64_t Nk) {
+  MassPlan p;
+  p.cols = dtype == DA_F32 ? 128 : 256;
+  p.rows = Hq / Hkv * Nq;
+  p.blocks0 = (p.rows + p.cols - 1) / p.cols;
+  p.blocks1 = (Nk + p.cols - 1) / p.cols;
+  p.split0 = mass_split(p.blocks0 * B * Hkv, Nk);
+  p.split1 = mass_split(p.blocks1 * B * Hkv, p.rows);
+  const int64_t p0 = p.split0 > 1 ? B * Hkv * p.rows * p.split0 * 2 : 0;
+  const int64_t p1 = p.split1 > 1 ? B * Hkv * Nk * p.split1 : 0;
+  p.part = p0 > p1 ? p0 : p1;
+  return p;
+}
+
+template <int DT>
+static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char* who) {
+  const unsigned bh = (unsigned)(a.B * a.Hkv);
+  a.split = p.split0;
+  hipLaunchKernelGGL((mass_kernel<DT, 0>), dim3((unsigned)p.blocks0, p.split0, bh), dim3(256), 0, st, a);
+  if (p.split0 > 1) {
+    const int64_t rows = bh * p.rows;
+    hipLaunchKernelGGL(mass_join_rows_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a.part, a.rowadd,
+                       rows, p.split0);
+  }
+  a.split = p.split1;
+  hipLaunchKernelGGL((mass_kernel<DT, 1>), dim3((unsigned)p.blocks1, p.split1, bh), dim3(256), 0, st, a);
+  if (p.split1 > 1) {
+    const int64_t cols = (int64_t)bh * a.Nk;
+    hipLaunchKernelGGL(mass_join_cols_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, st, a.part, a.mass,
+                       cols, p.split1);
+  }
+  return check_launch(who);
+}
+
+}  // namespace da
+
+using namespace da;
+
+// -lse of every query row, then the splits' parts (of whichever type needs more).
+extern "C" int64_t da_attention_mass_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq, int64_t Nk) {
+  if (B <= 0 || Hkv <= 0 || Hq < Hkv || Nq <= 0 || Nk <= 0) return 0;
+  const MassPlan p = mass_plan(DA_BF16, B, Hq, Hkv, Nq, Nk), p32 = mass_plan(DA_F32, B, Hq, Hkv, Nq, Nk);
+  const int64_t rows = (B * Hkv * p.rows + 3) / 4 * 4;
+  return (rows + (p.part > p32.part ? p.part : p32.part)) * (int64_t)sizeof(float);
+}
+
+extern "C" int da_attention_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Hq, int64_t Hkv,
+                                 int64_t Nq, int64_t Nk, int64_t D, int64_t sq_b, int64_t sq_h, int64_t sq_n,
+                                 int64_t sk_b, int64_t sk_h, int64_t sk_n, const int32_t* counts,
+                                 const int32_t* timestamps, const int32_t* lengths, int64_t q_start, float scale,
+                                 float* mass, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "da_attention_mass";
+  DA_REQUIRE(q && k && mass, "%s: null pointer", who);
+  if (dtype != DA_BF16 && dtype != DA_F16 && dtype != DA_F32)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: q and k must be bf16, fp16 or fp32", who);
+  if (D <= 0 || D > 128 || (D & 7))
+    return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128]", who);
+  DA_REQUIRE(B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Nq > 0 && Nk > 0, "%s: bad shape", who);
+  if (Hq / Hkv > 64) return set_error(DA_ERR_UNSUPPORTED, "%s: GQA group above 64", who);
+  if (Nk > (1 << 24) || Nq > (1 << 24) || Hq / Hkv * Nq >= (1ll << 30) || B * Hkv > 65535)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: more than 2^24 keys or queries, 2^30 query rows a KV head or 65535 "
+                     "(sequence, head) pairs", who);
+  const int64_t align = dtype == DA_F32 ? 3 : 7;
+  DA_REQUIRE(((sq_b | sq_h | sq_n | sk_b | sk_h | sk_n) & align) == 0 && (((uintptr_t)q | (uintptr_t)k) & 15) == 0,
+             "%s: rows must be 16-byte aligned", who);
+  DA_REQUIRE(scale > 0.0f, "%s: scale must be positive", who);
+  DA_REQUIRE(q_start > -(1ll << 40) && q_start < (1ll << 40), "%s: q_start out of range", who);
+  const int64_t need = da_attention_mass_workspace_size(B, Hq, Hkv, Nq, Nk);
+  if (!workspace || workspace_bytes < need)
+    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
+  DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
+  const MassPlan p = mass_plan(dtype, B, Hq, Hkv, Nq, Nk);
+  MassArgs a = {};
+  a.q = q; a.k = k;
+  a.sq_b = sq_b; a.sq_h = sq_h; a.sq_n = sq_n; a.sk_b = sk_b; a.sk_h = sk_h; a.sk_n = sk_n;
+  a.counts = counts; a.ts = timestamps; a.lengths = lengths; a.q_start = q_start;
+  a.scale_log2 = scale * kMLog2e;
+  a.rowadd = (float*)workspace;
+  a.part = a.rowadd + (B * Hkv * p.rows + 3) / 4 * 4;
+  a.mass = mass;
+  a.B = (int)B; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.Nq = (int)Nq; a.Nk = (int)Nk; a.D = (int)D;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DA_F32) return launch_mass<DA_F32>(a, p, st, who);
+  if (dtype == DA_F16) return launch_mass<DA_F16>(a, p, st, who);
+  return launch_mass<DA_BF16>(a, p, st, who);
+}

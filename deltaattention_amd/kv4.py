@@ -1,0 +1,373 @@
+"""A decode cache that stays bounded: rows in 4 bits, the attention weight each row received,
+eviction by it, and decode attention over 4-bit rows (include/deltaattn_cache.h).
+
+The compressed cache of the reference (deltaDecoding.py:111-233) keeps every anchor at full
+width; these operations have no counterpart there.  They follow ``ops``: GPU tensors, the
+current stream of the tensors' device, no synchronisation, no CPU fallback, errors as
+Python exceptions.  Users reach them as ``ops.KV4``, ``ops.attention_mass`` and so on;
+``deltaDecoding.FourBitCompressedCache`` is the cache object built on them.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from ._native import Kv4Block, check, dtype_code, lib, on_device
+
+__all__ = ["KV4", "attention_mass", "heavy_rows", "quantize_kv4", "dequantize_kv4", "evict_kv4",
+           "decode_attention_kv4"]
+
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
+
+
+def _want(t: Optional[torch.Tensor], name: str, shape, dtype, device) -> None:
+    """Refuse a tensor that is not contiguous, of this shape and type and on this device."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _gpu(t: torch.Tensor, name: str) -> torch.device:
+    if t.device.type != "cuda":
+        raise ValueError(f"deltaattention_amd operations take GPU tensors ({name} is on {t.device}); "
+                         "there is no CPU path")
+    return t.device
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with a contiguous head dimension and rows that begin at multiples of 16 bytes."""
+    per = 4 if t.dtype == _F32 else 8
+    s = t.stride()
+    if s[-1] == 1 and not any(x % per for x, n in zip(s[:-1], t.shape) if n > 1) and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    """Batch, head and row strides; 0 for a dimension of one, whose stride means nothing."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+class KV4:
+    """Key and value rows of one layer in 4 bits, for every (sequence, KV head).
+
+    A row of ``head_dim`` dims is cut into groups of 32; a group has one power of two and
+    elements 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times it, with a sign.  ``k_codes`` / ``v_codes``
+    [B, Hkv, capacity, 16 * groups] uint8 hold two elements a byte (even dim low),
+    ``k_scales`` / ``v_scales`` [B, Hkv, capacity, groups] uint8 the exponents plus 127 (255:
+    a group that held an infinity or NaN, which reads back as NaN).  ``counts`` and
+    ``timestamps`` [B, Hkv, capacity] int32 are those of the packed anchors (a row of count c
+    weighs like c keys), ``mass`` [B, Hkv, capacity] float32 (or None) the attention weight
+    each row has received, ``lengths`` [B, Hkv] int32 the rows in use.  All contiguous; the
+    tensors of an object are fixed, their contents are not.
+    """
+
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "counts", "timestamps", "lengths", "mass",
+                 "head_dim", "_block", "_ref")
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales, counts, timestamps, lengths, head_dim, mass=None):
+        D = int(head_dim)
+        if D <= 0 or D > 128 or D % 8:
+            raise ValueError(f"head_dim must be a multiple of 8 in [8, 128], got {head_dim}")
+        groups = (D + 31) // 32
+        if k_codes.dim() != 4:
+            raise ValueError("k_codes must have shape [B, Hkv, capacity, 16 * groups]")
+        device = _gpu(k_codes, "k_codes")
+        B, H, cap, _ = k_codes.shape
+        if not (B and H and cap):
+            raise ValueError("a cache needs sequences, heads and rows")
+        for t, name in ((k_codes, "k_codes"), (v_codes, "v_codes")):
+            _want(t, name, (B, H, cap, 16 * groups), _U8, device)
+            if t.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned")
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            _want(t, name, (B, H, cap, groups), _U8, device)
+        _want(counts, "counts", (B, H, cap), _I32, device)
+        _want(timestamps, "timestamps", (B, H, cap), _I32, device)
+        _want(lengths, "lengths", (B, H), _I32, device)
+        if mass is not None:
+            _want(mass, "mass", (B, H, cap), _F32, device)
+        put = object.__setattr__
+        put(self, "k_codes", k_codes)
+        put(self, "k_scales", k_scales)
+        put(self, "v_codes", v_codes)
+        put(self, "v_scales", v_scales)
+        put(self, "counts", counts)
+        put(self, "timestamps", timestamps)
+        put(self, "lengths", lengths)
+        put(self, "mass", mass)
+        put(self, "head_dim", D)
+        block = Kv4Block(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                         counts.data_ptr(), timestamps.data_ptr(), lengths.data_ptr(), _ptr(mass), cap)
+        put(self, "_block", block)
+        put(self, "_ref", ctypes.byref(block))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"KV4.{name} is fixed; build another KV4 from the tensors")
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, device="cuda", mass: bool = True) -> "KV4":
+        """A cache of ``capacity`` rows a head with undefined contents (``lengths`` too)."""
+        g = (head_dim + 31) // 32
+        new = torch.empty
+        shape = (batch, kv_heads, capacity)
+        return cls(new((*shape, 16 * g), dtype=_U8, device=device), new((*shape, g), dtype=_U8, device=device),
+                   new((*shape, 16 * g), dtype=_U8, device=device), new((*shape, g), dtype=_U8, device=device),
+                   new(shape, dtype=_I32, device=device), new(shape, dtype=_I32, device=device),
+                   new(shape[:2], dtype=_I32, device=device), head_dim,
+                   new(shape, dtype=_F32, device=device) if mass else None)
+
+    @property
+    def batch(self) -> int:
+        return self.k_codes.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k_codes.shape[1]
+
+    @property
+    def capacity(self) -> int:
+        return self.k_codes.shape[2]
+
+    @property
+    def device(self) -> torch.device:
+        return self.k_codes.device
+
+
+def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                   timestamps: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                   q_start: Optional[int] = None, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention weight every key receives from the queries: float32 [B, Hkv, Nk], summed over
+    the queries and the query heads of each KV head's group.
+
+    q [B, Hq, Nq, D] (usually the prompt's last queries, or all of them), k [B, Hkv, Nk, D].
+    Query i is at position ``q_start + i`` (default Nk - Nq, the last ones; needed with
+    ``timestamps``) and sees key j if j is below the head's ``lengths`` and its position
+    ``timestamps[b, g, j]`` (default j) is not past the query's.  ``counts`` adds log(count) to
+    the scores, as packed anchors have it; a count <= 0 hides the key.  A query that sees
+    nothing adds nothing; keys past the length get 0.
+    """
+    device = _gpu(q, "q")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k are [B, heads, tokens, head_dim]")
+    dt = dtype_code(q, k)
+    B, Hq, Nq, D = q.shape
+    H, N = k.shape[1], k.shape[2]
+    if k.device != device or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"k {list(k.shape)} on {k.device} does not fit q {list(q.shape)} on {device}")
+    if not (B and Nq and N and H and Hq) or Hq % H:
+        raise ValueError(f"{Hq} query heads over {H} KV heads, {Nq} queries, {N} keys")
+    if counts is not None:
+        _want(counts, "counts", (B, H, N), _I32, device)
+    if timestamps is not None:
+        _want(timestamps, "timestamps", (B, H, N), _I32, device)
+        if q_start is None:
+            raise ValueError("q_start (the position of the first query) is needed with timestamps")
+    if lengths is not None:
+        _want(lengths, "lengths", (B, H), _I32, device)
+    if out is None:
+        out = torch.empty((B, H, N), dtype=_F32, device=device)
+    else:
+        _want(out, "out", (B, H, N), _F32, device)
+    q, k = _rows(q), _rows(k)
+    n = lib().da_attention_mass_workspace_size(B, Hq, H, Nq, N)
+    ws = torch.empty((n,), dtype=_U8, device=device)
+    with on_device(device) as stream:
+        rc = lib().da_attention_mass(q.data_ptr(), k.data_ptr(), dt, B, Hq, H, Nq, N, D, *_strides(q), *_strides(k),
+                                     _ptr(counts), _ptr(timestamps), _ptr(lengths),
+                                     N - Nq if q_start is None else int(q_start),
+                                     D ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), n,
+                                     stream)
+    check(rc, "da_attention_mass")
+    return out
+
+
+def heavy_rows(mass: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
+               lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rows that a budget leaves: mass float32 [B, Hkv, N] -> (index [B, Hkv, budget] int32,
+    rows ascending and -1 past them, and their number [B, Hkv] int32).
+
+    A head with at most ``budget`` rows (``lengths``, default N) keeps all.  A longer one keeps
+    its first ``sinks`` rows, its last ``recent`` rows, and of those between the
+    budget - sinks - recent with the largest mass, ties to the lower row.
+    """
+    device = _gpu(mass, "mass")
+    if mass.dim() != 3:
+        raise ValueError("mass is [B, Hkv, N]")
+    B, H, N = mass.shape
+    _want(mass, "mass", (B, H, N), _F32, device)
+    if lengths is not None:
+        _want(lengths, "lengths", (B, H), _I32, device)
+    budget, sinks, recent = _budget(budget, sinks, recent)
+    index = torch.empty((B, H, budget), dtype=_I32, device=device)
+    kept = torch.empty((B, H), dtype=_I32, device=device)
+    n = lib().da_kv4_evict_workspace_size(B, H, N, budget)
+    ws = torch.empty((n,), dtype=_U8, device=device)
+    with on_device(device) as stream:
+        rc = lib().da_heavy_rows(mass.data_ptr(), _ptr(lengths), B, H, N, budget, sinks, recent, index.data_ptr(),
+                                 kept.data_ptr(), ws.data_ptr(), n, stream)
+    check(rc, "da_heavy_rows")
+    return index, kept
+
+
+def _budget(budget, sinks, recent):
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"needs sinks + recent <= budget and a positive budget, got {sinks} + {recent} and {budget}")
+    return budget, sinks, recent
+
+
+def quantize_kv4(k: torch.Tensor, v: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                 timestamps: Optional[torch.Tensor] = None, mass: Optional[torch.Tensor] = None,
+                 lengths: Optional[torch.Tensor] = None, index: Optional[torch.Tensor] = None,
+                 capacity: Optional[int] = None) -> KV4:
+    """k, v [B, Hkv, N, D] (any strides) into a new 4-bit cache of ``capacity`` rows a head.
+
+    Without ``index`` row m becomes row m; with it ([B, Hkv, M] int32, as ``heavy_rows`` gives
+    it) row index[b, g, m] does.  counts, timestamps and mass [B, Hkv, N] come along (default
+    1, the row's number, 0).  ``lengths`` [B, Hkv] are the rows in use (default: all of them);
+    rows past them, and those whose index is not a row of k, are zero with count 0, and rows
+    from N (M) to the capacity are undefined.
+    """
+    device = _gpu(k, "k")
+    if k.dim() != 4 or v.shape != k.shape or v.device != device:
+        raise ValueError("k and v are [B, Hkv, N, D] of one shape on one device")
+    dt = dtype_code(k, v)
+    B, H, N, D = k.shape
+    if not (B and H and N):
+        raise ValueError("k and v hold no rows")
+    for t, name, ty in ((counts, "counts", _I32), (timestamps, "timestamps", _I32), (mass, "mass", _F32)):
+        if t is not None:
+            _want(t, name, (B, H, N), ty, device)
+    M = N
+    if index is not None:
+        if index.dim() != 3 or index.shape[2] == 0:
+            raise ValueError("index is [B, Hkv, M]")
+        M = index.shape[2]
+        _want(index, "index", (B, H, M), _I32, device)
+    if lengths is not None:
+        _want(lengths, "lengths", (B, H), _I32, device)
+    capacity = M if capacity is None else int(capacity)
+    if capacity < M:
+        raise ValueError(f"{M} rows do not fit a capacity of {capacity}")
+    k, v = _rows(k), _rows(v)
+    out = KV4.empty(B, H, capacity, D, device)
+    with on_device(device) as stream:
+        rc = lib().da_kv4_quantize(k.data_ptr(), v.data_ptr(), dt, B, H, N, D, *_strides(k), *_strides(v),
+                                   _ptr(counts), _ptr(timestamps), _ptr(mass), _ptr(lengths), _ptr(index), M, out._ref,
+                                   stream)
+    check(rc, "da_kv4_quantize")
+    return out
+
+
+def dequantize_kv4(kv: KV4, dtype: torch.dtype = torch.bfloat16, rows: Optional[int] = None):
+    """(k, v) [B, Hkv, rows, D]: the values of the first ``rows`` (default: all) 4-bit rows, zero
+    past a head's length."""
+    N = kv.capacity if rows is None else int(rows)
+    if not 0 < N <= kv.capacity:
+        raise ValueError(f"rows must lie in [1, {kv.capacity}], got {N}")
+    shape = (kv.batch, kv.kv_heads, N, kv.head_dim)
+    k, v = (torch.empty(shape, dtype=dtype, device=kv.device) for _ in range(2))
+    dt = dtype_code(k)
+    with on_device(kv.device) as stream:
+        rc = lib().da_kv4_dequantize(kv._ref, *shape, k.data_ptr(), v.data_ptr(), dt, stream)
+    check(rc, "da_kv4_dequantize")
+    return k, v
+
+
+def evict_kv4(kv: KV4, budget: int, sinks: int = 0, recent: int = 0, capacity: Optional[int] = None) -> KV4:
+    """A new cache with the rows of ``kv`` that the budget leaves (the rule of ``heavy_rows`` on
+    ``kv.mass`` and ``kv.lengths``), in their order, with their counts, timestamps and mass.
+    Rows past those kept are zero up to the budget and undefined from there to ``capacity``
+    (default: the budget).  ``kv`` stays as it is."""
+    if kv.mass is None:
+        raise ValueError("eviction needs the cache's mass")
+    budget, sinks, recent = _budget(budget, sinks, recent)
+    capacity = budget if capacity is None else int(capacity)
+    if capacity < budget:
+        raise ValueError(f"a budget of {budget} rows does not fit a capacity of {capacity}")
+    B, H, cap, D, device = kv.batch, kv.kv_heads, kv.capacity, kv.head_dim, kv.device
+    out = KV4.empty(B, H, capacity, D, device)
+    n = lib().da_kv4_evict_workspace_size(B, H, cap, budget)
+    ws = torch.empty((n,), dtype=_U8, device=device)
+    with on_device(device) as stream:
+        rc = lib().da_kv4_evict(kv._ref, B, H, D, budget, sinks, recent, out._ref, None, ws.data_ptr(), n, stream)
+    check(rc, "da_kv4_evict")
+    return out
+
+
+def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tensor] = None,
+                         v_exact: Optional[torch.Tensor] = None, exact_len: Optional[int] = None,
+                         scale: Optional[float] = None, accumulate: bool = False,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One decode token: q [B, Hq, 1, D] (or [B, Hq, D]) -> the same shape, attention over the 4-bit
+    rows (scores + log(count)) and the first ``exact_len`` (default W) slots of the ring
+    k_exact, v_exact [B, Hkv, W, D] in q's type.
+
+    ``accumulate`` adds each row's softmax weight, summed over its group's query heads, to
+    ``kv.mass``.  A head without any key gives zeros.  Query head h reads KV head
+    h // (Hq // Hkv).
+    """
+    device = kv.device
+    if q.dim() == 4 and q.shape[2] == 1:
+        q3 = q.squeeze(2)
+    elif q.dim() == 3:
+        q3 = q
+    else:
+        raise ValueError("q is [B, Hq, 1, D] or [B, Hq, D]")
+    B, Hq, D = q3.shape
+    H = kv.kv_heads
+    if q.device != device or B != kv.batch or D != kv.head_dim or Hq % H or not Hq:
+        raise ValueError(f"q {list(q.shape)} on {q.device} does not fit a cache of {kv.batch} sequences, {H} KV heads "
+                         f"and head_dim {kv.head_dim} on {device}")
+    if (k_exact is None) != (v_exact is None):
+        raise ValueError("k_exact and v_exact come together")
+    if accumulate and kv.mass is None:
+        raise ValueError("accumulate needs the cache's mass")
+    dt = dtype_code(q, k_exact, v_exact, out)
+    sx = (0, 0, 0)
+    W = 0
+    if k_exact is not None:
+        W = k_exact.shape[2] if k_exact.dim() == 4 else 0
+        if k_exact.shape != (B, H, W, D) or v_exact.shape != k_exact.shape or k_exact.device != device \
+                or v_exact.device != device:
+            raise ValueError(f"k_exact and v_exact must be [{B}, {H}, W, {D}] on {device}")
+        sx = k_exact.stride()
+        if sx[3] != 1 or v_exact.stride() != sx:
+            k_exact, v_exact = (t.clone(memory_format=torch.contiguous_format) for t in (k_exact, v_exact))
+            sx = k_exact.stride()
+    n_exact = W if exact_len is None else int(exact_len)
+    if not 0 <= n_exact <= W:
+        raise ValueError(f"exact_len must lie in [0, {W}], got {n_exact}")
+    if q3.stride(2) != 1:
+        q3 = q3.contiguous()
+    if out is None:
+        out3 = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
+        result = out3.view(q.shape)
+    else:
+        if out.shape != q.shape or out.device != device or out.stride(-1) != 1:
+            raise ValueError("out must have q's shape and device and a contiguous head dimension")
+        out3, result = (out.squeeze(2) if out.dim() == 4 else out), out
+    native = lib()
+    n = native.da_kv4_attention_workspace_size(B, Hq, H, kv.capacity, 1 if accumulate else 0)
+    ws = torch.empty((n,), dtype=_U8, device=device)
+    sq, so = q3.stride(), out3.stride()
+    with on_device(device) as stream:
+        rc = native.da_kv4_attention(q3.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, _ptr(k_exact),
+                                     _ptr(v_exact), sx[0], sx[1], sx[2], n_exact,
+                                     D ** -0.5 if scale is None else float(scale), 1 if accumulate else 0,
+                                     out3.data_ptr(), so[0], so[1], ws.data_ptr(), n, stream)
+    check(rc, "da_kv4_attention")
+    return result
