@@ -221,14 +221,19 @@ __device__ __forceinline__ uint32_t mass_order(float m) {
 }
 
 constexpr int kHeavyThreads = 1024, kHeavyWaves = kHeavyThreads / 64, kHeavyBins = 2048;
+constexpr int kHeavyPer = 16;                              // masses a thread holds at once
+constexpr int kHeavyBatch = kHeavyThreads * kHeavyPer;     // rows of a batch
 
 // One workgroup per (sequence, head).  The border (the need-th largest mass between the
 // protected ends) comes from three histogram passes over 11, 11 and 10 bits of the order;
 // a last pass writes the rows above it, and as many of its equals as still fit, lowest row
-// first, in row order.
+// first, in row order.  Rows come in batches of 16384, 16 loads in flight a thread; a head of
+// one batch is read once.
 __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) {
   __shared__ uint32_t s_hist[kHeavyBins];
-  __shared__ uint32_t s_wave[2][kHeavyWaves];
+  __shared__ uint32_t s_wave[kHeavyWaves];
+  __shared__ uint32_t s_cnt[2][kHeavyPer * kHeavyWaves];  // rows above / at the border, in row order
+  __shared__ uint32_t s_all[2];
   __shared__ uint32_t s_pick[2];  // the chosen bin, the rows still needed from it
   const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int64_t n64 = a.lengths ? a.lengths[bh] : a.capacity;
@@ -243,26 +248,45 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
   }
   const float* const mass = a.mass + (int64_t)bh * a.capacity;
   const int lo = a.sinks, hi = n - a.recent;  // the rows that compete
+  for (int i = tid; i < a.sinks; i += kHeavyThreads) out[i] = i;
+  for (int i = tid; i < a.recent; i += kHeavyThreads) out[a.budget - a.recent + i] = hi + i;
   uint32_t need = (uint32_t)(a.budget - a.sinks - a.recent);
+  if (need == 0) return;
+  uint32_t u[kHeavyPer];
+  auto load = [&](int base) {
+    float m[kHeavyPer];
+#pragma unroll
+    for (int j = 0; j < kHeavyPer; ++j) {
+      const int i = base + j * kHeavyThreads + tid;
+      m[j] = mass[i < hi ? i : hi - 1];
+    }
+#pragma unroll
+    for (int j = 0; j < kHeavyPer; ++j) u[j] = mass_order(m[j]);
+  };
+  const bool one = hi - lo <= kHeavyBatch;
+  if (one) load(lo);
   uint32_t prefix = 0, mask = 0;  // bits of the border found so far
-  for (int pass = 0; pass < 3 && need > 0; ++pass) {
+  for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t bits = pass == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kHeavyBins; i += kHeavyThreads) s_hist[i] = 0;
+    s_hist[tid] = 0;
+    s_hist[tid + kHeavyThreads] = 0;
     __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += kHeavyThreads) {
-      const int i = i0 + tid;
-      const uint32_t u = i < hi ? mass_order(mass[i]) : 0;
-      const bool in = i < hi && (u & mask) == prefix;
-      const uint32_t bin = (u >> shift) & bits;
-      // lanes that share the first active lane's bin (rows of no weight at all, often most
-      // of them) add together; the others one by one
-      const uint64_t act = __ballot(in);
-      if (act) {
-        const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
-        const uint64_t same = __ballot(in && bin == lead);
-        if (lane == 0) atomicAdd(&s_hist[lead], (uint32_t)__popcll(same));
-        if (in && bin != lead) atomicAdd(&s_hist[bin], 1u);
+    for (int base = lo; base < hi; base += kHeavyBatch) {
+      if (!one) load(base);
+#pragma unroll
+      for (int j = 0; j < kHeavyPer; ++j) {
+        const bool in = base + j * kHeavyThreads + tid < hi && (u[j] & mask) == prefix;
+        const uint32_t bin = (u[j] >> shift) & bits;
+        // lanes that share the first active lane's bin (rows of no weight at all, often most
+        // of them) add together; the others one by one
+        const uint64_t act = __ballot(in);
+        if (act) {
+          const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
+          const uint64_t same = __ballot(in && bin == lead);
+          if (lane == 0) atomicAdd(&s_hist[lead], (uint32_t)__popcll(same));
+          if (in && bin != lead) atomicAdd(&s_hist[bin], 1u);
+        }
       }
     }
     __syncthreads();
@@ -275,11 +299,9 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
       const uint32_t up = (uint32_t)__shfl_down((int)suf, d, 64);
       suf += lane + d < 64 ? up : 0;
     }
-    if (lane == 0) s_wave[0][wid] = suf;
+    if (lane == 0) s_wave[wid] = suf;
     __syncthreads();
-    uint32_t above = 0;
-    for (int w = wid + 1; w < kHeavyWaves; ++w) above += s_wave[0][w];
-    suf += above;
+    for (int w = wid + 1; w < kHeavyWaves; ++w) suf += s_wave[w];
     const uint32_t after1 = suf - c0 - c1;  // rows in bins above 2 t + 1
     if (after1 < need && after1 + c1 >= need) {
       s_pick[0] = 2 * tid + 1;
@@ -292,43 +314,56 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
     prefix |= s_pick[0] << shift;
     mask |= bits << shift;
     need = s_pick[1];
-    __syncthreads();
   }
   // rows above the border, and the first `need` of its equals, in order
-  const bool any = a.budget > a.sinks + a.recent;
-  for (int i = tid; i < a.sinks; i += kHeavyThreads) out[i] = i;
-  for (int i = tid; i < a.recent; i += kHeavyThreads) out[a.budget - a.recent + i] = hi + i;
   uint32_t gt_before = 0, eq_before = 0;
-  if (any) {
-    for (int i0 = lo; i0 < hi; i0 += kHeavyThreads) {
-      const int i = i0 + tid;
-      const uint32_t u = i < hi ? mass_order(mass[i]) : 0;
-      const bool gt = i < hi && u > prefix, eq = i < hi && u == prefix;
-      const uint64_t bg = __ballot(gt), be = __ballot(eq);
-      if (lane == 0) {
-        s_wave[0][wid] = (uint32_t)__popcll(bg);
-        s_wave[1][wid] = (uint32_t)__popcll(be);
-      }
-      __syncthreads();
-      uint32_t g = gt_before, e = eq_before, gall = 0, eall = 0;
+  const uint64_t below = (1ull << lane) - 1;
+  for (int base = lo; base < hi; base += kHeavyBatch) {
+    if (!one) load(base);
+    uint64_t bg[kHeavyPer], be[kHeavyPer];
 #pragma unroll
-      for (int w = 0; w < kHeavyWaves; ++w) {
-        const uint32_t cg = s_wave[0][w], ce = s_wave[1][w];
-        if (w < wid) {
-          g += cg;
-          e += ce;
-        }
-        gall += cg;
-        eall += ce;
+    for (int j = 0; j < kHeavyPer; ++j) {
+      const bool in = base + j * kHeavyThreads + tid < hi;
+      bg[j] = __ballot(in && u[j] > prefix);
+      be[j] = __ballot(in && u[j] == prefix);
+      if (lane == 0) {
+        s_cnt[0][j * kHeavyWaves + wid] = (uint32_t)__popcll(bg[j]);
+        s_cnt[1][j * kHeavyWaves + wid] = (uint32_t)__popcll(be[j]);
       }
-      const uint64_t below = (1ull << lane) - 1;
-      g += (uint32_t)__popcll(bg & below);
-      e += (uint32_t)__popcll(be & below);
-      if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = i;
-      gt_before += gall;
-      eq_before += eall;
-      __syncthreads();
     }
+    __syncthreads();
+    if (wid < 2) {  // prefix sums of the 256 counts, four a lane: wave 0 above, wave 1 at the border
+      uint32_t c[4], run = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        c[j] = s_cnt[wid][4 * lane + j];
+        run += c[j];
+      }
+      uint32_t inc = run;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t dn = (uint32_t)__shfl_up((int)inc, d, 64);
+        inc += lane >= d ? dn : 0;
+      }
+      uint32_t at = inc - run;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s_cnt[wid][4 * lane + j] = at;
+        at += c[j];
+      }
+      if (lane == 63) s_all[wid] = inc;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kHeavyPer; ++j) {
+      const uint32_t g = gt_before + s_cnt[0][j * kHeavyWaves + wid] + (uint32_t)__popcll(bg[j] & below);
+      const uint32_t e = eq_before + s_cnt[1][j * kHeavyWaves + wid] + (uint32_t)__popcll(be[j] & below);
+      const bool gt = (bg[j] >> lane) & 1, eq = (be[j] >> lane) & 1;
+      if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = base + j * kHeavyThreads + tid;
+    }
+    gt_before += s_all[0];
+    eq_before += s_all[1];
+    __syncthreads();
   }
 }
 

@@ -359,32 +359,58 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Attn4Args a) {
   }
 }
 
-// Blocks [0, B Hq): one query head's splits joined (a thread a dim).  Blocks from there on add
-// the weights: kMassKeys keys of one (sequence, KV head) each, after the group's maxima and
-// sums over the splits.
+// Blocks [0, B Hq): one query head's splits joined, 32 lanes of four dims each, eight splits at a
+// time.  Blocks from there on add the weights: kMassKeys keys of one (sequence, KV head) each,
+// after the group's maxima and sums over the splits.
 constexpr int kMassKeys = 1024;
+// (max, sum) of a query head over the splits, by one wave
+__device__ __forceinline__ void join_stats(const float* part, int nsplit, int lane, float& m, float& l) {
+  m = -INFINITY;
+  l = 0.0f;
+  for (int s = lane; s < nsplit; s += 64) {
+    const float ms = part[(int64_t)s * kA4Part], ls = part[(int64_t)s * kA4Part + 1];
+    const float mm = __builtin_fmaxf(m, ms), base = is_neg_inf(mm) ? 0.0f : mm;
+    l = l * exp2_hw(m - base) + ls * exp2_hw(ms - base);
+    m = mm;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const float m2 = __shfl_xor(m, d, 64), l2 = __shfl_xor(l, d, 64);
+    const float mm = __builtin_fmaxf(m, m2), base = is_neg_inf(mm) ? 0.0f : mm;
+    l = l * exp2_hw(m - base) + l2 * exp2_hw(m2 - base);
+    m = mm;
+  }
+}
 template <int DT, bool MASS>
-__global__ __launch_bounds__(128) void kv4_join_kernel(Attn4Args a) {
+__global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
   __shared__ float s_m[64], s_l[64];
+  __shared__ __attribute__((aligned(16))) f32x4 s_o[8][32];
   const int Hq = a.Hkv * a.G;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int heads = a.B * Hq;
   if (!MASS || (int)blockIdx.x < heads) {
     const int bhq = blockIdx.x, b = bhq / Hq, hq = bhq - b * Hq;
     const float* part = a.part + (int64_t)bhq * a.nsplit * kA4Part;
-    float M = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) M = __builtin_fmaxf(M, part[s * kA4Part]);
-    const float base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, o = 0.0f;
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float m = part[s * kA4Part];
-      if (m == -INFINITY) continue;  // an empty split wrote no sums
+    const int c = tid & 31, sg = tid >> 5;  // dims 4 c .. 4 c + 3, splits sg, sg + 8, ...
+    float M, L;
+    join_stats(part, a.nsplit, lane, M, L);
+    const float base = is_neg_inf(M) ? 0.0f : M;
+    f32x4 o = f32x4{0, 0, 0, 0};
+    for (int s = sg; s < a.nsplit; s += 8) {
+      const float m = part[(int64_t)s * kA4Part];
+      if (is_neg_inf(m) || 4 * c >= a.D) continue;  // an empty split wrote no sums
       const float f = exp2_hw(m - base);
-      L += f * part[s * kA4Part + 1];
-      if (tid < a.D) o += f * part[s * kA4Part + 2 + tid];
+      const f32x2 v0 = *(const f32x2*)(part + (int64_t)s * kA4Part + 2 + 4 * c);
+      const f32x2 v1 = *(const f32x2*)(part + (int64_t)s * kA4Part + 4 + 4 * c);
+      o += f32x4{v0[0], v0[1], v1[0], v1[1]} * f;
     }
+    s_o[sg][c] = o;
+    __syncthreads();
     if (tid < a.D) {
-      const float v = zero_bits(L) ? 0.0f : o / L;
+      float v = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v += ((const float*)(const void*)s_o[s])[tid];
+      v = zero_bits(L) ? 0.0f : v / L;
       const int64_t at = b * a.so_b + hq * a.so_h + tid;
       if constexpr (DT == DA_F32) ((float*)a.out)[at] = v;
       else ((uint16_t*)a.out)[at] = E16<DT>::bits(v);
@@ -398,38 +424,29 @@ __global__ __launch_bounds__(128) void kv4_join_kernel(Attn4Args a) {
     n = n < 0 ? 0 : (n > a.capacity ? (int)a.capacity : n);
     const int first = chunk * kMassKeys;
     if (first >= n) return;
-    for (int h = wid; h < a.G; h += 2) {
-      const float* part = a.part + ((int64_t)bh * a.G + h) * a.nsplit * kA4Part;
-      float m = -INFINITY, l = 0.0f;
-      for (int s = lane; s < a.nsplit; s += 64) {
-        const float ms = part[s * kA4Part];
-        if (ms == -INFINITY) continue;
-        const float mm = __builtin_fmaxf(m, ms);
-        l = (m == -INFINITY ? 0.0f : l * exp2_hw(m - mm)) + part[s * kA4Part + 1] * exp2_hw(ms - mm);
-        m = mm;
-      }
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const float m2 = __shfl_xor(m, d, 64), l2 = __shfl_xor(l, d, 64);
-        const float mm = __builtin_fmaxf(m, m2);
-        const float base = mm == -INFINITY ? 0.0f : mm;
-        l = l * exp2_hw(m - base) + l2 * exp2_hw(m2 - base);
-        m = mm;
-      }
+    for (int h = wid; h < a.G; h += 4) {
+      float m, l;
+      join_stats(a.part + ((int64_t)bh * a.G + h) * a.nsplit * kA4Part, a.nsplit, lane, m, l);
       if (lane == 0) {
-        s_m[h] = m == -INFINITY ? 0.0f : m;
+        s_m[h] = is_neg_inf(m) ? 0.0f : m;
         s_l[h] = zero_bits(l) ? 0.0f : 1.0f / l;
       }
     }
     __syncthreads();
-    const int end = min(first + kMassKeys, n);
-    const float* score = a.score + (int64_t)bh * a.G * a.score_cap;
-    float* const mass = a.mass + (int64_t)bh * a.capacity;
-    for (int j = first + tid; j < end; j += 128) {
-      float w = 0.0f;
-      for (int h = 0; h < a.G; ++h) w += exp2_hw(score[h * a.score_cap + j] - s_m[h]) * s_l[h];
-      mass[j] += w;
+    // four keys a thread; the scores' rows are padded to whole tiles
+    const int j = first + 4 * tid;
+    if (j >= n) return;
+    const float* score = a.score + (int64_t)bh * a.G * a.score_cap + j;
+    float* const mass = a.mass + (int64_t)bh * a.capacity + j;
+    f32x4 w = f32x4{0, 0, 0, 0};
+    for (int h = 0; h < a.G; ++h) {
+      const f32x4 s = *(const f32x4*)(score + h * a.score_cap);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += exp2_hw(s[i] - s_m[h]) * s_l[h];
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i < n) mass[i] += w[i];
   }
 }
 
@@ -463,9 +480,9 @@ static int launch_attn4(const Attn4Args& a, bool mass, hipStream_t st, const cha
   const unsigned heads = (unsigned)(a.B * a.Hkv * a.G);
   if (mass) {
     const unsigned chunks = (unsigned)((a.capacity + kMassKeys - 1) / kMassKeys);
-    hipLaunchKernelGGL((kv4_join_kernel<DT, true>), dim3(heads + (unsigned)(a.B * a.Hkv) * chunks), dim3(128), 0, st, a);
+    hipLaunchKernelGGL((kv4_join_kernel<DT, true>), dim3(heads + (unsigned)(a.B * a.Hkv) * chunks), dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL((kv4_join_kernel<DT, false>), dim3(heads), dim3(128), 0, st, a);
+    hipLaunchKernelGGL((kv4_join_kernel<DT, false>), dim3(heads), dim3(256), 0, st, a);
   }
   return check_launch(who);
 }

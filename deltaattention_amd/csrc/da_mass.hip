@@ -28,10 +28,10 @@
 
 namespace da {
 
-constexpr int kMTile = 32;             // streamed rows a tile
 constexpr int kMRow = 256;             // bytes of a row in LDS (128 16-bit dims)
 constexpr float kMLog2e = 1.4426950408889634f;
 constexpr float kMLarge = 1.2676506e30f;  // 2^100: a tile's sum above it moves the maximum
+constexpr int kNever = 0x7fffffff;        // a time after every query's, and (negated) before every key's
 
 struct MassArgs {
   const void* q;
@@ -42,18 +42,22 @@ struct MassArgs {
   const int32_t* lengths;
   int64_t q_start;
   float scale_log2;
-  float* part;    // rows pass: [bh][R][split] (max, sum); columns pass: [split][bh][Nk] sums
-  float* rowadd;  // [bh][R]: -lse, or -inf where a query sees nothing
+  float* part;   // rows pass: [bh][R][split] (max, sum); columns pass: [split][bh][Nk] sums
+  float* stats;  // [bh][R] (-max, 1 / sum); (-inf, 0) where a query sees nothing
   float* mass;
-  int B, Hkv, G, Nq, Nk, D;
-  int split;
+  int B, Hkv, G, gshift, Nq, Nk, D;  // gshift: log2 G, or -1
+  int split, blocks;  // of the pass
 };
 
 __device__ __forceinline__ float mexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The position of query i, between the two values of kNever.
 __device__ __forceinline__ int mass_pos(const MassArgs& a, int i) {
   const int64_t p = a.q_start + i;
-  return p < -0x7ffffffe ? -0x7ffffffe : (p > 0x7fffffff ? 0x7fffffff : (int)p);
+  return p <= -kNever ? -kNever + 1 : (p >= kNever ? kNever - 1 : (int)p);
+}
+__device__ __forceinline__ int query_of(const MassArgs& a, int row) {
+  return a.gshift >= 0 ? row >> a.gshift : row / a.G;
 }
 
 // Eight fp32 elements as NP bf16 operands of eight, largest part first.
@@ -71,29 +75,45 @@ __device__ __forceinline__ void cut_chunk(f32x4 x0, f32x4 x1, u32x4 (&w)[NP]) {
     }
 }
 
+// What the columns pass needs of a query: its weights are 2^(s - max) / sum.  The maximum is kept
+// apart from the sum (not as one logarithm): s - max is small where the weight is large, so it
+// rounds finely there.
+__device__ __forceinline__ f32x2 row_stats(float M, float L) {
+  return zero_bits(L) ? f32x2{-INFINITY, 0.0f} : f32x2{-M, 1.0f / L};
+}
+
 // PASS 0: rows (stream keys, columns are queries); PASS 1: columns (stream queries, columns are
-// keys).  blockIdx: x = column block, y = split, z = (sequence, KV head).
+// keys).  The grid runs over (sequence, KV head), then the splits, then the column blocks, the
+// longest first; neighbours go to different XCDs, so one head's K and Q stay in few of their
+// caches.
 template <int DT, int PASS>
-__global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
+__global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   constexpr int NP = DT == DA_F32 ? 3 : 1;
   constexpr int NW = DT == DA_F32 ? 2 : 1;    // 16-byte loads of a chunk of 8 elements
   constexpr int NCB = DT == DA_F32 ? 1 : 2;   // column blocks of 32 a wave holds
+  constexpr int kTile = DT == DA_F32 ? 32 : 64;  // streamed rows a stage
+  constexpr int NU = kTile / 16;              // rows a thread stages
   constexpr int MT = DT == DA_F32 ? DA_BF16 : DT;
   constexpr int kCols = 4 * NCB * 32;
-  __shared__ __attribute__((aligned(16))) char s_y[2][NP * kMTile * kMRow];
-  __shared__ __attribute__((aligned(16))) float s_add[2][kMTile];
-  __shared__ __attribute__((aligned(16))) int s_t[2][kMTile];
-  __shared__ int s_flag[2], s_ext[2];
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  constexpr int kPart = kTile * kMRow;        // LDS bytes of one part of a stage
+  __shared__ __attribute__((aligned(16))) char s_y[2][NP * kPart];
+  // per row: PASS 0 log2(count); PASS 1 -max and 1 / sum
+  __shared__ __attribute__((aligned(16))) float s_add[2][kTile];
+  __shared__ __attribute__((aligned(16))) float s_mul[2][PASS == 1 ? kTile : 4];
+  __shared__ __attribute__((aligned(16))) int s_t[2][kTile];
+  __shared__ int s_flag[2], s_ext[4];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cl = lane & 31, hl = lane >> 5;
-  const int bh = blockIdx.z, b = bh / a.Hkv, g = bh - b * a.Hkv;
+  const int nbh = a.B * a.Hkv, id = blockIdx.x / nbh;
+  const int bh = blockIdx.x - id * nbh, b = bh / a.Hkv, g = bh - b * a.Hkv;
+  const int zb = id / a.split, part_id = id - zb * a.split;
   const int G = a.G;
   const int R = G * a.Nq;
   int n = a.lengths ? a.lengths[bh] : a.Nk;
   n = n < 0 ? 0 : (n > a.Nk ? a.Nk : n);
   const int ncol = PASS == 0 ? R : n;
-  // rows pass: later queries see more keys, so the last blocks go first
-  const int block = PASS == 0 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+  // rows pass: later queries see more keys; columns pass: earlier keys are seen by more queries
+  const int block = PASS == 0 ? a.blocks - 1 - zb : zb;
   const int c0 = block * kCols;
   const int KK = (a.D + 15) / 16;
   constexpr int es = DT == DA_F32 ? 4 : 2;
@@ -101,25 +121,101 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   const char* const kb = (const char*)a.k + (b * a.sk_b + g * a.sk_h) * es;
   const int32_t* const cnt = a.counts ? a.counts + (int64_t)bh * a.Nk : nullptr;
   const int32_t* const ts = a.ts ? a.ts + (int64_t)bh * a.Nk : nullptr;
-  float* const rowadd = a.rowadd + (int64_t)bh * R;
+  f32x2* const stats = (f32x2*)(void*)a.stats + (int64_t)bh * R;
 
   // ---- this workgroup's share of the streamed rows, in tiles ----
   const int c_last = min(c0 + kCols, ncol) - 1;  // below c0 where there is no column
-  int row_lo = 0, row_hi = PASS == 0 ? n : R;
+  const int nrow = PASS == 0 ? n : R;
+  int row_lo = 0, row_hi = nrow;
   if (!ts && c_last >= c0) {
     if (PASS == 0) {  // keys up to the last query's own place
-      const int p = mass_pos(a, c_last / G);
+      const int p = mass_pos(a, query_of(a, c_last));
       row_hi = p < row_hi ? p + 1 : row_hi;
     } else {  // from the first query that sees key c0
       const int64_t first = (int64_t)c0 - a.q_start;
       row_lo = first <= 0 ? 0 : (first >= a.Nq ? R : (int)first * G);
     }
   }
-  const int tile_lo = row_lo / kMTile, tile_hi = (row_hi + kMTile - 1) / kMTile;
+  const int tile_lo = row_lo / kTile, tile_hi = (row_hi + kTile - 1) / kTile;
   const int ntile = c_last >= c0 && tile_hi > tile_lo ? tile_hi - tile_lo : 0;
   const int per = (ntile + a.split - 1) / a.split;
-  const int t_begin = tile_lo + min((int)blockIdx.y * per, ntile);
+  const int t_begin = tile_lo + min(part_id * per, ntile);
   const int t_end = min(t_begin + per, tile_lo + ntile);
+
+  // ---- staging: 16 chunks of 8 elements a row, thread: rows tid / 16 + 16 u, chunk tid % 16 ----
+  const int sr = tid >> 4, sc = tid & 15;
+  u32x4 y[NU][NW];
+  float m_add = 0.0f, m_mul = 0.0f;
+  int m_t = 0;
+  auto load_tile = [&](int tile) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int row = tile * kTile + sr + 16 * u;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) y[u][w] = u32x4{0, 0, 0, 0};
+      if (row < nrow && 8 * sc < a.D) {
+        const char* src;
+        if (PASS == 0) {
+          src = kb + row * a.sk_n * es;
+        } else {
+          const int i = query_of(a, row), h = row - i * G;
+          src = qb + (h * a.sq_h + i * a.sq_n) * es;
+        }
+#pragma unroll
+        for (int w = 0; w < NW; ++w) y[u][w] = *(const u32x4*)(src + 8 * es * sc + 16 * w);
+      }
+    }
+    if (wid == 0 && lane < kTile) {
+      const int row = tile * kTile + lane;
+      m_add = -INFINITY;
+      m_mul = 0.0f;
+      m_t = PASS == 0 ? -kNever : kNever;  // past the end: no weight, a time that asks for no mask
+      if (row < nrow) {
+        if (PASS == 0) {
+          const int c = cnt ? cnt[row] : 1;
+          m_add = c <= 0 ? -INFINITY : (cnt ? __builtin_amdgcn_logf((float)c) : 0.0f);
+          m_t = c <= 0 ? kNever : (ts ? ts[row] : row);  // hidden keys: masked, whatever they hold
+        } else {
+          const f32x2 st = stats[row];
+          m_add = st[0];
+          m_mul = st[1];
+          // queries that see nothing: masked, whatever they hold
+          m_t = is_neg_inf(m_add) ? -kNever : mass_pos(a, query_of(a, row));
+        }
+      }
+    }
+  };
+  // An extreme time of the columns, to decide for whole tiles: rows pass, the earliest query (keys
+  // at or before it need no mask); columns pass, the latest key.
+  int ext = PASS == 0 ? mass_pos(a, query_of(a, c0)) : c_last;
+  auto store_tile = [&](int st) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int row = sr + 16 * u;
+      char* const at = s_y[st] + row * kMRow + ((sc ^ (row & 15)) << 4);
+      if constexpr (DT == DA_F32) {
+        u32x4 w[NP];
+        cut_chunk<NP>(__builtin_bit_cast(f32x4, y[u][0]), __builtin_bit_cast(f32x4, y[u][1]), w);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *(u32x4*)(at + p * kPart) = w[p];
+      } else {
+        *(u32x4*)at = y[u][0];
+      }
+    }
+    if (wid == 0) {
+      // bit 0 (rows pass): a key has a weight other than 1; bit 1: a row that some column may not see
+      const bool mine = lane < kTile;
+      if (mine) {
+        s_add[st][lane] = m_add;
+        if (PASS == 1) s_mul[st][lane] = m_mul;
+        s_t[st][lane] = m_t;
+      }
+      const uint64_t odd = __ballot(mine && !zero_bits(m_add));
+      const uint64_t late = __ballot(mine && (PASS == 0 ? m_t > ext : m_t < ext));
+      if (lane == 0) s_flag[st] = (odd ? 1 : 0) | (late ? 2 : 0);
+    }
+  };
+  if (t_begin < t_end) load_tile(t_begin);
 
   // ---- the columns' operand and times ----
   u32x4 x[NP][NCB][8];
@@ -129,10 +225,10 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
     const int c = c0 + (wid * NCB + cb) * 32 + cl;
     const bool have = c < ncol;
     const char* src = kb;
-    ct[cb] = 0;
+    ct[cb] = PASS == 0 ? kNever - 1 : -kNever + 1;
     if (have) {
       if (PASS == 0) {
-        const int i = c / G, h = c - i * G;
+        const int i = query_of(a, c), h = c - i * G;
         src = qb + (h * a.sq_h + i * a.sq_n) * es;
         ct[cb] = mass_pos(a, i);
       } else {
@@ -157,102 +253,16 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
       }
     }
   }
-  // an extreme time of the columns, to decide for whole tiles: rows pass, the earliest query (keys
-  // at or before it need no mask); columns pass, the wave's latest key
-  int ext = PASS == 0 ? mass_pos(a, c0 / G) : c_last;
   if (PASS == 1 && ts) {
-    ext = -0x7fffffff;
+    int e = -kNever + 1;
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb)
-      if (c0 + (wid * NCB + cb) * 32 + cl < ncol) ext = max(ext, ct[cb]);
+    for (int cb = 0; cb < NCB; ++cb) e = max(e, ct[cb]);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) ext = max(ext, __shfl_xor(ext, d, 64));
+    for (int d = 1; d < 64; d <<= 1) e = max(e, __shfl_xor(e, d, 64));
+    if (lane == 0) s_ext[wid] = e;
+    __syncthreads();
+    ext = max(max(s_ext[0], s_ext[1]), max(s_ext[2], s_ext[3]));
   }
-  ext = __builtin_amdgcn_readfirstlane(ext);
-
-  // ---- staging: 16 chunks of 8 elements a row, thread: rows tid / 16 + 16 u, chunk tid % 16 ----
-  const int sr = tid >> 4, sc = tid & 15;
-  u32x4 y[2][NW];
-  bool y_live[2];
-  float m_add = 0.0f;
-  int m_t = 0;
-  auto load_tile = [&](int tile) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = tile * kMTile + sr + 16 * u;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) y[u][w] = u32x4{0, 0, 0, 0};
-      y_live[u] = false;
-      if (row < (PASS == 0 ? n : R)) {
-        const char* src;
-        if (PASS == 0) {
-          src = kb + row * a.sk_n * es;
-          y_live[u] = !cnt || cnt[row] > 0;
-        } else {
-          const int i = row / G, h = row - i * G;
-          src = qb + (h * a.sq_h + i * a.sq_n) * es;
-          y_live[u] = !is_neg_inf(rowadd[row]);
-        }
-        if (8 * sc < a.D) {
-#pragma unroll
-          for (int w = 0; w < NW; ++w) y[u][w] = *(const u32x4*)(src + 8 * es * sc + 16 * w);
-        }
-      }
-    }
-    if (tid < kMTile) {
-      const int row = tile * kMTile + tid;
-      m_add = -INFINITY;
-      m_t = PASS == 0 ? -0x7fffffff : 0x7fffffff;  // past the end: no weight, a time that asks for no mask
-      if (PASS == 0) {
-        if (row < n) {
-          const int c = cnt ? cnt[row] : 1;
-          m_add = c <= 0 ? -INFINITY : (cnt ? __builtin_amdgcn_logf((float)c) : 0.0f);
-          m_t = ts ? ts[row] : row;
-        }
-      } else if (row < R) {
-        m_add = rowadd[row];
-        m_t = mass_pos(a, row / G);
-      }
-    }
-  };
-  auto store_tile = [&](int st) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = sr + 16 * u;
-      char* const at = s_y[st] + row * kMRow + ((sc ^ (row & 15)) << 4);
-      if (!y_live[u]) {  // a row without weight counts as zeros, whatever it holds
-#pragma unroll
-        for (int w = 0; w < NW; ++w) y[u][w] = u32x4{0, 0, 0, 0};
-      }
-      if constexpr (DT == DA_F32) {
-        u32x4 w[NP];
-        cut_chunk<NP>(__builtin_bit_cast(f32x4, y[u][0]), __builtin_bit_cast(f32x4, y[u][1]), w);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) *(u32x4*)(at + p * kMTile * kMRow) = w[p];
-      } else {
-        *(u32x4*)at = y[u][0];
-      }
-    }
-    if (wid == 0) {
-      // rows pass: whether any key has a weight other than 1; both: the extreme time of the rows
-      const bool mine = lane < kMTile;
-      if (mine) {
-        s_add[st][lane] = m_add;
-        s_t[st][lane] = m_t;
-      }
-      int e = mine ? m_t : (PASS == 0 ? -0x7fffffff : 0x7fffffff);
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_xor(e, d, 64);
-        e = PASS == 0 ? max(e, o) : min(e, o);
-      }
-      const uint64_t odd = __ballot(mine && !zero_bits(m_add));
-      if (lane == 0) {
-        s_flag[st] = odd != 0;
-        s_ext[st] = e;
-      }
-    }
-  };
 
   float m_run[NCB], sum[NCB];
 #pragma unroll
@@ -262,111 +272,112 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   }
   const float c2 = a.scale_log2;
 
-  if (t_begin < t_end) {
-    load_tile(t_begin);
-    store_tile(0);
-  }
+  if (t_begin < t_end) store_tile(0);
   __syncthreads();
   for (int tile = t_begin; tile < t_end; ++tile) {
     const int st = (tile - t_begin) & 1;
     const bool next = tile + 1 < t_end;
     if (next) load_tile(tile + 1);
-    f32x16 s[NCB];
+    const int flag = __builtin_amdgcn_readfirstlane(s_flag[st]);
+    const bool mask = (flag & 2) != 0;
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb)
+    for (int half = 0; half < kTile / 32; ++half) {
+      f32x16 s[NCB];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[cb][r] = 0.0f;
-    const char* const yb = s_y[st] + cl * kMRow;
+      for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      if (kk < KK) {
-        u32x4 f[NP];
+        for (int r = 0; r < 16; ++r) s[cb][r] = 0.0f;
+      const char* const yb = s_y[st] + (32 * half + cl) * kMRow;
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
-          f[p] = *(const u32x4*)(yb + p * kMTile * kMRow + (((2 * kk + hl) ^ (cl & 15)) << 4));
+      for (int kk = 0; kk < 8; ++kk) {
+        if (kk < KK) {
+          u32x4 f[NP];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) f[p] = *(const u32x4*)(yb + p * kPart + (((2 * kk + hl) ^ (cl & 15)) << 4));
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            if constexpr (NP == 1) {
+              s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
+            } else {  // the smallest products first
+              s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
+              s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
+              s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
+              s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
+              s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
+              s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
+            }
+          }
+        }
+      }
+      const float* const add_row = s_add[st] + 32 * half + 4 * hl;
+      const float* const mul_row = s_mul[st] + (PASS == 1 ? 32 * half + 4 * hl : 0);
+      const int* const t_row = s_t[st] + 32 * half + 4 * hl;
+      // register r of a block is row 8 (r / 4) + 4 hl + r % 4 of the half
+      if (PASS == 0) {
+        const bool plain = flag == 0;
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
-          if constexpr (NP == 1) {
-            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
-          } else {  // the smallest products first
-            s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
-          }
-        }
-      }
-    }
-    const int e = __builtin_amdgcn_readfirstlane(s_ext[st]);
-    const bool weights = __builtin_amdgcn_readfirstlane(s_flag[st]) != 0;
-    const bool mask = PASS == 0 ? e > ext : e < ext;
-    // register r of a block is row 8 (r / 4) + 4 hl + r % 4 of the tile
-    if (PASS == 0) {
-      const bool plain = !weights && !mask;
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        float p = 0.0f;
-        if (plain) {
+          float p = 0.0f;
           const float base = is_neg_inf(m_run[cb]) ? 0.0f : m_run[cb];
+          if (plain) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) p += mexp2(__builtin_fmaf(s[cb][r], c2, -base));
-        } else {
-          const float base = is_neg_inf(m_run[cb]) ? 0.0f : m_run[cb];
+            for (int r = 0; r < 16; ++r) p += mexp2(__builtin_fmaf(s[cb][r], c2, -base));
+          } else {
 #pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 add = *(const f32x4*)&s_add[st][8 * r4 + 4 * hl];
-            const int4 t4 = *(const int4*)&s_t[st][8 * r4 + 4 * hl];
-            const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+            for (int r4 = 0; r4 < 4; ++r4) {
+              const f32x4 add = *(const f32x4*)(add_row + 8 * r4);
+              const int4 t4 = *(const int4*)(t_row + 8 * r4);
+              const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float v = __builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]);
-              if (mask && tt[i] > ct[cb]) v = -INFINITY;
-              s[cb][4 * r4 + i] = v;
-              p += mexp2(v - base);
+              for (int i = 0; i < 4; ++i) {
+                float v = __builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]);
+                if (tt[i] > ct[cb]) v = -INFINITY;
+                s[cb][4 * r4 + i] = v;
+                p += mexp2(v - base);
+              }
             }
           }
-        }
-        if (__ballot(is_neg_inf(m_run[cb]) || p > kMLarge)) {
-          float mx = m_run[cb];
+          if (__ballot(is_neg_inf(m_run[cb]) || p > kMLarge)) {
+            float mx = m_run[cb];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if (plain) s[cb][r] *= c2;
-            mx = __builtin_fmaxf(mx, s[cb][r]);
+            for (int r = 0; r < 16; ++r) {
+              if (plain) s[cb][r] *= c2;
+              mx = __builtin_fmaxf(mx, s[cb][r]);
+            }
+            const float top = is_neg_inf(mx) ? 0.0f : mx;
+            sum[cb] *= mexp2(m_run[cb] - top);
+            p = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p += mexp2(s[cb][r] - top);
+            m_run[cb] = mx;
           }
-          const float base = is_neg_inf(mx) ? 0.0f : mx;
-          sum[cb] *= mexp2(m_run[cb] - base);
-          p = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) p += mexp2(s[cb][r] - base);
-          m_run[cb] = mx;
-        }
-        sum[cb] += p;
-      }
-    } else {
-      if (!mask) {
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 add = *(const f32x4*)&s_add[st][8 * r4 + 4 * hl];
-#pragma unroll
-          for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[cb] += mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]));
+          sum[cb] += p;
         }
       } else {
+        if (!mask) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 add = *(const f32x4*)&s_add[st][8 * r4 + 4 * hl];
-          const int4 t4 = *(const int4*)&s_t[st][8 * r4 + 4 * hl];
-          const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 add = *(const f32x4*)(add_row + 8 * r4), mul = *(const f32x4*)(mul_row + 8 * r4);
 #pragma unroll
-          for (int cb = 0; cb < NCB; ++cb)
+            for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]));
-              sum[cb] += tt[i] < ct[cb] ? 0.0f : p;
-            }
+              for (int i = 0; i < 4; ++i)
+                sum[cb] = __builtin_fmaf(mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])), mul[i], sum[cb]);
+          }
+        } else {
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 add = *(const f32x4*)(add_row + 8 * r4), mul = *(const f32x4*)(mul_row + 8 * r4);
+            const int4 t4 = *(const int4*)(t_row + 8 * r4);
+            const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float p = mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])) * mul[i];
+                sum[cb] += tt[i] < ct[cb] ? 0.0f : p;
+              }
+          }
         }
       }
     }
@@ -384,11 +395,10 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
       const float L = sum[cb] * mexp2(m_run[cb] - base) + l2 * mexp2(m2 - base);
       if (hl == 0 && c < R) {
         if (a.split == 1) {
-          rowadd[c] = zero_bits(L) ? -INFINITY : -(M + __builtin_amdgcn_logf(L));
+          stats[c] = row_stats(M, L);
         } else {
-          float* const p = a.part + (((int64_t)bh * R + c) * a.split + blockIdx.y) * 2;
-          p[0] = M;
-          p[1] = L;
+          float* const p = a.part + (((int64_t)bh * R + c) * a.split + part_id) * 2;
+          *(f32x2*)(void*)p = f32x2{M, L};
         }
       }
     } else {
@@ -397,23 +407,33 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
         float v = c < n ? t : 0.0f;
         if (cnt && c < n) v = cnt[c] > 0 ? t * (float)cnt[c] : 0.0f;
         if (a.split == 1) a.mass[(int64_t)bh * a.Nk + c] = v;
-        else a.part[((int64_t)blockIdx.y * gridDim.z + bh) * a.Nk + c] = v;
+        else a.part[((int64_t)part_id * nbh + bh) * a.Nk + c] = v;
       }
     }
   }
 }
 
-// A query's (max, sum) parts -> -lse, or -inf where it saw nothing.
-__global__ __launch_bounds__(256) void mass_join_rows_kernel(const float* part, float* rowadd, int64_t rows, int split) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows) return;
-  const f32x2* p = (const f32x2*)part + i * split;
-  float M = -INFINITY;
-  for (int s = 0; s < split; ++s) M = __builtin_fmaxf(M, p[s][0]);
-  const float base = is_neg_inf(M) ? 0.0f : M;
-  float L = 0.0f;
-  for (int s = 0; s < split; ++s) L += p[s][1] * mexp2(p[s][0] - base);
-  rowadd[i] = zero_bits(L) ? -INFINITY : -(M + __builtin_amdgcn_logf(L));
+// A query's (max, sum) parts, kJoinLanes lanes a query.
+constexpr int kJoinLanes = 16;
+__global__ __launch_bounds__(256) void mass_join_rows_kernel(const float* part, float* stats, int64_t rows, int split) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kJoinLanes;
+  const int l = threadIdx.x % kJoinLanes;
+  const f32x2* p = (const f32x2*)(const void*)part + (i < rows ? i : rows - 1) * split;
+  float M = -INFINITY, L = 0.0f;
+  for (int s = l; s < split; s += kJoinLanes) {
+    const f32x2 v = p[s];
+    const float m = __builtin_fmaxf(M, v[0]), base = is_neg_inf(m) ? 0.0f : m;
+    L = L * mexp2(M - base) + v[1] * mexp2(v[0] - base);
+    M = m;
+  }
+#pragma unroll
+  for (int d = 1; d < kJoinLanes; d <<= 1) {
+    const float m2 = __shfl_xor(M, d, 64), l2 = __shfl_xor(L, d, 64);
+    const float m = __builtin_fmaxf(M, m2), base = is_neg_inf(m) ? 0.0f : m;
+    L = L * mexp2(M - base) + l2 * mexp2(m2 - base);
+    M = m;
+  }
+  if (l == 0 && i < rows) ((f32x2*)(void*)stats)[i] = row_stats(M, L);
 }
 
 // The splits' column sums, added in order.
@@ -425,12 +445,11 @@ __global__ __launch_bounds__(256) void mass_join_cols_kernel(const float* part, 
   mass[i] = v;
 }
 
-// Splits of the streamed rows: workgroups for every CU a few times over, and at least
-// kMinTiles tiles each.
+// Splits of the streamed rows: workgroups for every CU a few times over, and at least 128 rows
+// each.
 static int mass_split(int64_t blocks, int64_t streamed) {
-  constexpr int64_t kMinTiles = 4;
   int64_t want = (1024 + blocks - 1) / blocks;
-  const int64_t most = (streamed + kMTile * kMinTiles - 1) / (kMTile * kMinTiles);
+  const int64_t most = (streamed + 127) / 128;
   if (want > most) want = most;
   if (want > 64) want = 64;
   return (int)(want < 1 ? 1 : want);
@@ -457,14 +476,16 @@ template <int DT>
 static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char* who) {
   const unsigned bh = (unsigned)(a.B * a.Hkv);
   a.split = p.split0;
-  hipLaunchKernelGGL((mass_kernel<DT, 0>), dim3((unsigned)p.blocks0, p.split0, bh), dim3(256), 0, st, a);
+  a.blocks = (int)p.blocks0;
+  hipLaunchKernelGGL((mass_kernel<DT, 0>), dim3(bh * p.split0 * (unsigned)p.blocks0), dim3(256), 0, st, a);
   if (p.split0 > 1) {
     const int64_t rows = bh * p.rows;
-    hipLaunchKernelGGL(mass_join_rows_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a.part, a.rowadd,
-                       rows, p.split0);
+    hipLaunchKernelGGL(mass_join_rows_kernel, dim3((unsigned)((rows * kJoinLanes + 255) / 256)), dim3(256), 0, st,
+                       a.part, a.stats, rows, p.split0);
   }
   a.split = p.split1;
-  hipLaunchKernelGGL((mass_kernel<DT, 1>), dim3((unsigned)p.blocks1, p.split1, bh), dim3(256), 0, st, a);
+  a.blocks = (int)p.blocks1;
+  hipLaunchKernelGGL((mass_kernel<DT, 1>), dim3(bh * p.split1 * (unsigned)p.blocks1), dim3(256), 0, st, a);
   if (p.split1 > 1) {
     const int64_t cols = (int64_t)bh * a.Nk;
     hipLaunchKernelGGL(mass_join_cols_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, st, a.part, a.mass,
@@ -477,11 +498,11 @@ static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char
 
 using namespace da;
 
-// -lse of every query row, then the splits' parts (of whichever type needs more).
+// The two statistics of every query row, then the splits' parts (of whichever type needs more).
 extern "C" int64_t da_attention_mass_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq, int64_t Nk) {
   if (B <= 0 || Hkv <= 0 || Hq < Hkv || Nq <= 0 || Nk <= 0) return 0;
   const MassPlan p = mass_plan(DA_BF16, B, Hq, Hkv, Nq, Nk), p32 = mass_plan(DA_F32, B, Hq, Hkv, Nq, Nk);
-  const int64_t rows = (B * Hkv * p.rows + 3) / 4 * 4;
+  const int64_t rows = (B * Hkv * p.rows * 2 + 3) / 4 * 4;
   return (rows + (p.part > p32.part ? p.part : p32.part)) * (int64_t)sizeof(float);
 }
 
@@ -498,9 +519,8 @@ extern "C" int da_attention_mass(const void* q, const void* k, int dtype, int64_
     return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128]", who);
   DA_REQUIRE(B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Nq > 0 && Nk > 0, "%s: bad shape", who);
   if (Hq / Hkv > 64) return set_error(DA_ERR_UNSUPPORTED, "%s: GQA group above 64", who);
-  if (Nk > (1 << 24) || Nq > (1 << 24) || Hq / Hkv * Nq >= (1ll << 30) || B * Hkv > 65535)
-    return set_error(DA_ERR_UNSUPPORTED, "%s: more than 2^24 keys or queries, 2^30 query rows a KV head or 65535 "
-                     "(sequence, head) pairs", who);
+  if (Nk > (1 << 24) || Nq > (1 << 24) || B * Hkv > 65535)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: more than 2^24 keys or queries, or 65535 (sequence, head) pairs", who);
   const int64_t align = dtype == DA_F32 ? 3 : 7;
   DA_REQUIRE(((sq_b | sq_h | sq_n | sk_b | sk_h | sk_n) & align) == 0 && (((uintptr_t)q | (uintptr_t)k) & 15) == 0,
              "%s: rows must be 16-byte aligned", who);
@@ -511,15 +531,18 @@ extern "C" int da_attention_mass(const void* q, const void* k, int dtype, int64_
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
   DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   const MassPlan p = mass_plan(dtype, B, Hq, Hkv, Nq, Nk);
+  if (p.rows >= (1ll << 30) || B * Hkv * p.split0 * p.blocks0 >= (1ll << 31) || B * Hkv * p.split1 * p.blocks1 >= (1ll << 31))
+    return set_error(DA_ERR_UNSUPPORTED, "%s: more than 2^30 query rows a KV head, or 2^31 workgroups", who);
   MassArgs a = {};
   a.q = q; a.k = k;
   a.sq_b = sq_b; a.sq_h = sq_h; a.sq_n = sq_n; a.sk_b = sk_b; a.sk_h = sk_h; a.sk_n = sk_n;
   a.counts = counts; a.ts = timestamps; a.lengths = lengths; a.q_start = q_start;
   a.scale_log2 = scale * kMLog2e;
-  a.rowadd = (float*)workspace;
-  a.part = a.rowadd + (B * Hkv * p.rows + 3) / 4 * 4;
+  a.stats = (float*)workspace;
+  a.part = a.stats + (B * Hkv * p.rows * 2 + 3) / 4 * 4;
   a.mass = mass;
   a.B = (int)B; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.Nq = (int)Nq; a.Nk = (int)Nk; a.D = (int)D;
+  a.gshift = (a.G & (a.G - 1)) == 0 ? __builtin_ctz(a.G) : -1;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) return launch_mass<DA_F32>(a, p, st, who);
   if (dtype == DA_F16) return launch_mass<DA_F16>(a, p, st, who);

@@ -10,6 +10,7 @@ Python exceptions.  Users reach them as ``ops.KV4``, ``ops.attention_mass`` and 
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -22,16 +23,17 @@ __all__ = ["KV4", "attention_mass", "heavy_rows", "quantize_kv4", "dequantize_kv
 _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
-def _want(t: Optional[torch.Tensor], name: str, shape, dtype, device) -> None:
+def _want(t: torch.Tensor, name: str, shape, dtype, device) -> None:
     """Refuse a tensor that is not contiguous, of this shape and type and on this device."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == device:
+        return
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _gpu(t: torch.Tensor, name: str) -> torch.device:
@@ -55,8 +57,21 @@ def _strides(t: torch.Tensor):
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
 
 
+@functools.lru_cache(maxsize=1024)
+def _mass_bytes(*shape) -> int:
+    return lib().da_attention_mass_workspace_size(*shape)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_bytes(*shape) -> int:
+    return lib().da_kv4_attention_workspace_size(*shape)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+_set = object.__setattr__
 
 
 class KV4:
@@ -74,7 +89,7 @@ class KV4:
     """
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "counts", "timestamps", "lengths", "mass",
-                 "head_dim", "_block", "_ref")
+                 "batch", "kv_heads", "capacity", "head_dim", "device", "_block", "_ref", "_own")
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales, counts, timestamps, lengths, head_dim, mass=None):
         D = int(head_dim)
@@ -87,62 +102,86 @@ class KV4:
         B, H, cap, _ = k_codes.shape
         if not (B and H and cap):
             raise ValueError("a cache needs sequences, heads and rows")
-        for t, name in ((k_codes, "k_codes"), (v_codes, "v_codes")):
-            _want(t, name, (B, H, cap, 16 * groups), _U8, device)
-            if t.data_ptr() % 16:
-                raise ValueError(f"{name} must be 16-byte aligned")
-        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-            _want(t, name, (B, H, cap, groups), _U8, device)
-        _want(counts, "counts", (B, H, cap), _I32, device)
-        _want(timestamps, "timestamps", (B, H, cap), _I32, device)
+        wide, narrow, rows = (B, H, cap, 16 * groups), (B, H, cap, groups), (B, H, cap)
+        _want(k_codes, "k_codes", wide, _U8, device)
+        _want(v_codes, "v_codes", wide, _U8, device)
+        _want(k_scales, "k_scales", narrow, _U8, device)
+        _want(v_scales, "v_scales", narrow, _U8, device)
+        _want(counts, "counts", rows, _I32, device)
+        _want(timestamps, "timestamps", rows, _I32, device)
         _want(lengths, "lengths", (B, H), _I32, device)
         if mass is not None:
-            _want(mass, "mass", (B, H, cap), _F32, device)
-        put = object.__setattr__
-        put(self, "k_codes", k_codes)
-        put(self, "k_scales", k_scales)
-        put(self, "v_codes", v_codes)
-        put(self, "v_scales", v_scales)
-        put(self, "counts", counts)
-        put(self, "timestamps", timestamps)
-        put(self, "lengths", lengths)
-        put(self, "mass", mass)
-        put(self, "head_dim", D)
-        block = Kv4Block(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
-                         counts.data_ptr(), timestamps.data_ptr(), lengths.data_ptr(), _ptr(mass), cap)
-        put(self, "_block", block)
-        put(self, "_ref", ctypes.byref(block))
+            _want(mass, "mass", rows, _F32, device)
+        kc, vc = k_codes.data_ptr(), v_codes.data_ptr()
+        if (kc | vc) % 16:
+            raise ValueError("k_codes and v_codes must be 16-byte aligned")
+        self._put(B, H, cap, D, device, Kv4Block(
+            kc, k_scales.data_ptr(), vc, v_scales.data_ptr(), counts.data_ptr(), timestamps.data_ptr(),
+            lengths.data_ptr(), None if mass is None else mass.data_ptr(), cap), None)
+        _set(self, "k_codes", k_codes)
+        _set(self, "k_scales", k_scales)
+        _set(self, "v_codes", v_codes)
+        _set(self, "v_scales", v_scales)
+        _set(self, "counts", counts)
+        _set(self, "timestamps", timestamps)
+        _set(self, "lengths", lengths)
+        _set(self, "mass", mass)
+
+    def _put(self, B, H, cap, D, device, block, own):
+        _set(self, "batch", B)
+        _set(self, "kv_heads", H)
+        _set(self, "capacity", cap)
+        _set(self, "head_dim", D)
+        _set(self, "device", device)
+        _set(self, "_block", block)
+        _set(self, "_ref", ctypes.byref(block))
+        _set(self, "_own", own)
 
     def __setattr__(self, name, value):
         raise AttributeError(f"KV4.{name} is fixed; build another KV4 from the tensors")
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, device="cuda", mass: bool = True) -> "KV4":
-        """A cache of ``capacity`` rows a head with undefined contents (``lengths`` too)."""
-        g = (head_dim + 31) // 32
-        new = torch.empty
-        shape = (batch, kv_heads, capacity)
-        return cls(new((*shape, 16 * g), dtype=_U8, device=device), new((*shape, g), dtype=_U8, device=device),
-                   new((*shape, 16 * g), dtype=_U8, device=device), new((*shape, g), dtype=_U8, device=device),
-                   new(shape, dtype=_I32, device=device), new(shape, dtype=_I32, device=device),
-                   new(shape[:2], dtype=_I32, device=device), head_dim,
-                   new(shape, dtype=_F32, device=device) if mass else None)
+        """A cache of ``capacity`` rows a head with undefined contents (``lengths`` too), in one
+        allocation; its tensors are views that are made when they are first asked for."""
+        B, H, cap, D = int(batch), int(kv_heads), int(capacity), int(head_dim)
+        if not (B > 0 and H > 0 and cap > 0) or D <= 0 or D > 128 or D % 8:
+            raise ValueError(f"no cache of {batch} sequences, {kv_heads} heads, {capacity} rows and head_dim {head_dim}")
+        n, g = B * H * cap, (D + 31) // 32
+        up = lambda x: (x + 255) & ~255  # noqa: E731
+        codes, scales, field, heads = up(16 * g * n), up(g * n), up(4 * n), up(4 * B * H)
+        at = {"k_codes": 0, "v_codes": codes, "k_scales": 2 * codes, "v_scales": 2 * codes + scales}
+        end = 2 * (codes + scales)
+        for name in ("counts", "timestamps", "mass") if mass else ("counts", "timestamps"):
+            at[name] = end
+            end += field
+        at["lengths"] = end
+        own = torch.empty((end + heads,), dtype=_U8, device=device)
+        device, p = _gpu(own, "the cache"), own.data_ptr()
+        self = cls.__new__(cls)
+        self._put(B, H, cap, D, device, Kv4Block(
+            p, p + 2 * codes, p + codes, p + 2 * codes + scales, p + at["counts"], p + at["timestamps"],
+            p + at["lengths"], p + at["mass"] if mass else None, cap), (own, at))
+        return self
 
-    @property
-    def batch(self) -> int:
-        return self.k_codes.shape[0]
-
-    @property
-    def kv_heads(self) -> int:
-        return self.k_codes.shape[1]
-
-    @property
-    def capacity(self) -> int:
-        return self.k_codes.shape[2]
-
-    @property
-    def device(self) -> torch.device:
-        return self.k_codes.device
+    def __getattr__(self, name):
+        # only for what is not there yet: a tensor of a cache that empty() made
+        if name not in ("k_codes", "k_scales", "v_codes", "v_scales", "counts", "timestamps", "lengths", "mass"):
+            raise AttributeError(name)
+        own, at = self._own
+        if name not in at:
+            t = None  # a cache without mass
+        else:
+            B, H, cap, g, first = self.batch, self.kv_heads, self.capacity, (self.head_dim + 31) // 32, at[name]
+            if name == "lengths":
+                t = own.view(_I32).as_strided((B, H), (H, 1), first // 4)
+            elif name in ("counts", "timestamps", "mass"):
+                t = own.view(_F32 if name == "mass" else _I32).as_strided((B, H, cap), (H * cap, cap, 1), first // 4)
+            else:
+                w = 16 * g if name.endswith("codes") else g
+                t = own.as_strided((B, H, cap, w), (H * cap * w, cap * w, w, 1), first)
+        _set(self, name, t)
+        return t
 
 
 def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tensor] = None,
@@ -182,7 +221,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tens
     else:
         _want(out, "out", (B, H, N), _F32, device)
     q, k = _rows(q), _rows(k)
-    n = lib().da_attention_mass_workspace_size(B, Hq, H, Nq, N)
+    n = _mass_bytes(B, Hq, H, Nq, N)
     ws = torch.empty((n,), dtype=_U8, device=device)
     with on_device(device) as stream:
         rc = lib().da_attention_mass(q.data_ptr(), k.data_ptr(), dt, B, Hq, H, Nq, N, D, *_strides(q), *_strides(k),
@@ -320,54 +359,50 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
     ``kv.mass``.  A head without any key gives zeros.  Query head h reads KV head
     h // (Hq // Hkv).
     """
-    device = kv.device
-    if q.dim() == 4 and q.shape[2] == 1:
-        q3 = q.squeeze(2)
-    elif q.dim() == 3:
-        q3 = q
+    device, H = kv.device, kv.kv_heads
+    shape = q.shape
+    if len(shape) == 4 and shape[2] == 1:
+        B, Hq, _, D = shape
+    elif len(shape) == 3:
+        B, Hq, D = shape
     else:
         raise ValueError("q is [B, Hq, 1, D] or [B, Hq, D]")
-    B, Hq, D = q3.shape
-    H = kv.kv_heads
     if q.device != device or B != kv.batch or D != kv.head_dim or Hq % H or not Hq:
-        raise ValueError(f"q {list(q.shape)} on {q.device} does not fit a cache of {kv.batch} sequences, {H} KV heads "
+        raise ValueError(f"q {list(shape)} on {q.device} does not fit a cache of {kv.batch} sequences, {H} KV heads "
                          f"and head_dim {kv.head_dim} on {device}")
     if (k_exact is None) != (v_exact is None):
         raise ValueError("k_exact and v_exact come together")
     if accumulate and kv.mass is None:
         raise ValueError("accumulate needs the cache's mass")
     dt = dtype_code(q, k_exact, v_exact, out)
-    sx = (0, 0, 0)
-    W = 0
+    sx, W, kx, vx = (0, 0, 0), 0, None, None
     if k_exact is not None:
-        W = k_exact.shape[2] if k_exact.dim() == 4 else 0
-        if k_exact.shape != (B, H, W, D) or v_exact.shape != k_exact.shape or k_exact.device != device \
+        xs = k_exact.shape
+        if len(xs) != 4 or xs[0] != B or xs[1] != H or xs[3] != D or v_exact.shape != xs or k_exact.device != device \
                 or v_exact.device != device:
             raise ValueError(f"k_exact and v_exact must be [{B}, {H}, W, {D}] on {device}")
-        sx = k_exact.stride()
+        W, sx = xs[2], k_exact.stride()
         if sx[3] != 1 or v_exact.stride() != sx:
             k_exact, v_exact = (t.clone(memory_format=torch.contiguous_format) for t in (k_exact, v_exact))
             sx = k_exact.stride()
+        kx, vx = k_exact.data_ptr(), v_exact.data_ptr()
     n_exact = W if exact_len is None else int(exact_len)
     if not 0 <= n_exact <= W:
         raise ValueError(f"exact_len must lie in [0, {W}], got {n_exact}")
-    if q3.stride(2) != 1:
-        q3 = q3.contiguous()
+    sq = q.stride()
+    if sq[-1] != 1:
+        q = q.contiguous()
+        sq = q.stride()
     if out is None:
-        out3 = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
-        result = out3.view(q.shape)
-    else:
-        if out.shape != q.shape or out.device != device or out.stride(-1) != 1:
-            raise ValueError("out must have q's shape and device and a contiguous head dimension")
-        out3, result = (out.squeeze(2) if out.dim() == 4 else out), out
-    native = lib()
-    n = native.da_kv4_attention_workspace_size(B, Hq, H, kv.capacity, 1 if accumulate else 0)
+        out = torch.empty(shape, dtype=q.dtype, device=device)
+    elif out.shape != shape or out.device != device or out.stride(-1) != 1:
+        raise ValueError("out must have q's shape and device and a contiguous head dimension")
+    so = out.stride()
+    n = _attention_bytes(B, Hq, H, kv.capacity, 1 if accumulate else 0)
     ws = torch.empty((n,), dtype=_U8, device=device)
-    sq, so = q3.stride(), out3.stride()
     with on_device(device) as stream:
-        rc = native.da_kv4_attention(q3.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, _ptr(k_exact),
-                                     _ptr(v_exact), sx[0], sx[1], sx[2], n_exact,
-                                     D ** -0.5 if scale is None else float(scale), 1 if accumulate else 0,
-                                     out3.data_ptr(), so[0], so[1], ws.data_ptr(), n, stream)
+        rc = lib().da_kv4_attention(q.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, kx, vx, sx[0], sx[1], sx[2],
+                                    n_exact, D ** -0.5 if scale is None else scale, 1 if accumulate else 0,
+                                    out.data_ptr(), so[0], so[1], ws.data_ptr(), n, stream)
     check(rc, "da_kv4_attention")
-    return result
+    return out
