@@ -28,7 +28,7 @@ struct Quant4Args {
   float* o_mass;
   int32_t* o_lengths;
   int64_t N, M, capacity;
-  int H, D;
+  int B, H, D;
 };
 
 // Eight consecutive elements of a row, as fp32.
@@ -72,27 +72,33 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 // A lane takes 8 dims: 16 bytes of a 16-bit row (32 of an fp32 one), 4 bytes of codes; the
 // four lanes of a quad are one group, whose largest magnitude is two quad permutes away.
 // Lanes per row: 4 NG.  Each thread takes kQuantItems of them, a block's width apart, with
-// all of its loads in flight.  blockIdx.y = (sequence, head), z = key or value.
+// all of its loads in flight.  The grid runs over (sequence, head) first: neighbours read the
+// same rows' heads, which projections lay side by side.  blockIdx.y = key or value.
 constexpr int kQuantItems = 4;
 template <int DT, int NG>
 __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
-  constexpr int kLpr = 4 * NG;
-  const int bh = blockIdx.y, z = blockIdx.z;
+  constexpr uint32_t kLpr = 4 * NG;
+  const uint32_t nbh = a.B * a.H, blk = blockIdx.x / nbh;
+  const int bh = blockIdx.x - blk * nbh, z = blockIdx.y;
   const int b = bh / a.H, h = bh - b * a.H;
-  int64_t len = a.lengths ? a.lengths[bh] : a.M;
-  len = len < 0 ? 0 : (len > a.M ? a.M : len);
+  const uint32_t M = (uint32_t)a.M;
+  uint32_t len = M;
+  if (a.lengths) {
+    const int n = a.lengths[bh];
+    len = n < 0 ? 0 : ((uint32_t)n > M ? M : (uint32_t)n);
+  }
   const char* base = (const char*)a.x[z] + (b * a.s_b[z] + h * a.s_h[z]) * (DT == DA_F32 ? 4 : 2);
-  const int64_t first = (int64_t)blockIdx.x * 256 * kQuantItems + threadIdx.x;
+  const uint32_t first = blk * 256 * kQuantItems + threadIdx.x;  // below 2^31: capacity <= 2^26
   float x[kQuantItems][8];
-  int64_t src[kQuantItems];
+  int src[kQuantItems];
 #pragma unroll
   for (int u = 0; u < kQuantItems; ++u) {
-    const int64_t it = first + u * 256, m = it / kLpr;
-    int64_t s = -1;
+    const uint32_t m = (first + u * 256) / kLpr;
+    int s = -1;
     if (m < len) {
-      s = m;
+      s = (int)m;
       if (a.index) {
-        s = a.index[bh * a.M + m];
+        s = a.index[(int64_t)bh * M + m];
         if (s >= a.N) s = -1;
       }
     }
@@ -100,15 +106,14 @@ __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
   }
 #pragma unroll
   for (int u = 0; u < kQuantItems; ++u) {
-    const int64_t it = first + u * 256;
-    const int d = 8 * (int)(it - it / kLpr * kLpr);
+    const int d = 8 * (int)((first + u * 256) % kLpr);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[u][i] = 0.0f;
     if (src[u] >= 0 && d < a.D) load8<DT>(base, src[u] * a.s_n[z] + d, x[u]);
   }
 #pragma unroll
   for (int u = 0; u < kQuantItems; ++u) {
-    const int64_t it = first + u * 256, m = it / kLpr;
+    const uint32_t it = first + u * 256, m = it / kLpr;
     const int c = (int)(it - m * kLpr);
     uint32_t top = 0;
 #pragma unroll
@@ -131,7 +136,7 @@ __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
       codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][4], x[u][5], 1.0f, 2);
       codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][6], x[u][7], 1.0f, 3);
     }
-    if (m < a.M) {
+    if (m < M) {
       const int64_t row = bh * a.capacity + m;
       ((uint32_t*)a.codes[z])[row * kLpr + c] = codes;
       if ((c & 3) == 0) a.scales[z][row * NG + (c >> 2)] = (uint8_t)(src[u] < 0 ? 0u : e);
@@ -162,28 +167,28 @@ struct Dequant4Args {
 // A lane turns 4 bytes of codes into 8 elements; kQuantItems of them in flight a thread.
 template <int DT, int NG>
 __global__ __launch_bounds__(256) void dequantize4_kernel(Dequant4Args a) {
-  constexpr int kLpr = 4 * NG;
+  constexpr uint32_t kLpr = 4 * NG;
   const int bh = blockIdx.y, z = blockIdx.z;
-  int64_t len = a.lengths[bh];
-  len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
-  const int64_t first = (int64_t)blockIdx.x * 256 * kQuantItems + threadIdx.x;
+  const int n = a.lengths[bh];
+  const uint32_t len = n < 0 ? 0 : (n > a.N ? (uint32_t)a.N : (uint32_t)n);
+  const uint32_t first = blockIdx.x * 256 * kQuantItems + threadIdx.x;
   uint32_t w[kQuantItems], e[kQuantItems];
 #pragma unroll
   for (int u = 0; u < kQuantItems; ++u) {
-    const int64_t it = first + u * 256, m = it / kLpr;
+    const uint32_t it = first + u * 256, m = it / kLpr;
     const int c = (int)(it - m * kLpr);
     const int64_t row = bh * a.capacity + m;
     w[u] = e[u] = 0;
-    if (m < a.N && m < len) {
+    if (m < len) {
       w[u] = ((const uint32_t*)a.codes[z])[row * kLpr + c];
       e[u] = a.scales[z][row * NG + (c >> 2)];
     }
   }
 #pragma unroll
   for (int u = 0; u < kQuantItems; ++u) {
-    const int64_t it = first + u * 256, m = it / kLpr;
+    const uint32_t it = first + u * 256, m = it / kLpr;
     const int d = 8 * (int)(it - m * kLpr);
-    if (m >= a.N || d >= a.D) continue;
+    if (m >= (uint32_t)a.N || d >= a.D) continue;
     const float s = __uint_as_float(e[u] << 23);
     const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], s, 0);
     const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], s, 1);
@@ -223,25 +228,33 @@ __device__ __forceinline__ uint32_t mass_order(float m) {
 constexpr int kHeavyThreads = 1024, kHeavyWaves = kHeavyThreads / 64, kHeavyBins = 2048;
 constexpr int kHeavyPer = 16;                              // masses a thread holds at once
 constexpr int kHeavyBatch = kHeavyThreads * kHeavyPer;     // rows of a batch
+constexpr int kHeavyList = 16384;                          // rows of the border's first bin kept in LDS
 
 // One workgroup per (sequence, head).  The border (the need-th largest mass between the
 // protected ends) comes from three histogram passes over 11, 11 and 10 bits of the order;
 // a last pass writes the rows above it, and as many of its equals as still fit, lowest row
-// first, in row order.  Rows come in batches of 16384, 16 loads in flight a thread; a head of
-// one batch is read once.
+// first, in row order.  Rows come in batches of 16384, 16 loads in flight a thread.  A head of
+// one batch is read once.  A longer one is read three times: the second reading collects the
+// rows of the first pass's bin in LDS, where the other passes find them (unless they are too
+// many: then those read the row again).
 __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) {
+  __shared__ uint32_t s_list[kHeavyList];
   __shared__ uint32_t s_hist[kHeavyBins];
   __shared__ uint32_t s_wave[kHeavyWaves];
   __shared__ uint32_t s_cnt[2][kHeavyPer * kHeavyWaves];  // rows above / at the border, in row order
   __shared__ uint32_t s_all[2];
-  __shared__ uint32_t s_pick[2];  // the chosen bin, the rows still needed from it
+  __shared__ uint32_t s_pick[3];  // the chosen bin, the rows still needed from it, the rows it holds
+  __shared__ uint32_t s_fill;
   const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int64_t n64 = a.lengths ? a.lengths[bh] : a.capacity;
   n64 = n64 < 0 ? 0 : (n64 > a.capacity ? a.capacity : n64);
   const int n = (int)n64;
   int32_t* const out = a.index + (int64_t)bh * a.budget;
   const int kept = n < a.budget ? n : a.budget;
-  if (tid == 0) a.kept[bh] = kept;
+  if (tid == 0) {
+    a.kept[bh] = kept;
+    s_fill = 0;
+  }
   if (n <= a.budget) {
     for (int i = tid; i < a.budget; i += kHeavyThreads) out[i] = i < n ? i : -1;
     return;
@@ -263,7 +276,20 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
 #pragma unroll
     for (int j = 0; j < kHeavyPer; ++j) u[j] = mass_order(m[j]);
   };
+  // one more row of `bin` for the active lanes: lanes that share the first one's bin (rows of no
+  // weight at all, often most of them) add together, the others one by one
+  auto count = [&](bool in, uint32_t bin) {
+    const uint64_t act = __ballot(in);
+    if (act) {
+      const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
+      const uint64_t same = __ballot(in && bin == lead);
+      if (lane == 0) atomicAdd(&s_hist[lead], (uint32_t)__popcll(same));
+      if (in && bin != lead) atomicAdd(&s_hist[bin], 1u);
+    }
+  };
   const bool one = hi - lo <= kHeavyBatch;
+  bool listed = false;
+  uint32_t nlist = 0;
   if (one) load(lo);
   uint32_t prefix = 0, mask = 0;  // bits of the border found so far
   for (int pass = 0; pass < 3; ++pass) {
@@ -272,20 +298,29 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
     s_hist[tid] = 0;
     s_hist[tid + kHeavyThreads] = 0;
     __syncthreads();
-    for (int base = lo; base < hi; base += kHeavyBatch) {
-      if (!one) load(base);
+    if (listed && pass == 2) {
+      for (uint32_t i0 = 0; i0 < nlist; i0 += kHeavyThreads) {
+        const uint32_t i = i0 + tid, v = i < nlist ? s_list[i] : 0;
+        count(i < nlist && (v & mask) == prefix, v & bits);
+      }
+    } else {
+      for (int base = lo; base < hi; base += kHeavyBatch) {
+        if (!one) load(base);
 #pragma unroll
-      for (int j = 0; j < kHeavyPer; ++j) {
-        const bool in = base + j * kHeavyThreads + tid < hi && (u[j] & mask) == prefix;
-        const uint32_t bin = (u[j] >> shift) & bits;
-        // lanes that share the first active lane's bin (rows of no weight at all, often most
-        // of them) add together; the others one by one
-        const uint64_t act = __ballot(in);
-        if (act) {
-          const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
-          const uint64_t same = __ballot(in && bin == lead);
-          if (lane == 0) atomicAdd(&s_hist[lead], (uint32_t)__popcll(same));
-          if (in && bin != lead) atomicAdd(&s_hist[bin], 1u);
+        for (int j = 0; j < kHeavyPer; ++j) {
+          const int row = base + j * kHeavyThreads;
+          if (row >= hi) break;
+          const bool in = row + tid < hi && (u[j] & mask) == prefix;
+          if (listed) {  // pass 1: into the list as well
+            const uint64_t act = __ballot(in);
+            if (act) {
+              uint32_t at = 0;
+              if (lane == 0) at = atomicAdd(&s_fill, (uint32_t)__popcll(act));
+              at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(act & ((1ull << lane) - 1));
+              if (in) s_list[at] = u[j];
+            }
+          }
+          count(in, (u[j] >> shift) & bits);
         }
       }
     }
@@ -306,14 +341,20 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
     if (after1 < need && after1 + c1 >= need) {
       s_pick[0] = 2 * tid + 1;
       s_pick[1] = need - after1;
+      s_pick[2] = c1;
     } else if (after1 + c1 < need && suf >= need) {
       s_pick[0] = 2 * tid;
       s_pick[1] = need - after1 - c1;
+      s_pick[2] = c0;
     }
     __syncthreads();
     prefix |= s_pick[0] << shift;
     mask |= bits << shift;
     need = s_pick[1];
+    if (pass == 0) {
+      nlist = s_pick[2];
+      listed = !one && nlist <= kHeavyList;
+    }
   }
   // rows above the border, and the first `need` of its equals, in order
   uint32_t gt_before = 0, eq_before = 0;
@@ -391,27 +432,26 @@ struct Move4Args {
 constexpr int kMoveItems = 2;
 template <int NG>
 __global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
-  constexpr int kLpr = 2 * NG;
+  constexpr uint32_t kLpr = 2 * NG;
   const int bh = blockIdx.y;
-  const int64_t first = (int64_t)blockIdx.x * 256 * kMoveItems + threadIdx.x;
+  const uint32_t first = blockIdx.x * 256 * kMoveItems + threadIdx.x;
   u32x4 w[kMoveItems];
   int src[kMoveItems];
 #pragma unroll
   for (int u = 0; u < kMoveItems; ++u) {
-    const int64_t m = (first + u * 256) / kLpr;
-    src[u] = m < a.budget ? a.index[(int64_t)bh * a.budget + m] : -1;
+    const uint32_t m = (first + u * 256) / kLpr;
+    src[u] = m < (uint32_t)a.budget ? a.index[(int64_t)bh * a.budget + m] : -1;
   }
 #pragma unroll
   for (int u = 0; u < kMoveItems; ++u) {
-    const int64_t it = first + u * 256;
-    const int c = (int)(it % kLpr), z = c >= NG ? 1 : 0;
+    const int c = (int)((first + u * 256) % kLpr), z = c >= NG ? 1 : 0;
     w[u] = u32x4{0, 0, 0, 0};
     if (src[u] >= 0) w[u] = *(const u32x4*)(a.codes[z] + ((bh * a.capacity + src[u]) * NG + (c - z * NG)) * 16);
   }
 #pragma unroll
   for (int u = 0; u < kMoveItems; ++u) {
-    const int64_t it = first + u * 256, m = it / kLpr;
-    if (m >= a.budget) continue;
+    const uint32_t it = first + u * 256, m = it / kLpr;
+    if (m >= (uint32_t)a.budget) continue;
     const int c = (int)(it - m * kLpr), z = c >= NG ? 1 : 0, cc = c - z * NG;
     const int64_t to = bh * a.o_capacity + m, from = bh * a.capacity + src[u];
     const bool real = src[u] >= 0;
@@ -434,7 +474,7 @@ static int check_kv4(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, bool ma
     return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128]", who);
   DA_REQUIRE(B > 0 && Hkv > 0 && kv->capacity > 0, "%s: empty shape", who);
   DA_REQUIRE(B * Hkv <= 65535, "%s: at most 65535 (sequence, head) pairs", who);
-  DA_REQUIRE(kv->capacity < (1ll << 31) - 65536, "%s: capacity must be below 2^31 - 65536", who);
+  if (kv->capacity > (1 << 26)) return set_error(DA_ERR_UNSUPPORTED, "%s: capacity above 2^26 rows", who);
   DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
   return DA_OK;
 }
@@ -459,9 +499,9 @@ static void launch_dequantize(const Dequant4Args& a, int groups, dim3 grid, hipS
 }
 
 static int check_budget(int64_t budget, int64_t sinks, int64_t recent, const char* who) {
-  DA_REQUIRE(budget > 0 && budget < (1ll << 31) - 65536 && sinks >= 0 && recent >= 0 && sinks <= budget &&
+  DA_REQUIRE(budget > 0 && budget <= (1 << 26) && sinks >= 0 && recent >= 0 && sinks <= budget &&
                  recent <= budget - sinks,
-             "%s: needs sinks + recent <= budget, budget positive", who);
+             "%s: needs sinks + recent <= budget, budget in [1, 2^26]", who);
   return DA_OK;
 }
 
@@ -490,7 +530,7 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   if (int rc = check_kv4(out, B, Hkv, D, false, who)) return rc;
   if (dtype != DA_BF16 && dtype != DA_F16 && dtype != DA_F32)
     return set_error(DA_ERR_UNSUPPORTED, "%s: rows must be bf16, fp16 or fp32", who);
-  DA_REQUIRE(N > 0 && N < (1ll << 31) && M > 0 && M <= out->capacity && (index || M == N),
+  DA_REQUIRE(N > 0 && N <= (1 << 26) && M > 0 && M <= out->capacity && (index || M == N),
              "%s: needs 0 < M <= capacity, and M = N without an index", who);
   const int64_t align = dtype == DA_F32 ? 3 : 7;
   DA_REQUIRE(((sk_b | sk_h | sk_n | sv_b | sv_h | sv_n) & align) == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
@@ -502,10 +542,11 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   a.scales[0] = out->k_scales; a.scales[1] = out->v_scales;
   a.counts = counts; a.ts = timestamps; a.mass = mass; a.lengths = lengths; a.index = index;
   a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass; a.o_lengths = out->lengths;
-  a.N = N; a.M = M; a.capacity = out->capacity; a.H = (int)Hkv; a.D = (int)D;
+  a.N = N; a.M = M; a.capacity = out->capacity; a.B = (int)B; a.H = (int)Hkv; a.D = (int)D;
   const int groups = (int)((D + 31) / 32);
   const int64_t blocks = (M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems);
-  const dim3 grid((unsigned)blocks, (unsigned)(B * Hkv), 2);
+  DA_REQUIRE(blocks * B * Hkv < (1ll << 31), "%s: more than 2^31 workgroups", who);
+  const dim3 grid((unsigned)(blocks * B * Hkv), 2);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) launch_quantize<DA_F32>(a, groups, grid, st);
   else if (dtype == DA_F16) launch_quantize<DA_F16>(a, groups, grid, st);
@@ -586,7 +627,7 @@ extern "C" int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t 
   (void)workspace;
   (void)workspace_bytes;
   DA_REQUIRE(mass && index && kept, "%s: null pointer", who);
-  DA_REQUIRE(B > 0 && Hkv > 0 && N > 0 && N < (1ll << 31) - 65536 && B * Hkv <= 65535, "%s: bad shape", who);
+  DA_REQUIRE(B > 0 && Hkv > 0 && N > 0 && N <= (1 << 26) && B * Hkv <= 65535, "%s: bad shape", who);
   if (int rc = check_budget(budget, sinks, recent, who)) return rc;
   return launch_heavy(mass, lengths, B * Hkv, N, budget, sinks, recent, index, kept, (hipStream_t)stream, who);
 }

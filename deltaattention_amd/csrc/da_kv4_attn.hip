@@ -68,16 +68,6 @@ constexpr int kA4Part = 2 + 128;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 
-// x = sum of N bf16 parts, largest first (exact for bf16 with 1, for fp16 with 2).
-template <int N>
-__device__ __forceinline__ void split_bf16(float x, uint16_t (&p)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    p[i] = E16<DA_BF16>::bits(x);
-    x -= E16<DA_BF16>::one(p[i]);
-  }
-}
-
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                  0, 0);
@@ -103,28 +93,97 @@ __device__ __forceinline__ float cols_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-template <int DT>
-__device__ __forceinline__ float load_elem(const void* p, int64_t at) {
-  if constexpr (DT == DA_F32) return ((const float*)p)[at];
-  else return E16<DT>::one(((const uint16_t*)p)[at]);
+// Two fp32 values into N words of bf16 pairs, largest part first.
+template <int N>
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = pack_bf16x2(x0, x1);
+    if (i + 1 < N) {
+      x0 -= bf16_lo(w[i]);
+      x1 -= bf16_hi(w[i]);
+    }
+  }
 }
+
+// Eight elements of a row as they are, and element e of them as fp32.
+template <int DT>
+struct Row8 {
+  u32x4 w[DT == DA_F32 ? 2 : 1];
+  __device__ __forceinline__ void clear() {
+    w[0] = u32x4{0, 0, 0, 0};
+    if constexpr (DT == DA_F32) w[1] = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    if constexpr (DT == DA_F32) {
+      w[0] = *(const u32x4*)((const float*)p + at);
+      w[1] = *(const u32x4*)((const float*)p + at + 4);
+    } else {
+      w[0] = *(const u32x4*)((const uint16_t*)p + at);
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (DT == DA_F32) return __uint_as_float(w[e >> 2][e & 3]);
+    else return e & 1 ? E16<DT>::hi(w[0][e >> 1]) : E16<DT>::lo(w[0][e >> 1]);
+  }
+};
+
+// Orders a wave's own LDS accesses (its tile is its own).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+// What a wave loads of 32 rows: lane (r, t) group t of rows r and 16 + r, and row lane % 32's count.
+struct Tile4 {
+  u32x4 kc[2], vc[2];
+  uint32_t ks[2], vs[2];
+  int count;
+};
 
 // One workgroup: (sequence, KV head) blockIdx.x, split blockIdx.y, heads 16 z .. of the group.
 template <int DT, int NG, bool MASS>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Attn4Args a) {
+__global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Attn4Args a) {
   constexpr int QP = DT == DA_BF16 ? 1 : DT == DA_F16 ? 2 : 3;
   constexpr int PP = DT == DA_F32 ? 3 : 2;
   constexpr int NJ = 2 * NG;  // output tiles of 16 dims
   constexpr int kTileBytes = kA4Tile * kA4VRow;
+  constexpr int kRingRow = 128 + 4;  // floats of a ring row in LDS
+  static_assert(16 * kRingRow * 4 <= kTileBytes, "16 ring rows must fit a wave's tile");
   __shared__ __attribute__((aligned(16))) char s_v[kA4Waves][kTileBytes];
+  __shared__ __attribute__((aligned(16))) float s_bias[kA4Waves][kA4Tile];
   __shared__ float s_ml[kA4Waves][2][kA4Cols];
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, t = lane >> 4;
   const int bh = blockIdx.x, split = blockIdx.y;
   const int b = bh / a.Hkv, g = bh - b * a.Hkv;
   const int h0 = blockIdx.z * kA4Cols;
   const int cols = min(a.G - h0, kA4Cols);
   int n = a.lengths[bh];
+
+  // ---- q in bf16 parts, the B operand: lane (head r, t), slot e of MFMA m: dim 32 t + 8 m + e
+  const bool have = r < cols;
+  u32x4 qf[QP][4];
+  {
+    const int64_t q_at = b * a.sq_b + (int64_t)(g * a.G + h0 + (have ? r : 0)) * a.sq_h;
+    Row8<DT> x[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      x[m].clear();
+      if (have && 32 * t + 8 * m < a.D) x[m].load(a.q, q_at + 32 * t + 8 * m);
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t p[QP];
+        split_pair<QP>(x[m].get(2 * w), x[m].get(2 * w + 1), p);
+#pragma unroll
+        for (int i = 0; i < QP; ++i) qf[i][m][w] = p[i];
+      }
+  }
+
   n = n < 0 ? 0 : (n > a.capacity ? (int)a.capacity : n);
   const int tiles = (n + kA4Tile - 1) / kA4Tile;
   const int rtiles = (a.exact_len + 15) / 16;
@@ -144,75 +203,125 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Attn4Args a) {
     return;
   }
 
-  // ---- q in bf16 parts, the B operand: lane (head r, t), slot e of MFMA m: dim 32 t + 8 m + e
-  const bool have = r < cols;
-  const int64_t q_at = b * a.sq_b + (int64_t)(g * a.G + h0 + (have ? r : 0)) * a.sq_h;
-  u32x4 qf[QP][4];
+  const bool grp = t < NG;
+  const int tg = grp ? t : 0;
+  const int64_t row0 = (int64_t)bh * a.capacity;
+  const uint8_t* const kc0 = a.kc + row0 * NG * 16;
+  const uint8_t* const vc0 = a.vc + row0 * NG * 16;
+  const uint8_t* const ks0 = a.ks + row0 * NG;
+  const uint8_t* const vs0 = a.vs + row0 * NG;
+  const int32_t* const cnt0 = a.counts + row0;
+  // rows past the length read the last one and carry no weight
+  auto load_tile = [&](int tile, Tile4& x) {
+    const int j0 = tile * kA4Tile;
 #pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    uint16_t p[8][QP];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = 32 * t + 8 * m + e;
-      split_bf16<QP>(have && d < a.D ? load_elem<DT>(a.q, q_at + d) : 0.0f, p[e]);
+    for (int u = 0; u < 2; ++u) {
+      const int64_t at = (int64_t)min(j0 + 16 * u + r, n - 1) * NG + tg;
+      x.kc[u] = *(const u32x4*)(kc0 + at * 16);
+      x.vc[u] = *(const u32x4*)(vc0 + at * 16);
+      x.ks[u] = ks0[at];
+      x.vs[u] = vs0[at];
     }
-#pragma unroll
-    for (int i = 0; i < QP; ++i)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) qf[i][m][w] = p[2 * w][i] | ((uint32_t)p[2 * w + 1][i] << 16);
-  }
+    x.count = cnt0[min(j0 + (lane & 31), n - 1)];
+  };
+  Tile4 cur;
+  if (t_begin + wid < t_end) load_tile(t_begin + wid, cur);
 
   f32x4 acc[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
   float m_run = -INFINITY, l_run = 0.0f;
-
-  const int64_t row0 = (int64_t)bh * a.capacity;
-  const bool grp = t < NG;
-  const int tg = grp ? t : 0;
+  // a new maximum: what was summed shrinks by 2^(old - new)
+  auto raise = [&](float mx) {
+    mx = cols_max(mx);
+    if (__ballot(mx > m_run)) {
+      const float m_new = __builtin_fmaxf(mx, m_run);
+      const float f = is_neg_inf(m_run) ? 0.0f : exp2_hw(m_run - m_new);
+      l_run *= f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
+      m_run = m_new;
+    }
+    return is_neg_inf(m_run) ? 0.0f : m_run;
+  };
   char* const vt = s_v[wid];
-  float* const score = MASS ? a.score + ((int64_t)bh * a.G + h0 + (have ? r : 0)) * a.score_cap : nullptr;
+  float* const bias = s_bias[wid];
 
-  // ---- the rows, 32 at a time ----
+  // ---- the ring, 16 slots at a time, in fp32: lane (r, t) loads dims 32 t + 8 m + e of slot r ----
+  const int64_t x_at = b * a.sx_b + g * a.sx_h;
+  for (int rt = rfirst; rt < rtiles; rt += nwave) {
+    const int j0 = rt * 16;
+    const bool slot = j0 + r < a.exact_len;
+    const int64_t at = x_at + (int64_t)(slot ? j0 + r : 0) * a.sx_s + 32 * t;
+    f32x4 s = f32x4{0, 0, 0, 0};
+    Row8<DT> kx[4], vx[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      kx[m].clear();
+      vx[m].clear();
+      if (slot && 32 * t + 8 * m < a.D) {
+        kx[m].load(a.kx, at + 8 * m);
+        vx[m].load(a.vx, at + 8 * m);
+      }
+    }
+    float* const rv = (float*)(void*)vt;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float qv = 0.0f;  // the parts' sum is q itself
+#pragma unroll
+        for (int i = QP - 1; i >= 0; --i) qv += (e & 1) ? bf16_hi(qf[i][m][e >> 1]) : bf16_lo(qf[i][m][e >> 1]);
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[m].get(e), qv, s, 0, 0, 0);
+      }
+      if (grp) {
+        *(f32x4*)(rv + r * kRingRow + 32 * t + 8 * m) = f32x4{vx[m].get(0), vx[m].get(1), vx[m].get(2), vx[m].get(3)};
+        *(f32x4*)(rv + r * kRingRow + 32 * t + 8 * m + 4) = f32x4{vx[m].get(4), vx[m].get(5), vx[m].get(6), vx[m].get(7)};
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = j0 + 4 * t + i < a.exact_len ? s[i] * a.scale_log2 : -INFINITY;
+      mx = __builtin_fmaxf(mx, s[i]);
+    }
+    const float base = raise(mx);
+    wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = exp2_hw(s[i] - base);
+      l_run += p;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(rv[(4 * t + i) * kRingRow + 16 * j + r], p, acc[j], 0, 0, 0);
+    }
+    wave_lds_fence();
+  }
+
+  // ---- the rows, 32 at a time, the next tile's loads under this one's work ----
+  float* const score = MASS ? a.score + ((int64_t)bh * a.G + h0 + (have ? r : 0)) * a.score_cap : nullptr;
   for (int tile = t_begin + wid; tile < t_end; tile += kA4Waves) {
     const int j0 = tile * kA4Tile;
-    u32x4 kc[2], vc[2];
-    uint32_t ksc[2], vsc[2];
-    int cnt[2][4], vcnt[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      // rows past the length read the last one and carry no weight
-      const int64_t row = row0 + min(j0 + 16 * u + r, n - 1);
-      kc[u] = *(const u32x4*)(a.kc + (row * NG + tg) * 16);
-      vc[u] = *(const u32x4*)(a.vc + (row * NG + tg) * 16);
-      ksc[u] = a.ks[row * NG + tg];
-      vsc[u] = a.vs[row * NG + tg];
-      vcnt[u] = a.counts[row];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cnt[u][i] = a.counts[row0 + min(j0 + 16 * u + 4 * t + i, n - 1)];
-    }
-    // ---- scores ----
+    Tile4 nxt;
+    if (tile + kA4Waves < t_end) load_tile(tile + kA4Waves, nxt);
+    // log2(count), or -inf for a row without weight, once a row
+    if (lane < kA4Tile)
+      bias[lane] = cur.count > 0 && j0 + lane < n ? __builtin_amdgcn_logf((float)cur.count) : -INFINITY;
+    wave_lds_fence();
     f32x4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float sc = __uint_as_float(ksc[u] << 23);
+      const float ksc = __uint_as_float(cur.ks[u] << 23), vsc = __uint_as_float(cur.vs[u] << 23);
+      const bool live = !is_neg_inf(bias[16 * u + r]);
       s[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        u32x4 kf = fp4_to_bf16x8(kc[u][m], sc);
+        u32x4 kf = fp4_to_bf16x8(cur.kc[u][m], ksc);
         if (NG < 4 && !grp) kf = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = QP - 1; i >= 0; --i) s[u] = mfma16(kf, qf[i][m], s[u]);
-      }
-    }
-    // ---- V to LDS as bf16; a row without weight as zeros, whatever it holds ----
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const bool live = vcnt[u] > 0 && j0 + 16 * u + r < n;
-      const float sc = __uint_as_float(vsc[u] << 23);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        u32x4 v = fp4_to_bf16x8(vc[u][m], sc);
+        // V to LDS as bf16; a row without weight as zeros, whatever it holds
+        u32x4 v = fp4_to_bf16x8(cur.vc[u][m], vsc);
         if (!live) v = u32x4{0, 0, 0, 0};
         if (grp) *(u32x4*)(vt + (16 * u + r) * kA4VRow + 64 * t + 16 * m) = v;
       }
@@ -220,47 +329,34 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Attn4Args a) {
     // ---- softmax: lane (head r), keys 4 t + i of both halves ----
     float mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
+      const f32x4 add = *(const f32x4*)(bias + 16 * u + 4 * t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = j0 + 16 * u + 4 * t + i;
-        const bool live = cnt[u][i] > 0 && key < n;
-        s[u][i] = live ? s[u][i] * a.scale_log2 + __builtin_amdgcn_logf((float)cnt[u][i]) : -INFINITY;
+        s[u][i] = is_neg_inf(add[i]) ? -INFINITY : __builtin_fmaf(s[u][i], a.scale_log2, add[i]);
         mx = __builtin_fmaxf(mx, s[u][i]);
       }
+    }
     if (MASS) {
       if (have)
 #pragma unroll
         for (int u = 0; u < 2; ++u) *(f32x4*)(score + j0 + 16 * u + 4 * t) = s[u];
     }
-    mx = cols_max(mx);
-    if (__ballot(mx > m_run)) {
-      const float m_new = __builtin_fmaxf(mx, m_run);
-      const float f = m_run == -INFINITY ? 0.0f : exp2_hw(m_run - m_new);
-      l_run *= f;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[j] *= f;
-      m_run = m_new;
-    }
-    const float base = m_run == -INFINITY ? 0.0f : m_run;
-    uint16_t pp[8][PP];
+    const float base = raise(mx);
+    u32x4 pf[PP];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = exp2_hw(s[u][i] - base);
-        l_run += p;
-        split_bf16<PP>(p, pp[4 * u + i]);
+      for (int w = 0; w < 2; ++w) {
+        const float p0 = exp2_hw(s[u][2 * w] - base), p1 = exp2_hw(s[u][2 * w + 1] - base);
+        l_run += p0 + p1;
+        uint32_t p[PP];
+        split_pair<PP>(p0, p1, p);
+#pragma unroll
+        for (int i = 0; i < PP; ++i) pf[i][2 * u + w] = p[i];
       }
-    u32x4 pf[PP];
-#pragma unroll
-    for (int i = 0; i < PP; ++i)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) pf[i][w] = pp[2 * w][i] | ((uint32_t)pp[2 * w + 1][i] << 16);
     // ---- O^T += V^T P^T ----
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       // in each group of 16 lanes, lane i receives element i % 4 of the 8 bytes that lanes
@@ -276,54 +372,8 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Attn4Args a) {
 #pragma unroll
       for (int i = PP - 1; i >= 0; --i) acc[j] = mfma16(vf, pf[i], acc[j]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-  }
-
-  // ---- the ring, 16 slots at a time, in fp32 ----
-  const int64_t x_at = b * a.sx_b + g * a.sx_h;
-  for (int rt = rfirst; rt < rtiles; rt += nwave) {
-    const int j0 = rt * 16;
-    const int64_t krow = x_at + (int64_t)min(j0 + r, a.exact_len - 1) * a.sx_s;
-    f32x4 s = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int u = 0; u < 2 * NG; ++u) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 16 * u + 4 * t + i;
-        const float kf = d < a.D ? load_elem<DT>(a.kx, krow + d) : 0.0f;
-        const float qv = have && d < a.D ? load_elem<DT>(a.q, q_at + d) : 0.0f;
-        s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, qv, s, 0, 0, 0);
-      }
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = j0 + 4 * t + i < a.exact_len ? s[i] * a.scale_log2 : -INFINITY;
-      mx = __builtin_fmaxf(mx, s[i]);
-    }
-    mx = cols_max(mx);
-    const float m_new = __builtin_fmaxf(mx, m_run);
-    const float f = m_run == -INFINITY ? 0.0f : exp2_hw(m_run - m_new);
-    l_run *= f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[j] *= f;
-    m_run = m_new;
-    const float base = m_run == -INFINITY ? 0.0f : m_run;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float p = exp2_hw(s[i] - base);
-      l_run += p;
-      const int slot = j0 + 4 * t + i;
-      const int64_t vrow = x_at + (int64_t)min(slot, a.exact_len - 1) * a.sx_s;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int d = 16 * j + r;
-        const float v = d < a.D && slot < a.exact_len ? load_elem<DT>(a.vx, vrow + d) : 0.0f;
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p, acc[j], 0, 0, 0);
-      }
-    }
+    wave_lds_fence();
+    cur = nxt;
   }
 
   // ---- join the four waves; the V tiles' LDS holds their sums ----
@@ -518,6 +568,10 @@ extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq,
   DA_REQUIRE(kv->capacity > 0 && exact_len >= 0 && exact_len < (1 << 24), "%s: bad cache lengths", who);
   if (kv->capacity > (1 << 24)) return set_error(DA_ERR_UNSUPPORTED, "%s: capacity above 2^24 rows", who);
   DA_REQUIRE(exact_len == 0 || (k_exact && v_exact), "%s: null ring", who);
+  const int64_t align = dtype == DA_F32 ? 3 : 7;
+  DA_REQUIRE(((sq_b | sq_h) & align) == 0 && ((uintptr_t)q & 15) == 0 &&
+                 (exact_len == 0 || (((sx_b | sx_h | sx_s) & align) == 0 && (((uintptr_t)k_exact | (uintptr_t)v_exact) & 15) == 0)),
+             "%s: q and ring rows must be 16-byte aligned", who);
   DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
   DA_REQUIRE(scale > 0.0f, "%s: scale must be positive", who);
   const int64_t need = da_kv4_attention_workspace_size(B, Hq, Hkv, kv->capacity, accumulate);

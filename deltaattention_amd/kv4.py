@@ -45,10 +45,13 @@ def _gpu(t: torch.Tensor, name: str) -> torch.device:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with a contiguous head dimension and rows that begin at multiples of 16 bytes."""
-    per = 4 if t.dtype == _F32 else 8
-    s = t.stride()
-    if s[-1] == 1 and not any(x % per for x, n in zip(s[:-1], t.shape) if n > 1) and t.data_ptr() % 16 == 0:
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():  # a head dimension is a multiple of 8 elements
+            return t
+        per = 4 if t.dtype == _F32 else 8
+        s = t.stride()
+        if s[-1] == 1 and not any(x % per for x, n in zip(s[:-1], t.shape) if n > 1):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -381,18 +384,19 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
         if len(xs) != 4 or xs[0] != B or xs[1] != H or xs[3] != D or v_exact.shape != xs or k_exact.device != device \
                 or v_exact.device != device:
             raise ValueError(f"k_exact and v_exact must be [{B}, {H}, W, {D}] on {device}")
-        W, sx = xs[2], k_exact.stride()
-        if sx[3] != 1 or v_exact.stride() != sx:
-            k_exact, v_exact = (t.clone(memory_format=torch.contiguous_format) for t in (k_exact, v_exact))
-            sx = k_exact.stride()
+        W = xs[2]
+        if W:
+            k_exact, v_exact = _rows(k_exact), _rows(v_exact)
+            sx = _strides(k_exact)
+            if _strides(v_exact) != sx:
+                k_exact, v_exact = (t.clone(memory_format=torch.contiguous_format) for t in (k_exact, v_exact))
+                sx = _strides(k_exact)
         kx, vx = k_exact.data_ptr(), v_exact.data_ptr()
     n_exact = W if exact_len is None else int(exact_len)
     if not 0 <= n_exact <= W:
         raise ValueError(f"exact_len must lie in [0, {W}], got {n_exact}")
-    sq = q.stride()
-    if sq[-1] != 1:
-        q = q.contiguous()
-        sq = q.stride()
+    q = _rows(q)
+    sq = _strides(q)
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=device)
     elif out.shape != shape or out.device != device or out.stride(-1) != 1:

@@ -29,7 +29,8 @@ extern "C" {
  * All arrays are contiguous: codes [B, Hkv, capacity, 16 groups], exponents [B, Hkv,
  * capacity, groups], counts / timestamps / mass [B, Hkv, capacity], lengths [B, Hkv] (rows in
  * use; clamped into [0, capacity] where read).  Codes must be 16-byte aligned.  mass (the
- * attention weight each row has received) may be null where a call does not use it.
+ * attention weight each row has received) may be null where a call does not use it.  At most
+ * 2^26 rows a head and 65535 (sequence, head) pairs.
  */
 typedef struct DaKv4 {
   uint8_t* k_codes;
@@ -73,7 +74,7 @@ int da_kv4_dequantize(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t N, int64_
  * sinks + recent <= budget <= out->capacity.  Rows [kept, budget) of `out` are zero, rows from
  * budget on are not written; out->lengths receives the rows kept.  kv->mass and out->mass are
  * needed.  index, if not null ([B, Hkv, budget] int32), receives the rows kept, -1 past them.
- * kv->capacity < 2^31, workspace: da_kv4_evict_workspace_size() bytes.
+ * workspace: da_kv4_evict_workspace_size() bytes.
  */
 int64_t da_kv4_evict_workspace_size(int64_t B, int64_t Hkv, int64_t capacity, int64_t budget);
 int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, int64_t budget, int64_t sinks, int64_t recent,
