@@ -174,30 +174,20 @@ def device_stream(device: torch.device) -> int:
     return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
 
 
+_get_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _raw_stream(index: int) -> int:
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if get is None:  # pragma: no cover - older torch
+    if _get_raw_stream is None:  # pragma: no cover - older torch
         return torch.cuda.current_stream(index).cuda_stream
-    return get(index)
+    return _get_raw_stream(index)
 
 
-class on_device:
-    """``with on_device(device) as stream``: ``device`` is the current one inside, whichever was
-    before, and ``stream`` the handle of its current stream."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self) -> int:
-        self.before = torch.cuda.current_device()
-        if self.index is None:
-            self.index = self.before
-        if self.index != self.before:
-            torch.cuda.set_device(self.index)
-        return _raw_stream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.index != self.before:
-            torch.cuda.set_device(self.before)
+def call_on(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` with ``device`` current (whichever was before) and the handle of its
+    current stream."""
+    index, now = device.index, torch.cuda.current_device()
+    if index == now:
+        return fn(*args, _raw_stream(now))
+    with torch.cuda.device(device):
+        return fn(*args, _raw_stream(index))

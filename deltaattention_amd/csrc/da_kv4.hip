@@ -226,71 +226,88 @@ __device__ __forceinline__ uint32_t mass_order(float m) {
 }
 
 constexpr int kHeavyThreads = 1024, kHeavyWaves = kHeavyThreads / 64, kHeavyBins = 2048;
-constexpr int kHeavyPer = 16;                              // masses a thread holds at once
-constexpr int kHeavyBatch = kHeavyThreads * kHeavyPer;     // rows of a batch
-constexpr int kHeavyList = 16384;                          // rows of the border's first bin kept in LDS
+constexpr int kHeavyPer = 16;                              // masses a thread of heavy_rows_kernel holds
+constexpr int kHeavyShort = kHeavyThreads * kHeavyPer;     // rows of a head that one workgroup sorts out
 
-// One workgroup per (sequence, head).  The border (the need-th largest mass between the
-// protected ends) comes from three histogram passes over 11, 11 and 10 bits of the order;
-// a last pass writes the rows above it, and as many of its equals as still fit, lowest row
-// first, in row order.  Rows come in batches of 16384, 16 loads in flight a thread.  A head of
-// one batch is read once.  A longer one is read three times: the second reading collects the
-// rows of the first pass's bin in LDS, where the other passes find them (unless they are too
-// many: then those read the row again).
+// One more row of `bin` for the lanes that are `in`: lanes that share the first one's bin (rows of
+// no weight at all, often most of them) add together, the others one by one.
+__device__ __forceinline__ void count_bin(uint32_t* hist, bool in, uint32_t bin, int lane) {
+  const uint64_t act = __ballot(in);
+  if (act) {
+    const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
+    const uint64_t same = __ballot(in && bin == lead);
+    if (lane == 0) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
+    if (in && bin != lead) atomicAdd(&hist[bin], 1u);
+  }
+}
+
+// The highest bin such that it and those above hold at least `need` rows, and how many of its own
+// rows are needed.  Thread t brings the counts of bins 2 t and 2 t + 1; called by all threads, the
+// counts' writes already waited for.
+__device__ __forceinline__ void pick_bin(uint32_t c0, uint32_t c1, uint32_t& need, uint32_t& bin, uint32_t* s_wave,
+                                         uint32_t* s_pick, int tid) {
+  const int lane = tid & 63, wid = tid >> 6;
+  uint32_t suf = c0 + c1;  // becomes the sum over this thread's bins and those above
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = (uint32_t)__shfl_down((int)suf, d, 64);
+    suf += lane + d < 64 ? up : 0;
+  }
+  if (lane == 0) s_wave[wid] = suf;
+  __syncthreads();
+  for (int w = wid + 1; w < kHeavyWaves; ++w) suf += s_wave[w];
+  const uint32_t after1 = suf - c0 - c1;  // rows in bins above 2 t + 1
+  if (after1 < need && after1 + c1 >= need) {
+    s_pick[0] = 2 * tid + 1;
+    s_pick[1] = need - after1;
+  } else if (after1 + c1 < need && suf >= need) {
+    s_pick[0] = 2 * tid;
+    s_pick[1] = need - after1 - c1;
+  }
+  __syncthreads();
+  bin = s_pick[0];
+  need = s_pick[1];
+}
+
+__device__ __forceinline__ int heavy_length(const HeavyArgs& a, int bh) {
+  const int n = a.lengths ? a.lengths[bh] : (int)a.capacity;
+  return n < 0 ? 0 : (n > a.capacity ? (int)a.capacity : n);
+}
+
+// Heads of at most kHeavyShort rows, one workgroup each, every mass read once and kept in
+// registers.  The border (the need-th largest mass between the protected ends) comes from three
+// histogram passes over 11, 11 and 10 bits of the order; then the rows above it are written, and as
+// many of its equals as still fit, lowest row first, in row order.
 __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) {
-  __shared__ uint32_t s_list[kHeavyList];
   __shared__ uint32_t s_hist[kHeavyBins];
   __shared__ uint32_t s_wave[kHeavyWaves];
   __shared__ uint32_t s_cnt[2][kHeavyPer * kHeavyWaves];  // rows above / at the border, in row order
-  __shared__ uint32_t s_all[2];
-  __shared__ uint32_t s_pick[3];  // the chosen bin, the rows still needed from it, the rows it holds
-  __shared__ uint32_t s_fill;
+  __shared__ uint32_t s_pick[2];
   const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  int64_t n64 = a.lengths ? a.lengths[bh] : a.capacity;
-  n64 = n64 < 0 ? 0 : (n64 > a.capacity ? a.capacity : n64);
-  const int n = (int)n64;
+  const int n = heavy_length(a, bh);
   int32_t* const out = a.index + (int64_t)bh * a.budget;
-  const int kept = n < a.budget ? n : a.budget;
-  if (tid == 0) {
-    a.kept[bh] = kept;
-    s_fill = 0;
-  }
+  if (tid == 0) a.kept[bh] = n < a.budget ? n : a.budget;
   if (n <= a.budget) {
     for (int i = tid; i < a.budget; i += kHeavyThreads) out[i] = i < n ? i : -1;
     return;
   }
   const float* const mass = a.mass + (int64_t)bh * a.capacity;
   const int lo = a.sinks, hi = n - a.recent;  // the rows that compete
+  uint32_t u[kHeavyPer];
+  {
+    float m[kHeavyPer];
+#pragma unroll
+    for (int j = 0; j < kHeavyPer; ++j) {
+      const int i = lo + j * kHeavyThreads + tid;
+      m[j] = i < hi ? mass[i] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kHeavyPer; ++j) u[j] = mass_order(m[j]);
+  }
   for (int i = tid; i < a.sinks; i += kHeavyThreads) out[i] = i;
   for (int i = tid; i < a.recent; i += kHeavyThreads) out[a.budget - a.recent + i] = hi + i;
   uint32_t need = (uint32_t)(a.budget - a.sinks - a.recent);
   if (need == 0) return;
-  uint32_t u[kHeavyPer];
-  auto load = [&](int base) {
-    float m[kHeavyPer];
-#pragma unroll
-    for (int j = 0; j < kHeavyPer; ++j) {
-      const int i = base + j * kHeavyThreads + tid;
-      m[j] = mass[i < hi ? i : hi - 1];
-    }
-#pragma unroll
-    for (int j = 0; j < kHeavyPer; ++j) u[j] = mass_order(m[j]);
-  };
-  // one more row of `bin` for the active lanes: lanes that share the first one's bin (rows of no
-  // weight at all, often most of them) add together, the others one by one
-  auto count = [&](bool in, uint32_t bin) {
-    const uint64_t act = __ballot(in);
-    if (act) {
-      const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)act) - 1);
-      const uint64_t same = __ballot(in && bin == lead);
-      if (lane == 0) atomicAdd(&s_hist[lead], (uint32_t)__popcll(same));
-      if (in && bin != lead) atomicAdd(&s_hist[bin], 1u);
-    }
-  };
-  const bool one = hi - lo <= kHeavyBatch;
-  bool listed = false;
-  uint32_t nlist = 0;
-  if (one) load(lo);
   uint32_t prefix = 0, mask = 0;  // bits of the border found so far
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
@@ -298,115 +315,280 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
     s_hist[tid] = 0;
     s_hist[tid + kHeavyThreads] = 0;
     __syncthreads();
-    if (listed && pass == 2) {
-      for (uint32_t i0 = 0; i0 < nlist; i0 += kHeavyThreads) {
-        const uint32_t i = i0 + tid, v = i < nlist ? s_list[i] : 0;
-        count(i < nlist && (v & mask) == prefix, v & bits);
-      }
-    } else {
-      for (int base = lo; base < hi; base += kHeavyBatch) {
-        if (!one) load(base);
 #pragma unroll
-        for (int j = 0; j < kHeavyPer; ++j) {
-          const int row = base + j * kHeavyThreads;
-          if (row >= hi) break;
-          const bool in = row + tid < hi && (u[j] & mask) == prefix;
-          if (listed) {  // pass 1: into the list as well
-            const uint64_t act = __ballot(in);
-            if (act) {
-              uint32_t at = 0;
-              if (lane == 0) at = atomicAdd(&s_fill, (uint32_t)__popcll(act));
-              at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(act & ((1ull << lane) - 1));
-              if (in) s_list[at] = u[j];
-            }
-          }
-          count(in, (u[j] >> shift) & bits);
-        }
-      }
+    for (int j = 0; j < kHeavyPer; ++j) {
+      const int row = lo + j * kHeavyThreads;
+      if (row < hi) count_bin(s_hist, row + tid < hi && (u[j] & mask) == prefix, (u[j] >> shift) & bits, lane);
     }
     __syncthreads();
-    // the highest bin such that it and those above hold at least `need` rows: thread t owns
-    // bins 2 t and 2 t + 1, suffix sums over the threads
-    const uint32_t c0 = s_hist[2 * tid], c1 = s_hist[2 * tid + 1];
-    uint32_t suf = c0 + c1;  // becomes the sum over this thread's bins and those above
+    uint32_t bin;
+    pick_bin(s_hist[2 * tid], s_hist[2 * tid + 1], need, bin, s_wave, s_pick, tid);
+    prefix |= bin << shift;
+    mask |= bits << shift;
+  }
+  uint64_t bg[kHeavyPer], be[kHeavyPer];
+#pragma unroll
+  for (int j = 0; j < kHeavyPer; ++j) {
+    const bool in = lo + j * kHeavyThreads + tid < hi;
+    bg[j] = __ballot(in && u[j] > prefix);
+    be[j] = __ballot(in && u[j] == prefix);
+    if (lane == 0) {
+      s_cnt[0][j * kHeavyWaves + wid] = (uint32_t)__popcll(bg[j]);
+      s_cnt[1][j * kHeavyWaves + wid] = (uint32_t)__popcll(be[j]);
+    }
+  }
+  __syncthreads();
+  if (wid < 2) {  // prefix sums of the 256 counts, four a lane: wave 0 above, wave 1 at the border
+    uint32_t c[4], run = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j] = s_cnt[wid][4 * lane + j];
+      run += c[j];
+    }
+    uint32_t inc = run;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t up = (uint32_t)__shfl_down((int)suf, d, 64);
-      suf += lane + d < 64 ? up : 0;
+      const uint32_t dn = (uint32_t)__shfl_up((int)inc, d, 64);
+      inc += lane >= d ? dn : 0;
     }
-    if (lane == 0) s_wave[wid] = suf;
-    __syncthreads();
-    for (int w = wid + 1; w < kHeavyWaves; ++w) suf += s_wave[w];
-    const uint32_t after1 = suf - c0 - c1;  // rows in bins above 2 t + 1
-    if (after1 < need && after1 + c1 >= need) {
-      s_pick[0] = 2 * tid + 1;
-      s_pick[1] = need - after1;
-      s_pick[2] = c1;
-    } else if (after1 + c1 < need && suf >= need) {
-      s_pick[0] = 2 * tid;
-      s_pick[1] = need - after1 - c1;
-      s_pick[2] = c0;
-    }
-    __syncthreads();
-    prefix |= s_pick[0] << shift;
-    mask |= bits << shift;
-    need = s_pick[1];
-    if (pass == 0) {
-      nlist = s_pick[2];
-      listed = !one && nlist <= kHeavyList;
+    uint32_t at = inc - run;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s_cnt[wid][4 * lane + j] = at;
+      at += c[j];
     }
   }
-  // rows above the border, and the first `need` of its equals, in order
-  uint32_t gt_before = 0, eq_before = 0;
+  __syncthreads();
   const uint64_t below = (1ull << lane) - 1;
-  for (int base = lo; base < hi; base += kHeavyBatch) {
-    if (!one) load(base);
-    uint64_t bg[kHeavyPer], be[kHeavyPer];
 #pragma unroll
-    for (int j = 0; j < kHeavyPer; ++j) {
-      const bool in = base + j * kHeavyThreads + tid < hi;
-      bg[j] = __ballot(in && u[j] > prefix);
-      be[j] = __ballot(in && u[j] == prefix);
-      if (lane == 0) {
-        s_cnt[0][j * kHeavyWaves + wid] = (uint32_t)__popcll(bg[j]);
-        s_cnt[1][j * kHeavyWaves + wid] = (uint32_t)__popcll(be[j]);
-      }
-    }
-    __syncthreads();
-    if (wid < 2) {  // prefix sums of the 256 counts, four a lane: wave 0 above, wave 1 at the border
-      uint32_t c[4], run = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        c[j] = s_cnt[wid][4 * lane + j];
-        run += c[j];
-      }
-      uint32_t inc = run;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t dn = (uint32_t)__shfl_up((int)inc, d, 64);
-        inc += lane >= d ? dn : 0;
-      }
-      uint32_t at = inc - run;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s_cnt[wid][4 * lane + j] = at;
-        at += c[j];
-      }
-      if (lane == 63) s_all[wid] = inc;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kHeavyPer; ++j) {
-      const uint32_t g = gt_before + s_cnt[0][j * kHeavyWaves + wid] + (uint32_t)__popcll(bg[j] & below);
-      const uint32_t e = eq_before + s_cnt[1][j * kHeavyWaves + wid] + (uint32_t)__popcll(be[j] & below);
-      const bool gt = (bg[j] >> lane) & 1, eq = (be[j] >> lane) & 1;
-      if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = base + j * kHeavyThreads + tid;
-    }
-    gt_before += s_all[0];
-    eq_before += s_all[1];
-    __syncthreads();
+  for (int j = 0; j < kHeavyPer; ++j) {
+    const uint32_t g = s_cnt[0][j * kHeavyWaves + wid] + (uint32_t)__popcll(bg[j] & below);
+    const uint32_t e = s_cnt[1][j * kHeavyWaves + wid] + (uint32_t)__popcll(be[j] & below);
+    const bool gt = (bg[j] >> lane) & 1, eq = (be[j] >> lane) & 1;
+    if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = lo + j * kHeavyThreads + tid;
   }
 }
+
+// Longer heads in chunks of kChunk rows, a workgroup each, in five launches that take the chip:
+// histogram of the top 11 bits a chunk; the border's bin a head; the rows of that bin, listed a
+// chunk; the border itself from the lists, and what every chunk keeps; the rows' numbers.  (One
+// workgroup a head took 120 us for 131072 rows, where these take a quarter.)
+constexpr int kChunkPer = 4, kChunk = kHeavyThreads * kChunkPer;
+
+struct HeavyWork {      // per head and chunk, in the workspace
+  uint32_t* hist;       // [bh][chunks][kHeavyBins]
+  uint32_t* list;       // [bh][chunks][kChunk]: orders of the rows of the border's bin
+  uint32_t* count;      // [bh][chunks][4]: rows in the list; rows above and at the border before the chunk
+  uint32_t* border;     // [bh][4]: bin, rows needed of it; border, equals needed
+  int chunks;
+};
+
+__device__ __forceinline__ void chunk_masses(const HeavyArgs& a, int bh, int first, int lo, int hi,
+                                             uint32_t (&u)[kChunkPer], bool (&in)[kChunkPer]) {
+  const float* const mass = a.mass + (int64_t)bh * a.capacity;
+  float m[kChunkPer];
+#pragma unroll
+  for (int j = 0; j < kChunkPer; ++j) {
+    const int i = first + j * kHeavyThreads + (int)threadIdx.x;
+    in[j] = i >= lo && i < hi;
+    m[j] = in[j] ? mass[i] : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < kChunkPer; ++j) u[j] = mass_order(m[j]);
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heavy_hist_kernel(HeavyArgs a, HeavyWork w) {
+  __shared__ uint32_t s_hist[kHeavyBins];
+  const int bh = blockIdx.x / w.chunks, c = blockIdx.x - bh * w.chunks, tid = threadIdx.x;
+  const int n = heavy_length(a, bh);
+  if (n <= a.budget) return;
+  s_hist[tid] = 0;
+  s_hist[tid + kHeavyThreads] = 0;
+  uint32_t u[kChunkPer];
+  bool in[kChunkPer];
+  chunk_masses(a, bh, c * kChunk, a.sinks, n - a.recent, u, in);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kChunkPer; ++j) count_bin(s_hist, in[j], u[j] >> 21, tid & 63);
+  __syncthreads();
+  uint32_t* const h = w.hist + (int64_t)blockIdx.x * kHeavyBins;
+  h[tid] = s_hist[tid];
+  h[tid + kHeavyThreads] = s_hist[tid + kHeavyThreads];
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heavy_bin_kernel(HeavyArgs a, HeavyWork w) {
+  __shared__ uint32_t s_wave[kHeavyWaves];
+  __shared__ uint32_t s_pick[2];
+  const int bh = blockIdx.x, tid = threadIdx.x;
+  const int n = heavy_length(a, bh);
+  if (tid == 0) a.kept[bh] = n < a.budget ? n : a.budget;
+  uint32_t need = (uint32_t)(a.budget - a.sinks - a.recent), bin = kHeavyBins;  // none: no row competes for a place
+  if (n > a.budget && need > 0) {
+    uint32_t c0 = 0, c1 = 0;
+    const u32x2* h = (const u32x2*)(const void*)(w.hist + (int64_t)bh * w.chunks * kHeavyBins) + tid;
+    for (int c = 0; c < w.chunks; ++c) {
+      const u32x2 v = h[(int64_t)c * (kHeavyBins / 2)];
+      c0 += v[0];
+      c1 += v[1];
+    }
+    pick_bin(c0, c1, need, bin, s_wave, s_pick, tid);
+  }
+  if (tid == 0) {
+    w.border[4 * bh] = bin;
+    w.border[4 * bh + 1] = need;
+  }
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heavy_list_kernel(HeavyArgs a, HeavyWork w) {
+  __shared__ uint32_t s_fill;
+  const int bh = blockIdx.x / w.chunks, c = blockIdx.x - bh * w.chunks, tid = threadIdx.x, lane = tid & 63;
+  const int n = heavy_length(a, bh);
+  if (n <= a.budget) return;
+  const uint32_t bin = w.border[4 * bh];
+  if (tid == 0) s_fill = 0;
+  uint32_t u[kChunkPer];
+  bool in[kChunkPer];
+  chunk_masses(a, bh, c * kChunk, a.sinks, n - a.recent, u, in);
+  __syncthreads();
+  uint32_t* const list = w.list + (int64_t)blockIdx.x * kChunk;
+#pragma unroll
+  for (int j = 0; j < kChunkPer; ++j) {
+    const bool hit = in[j] && (u[j] >> 21) == bin;
+    const uint64_t act = __ballot(hit);
+    if (act) {
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&s_fill, (uint32_t)__popcll(act));
+      at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(act & ((1ull << lane) - 1));
+      if (hit) list[at] = u[j];
+    }
+  }
+  __syncthreads();
+  if (tid == 0) w.count[4 * blockIdx.x] = s_fill;
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heavy_border_kernel(HeavyArgs a, HeavyWork w) {
+  __shared__ uint32_t s_hist[kHeavyBins];
+  __shared__ uint32_t s_wave[kHeavyWaves];
+  __shared__ uint32_t s_pick[2];
+  const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int n = heavy_length(a, bh);
+  if (n <= a.budget) return;
+  const uint32_t bin = w.border[4 * bh];
+  uint32_t need = w.border[4 * bh + 1];
+  uint32_t prefix = bin << 21, mask = 2047u << 21;
+  uint32_t* const count = w.count + (int64_t)bh * w.chunks * 4;
+  const uint32_t* const list = w.list + (int64_t)bh * w.chunks * kChunk;
+  const bool any = bin < kHeavyBins;
+  if (any) {
+    for (int pass = 1; pass < 3; ++pass) {
+      const int shift = pass == 1 ? 10 : 0;
+      const uint32_t bits = pass == 1 ? 2047u : 1023u;
+      s_hist[tid] = 0;
+      s_hist[tid + kHeavyThreads] = 0;
+      __syncthreads();
+      for (int c = wid; c < w.chunks; c += kHeavyWaves) {
+        const uint32_t fill = count[4 * c];
+        for (uint32_t i0 = 0; i0 < fill; i0 += 64) {
+          const uint32_t i = i0 + lane, v = i < fill ? list[(int64_t)c * kChunk + i] : 0;
+          count_bin(s_hist, i < fill && (v & mask) == prefix, (v >> shift) & bits, lane);
+        }
+      }
+      __syncthreads();
+      uint32_t b2;
+      pick_bin(s_hist[2 * tid], s_hist[2 * tid + 1], need, b2, s_wave, s_pick, tid);
+      prefix |= b2 << shift;
+      mask |= bits << shift;
+    }
+  }
+  if (tid == 0) {
+    w.border[4 * bh + 2] = any ? prefix : 0xffffffffu;
+    w.border[4 * bh + 3] = any ? need : 0;
+  }
+  // rows of each chunk above the border (higher bins, and in the list) and at it
+  for (int c = wid; c < w.chunks; c += kHeavyWaves) {
+    uint32_t g = 0, e = 0;
+    if (any) {
+      const uint32_t* const h = w.hist + ((int64_t)bh * w.chunks + c) * kHeavyBins;
+      for (uint32_t i = bin + 1 + lane; i < kHeavyBins; i += 64) g += h[i];
+      const uint32_t fill = count[4 * c];
+      for (uint32_t i = lane; i < fill; i += 64) {
+        const uint32_t v = list[(int64_t)c * kChunk + i];
+        g += v > prefix ? 1 : 0;
+        e += v == prefix ? 1 : 0;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        g += (uint32_t)__shfl_xor((int)g, d, 64);
+        e += (uint32_t)__shfl_xor((int)e, d, 64);
+      }
+    }
+    if (lane == 0) {
+      count[4 * c + 1] = g;
+      count[4 * c + 2] = e;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heavy_index_kernel(HeavyArgs a, HeavyWork w) {
+  __shared__ uint32_t s_cnt[2][kChunkPer * kHeavyWaves];
+  __shared__ uint32_t s_before[2];
+  const int bh = blockIdx.x / w.chunks, c = blockIdx.x - bh * w.chunks;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int n = heavy_length(a, bh);
+  int32_t* const out = a.index + (int64_t)bh * a.budget;
+  const int first = c * kChunk;
+  if (n <= a.budget) {  // all rows, then -1 (the last chunk's workgroup writes what is past the chunks)
+    const int end = c == w.chunks - 1 ? a.budget : min(first + kChunk, a.budget);
+    for (int i = first + tid; i < end; i += kHeavyThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int lo = a.sinks, hi = n - a.recent;
+  const uint32_t border = w.border[4 * bh + 2], need = w.border[4 * bh + 3];
+  uint32_t u[kChunkPer];
+  bool in[kChunkPer];
+  chunk_masses(a, bh, first, lo, hi, u, in);
+  if (wid < 2) {  // rows above / at the border in the chunks before
+    uint32_t v = 0;
+    for (int i = lane; i < c; i += 64) v += w.count[((int64_t)bh * w.chunks + i) * 4 + 1 + wid];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += (uint32_t)__shfl_xor((int)v, d, 64);
+    if (lane == 0) s_before[wid] = v;
+  }
+  uint64_t bg[kChunkPer], be[kChunkPer];
+#pragma unroll
+  for (int j = 0; j < kChunkPer; ++j) {
+    bg[j] = __ballot(in[j] && u[j] > border);
+    be[j] = __ballot(in[j] && u[j] == border);
+    if (lane == 0) {
+      s_cnt[0][j * kHeavyWaves + wid] = (uint32_t)__popcll(bg[j]);
+      s_cnt[1][j * kHeavyWaves + wid] = (uint32_t)__popcll(be[j]);
+    }
+  }
+  __syncthreads();
+  if (wid < 2) {
+    const uint32_t own = s_cnt[wid][lane];
+    uint32_t inc = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t dn = (uint32_t)__shfl_up((int)inc, d, 64);
+      inc += lane >= d ? dn : 0;
+    }
+    s_cnt[wid][lane] = inc - own + s_before[wid];
+  }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int j = 0; j < kChunkPer; ++j) {
+    const int row = first + j * kHeavyThreads + tid;
+    const uint32_t g = s_cnt[0][j * kHeavyWaves + wid] + (uint32_t)__popcll(bg[j] & below);
+    const uint32_t e = s_cnt[1][j * kHeavyWaves + wid] + (uint32_t)__popcll(be[j] & below);
+    const bool gt = (bg[j] >> lane) & 1, eq = (be[j] >> lane) & 1;
+    if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = row;
+    else if (row < lo) out[row] = row;
+    else if (row >= hi && row < n) out[a.budget - n + row] = row;
+  }
+}
+static_assert(kChunkPer * kHeavyWaves == 64, "one count a lane");
 
 // ------------------------------------------------------------------------------------
 // eviction: the rows moved
@@ -505,14 +687,39 @@ static int check_budget(int64_t budget, int64_t sinks, int64_t recent, const cha
   return DA_OK;
 }
 
+// The choice's scratch for heads that may be longer than kHeavyShort rows, after `at`.
+static HeavyWork heavy_work(int64_t BH, int64_t capacity, uint32_t* at, int64_t* bytes) {
+  HeavyWork w = {};
+  w.chunks = capacity > kHeavyShort ? (int)((capacity + kChunk - 1) / kChunk) : 0;
+  const int64_t n = BH * w.chunks;
+  w.hist = at;
+  w.list = w.hist + n * kHeavyBins;
+  w.count = w.list + n * kChunk;
+  w.border = w.count + n * 4;
+  *bytes = (n * (kHeavyBins + kChunk + 4) + (n ? BH * 4 : 0)) * (int64_t)sizeof(uint32_t);
+  return w;
+}
+
 static int launch_heavy(const float* mass, const int32_t* lengths, int64_t BH, int64_t capacity, int64_t budget,
-                        int64_t sinks, int64_t recent, int32_t* index, int32_t* kept, hipStream_t st,
+                        int64_t sinks, int64_t recent, int32_t* index, int32_t* kept, void* workspace, hipStream_t st,
                         const char* who) {
   HeavyArgs a = {};
   a.mass = mass; a.lengths = lengths; a.capacity = capacity;
   a.budget = (int)budget; a.sinks = (int)sinks; a.recent = (int)recent;
   a.index = index; a.kept = kept;
-  hipLaunchKernelGGL(heavy_rows_kernel, dim3((unsigned)BH), dim3(kHeavyThreads), 0, st, a);
+  int64_t bytes;
+  const HeavyWork w = heavy_work(BH, capacity, (uint32_t*)workspace, &bytes);
+  if (w.chunks == 0) {
+    hipLaunchKernelGGL(heavy_rows_kernel, dim3((unsigned)BH), dim3(kHeavyThreads), 0, st, a);
+    return check_launch(who);
+  }
+  DA_REQUIRE(BH * w.chunks < (1ll << 31), "%s: more than 2^31 workgroups", who);
+  const dim3 all((unsigned)(BH * w.chunks)), heads((unsigned)BH);
+  hipLaunchKernelGGL(heavy_hist_kernel, all, dim3(kHeavyThreads), 0, st, a, w);
+  hipLaunchKernelGGL(heavy_bin_kernel, heads, dim3(kHeavyThreads), 0, st, a, w);
+  hipLaunchKernelGGL(heavy_list_kernel, all, dim3(kHeavyThreads), 0, st, a, w);
+  hipLaunchKernelGGL(heavy_border_kernel, heads, dim3(kHeavyThreads), 0, st, a, w);
+  hipLaunchKernelGGL(heavy_index_kernel, all, dim3(kHeavyThreads), 0, st, a, w);
   return check_launch(who);
 }
 
@@ -533,7 +740,9 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   DA_REQUIRE(N > 0 && N <= (1 << 26) && M > 0 && M <= out->capacity && (index || M == N),
              "%s: needs 0 < M <= capacity, and M = N without an index", who);
   const int64_t align = dtype == DA_F32 ? 3 : 7;
-  DA_REQUIRE(((sk_b | sk_h | sk_n | sv_b | sv_h | sv_n) & align) == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
+  // a dimension of one has no stride
+  const int64_t strides = (B > 1 ? sk_b | sv_b : 0) | (Hkv > 1 ? sk_h | sv_h : 0) | (N > 1 ? sk_n | sv_n : 0);
+  DA_REQUIRE((strides & align) == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
              "%s: rows must be 16-byte aligned", who);
   Quant4Args a = {};
   a.x[0] = k; a.s_b[0] = sk_b; a.s_h[0] = sk_h; a.s_n[0] = sk_n;
@@ -576,10 +785,12 @@ extern "C" int da_kv4_dequantize(const DaKv4* kv, int64_t B, int64_t Hkv, int64_
   return check_launch(who);
 }
 
-// The rows kept, [B, Hkv, budget].
+// The choice's scratch, then the rows kept, [B, Hkv, budget].
 extern "C" int64_t da_kv4_evict_workspace_size(int64_t B, int64_t Hkv, int64_t capacity, int64_t budget) {
-  (void)capacity;
-  return B * Hkv * budget * (int64_t)sizeof(int32_t);
+  if (B <= 0 || Hkv <= 0 || capacity <= 0 || budget <= 0) return 0;
+  int64_t bytes;
+  heavy_work(B * Hkv, capacity, nullptr, &bytes);
+  return bytes + B * Hkv * budget * (int64_t)sizeof(int32_t);
 }
 
 extern "C" int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, int64_t budget, int64_t sinks,
@@ -594,12 +805,15 @@ extern "C" int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, 
                  kv->counts != out->counts && kv->lengths != out->lengths,
              "%s: the rows move to other memory", who);
   const int64_t need = da_kv4_evict_workspace_size(B, Hkv, kv->capacity, budget);
-  if (!index && (!workspace || workspace_bytes < need))
+  if (!workspace || workspace_bytes < need)
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
-  int32_t* rows = index ? index : (int32_t*)workspace;
+  DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
+  int64_t scratch;
+  heavy_work(B * Hkv, kv->capacity, nullptr, &scratch);
+  int32_t* rows = index ? index : (int32_t*)((char*)workspace + scratch);
   hipStream_t st = (hipStream_t)stream;
   if (int rc = launch_heavy(kv->mass, kv->lengths, B * Hkv, kv->capacity, budget, sinks, recent, rows, out->lengths,
-                            st, who))
+                            workspace, st, who))
     return rc;
   Move4Args a = {};
   a.codes[0] = kv->k_codes; a.codes[1] = kv->v_codes;
@@ -624,10 +838,13 @@ extern "C" int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t 
                              int64_t budget, int64_t sinks, int64_t recent, int32_t* index, int32_t* kept,
                              void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = "da_heavy_rows";
-  (void)workspace;
-  (void)workspace_bytes;
   DA_REQUIRE(mass && index && kept, "%s: null pointer", who);
   DA_REQUIRE(B > 0 && Hkv > 0 && N > 0 && N <= (1 << 26) && B * Hkv <= 65535, "%s: bad shape", who);
   if (int rc = check_budget(budget, sinks, recent, who)) return rc;
-  return launch_heavy(mass, lengths, B * Hkv, N, budget, sinks, recent, index, kept, (hipStream_t)stream, who);
+  const int64_t need = da_kv4_evict_workspace_size(B, Hkv, N, budget);
+  if (!workspace || workspace_bytes < need)
+    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
+  DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
+  return launch_heavy(mass, lengths, B * Hkv, N, budget, sinks, recent, index, kept, workspace, (hipStream_t)stream,
+                      who);
 }

@@ -569,8 +569,10 @@ extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq,
   if (kv->capacity > (1 << 24)) return set_error(DA_ERR_UNSUPPORTED, "%s: capacity above 2^24 rows", who);
   DA_REQUIRE(exact_len == 0 || (k_exact && v_exact), "%s: null ring", who);
   const int64_t align = dtype == DA_F32 ? 3 : 7;
-  DA_REQUIRE(((sq_b | sq_h) & align) == 0 && ((uintptr_t)q & 15) == 0 &&
-                 (exact_len == 0 || (((sx_b | sx_h | sx_s) & align) == 0 && (((uintptr_t)k_exact | (uintptr_t)v_exact) & 15) == 0)),
+  // a dimension of one has no stride
+  const int64_t strides = (B > 1 ? sq_b | sx_b : 0) | (Hq > 1 ? sq_h : 0) | (Hkv > 1 ? sx_h : 0) | (exact_len > 1 ? sx_s : 0);
+  DA_REQUIRE((strides & align) == 0 && ((uintptr_t)q & 15) == 0 &&
+                 (exact_len == 0 || (((uintptr_t)k_exact | (uintptr_t)v_exact) & 15) == 0),
              "%s: q and ring rows must be 16-byte aligned", who);
   DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
   DA_REQUIRE(scale > 0.0f, "%s: scale must be positive", who);

@@ -522,7 +522,10 @@ extern "C" int da_attention_mass(const void* q, const void* k, int dtype, int64_
   if (Nk > (1 << 24) || Nq > (1 << 24) || B * Hkv > 65535)
     return set_error(DA_ERR_UNSUPPORTED, "%s: more than 2^24 keys or queries, or 65535 (sequence, head) pairs", who);
   const int64_t align = dtype == DA_F32 ? 3 : 7;
-  DA_REQUIRE(((sq_b | sq_h | sq_n | sk_b | sk_h | sk_n) & align) == 0 && (((uintptr_t)q | (uintptr_t)k) & 15) == 0,
+  // a dimension of one has no stride
+  const int64_t strides = (B > 1 ? sq_b | sk_b : 0) | (Hq > 1 ? sq_h : 0) | (Hkv > 1 ? sk_h : 0) | (Nq > 1 ? sq_n : 0) |
+                          (Nk > 1 ? sk_n : 0);
+  DA_REQUIRE((strides & align) == 0 && (((uintptr_t)q | (uintptr_t)k) & 15) == 0,
              "%s: rows must be 16-byte aligned", who);
   DA_REQUIRE(scale > 0.0f, "%s: scale must be positive", who);
   DA_REQUIRE(q_start > -(1ll << 40) && q_start < (1ll << 40), "%s: q_start out of range", who);

@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._native import Kv4Block, check, dtype_code, lib, on_device
+from ._native import Kv4Block, call_on, check, dtype_code, lib
 
 __all__ = ["KV4", "attention_mass", "heavy_rows", "quantize_kv4", "dequantize_kv4", "evict_kv4",
            "decode_attention_kv4"]
@@ -66,6 +66,11 @@ def _mass_bytes(*shape) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
+def _evict_bytes(*shape) -> int:
+    return lib().da_kv4_evict_workspace_size(*shape)
+
+
+@functools.lru_cache(maxsize=1024)
 def _attention_bytes(*shape) -> int:
     return lib().da_kv4_attention_workspace_size(*shape)
 
@@ -75,6 +80,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 _set = object.__setattr__
+_TENSORS = ("k_codes", "k_scales", "v_codes", "v_scales", "counts", "timestamps", "lengths", "mass")
 
 
 class KV4:
@@ -164,25 +170,30 @@ class KV4:
         self = cls.__new__(cls)
         self._put(B, H, cap, D, device, Kv4Block(
             p, p + 2 * codes, p + codes, p + 2 * codes + scales, p + at["counts"], p + at["timestamps"],
-            p + at["lengths"], p + at["mass"] if mass else None, cap), (own, at))
+            p + at["lengths"], p + at["mass"] if mass else None, cap), [at, own, None, None])
         return self
 
     def __getattr__(self, name):
         # only for what is not there yet: a tensor of a cache that empty() made
-        if name not in ("k_codes", "k_scales", "v_codes", "v_scales", "counts", "timestamps", "lengths", "mass"):
+        if name not in _TENSORS:
             raise AttributeError(name)
-        own, at = self._own
-        if name not in at:
-            t = None  # a cache without mass
+        at, own, ints, floats = self._own
+        first = at.get(name)
+        B, H, cap, g = self.batch, self.kv_heads, self.capacity, (self.head_dim + 31) // 32
+        if first is None:  # a cache without mass
+            t = None
+        elif name in ("counts", "timestamps", "lengths"):
+            if ints is None:
+                ints = self._own[2] = own.view(_I32)
+            t = ints.as_strided((B, H), (H, 1), first // 4) if name == "lengths" else \
+                ints.as_strided((B, H, cap), (H * cap, cap, 1), first // 4)
+        elif name == "mass":
+            if floats is None:
+                floats = self._own[3] = own.view(_F32)
+            t = floats.as_strided((B, H, cap), (H * cap, cap, 1), first // 4)
         else:
-            B, H, cap, g, first = self.batch, self.kv_heads, self.capacity, (self.head_dim + 31) // 32, at[name]
-            if name == "lengths":
-                t = own.view(_I32).as_strided((B, H), (H, 1), first // 4)
-            elif name in ("counts", "timestamps", "mass"):
-                t = own.view(_F32 if name == "mass" else _I32).as_strided((B, H, cap), (H * cap, cap, 1), first // 4)
-            else:
-                w = 16 * g if name.endswith("codes") else g
-                t = own.as_strided((B, H, cap, w), (H * cap * w, cap * w, w, 1), first)
+            w = 16 * g if name in ("k_codes", "v_codes") else g
+            t = own.as_strided((B, H, cap, w), (H * cap * w, cap * w, w, 1), first)
         _set(self, name, t)
         return t
 
@@ -226,12 +237,11 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tens
     q, k = _rows(q), _rows(k)
     n = _mass_bytes(B, Hq, H, Nq, N)
     ws = torch.empty((n,), dtype=_U8, device=device)
-    with on_device(device) as stream:
-        rc = lib().da_attention_mass(q.data_ptr(), k.data_ptr(), dt, B, Hq, H, Nq, N, D, *_strides(q), *_strides(k),
-                                     _ptr(counts), _ptr(timestamps), _ptr(lengths),
-                                     N - Nq if q_start is None else int(q_start),
-                                     D ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), n,
-                                     stream)
+    sq, sk = q.stride(), k.stride()
+    rc = call_on(device, lib().da_attention_mass, q.data_ptr(), k.data_ptr(), dt, B, Hq, H, Nq, N, D, sq[0], sq[1], sq[2],
+                 sk[0], sk[1], sk[2], _ptr(counts), _ptr(timestamps), _ptr(lengths),
+                 N - Nq if q_start is None else int(q_start), D ** -0.5 if scale is None else scale, out.data_ptr(),
+                 ws.data_ptr(), n)
     check(rc, "da_attention_mass")
     return out
 
@@ -255,11 +265,10 @@ def heavy_rows(mass: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
     budget, sinks, recent = _budget(budget, sinks, recent)
     index = torch.empty((B, H, budget), dtype=_I32, device=device)
     kept = torch.empty((B, H), dtype=_I32, device=device)
-    n = lib().da_kv4_evict_workspace_size(B, H, N, budget)
+    n = _evict_bytes(B, H, N, budget)
     ws = torch.empty((n,), dtype=_U8, device=device)
-    with on_device(device) as stream:
-        rc = lib().da_heavy_rows(mass.data_ptr(), _ptr(lengths), B, H, N, budget, sinks, recent, index.data_ptr(),
-                                 kept.data_ptr(), ws.data_ptr(), n, stream)
+    rc = call_on(device, lib().da_heavy_rows, mass.data_ptr(), _ptr(lengths), B, H, N, budget, sinks, recent,
+                 index.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
     check(rc, "da_heavy_rows")
     return index, kept
 
@@ -306,10 +315,9 @@ def quantize_kv4(k: torch.Tensor, v: torch.Tensor, counts: Optional[torch.Tensor
         raise ValueError(f"{M} rows do not fit a capacity of {capacity}")
     k, v = _rows(k), _rows(v)
     out = KV4.empty(B, H, capacity, D, device)
-    with on_device(device) as stream:
-        rc = lib().da_kv4_quantize(k.data_ptr(), v.data_ptr(), dt, B, H, N, D, *_strides(k), *_strides(v),
-                                   _ptr(counts), _ptr(timestamps), _ptr(mass), _ptr(lengths), _ptr(index), M, out._ref,
-                                   stream)
+    sk, sv = k.stride(), v.stride()
+    rc = call_on(device, lib().da_kv4_quantize, k.data_ptr(), v.data_ptr(), dt, B, H, N, D, sk[0], sk[1], sk[2], sv[0],
+                 sv[1], sv[2], _ptr(counts), _ptr(timestamps), _ptr(mass), _ptr(lengths), _ptr(index), M, out._ref)
     check(rc, "da_kv4_quantize")
     return out
 
@@ -323,8 +331,7 @@ def dequantize_kv4(kv: KV4, dtype: torch.dtype = torch.bfloat16, rows: Optional[
     shape = (kv.batch, kv.kv_heads, N, kv.head_dim)
     k, v = (torch.empty(shape, dtype=dtype, device=kv.device) for _ in range(2))
     dt = dtype_code(k)
-    with on_device(kv.device) as stream:
-        rc = lib().da_kv4_dequantize(kv._ref, *shape, k.data_ptr(), v.data_ptr(), dt, stream)
+    rc = call_on(kv.device, lib().da_kv4_dequantize, kv._ref, *shape, k.data_ptr(), v.data_ptr(), dt)
     check(rc, "da_kv4_dequantize")
     return k, v
 
@@ -342,10 +349,9 @@ def evict_kv4(kv: KV4, budget: int, sinks: int = 0, recent: int = 0, capacity: O
         raise ValueError(f"a budget of {budget} rows does not fit a capacity of {capacity}")
     B, H, cap, D, device = kv.batch, kv.kv_heads, kv.capacity, kv.head_dim, kv.device
     out = KV4.empty(B, H, capacity, D, device)
-    n = lib().da_kv4_evict_workspace_size(B, H, cap, budget)
+    n = _evict_bytes(B, H, cap, budget)
     ws = torch.empty((n,), dtype=_U8, device=device)
-    with on_device(device) as stream:
-        rc = lib().da_kv4_evict(kv._ref, B, H, D, budget, sinks, recent, out._ref, None, ws.data_ptr(), n, stream)
+    rc = call_on(device, lib().da_kv4_evict, kv._ref, B, H, D, budget, sinks, recent, out._ref, None, ws.data_ptr(), n)
     check(rc, "da_kv4_evict")
     return out
 
@@ -386,17 +392,17 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
             raise ValueError(f"k_exact and v_exact must be [{B}, {H}, W, {D}] on {device}")
         W = xs[2]
         if W:
-            k_exact, v_exact = _rows(k_exact), _rows(v_exact)
-            sx = _strides(k_exact)
-            if _strides(v_exact) != sx:
-                k_exact, v_exact = (t.clone(memory_format=torch.contiguous_format) for t in (k_exact, v_exact))
-                sx = _strides(k_exact)
+            if not (k_exact.is_contiguous() and v_exact.is_contiguous() and (k_exact.data_ptr() | v_exact.data_ptr()) % 16 == 0):
+                k_exact, v_exact = _rows(k_exact), _rows(v_exact)
+                if _strides(v_exact) != _strides(k_exact):
+                    k_exact, v_exact = (t.clone(memory_format=torch.contiguous_format) for t in (k_exact, v_exact))
+            sx = k_exact.stride()
         kx, vx = k_exact.data_ptr(), v_exact.data_ptr()
     n_exact = W if exact_len is None else int(exact_len)
     if not 0 <= n_exact <= W:
         raise ValueError(f"exact_len must lie in [0, {W}], got {n_exact}")
     q = _rows(q)
-    sq = _strides(q)
+    sq = q.stride()
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=device)
     elif out.shape != shape or out.device != device or out.stride(-1) != 1:
@@ -404,9 +410,8 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
     so = out.stride()
     n = _attention_bytes(B, Hq, H, kv.capacity, 1 if accumulate else 0)
     ws = torch.empty((n,), dtype=_U8, device=device)
-    with on_device(device) as stream:
-        rc = lib().da_kv4_attention(q.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, kx, vx, sx[0], sx[1], sx[2],
-                                    n_exact, D ** -0.5 if scale is None else scale, 1 if accumulate else 0,
-                                    out.data_ptr(), so[0], so[1], ws.data_ptr(), n, stream)
+    rc = call_on(device, lib().da_kv4_attention, q.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, kx, vx, sx[0],
+                 sx[1], sx[2], n_exact, D ** -0.5 if scale is None else scale, 1 if accumulate else 0, out.data_ptr(),
+                 so[0], so[1], ws.data_ptr(), n)
     check(rc, "da_kv4_attention")
     return out
