@@ -86,7 +86,9 @@ __device__ __forceinline__ f32x2 row_stats(float M, float L) {
 // keys).  The grid runs over (sequence, KV head), then the splits, then the column blocks, the
 // longest first; neighbours go to different XCDs, so one head's K and Q stay in few of their
 // caches.
-template <int DT, int PASS>
+// KK: k steps of 16 dims a score takes (2, 4, 6 or 8: the steps are not left to a run-time bound,
+// which costs a copy of the accumulators each).
+template <int DT, int PASS, int KK>
 __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   constexpr int NP = DT == DA_F32 ? 3 : 1;
   constexpr int NW = DT == DA_F32 ? 2 : 1;    // 16-byte loads of a chunk of 8 elements
@@ -115,7 +117,6 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   // rows pass: later queries see more keys; columns pass: earlier keys are seen by more queries
   const int block = PASS == 0 ? a.blocks - 1 - zb : zb;
   const int c0 = block * kCols;
-  const int KK = (a.D + 15) / 16;
   constexpr int es = DT == DA_F32 ? 4 : 2;
   const char* const qb = (const char*)a.q + (b * a.sq_b + (int64_t)g * G * a.sq_h) * es;
   const char* const kb = (const char*)a.k + (b * a.sk_b + g * a.sk_h) * es;
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   if (t_begin < t_end) load_tile(t_begin);
 
   // ---- the columns' operand and times ----
-  u32x4 x[NP][NCB][8];
+  u32x4 x[NP][NCB][KK];
   int ct[NCB];
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
       }
     }
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
+    for (int kk = 0; kk < KK; ++kk) {
       const int d = 16 * kk + 8 * hl;
 #pragma unroll
       for (int p = 0; p < NP; ++p) x[p][cb][kk] = u32x4{0, 0, 0, 0};
@@ -289,23 +290,21 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
         for (int r = 0; r < 16; ++r) s[cb][r] = 0.0f;
       const char* const yb = s_y[st] + (32 * half + cl) * kMRow;
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        if (kk < KK) {
-          u32x4 f[NP];
+      for (int kk = 0; kk < KK; ++kk) {
+        u32x4 f[NP];
 #pragma unroll
-          for (int p = 0; p < NP; ++p) f[p] = *(const u32x4*)(yb + p * kPart + (((2 * kk + hl) ^ (cl & 15)) << 4));
+        for (int p = 0; p < NP; ++p) f[p] = *(const u32x4*)(yb + p * kPart + (((2 * kk + hl) ^ (cl & 15)) << 4));
 #pragma unroll
-          for (int cb = 0; cb < NCB; ++cb) {
-            if constexpr (NP == 1) {
-              s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
-            } else {  // the smallest products first
-              s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
-              s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
-              s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
-              s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
-              s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
-              s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
-            }
+        for (int cb = 0; cb < NCB; ++cb) {
+          if constexpr (NP == 1) {
+            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
+          } else {  // the smallest products first
+            s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
+            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
           }
         }
       }
@@ -472,12 +471,22 @@ static MassPlan mass_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t
   return p;
 }
 
+template <int DT, int PASS>
+static void launch_pass(const MassArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.B * a.Hkv) * a.split * a.blocks);
+  switch ((a.D + 31) / 32) {
+    case 1: hipLaunchKernelGGL((mass_kernel<DT, PASS, 2>), grid, dim3(256), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((mass_kernel<DT, PASS, 4>), grid, dim3(256), 0, st, a); break;
+    case 3: hipLaunchKernelGGL((mass_kernel<DT, PASS, 6>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((mass_kernel<DT, PASS, 8>), grid, dim3(256), 0, st, a); break;
+  }
+}
 template <int DT>
 static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char* who) {
-  const unsigned bh = (unsigned)(a.B * a.Hkv);
+  const int64_t bh = (int64_t)a.B * a.Hkv;
   a.split = p.split0;
   a.blocks = (int)p.blocks0;
-  hipLaunchKernelGGL((mass_kernel<DT, 0>), dim3(bh * p.split0 * (unsigned)p.blocks0), dim3(256), 0, st, a);
+  launch_pass<DT, 0>(a, st);
   if (p.split0 > 1) {
     const int64_t rows = bh * p.rows;
     hipLaunchKernelGGL(mass_join_rows_kernel, dim3((unsigned)((rows * kJoinLanes + 255) / 256)), dim3(256), 0, st,
@@ -485,9 +494,9 @@ static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char
   }
   a.split = p.split1;
   a.blocks = (int)p.blocks1;
-  hipLaunchKernelGGL((mass_kernel<DT, 1>), dim3(bh * p.split1 * (unsigned)p.blocks1), dim3(256), 0, st, a);
+  launch_pass<DT, 1>(a, st);
   if (p.split1 > 1) {
-    const int64_t cols = (int64_t)bh * a.Nk;
+    const int64_t cols = bh * a.Nk;
     hipLaunchKernelGGL(mass_join_cols_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, st, a.part, a.mass,
                        cols, p.split1);
   }
