@@ -72,14 +72,18 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 // A lane takes 8 dims: 16 bytes of a 16-bit row (32 of an fp32 one), 4 bytes of codes; the
 // four lanes of a quad are one group, whose largest magnitude is two quad permutes away.
 // Lanes per row: 4 NG.  Each thread takes kQuantItems of them, a block's width apart, with
-// all of its loads in flight.  The grid runs over (sequence, head) first: neighbours read the
-// same rows' heads, which projections lay side by side.  blockIdx.y = key or value.
+// all of its loads in flight.  blockIdx.y = key or value.  Workgroups go to the XCDs in turn, so
+// eight row blocks are interleaved and the (sequence, head) pairs of one follow each other on one
+// XCD: where projections lay the heads of a token side by side, that XCD reads whole tokens (by
+// head, each L2 would see one 256-byte piece in 2 KiB, two of its 16 channels: 101 us a 64K-token
+// prompt against XXX).
 constexpr int kQuantItems = 4;
 template <int DT, int NG>
 __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
   constexpr uint32_t kLpr = 4 * NG;
-  const uint32_t nbh = a.B * a.H, blk = blockIdx.x / nbh;
-  const int bh = blockIdx.x - blk * nbh, z = blockIdx.y;
+  const uint32_t nbh = a.B * a.H, turn = blockIdx.x >> 3, eight = turn / nbh;
+  const uint32_t blk = 8 * eight + (blockIdx.x & 7);
+  const int bh = turn - eight * nbh, z = blockIdx.y;
   const int b = bh / a.H, h = bh - b * a.H;
   const uint32_t M = (uint32_t)a.M;
   uint32_t len = M;
@@ -426,6 +430,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_bin_kernel(HeavyArgs a, H
   if (n > a.budget && need > 0) {
     uint32_t c0 = 0, c1 = 0;
     const u32x2* h = (const u32x2*)(const void*)(w.hist + (int64_t)bh * w.chunks * kHeavyBins) + tid;
+#pragma unroll 8
     for (int c = 0; c < w.chunks; ++c) {
       const u32x2 v = h[(int64_t)c * (kHeavyBins / 2)];
       c0 += v[0];
@@ -509,6 +514,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_border_kernel(HeavyArgs a
     uint32_t g = 0, e = 0;
     if (any) {
       const uint32_t* const h = w.hist + ((int64_t)bh * w.chunks + c) * kHeavyBins;
+#pragma unroll 8
       for (uint32_t i = bin + 1 + lane; i < kHeavyBins; i += 64) g += h[i];
       const uint32_t fill = count[4 * c];
       for (uint32_t i = lane; i < fill; i += 64) {
@@ -611,7 +617,7 @@ struct Move4Args {
 
 // A lane moves 16 bytes of codes (2 NG lanes a row, keys then values) and the first lanes of
 // a row its small fields.
-constexpr int kMoveItems = 2;
+constexpr int kMoveItems = 4;
 template <int NG>
 __global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
   constexpr uint32_t kLpr = 2 * NG;
@@ -753,9 +759,9 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass; a.o_lengths = out->lengths;
   a.N = N; a.M = M; a.capacity = out->capacity; a.B = (int)B; a.H = (int)Hkv; a.D = (int)D;
   const int groups = (int)((D + 31) / 32);
-  const int64_t blocks = (M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems);
+  const int64_t blocks = ((M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems) + 7) / 8 * 8;
   DA_REQUIRE(blocks * B * Hkv < (1ll << 31), "%s: more than 2^31 workgroups", who);
-  const dim3 grid((unsigned)(blocks * B * Hkv), 2);
+  const dim3 grid((unsigned)(blocks * B * Hkv), 2);  // blocks: a multiple of eight
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) launch_quantize<DA_F32>(a, groups, grid, st);
   else if (dtype == DA_F16) launch_quantize<DA_F16>(a, groups, grid, st);

@@ -144,29 +144,38 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   const int t_end = min(t_begin + per, tile_lo + ntile);
 
   // ---- staging: 16 chunks of 8 elements a row, thread: rows tid / 16 + 16 u, chunk tid % 16 ----
+  // Where a stage's rows are at a fixed distance from the last one's (keys; queries of a group
+  // that divides a stage) the addresses are stepped, else formed again.  The waves take turns with
+  // the rows' times and weights.
   const int sr = tid >> 4, sc = tid & 15;
+  const bool chunk = 8 * sc < a.D;  // chunks past the head dimension stay zero
+  const bool stepped = PASS == 0 || a.gshift >= 0;
+  const int64_t step = (PASS == 0 ? kTile * a.sk_n : (int64_t)(kTile >> (a.gshift >= 0 ? a.gshift : 0)) * a.sq_n) * es;
+  auto row_src = [&](int row) {
+    if (PASS == 0) return kb + row * a.sk_n * es;
+    const int i = query_of(a, row), h = row - i * G;
+    return qb + (h * a.sq_h + i * a.sq_n) * es;
+  };
+  const char* src[NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) src[u] = row_src(t_begin * kTile + sr + 16 * u) + 8 * es * sc;
   u32x4 y[NU][NW];
   float m_add = 0.0f, m_mul = 0.0f;
   int m_t = 0;
   auto load_tile = [&](int tile) {
+    const int row0 = tile * kTile + sr;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int row = tile * kTile + sr + 16 * u;
+      if (!stepped) src[u] = row_src(row0 + 16 * u) + 8 * es * sc;
 #pragma unroll
       for (int w = 0; w < NW; ++w) y[u][w] = u32x4{0, 0, 0, 0};
-      if (row < nrow && 8 * sc < a.D) {
-        const char* src;
-        if (PASS == 0) {
-          src = kb + row * a.sk_n * es;
-        } else {
-          const int i = query_of(a, row), h = row - i * G;
-          src = qb + (h * a.sq_h + i * a.sq_n) * es;
-        }
+      if (chunk && row0 + 16 * u < nrow) {
 #pragma unroll
-        for (int w = 0; w < NW; ++w) y[u][w] = *(const u32x4*)(src + 8 * es * sc + 16 * w);
+        for (int w = 0; w < NW; ++w) y[u][w] = *(const u32x4*)(src[u] + 16 * w);
       }
+      src[u] += step;
     }
-    if (wid == 0 && lane < kTile) {
+    if (wid == (tile & 3) && lane < kTile) {
       const int row = tile * kTile + lane;
       m_add = -INFINITY;
       m_mul = 0.0f;
@@ -189,21 +198,23 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   // An extreme time of the columns, to decide for whole tiles: rows pass, the earliest query (keys
   // at or before it need no mask); columns pass, the latest key.
   int ext = PASS == 0 ? mass_pos(a, query_of(a, c0)) : c_last;
-  auto store_tile = [&](int st) {
+  auto store_tile = [&](int st, int tile) {
+    char* const at0 = s_y[st] + sr * kMRow + ((sc ^ sr) << 4);  // row % 16 is sr
+    if (chunk) {
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int row = sr + 16 * u;
-      char* const at = s_y[st] + row * kMRow + ((sc ^ (row & 15)) << 4);
-      if constexpr (DT == DA_F32) {
-        u32x4 w[NP];
-        cut_chunk<NP>(__builtin_bit_cast(f32x4, y[u][0]), __builtin_bit_cast(f32x4, y[u][1]), w);
+      for (int u = 0; u < NU; ++u) {
+        char* const at = at0 + 16 * u * kMRow;
+        if constexpr (DT == DA_F32) {
+          u32x4 w[NP];
+          cut_chunk<NP>(__builtin_bit_cast(f32x4, y[u][0]), __builtin_bit_cast(f32x4, y[u][1]), w);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) *(u32x4*)(at + p * kPart) = w[p];
-      } else {
-        *(u32x4*)at = y[u][0];
+          for (int p = 0; p < NP; ++p) *(u32x4*)(at + p * kPart) = w[p];
+        } else {
+          *(u32x4*)at = y[u][0];
+        }
       }
     }
-    if (wid == 0) {
+    if (wid == (tile & 3)) {
       // bit 0 (rows pass): a key has a weight other than 1; bit 1: a row that some column may not see
       const bool mine = lane < kTile;
       if (mine) {
@@ -216,6 +227,11 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
       if (lane == 0) s_flag[st] = (odd ? 1 : 0) | (late ? 2 : 0);
     }
   };
+  if (!chunk) {
+#pragma unroll
+    for (int i = 0; i < 2 * NP * NU; ++i)
+      *(u32x4*)(&s_y[0][0] + (16 * i + sr) * kMRow + ((sc ^ sr) << 4)) = u32x4{0, 0, 0, 0};
+  }
   if (t_begin < t_end) load_tile(t_begin);
 
   // ---- the columns' operand and times ----
@@ -273,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   }
   const float c2 = a.scale_log2;
 
-  if (t_begin < t_end) store_tile(0);
+  if (t_begin < t_end) store_tile(0, t_begin);
   __syncthreads();
   for (int tile = t_begin; tile < t_end; ++tile) {
     const int st = (tile - t_begin) & 1;
@@ -380,7 +396,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
         }
       }
     }
-    if (next) store_tile(st ^ 1);
+    if (next) store_tile(st ^ 1, tile + 1);
     __syncthreads();
   }
 
