@@ -31,18 +31,19 @@ struct Quant4Args {
   int B, H, D;
 };
 
-// Eight consecutive elements of a row, as fp32.
+// Eight consecutive elements of a row, as fp32.  The rows are read once: they pass the caches by.
 template <int DT>
 __device__ __forceinline__ void load8(const void* row, int64_t at, float (&x)[8]) {
   if constexpr (DT == DA_F32) {
-    const f32x4 a = *(const f32x4*)((const float*)row + at), b = *(const f32x4*)((const float*)row + at + 4);
+    const f32x4 a = __builtin_nontemporal_load((const f32x4*)((const float*)row + at));
+    const f32x4 b = __builtin_nontemporal_load((const f32x4*)((const float*)row + at + 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[i] = a[i];
       x[4 + i] = b[i];
     }
   } else {
-    const u32x4 w = *(const u32x4*)((const uint16_t*)row + at);
+    const u32x4 w = __builtin_nontemporal_load((const u32x4*)((const uint16_t*)row + at));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[2 * i] = E16<DT>::lo(w[i]);
@@ -77,7 +78,7 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 // XCD: where projections lay the heads of a token side by side, that XCD reads whole tokens (by
 // head, each L2 would see one 256-byte piece in 2 KiB, two of its 16 channels: 101 us a 64K-token
 // prompt against XXX).
-constexpr int kQuantItems = 4;
+constexpr int kQuantItems = 2;
 template <int DT, int NG>
 __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
   constexpr uint32_t kLpr = 4 * NG;
@@ -617,7 +618,7 @@ struct Move4Args {
 
 // A lane moves 16 bytes of codes (2 NG lanes a row, keys then values) and the first lanes of
 // a row its small fields.
-constexpr int kMoveItems = 4;
+constexpr int kMoveItems = 2;
 template <int NG>
 __global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
   constexpr uint32_t kLpr = 2 * NG;

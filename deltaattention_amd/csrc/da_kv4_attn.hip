@@ -56,14 +56,15 @@ struct Attn4Args {
   void* out;
   int64_t so_b, so_h;
   float* mass;
-  float* part;   // [bh][G][nsplit][2 + 128]: max and sum (log2 units), P.V
+  float* part;   // [bh][G][nsplit][128]: P.V
+  float* stat;   // [bh][G][nsplit][2]: max (log2 units) and sum
   float* score;  // [bh][G][score_cap]: scores (log2 units), where the weights are wanted
   int64_t score_cap;
   int nsplit;
   int B, Hkv, G, D;
 };
 
-constexpr int kA4Part = 2 + 128;
+constexpr int kA4Part = 128;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -83,14 +84,18 @@ __device__ __forceinline__ u32x4 fp4_to_bf16x8(uint32_t w, float scale) {
                fp4_to_bf16x2<3>(w, scale)};
 }
 
-// max / sum over the four lanes l % 16 + 16 t
+// max / sum over the four lanes l % 16 + 16 t, in registers
 __device__ __forceinline__ float cols_max(float v) {
-  v = __builtin_fmaxf(v, __shfl_xor(v, 16, 64));
-  return __builtin_fmaxf(v, __shfl_xor(v, 32, 64));
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __builtin_fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 __device__ __forceinline__ float cols_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
 }
 
 // Two fp32 values into N words of bf16 pairs, largest part first.
@@ -193,13 +198,9 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
   const int t_begin = min(split * per, tiles), t_end = min(t_begin + per, tiles);
   const int nwave = a.nsplit * kA4Waves;
   const int rfirst = nwave - 1 - (split * kA4Waves + wid);
-  float* const part = a.part + (((int64_t)bh * a.G + h0) * a.nsplit + split) * kA4Part;
-  const int64_t pstride = (int64_t)a.nsplit * kA4Part;
+  const int64_t head_part = ((int64_t)bh * a.G + h0) * a.nsplit + split;  // of column 0; nsplit a column
   if (t_begin >= t_end && nwave - 1 - (split * kA4Waves + kA4Waves - 1) >= rtiles) {  // nothing to do
-    if (tid < cols) {
-      part[tid * pstride] = -INFINITY;
-      part[tid * pstride + 1] = 0.0f;
-    }
+    if (tid < cols) *(f32x2*)(void*)(a.stat + 2 * (head_part + (int64_t)tid * a.nsplit)) = f32x2{-INFINITY, 0.0f};
     return;
   }
 
@@ -217,8 +218,8 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int64_t at = (int64_t)min(j0 + 16 * u + r, n - 1) * NG + tg;
-      x.kc[u] = *(const u32x4*)(kc0 + at * 16);
-      x.vc[u] = *(const u32x4*)(vc0 + at * 16);
+      x.kc[u] = __builtin_nontemporal_load((const u32x4*)(kc0 + at * 16));
+      x.vc[u] = __builtin_nontemporal_load((const u32x4*)(vc0 + at * 16));
       x.ks[u] = ks0[at];
       x.vs[u] = vs0[at];
     }
@@ -231,10 +232,11 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
   float m_run = -INFINITY, l_run = 0.0f;
-  // a new maximum: what was summed shrinks by 2^(old - new)
+  // a new maximum: what was summed shrinks by 2^(old - new).  Everything is in fp32 (and p's parts
+  // keep their relative precision), so the maximum moves only where p would pass 2^16.
   auto raise = [&](float mx) {
     mx = cols_max(mx);
-    if (__ballot(mx > m_run)) {
+    if (__ballot(mx > m_run + 16.0f)) {
       const float m_new = __builtin_fmaxf(mx, m_run);
       const float f = is_neg_inf(m_run) ? 0.0f : exp2_hw(m_run - m_new);
       l_run *= f;
@@ -311,8 +313,10 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
     f32x4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float ksc = __uint_as_float(cur.ks[u] << 23), vsc = __uint_as_float(cur.vs[u] << 23);
+      // a row without weight as good as zeros (its codes times 2^-127), whatever it holds: its score
+      // is then finite, its weight 0
       const bool live = !is_neg_inf(bias[16 * u + r]);
+      const float ksc = __uint_as_float(live ? cur.ks[u] << 23 : 0u), vsc = __uint_as_float(live ? cur.vs[u] << 23 : 0u);
       s[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
@@ -320,9 +324,8 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
         if (NG < 4 && !grp) kf = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = QP - 1; i >= 0; --i) s[u] = mfma16(kf, qf[i][m], s[u]);
-        // V to LDS as bf16; a row without weight as zeros, whatever it holds
-        u32x4 v = fp4_to_bf16x8(cur.vc[u][m], vsc);
-        if (!live) v = u32x4{0, 0, 0, 0};
+        // V to LDS as bf16
+        const u32x4 v = fp4_to_bf16x8(cur.vc[u][m], vsc);
         if (grp) *(u32x4*)(vt + (16 * u + r) * kA4VRow + 64 * t + 16 * m) = v;
       }
     }
@@ -333,7 +336,7 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
       const f32x4 add = *(const f32x4*)(bias + 16 * u + 4 * t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[u][i] = is_neg_inf(add[i]) ? -INFINITY : __builtin_fmaf(s[u][i], a.scale_log2, add[i]);
+        s[u][i] = __builtin_fmaf(s[u][i], a.scale_log2, add[i]);
         mx = __builtin_fmaxf(mx, s[u][i]);
       }
     }
@@ -401,26 +404,24 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
       o += f * ((const float*)(const void*)s_v[w])[c * kRow + d];
       L += f * s_ml[w][1][c];
     }
-    part[c * pstride + 2 + d] = o;
-    if (d == 0) {
-      part[c * pstride] = M;
-      part[c * pstride + 1] = L;
-    }
+    const int64_t to = head_part + (int64_t)c * a.nsplit;
+    a.part[to * kA4Part + d] = o;
+    if (d == 0) *(f32x2*)(void*)(a.stat + 2 * to) = f32x2{M, L};
   }
 }
 
 // Blocks [0, B Hq): one query head's splits joined, 32 lanes of four dims each, eight splits at a
-// time.  Blocks from there on add the weights: kMassKeys keys of one (sequence, KV head) each,
-// after the group's maxima and sums over the splits.
+// time with four in flight.  Blocks from there on add the weights: kMassKeys keys of one
+// (sequence, KV head) each, after the group's maxima and sums over the splits.
 constexpr int kMassKeys = 1024;
 // (max, sum) of a query head over the splits, by one wave
-__device__ __forceinline__ void join_stats(const float* part, int nsplit, int lane, float& m, float& l) {
+__device__ __forceinline__ void join_stats(const float* stat, int nsplit, int lane, float& m, float& l) {
   m = -INFINITY;
   l = 0.0f;
   for (int s = lane; s < nsplit; s += 64) {
-    const float ms = part[(int64_t)s * kA4Part], ls = part[(int64_t)s * kA4Part + 1];
-    const float mm = __builtin_fmaxf(m, ms), base = is_neg_inf(mm) ? 0.0f : mm;
-    l = l * exp2_hw(m - base) + ls * exp2_hw(ms - base);
+    const f32x2 v = *(const f32x2*)(const void*)(stat + 2 * s);
+    const float mm = __builtin_fmaxf(m, v[0]), base = is_neg_inf(mm) ? 0.0f : mm;
+    l = l * exp2_hw(m - base) + v[1] * exp2_hw(v[0] - base);
     m = mm;
   }
 #pragma unroll
@@ -441,29 +442,40 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
   if (!MASS || (int)blockIdx.x < heads) {
     const int bhq = blockIdx.x, b = bhq / Hq, hq = bhq - b * Hq;
     const float* part = a.part + (int64_t)bhq * a.nsplit * kA4Part;
+    const float* stat = a.stat + (int64_t)bhq * a.nsplit * 2;
     const int c = tid & 31, sg = tid >> 5;  // dims 4 c .. 4 c + 3, splits sg, sg + 8, ...
+    const int cd = 4 * c < a.D ? 4 * c : 0;
+    f32x4 v[4];
+    float ms[4];
+    auto load = [&](int s0) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = min(s0 + 8 * u, a.nsplit - 1);
+        ms[u] = s0 + 8 * u < a.nsplit ? stat[2 * s] : -INFINITY;
+        v[u] = *(const f32x4*)(part + (int64_t)s * kA4Part + cd);
+      }
+    };
+    load(sg);
     float M, L;
-    join_stats(part, a.nsplit, lane, M, L);
+    join_stats(stat, a.nsplit, lane, M, L);
     const float base = is_neg_inf(M) ? 0.0f : M;
     f32x4 o = f32x4{0, 0, 0, 0};
-    for (int s = sg; s < a.nsplit; s += 8) {
-      const float m = part[(int64_t)s * kA4Part];
-      if (is_neg_inf(m) || 4 * c >= a.D) continue;  // an empty split wrote no sums
-      const float f = exp2_hw(m - base);
-      const f32x2 v0 = *(const f32x2*)(part + (int64_t)s * kA4Part + 2 + 4 * c);
-      const f32x2 v1 = *(const f32x2*)(part + (int64_t)s * kA4Part + 4 + 4 * c);
-      o += f32x4{v0[0], v0[1], v1[0], v1[1]} * f;
+    for (int s0 = sg; s0 < a.nsplit; s0 += 32) {
+      if (s0 != sg) load(s0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (!is_neg_inf(ms[u])) o += v[u] * exp2_hw(ms[u] - base);  // an empty split wrote no sums
     }
     s_o[sg][c] = o;
     __syncthreads();
     if (tid < a.D) {
-      float v = 0.0f;
+      float w = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) v += ((const float*)(const void*)s_o[s])[tid];
-      v = zero_bits(L) ? 0.0f : v / L;
+      for (int s = 0; s < 8; ++s) w += ((const float*)(const void*)s_o[s])[tid];
+      w = zero_bits(L) ? 0.0f : w / L;
       const int64_t at = b * a.so_b + hq * a.so_h + tid;
-      if constexpr (DT == DA_F32) ((float*)a.out)[at] = v;
-      else ((uint16_t*)a.out)[at] = E16<DT>::bits(v);
+      if constexpr (DT == DA_F32) ((float*)a.out)[at] = w;
+      else ((uint16_t*)a.out)[at] = E16<DT>::bits(w);
     }
     return;
   }
@@ -476,7 +488,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
     if (first >= n) return;
     for (int h = wid; h < a.G; h += 4) {
       float m, l;
-      join_stats(a.part + ((int64_t)bh * a.G + h) * a.nsplit * kA4Part, a.nsplit, lane, m, l);
+      join_stats(a.stat + ((int64_t)bh * a.G + h) * a.nsplit * 2, a.nsplit, lane, m, l);
       if (lane == 0) {
         s_m[h] = is_neg_inf(m) ? 0.0f : m;
         s_l[h] = zero_bits(l) ? 0.0f : 1.0f / l;
@@ -505,8 +517,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
 static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
   const int64_t units = B * Hkv * ((G + kA4Cols - 1) / kA4Cols);
   const int64_t most = (capacity + kA4Tile * kA4Waves - 1) / (kA4Tile * kA4Waves);
-  int64_t want = (1024 + units - 1) / units;
-  if (want > 128) want = 128;
+  int64_t want = (768 + units - 1) / units;
+  if (want > 64) want = 64;
   if (want > most) want = most;
   return (int)(want < 1 ? 1 : want);
 }
@@ -541,13 +553,14 @@ static int launch_attn4(const Attn4Args& a, bool mass, hipStream_t st, const cha
 
 using namespace da;
 
-// The splits' partials, then (accumulate) the scores.
+// The splits' P.V and statistics, then (accumulate) the scores.
+static int64_t kv4_stat_floats(int64_t n) { return (2 * n + 3) / 4 * 4; }
 extern "C" int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t capacity,
                                                    int accumulate) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || capacity <= 0) return 0;
-  const int64_t parts = B * Hq * kv4_splits(B, Hkv, Hq / Hkv, capacity) * kA4Part;
+  const int64_t n = B * Hq * kv4_splits(B, Hkv, Hq / Hkv, capacity);
   const int64_t scores = accumulate ? B * Hq * kv4_score_cap(capacity) : 0;
-  return ((parts + 3) / 4 * 4 + scores) * (int64_t)sizeof(float);
+  return (n * kA4Part + kv4_stat_floats(n) + scores) * (int64_t)sizeof(float);
 }
 
 extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t sq_b,
@@ -591,7 +604,9 @@ extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq,
   a.nsplit = kv4_splits(B, Hkv, a.G, kv->capacity);
   a.part = (float*)workspace;
   a.score_cap = kv4_score_cap(kv->capacity);
-  a.score = a.part + (B * Hq * a.nsplit * (int64_t)kA4Part + 3) / 4 * 4;
+  const int64_t n = B * Hq * a.nsplit;
+  a.stat = a.part + n * kA4Part;
+  a.score = a.stat + kv4_stat_floats(n);
   const unsigned long long blocks = (unsigned long long)(B * Hq) + (unsigned long long)(B * Hkv) * ((kv->capacity + kMassKeys - 1) / kMassKeys);
   DA_REQUIRE(B * Hkv < (1ll << 31) && blocks < (1ull << 31), "%s: too many heads", who);
   hipStream_t st = (hipStream_t)stream;
