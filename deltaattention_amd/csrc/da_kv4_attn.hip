@@ -32,7 +32,7 @@ namespace da {
 
 typedef short i16x4v __attribute__((ext_vector_type(4)));
 
-constexpr int kA4Waves = 4;
+constexpr int kA4Waves = 4;                 // of a split's workgroup
 constexpr int kA4Tile = 32;                 // keys a wave takes at once
 constexpr int kA4VRow = 128 * 2 + 16;       // bytes of a bf16 V row in LDS, padded off the banks
 constexpr int kA4Cols = 16;                 // query heads of one workgroup
@@ -140,6 +140,15 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
+// Dim d of a query head: the weighted sum over the weights' sum, 0 where no key has a weight.
+template <int DT>
+__device__ __forceinline__ void store_out(const Attn4Args& a, int b, int hq, int d, float o, float L) {
+  const float v = zero_bits(L) ? 0.0f : o / L;
+  const int64_t at = b * a.so_b + hq * a.so_h + d;
+  if constexpr (DT == DA_F32) ((float*)a.out)[at] = v;
+  else ((uint16_t*)a.out)[at] = E16<DT>::bits(v);
+}
+
 // What a wave loads of 32 rows: lane (r, t) group t of rows r and 16 + r, and row lane % 32's count.
 struct Tile4 {
   u32x4 kc[2], vc[2];
@@ -148,17 +157,23 @@ struct Tile4 {
 };
 
 // One workgroup: (sequence, KV head) blockIdx.x, split blockIdx.y, heads 16 z .. of the group.
-template <int DT, int NG, bool MASS>
-__global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Attn4Args a) {
+// MODE kParts: `nsplit` workgroups a head leave their partials; kScores: and the scores; kWhole: one
+// workgroup of eight waves takes the head and writes the output itself.
+enum Mode4 : int { kParts = 0, kScores = 1, kWhole = 2 };
+template <int DT, int NG, int MODE>
+__global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(
+    Attn4Args a) {
+  constexpr bool MASS = MODE == kScores;
+  constexpr int NW = MODE == kWhole ? 8 : kA4Waves;
   constexpr int QP = DT == DA_BF16 ? 1 : DT == DA_F16 ? 2 : 3;
   constexpr int PP = DT == DA_F32 ? 3 : 2;
   constexpr int NJ = 2 * NG;  // output tiles of 16 dims
   constexpr int kTileBytes = kA4Tile * kA4VRow;
   constexpr int kRingRow = 128 + 4;  // floats of a ring row in LDS
   static_assert(16 * kRingRow * 4 <= kTileBytes, "16 ring rows must fit a wave's tile");
-  __shared__ __attribute__((aligned(16))) char s_v[kA4Waves][kTileBytes];
-  __shared__ __attribute__((aligned(16))) float s_bias[kA4Waves][kA4Tile];
-  __shared__ float s_ml[kA4Waves][2][kA4Cols];
+  __shared__ __attribute__((aligned(16))) char s_v[NW][kTileBytes];
+  __shared__ __attribute__((aligned(16))) float s_bias[NW][kA4Tile];
+  __shared__ float s_ml[NW][2][kA4Cols];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, t = lane >> 4;
   const int bh = blockIdx.x, split = blockIdx.y;
@@ -196,10 +211,10 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
   // the last one on
   const int per = (tiles + a.nsplit - 1) / a.nsplit;
   const int t_begin = min(split * per, tiles), t_end = min(t_begin + per, tiles);
-  const int nwave = a.nsplit * kA4Waves;
-  const int rfirst = nwave - 1 - (split * kA4Waves + wid);
+  const int nwave = a.nsplit * NW;
+  const int rfirst = nwave - 1 - (split * NW + wid);
   const int64_t head_part = ((int64_t)bh * a.G + h0) * a.nsplit + split;  // of column 0; nsplit a column
-  if (t_begin >= t_end && nwave - 1 - (split * kA4Waves + kA4Waves - 1) >= rtiles) {  // nothing to do
+  if (MODE != kWhole && t_begin >= t_end && nwave - 1 - (split * NW + NW - 1) >= rtiles) {  // nothing to do
     if (tid < cols) *(f32x2*)(void*)(a.stat + 2 * (head_part + (int64_t)tid * a.nsplit)) = f32x2{-INFINITY, 0.0f};
     return;
   }
@@ -302,10 +317,10 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
 
   // ---- the rows, 32 at a time, the next tile's loads under this one's work ----
   float* const score = MASS ? a.score + ((int64_t)bh * a.G + h0 + (have ? r : 0)) * a.score_cap : nullptr;
-  for (int tile = t_begin + wid; tile < t_end; tile += kA4Waves) {
+  for (int tile = t_begin + wid; tile < t_end; tile += NW) {
     const int j0 = tile * kA4Tile;
     Tile4 nxt;
-    if (tile + kA4Waves < t_end) load_tile(tile + kA4Waves, nxt);
+    if (tile + NW < t_end) load_tile(tile + NW, nxt);
     // log2(count), or -inf for a row without weight, once a row
     if (lane < kA4Tile)
       bias[lane] = cur.count > 0 && j0 + lane < n ? __builtin_amdgcn_logf((float)cur.count) : -INFINITY;
@@ -391,22 +406,26 @@ __global__ __launch_bounds__(256, DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(Att
 #pragma unroll
   for (int j = 0; j < NJ; ++j) *(f32x4*)(so + r * kRow + 16 * j + 4 * t) = acc[j];
   __syncthreads();
-  for (int i = tid; i < cols * 16 * NJ; i += 256) {
+  for (int i = tid; i < cols * 16 * NJ; i += 64 * NW) {
     const int c = i / (16 * NJ), d = i - c * (16 * NJ);
     float M = s_ml[0][0][c];
 #pragma unroll
-    for (int w = 1; w < kA4Waves; ++w) M = __builtin_fmaxf(M, s_ml[w][0][c]);
+    for (int w = 1; w < NW; ++w) M = __builtin_fmaxf(M, s_ml[w][0][c]);
     const float base = M == -INFINITY ? 0.0f : M;
     float o = 0.0f, L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kA4Waves; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = exp2_hw(s_ml[w][0][c] - base);
       o += f * ((const float*)(const void*)s_v[w])[c * kRow + d];
       L += f * s_ml[w][1][c];
     }
-    const int64_t to = head_part + (int64_t)c * a.nsplit;
-    a.part[to * kA4Part + d] = o;
-    if (d == 0) *(f32x2*)(void*)(a.stat + 2 * to) = f32x2{M, L};
+    if (MODE == kWhole) {
+      if (d < a.D) store_out<DT>(a, b, g * a.G + h0 + c, d, o, L);
+    } else {
+      const int64_t to = head_part + (int64_t)c * a.nsplit;
+      a.part[to * kA4Part + d] = o;
+      if (d == 0) *(f32x2*)(void*)(a.stat + 2 * to) = f32x2{M, L};
+    }
   }
 }
 
@@ -472,10 +491,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
       float w = 0.0f;
 #pragma unroll
       for (int s = 0; s < 8; ++s) w += ((const float*)(const void*)s_o[s])[tid];
-      w = zero_bits(L) ? 0.0f : w / L;
-      const int64_t at = b * a.so_b + hq * a.so_h + tid;
-      if constexpr (DT == DA_F32) ((float*)a.out)[at] = w;
-      else ((uint16_t*)a.out)[at] = E16<DT>::bits(w);
+      store_out<DT>(a, b, hq, tid, w, L);
     }
     return;
   }
@@ -512,10 +528,14 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
   }
 }
 
-// Workgroups of the attention launch: enough to fill the chip's 256 CUs a few times over, and
-// no split shorter than one tile a wave.
+// Workgroups of the attention launch: three a CU run at once (its registers), and no split is
+// shorter than a tile a wave; 64 splits are the most that pay their joining (8297 rows x 8 heads:
+// 64 10.2 us, 32 11.8).  A short cache is one workgroup of eight waves a head, without a second
+// launch (8 heads, 500 rows: 8.1 against 9.2 us, 750: 9.7 / 9.3, 1000: 10.9 / 9.2; a launch is 3.4 us
+// of the caller's time as well); 256 heads fill the chip like that (1000 rows: 15.4 / 20.0).
 static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
   const int64_t units = B * Hkv * ((G + kA4Cols - 1) / kA4Cols);
+  if (capacity <= (units >= 256 ? 1024 : 768)) return 1;
   const int64_t most = (capacity + kA4Tile * kA4Waves - 1) / (kA4Tile * kA4Waves);
   int64_t want = (768 + units - 1) / units;
   if (want > 64) want = 64;
@@ -525,20 +545,22 @@ static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
 static int64_t kv4_score_cap(int64_t capacity) { return (capacity + kA4Tile - 1) / kA4Tile * kA4Tile; }
 
 template <int DT, int NG>
-static void launch_attn4_ng(const Attn4Args& a, dim3 grid, bool mass, hipStream_t st) {
-  if (mass) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, false>), grid, dim3(256), 0, st, a);
+static void launch_attn4_ng(const Attn4Args& a, dim3 grid, int mode, hipStream_t st) {
+  if (mode == kWhole) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kWhole>), grid, dim3(512), 0, st, a);
+  else if (mode == kScores) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kScores>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kParts>), grid, dim3(256), 0, st, a);
 }
 template <int DT>
 static int launch_attn4(const Attn4Args& a, bool mass, hipStream_t st, const char* who) {
   const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)a.nsplit, (unsigned)((a.G + kA4Cols - 1) / kA4Cols));
+  const int mode = mass ? kScores : a.nsplit == 1 ? kWhole : kParts;
   switch ((a.D + 31) / 32) {
-    case 1: launch_attn4_ng<DT, 1>(a, grid, mass, st); break;
-    case 2: launch_attn4_ng<DT, 2>(a, grid, mass, st); break;
-    case 3: launch_attn4_ng<DT, 3>(a, grid, mass, st); break;
-    default: launch_attn4_ng<DT, 4>(a, grid, mass, st); break;
+    case 1: launch_attn4_ng<DT, 1>(a, grid, mode, st); break;
+    case 2: launch_attn4_ng<DT, 2>(a, grid, mode, st); break;
+    case 3: launch_attn4_ng<DT, 3>(a, grid, mode, st); break;
+    default: launch_attn4_ng<DT, 4>(a, grid, mode, st); break;
   }
-  if (int rc = check_launch(who)) return rc;
+  if (mode == kWhole) return check_launch(who);
   const unsigned heads = (unsigned)(a.B * a.Hkv * a.G);
   if (mass) {
     const unsigned chunks = (unsigned)((a.capacity + kMassKeys - 1) / kMassKeys);
