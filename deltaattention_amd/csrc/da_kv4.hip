@@ -73,7 +73,8 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 // A lane takes 8 dims: 16 bytes of a 16-bit row (32 of an fp32 one), 4 bytes of codes; the
 // four lanes of a quad are one group, whose largest magnitude is two quad permutes away.
 // Lanes per row: 4 NG.  Each thread takes kQuantItems of them, a block's width apart, with
-// all of its loads in flight.  blockIdx.y = key or value.  Workgroups go to the XCDs in turn, so
+// all of its loads in flight.  blockIdx.y = key, value or the
+// rows' small fields.  Workgroups go to the XCDs in turn, so
 // eight row blocks are interleaved and the (sequence, head) pairs of one follow each other on one
 // XCD: where projections lay the heads of a token side by side, that XCD reads whole tokens (by
 // head, each L2 would see one 256-byte piece in 2 KiB, two of its 16 channels: 101 us a 64K-token
@@ -91,6 +92,18 @@ __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
   if (a.lengths) {
     const int n = a.lengths[bh];
     len = n < 0 ? 0 : ((uint32_t)n > M ? M : (uint32_t)n);
+  }
+  if (z == 2) {  // the rows' small fields, a lane each
+    for (uint32_t m = blk * 256 + threadIdx.x; m < M; m += gridDim.x / nbh * 256) {
+      int s = m < len ? (a.index ? a.index[(int64_t)bh * M + m] : (int)m) : -1;
+      const bool real = s >= 0 && s < a.N;
+      const int64_t row = bh * a.capacity + m, from = bh * a.N + (real ? s : 0);
+      a.o_counts[row] = real ? (a.counts ? a.counts[from] : 1) : 0;
+      a.o_ts[row] = real ? (a.ts ? a.ts[from] : s) : 0;
+      if (a.o_mass) a.o_mass[row] = real && a.mass ? a.mass[from] : 0.0f;
+      if (m == 0) a.o_lengths[bh] = (int32_t)len;
+    }
+    return;
   }
   const char* base = (const char*)a.x[z] + (b * a.s_b[z] + h * a.s_h[z]) * (DT == DA_F32 ? 4 : 2);
   const uint32_t first = blk * 256 * kQuantItems + threadIdx.x;  // below 2^31: capacity <= 2^26
@@ -145,14 +158,6 @@ __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
       const int64_t row = bh * a.capacity + m;
       ((uint32_t*)a.codes[z])[row * kLpr + c] = codes;
       if ((c & 3) == 0) a.scales[z][row * NG + (c >> 2)] = (uint8_t)(src[u] < 0 ? 0u : e);
-      if (z == 0 && c == 0) {
-        const int64_t s = bh * a.N + src[u];
-        const bool real = src[u] >= 0;
-        a.o_counts[row] = real ? (a.counts ? a.counts[s] : 1) : 0;
-        a.o_ts[row] = real ? (a.ts ? a.ts[s] : (int32_t)src[u]) : 0;
-        if (a.o_mass) a.o_mass[row] = real && a.mass ? a.mass[s] : 0.0f;
-        if (m == 0) a.o_lengths[bh] = (int32_t)len;
-      }
     }
   }
 }
@@ -616,41 +621,79 @@ struct Move4Args {
   int budget;
 };
 
-// A lane moves 16 bytes of codes (2 NG lanes a row, keys then values) and the first lanes of
-// a row its small fields.
+// A row's exponent bytes, as one access where they are 1, 2 or 4.
+template <int NG>
+__device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
+  if constexpr (NG == 4) return *(const uint32_t*)p;
+  else if constexpr (NG == 2) return *(const uint16_t*)p;
+  else if constexpr (NG == 1) return *p;
+  else return p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16;
+}
+template <int NG>
+__device__ __forceinline__ void store_scales(uint8_t* p, uint32_t v) {
+  if constexpr (NG == 4) *(uint32_t*)p = v;
+  else if constexpr (NG == 2) *(uint16_t*)p = (uint16_t)v;
+  else if constexpr (NG == 1) *p = (uint8_t)v;
+  else {
+    p[0] = (uint8_t)v;
+    p[1] = (uint8_t)(v >> 8);
+    p[2] = (uint8_t)(v >> 16);
+  }
+}
+
+// blockIdx.z = 0: a lane moves 16 bytes of codes (2 NG lanes a row, keys then values), read once and
+// past the caches; z = 1: a lane moves a row's small fields.  (With the fields on the codes' lanes the
+// memory instructions a row were three times as many: 131072 rows x 8 heads to 32768
+// took 29 us against 22, a ragged batch of 16 47 against 31, 4.9 TB/s.)
 constexpr int kMoveItems = 2;
 template <int NG>
 __global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
   constexpr uint32_t kLpr = 2 * NG;
   const int bh = blockIdx.y;
+  const int32_t* const index = a.index + (int64_t)bh * a.budget;
+  if (blockIdx.z == 1) {
+    for (int m = blockIdx.x * 256 + threadIdx.x; m < a.budget; m += gridDim.x * 256) {
+      const int src = index[m];
+      const int64_t to = bh * a.o_capacity + m, from = bh * a.capacity + src;
+      uint32_t ks = 0, vs = 0;
+      int c = 0, t = 0;
+      float w = 0.0f;
+      if (src >= 0) {
+        ks = load_scales<NG>(a.scales[0] + from * NG);
+        vs = load_scales<NG>(a.scales[1] + from * NG);
+        c = a.counts[from];
+        t = a.ts[from];
+        w = a.mass[from];
+      }
+      store_scales<NG>(a.o_scales[0] + to * NG, ks);
+      store_scales<NG>(a.o_scales[1] + to * NG, vs);
+      a.o_counts[to] = c;
+      a.o_ts[to] = t;
+      a.o_mass[to] = w;
+    }
+    return;
+  }
   const uint32_t first = blockIdx.x * 256 * kMoveItems + threadIdx.x;
   u32x4 w[kMoveItems];
   int src[kMoveItems];
 #pragma unroll
   for (int u = 0; u < kMoveItems; ++u) {
     const uint32_t m = (first + u * 256) / kLpr;
-    src[u] = m < (uint32_t)a.budget ? a.index[(int64_t)bh * a.budget + m] : -1;
+    src[u] = m < (uint32_t)a.budget ? index[m] : -1;
   }
 #pragma unroll
   for (int u = 0; u < kMoveItems; ++u) {
     const int c = (int)((first + u * 256) % kLpr), z = c >= NG ? 1 : 0;
     w[u] = u32x4{0, 0, 0, 0};
-    if (src[u] >= 0) w[u] = *(const u32x4*)(a.codes[z] + ((bh * a.capacity + src[u]) * NG + (c - z * NG)) * 16);
+    if (src[u] >= 0)
+      w[u] = __builtin_nontemporal_load((const u32x4*)(a.codes[z] + ((bh * a.capacity + src[u]) * NG + (c - z * NG)) * 16));
   }
 #pragma unroll
   for (int u = 0; u < kMoveItems; ++u) {
     const uint32_t it = first + u * 256, m = it / kLpr;
     if (m >= (uint32_t)a.budget) continue;
     const int c = (int)(it - m * kLpr), z = c >= NG ? 1 : 0, cc = c - z * NG;
-    const int64_t to = bh * a.o_capacity + m, from = bh * a.capacity + src[u];
-    const bool real = src[u] >= 0;
-    *(u32x4*)(a.o_codes[z] + (to * NG + cc) * 16) = w[u];
-    a.o_scales[z][to * NG + cc] = real ? a.scales[z][from * NG + cc] : (uint8_t)0;
-    if (c == 0) {
-      a.o_counts[to] = real ? a.counts[from] : 0;
-      a.o_ts[to] = real ? a.ts[from] : 0;
-      a.o_mass[to] = real ? a.mass[from] : 0.0f;
-    }
+    *(u32x4*)(a.o_codes[z] + ((bh * a.o_capacity + m) * NG + cc) * 16) = w[u];
   }
 }
 
@@ -665,6 +708,7 @@ static int check_kv4(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, bool ma
   DA_REQUIRE(B * Hkv <= 65535, "%s: at most 65535 (sequence, head) pairs", who);
   if (kv->capacity > (1 << 26)) return set_error(DA_ERR_UNSUPPORTED, "%s: capacity above 2^26 rows", who);
   DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
+  DA_REQUIRE((((uintptr_t)kv->k_scales | (uintptr_t)kv->v_scales) & 3) == 0, "%s: exponents must be 4-byte aligned", who);
   return DA_OK;
 }
 
@@ -762,7 +806,7 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   const int groups = (int)((D + 31) / 32);
   const int64_t blocks = ((M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems) + 7) / 8 * 8;
   DA_REQUIRE(blocks * B * Hkv < (1ll << 31), "%s: more than 2^31 workgroups", who);
-  const dim3 grid((unsigned)(blocks * B * Hkv), 2);  // blocks: a multiple of eight
+  const dim3 grid((unsigned)(blocks * B * Hkv), 3);  // blocks: a multiple of eight
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) launch_quantize<DA_F32>(a, groups, grid, st);
   else if (dtype == DA_F16) launch_quantize<DA_F16>(a, groups, grid, st);
@@ -831,7 +875,7 @@ extern "C" int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, 
   a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass;
   a.index = rows; a.capacity = kv->capacity; a.o_capacity = out->capacity; a.budget = (int)budget;
   const int groups = (int)((D + 31) / 32);
-  const dim3 grid((unsigned)((budget * 2 * groups + 256 * kMoveItems - 1) / (256 * kMoveItems)), (unsigned)(B * Hkv));
+  const dim3 grid((unsigned)((budget * 2 * groups + 256 * kMoveItems - 1) / (256 * kMoveItems)), (unsigned)(B * Hkv), 2);
   switch (groups) {
     case 1: hipLaunchKernelGGL((move4_kernel<1>), grid, dim3(256), 0, st, a); break;
     case 2: hipLaunchKernelGGL((move4_kernel<2>), grid, dim3(256), 0, st, a); break;

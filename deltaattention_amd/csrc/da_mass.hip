@@ -369,6 +369,9 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
           sum[cb] += p;
         }
       } else {
+        float part[NCB];  // a half's 16 rows by themselves: long sums lose less
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) part[cb] = 0.0f;
         if (!mask) {
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
             for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                sum[cb] = __builtin_fmaf(mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])), mul[i], sum[cb]);
+                part[cb] = __builtin_fmaf(mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])), mul[i], part[cb]);
           }
         } else {
 #pragma unroll
@@ -390,10 +393,12 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float p = mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])) * mul[i];
-                sum[cb] += tt[i] < ct[cb] ? 0.0f : p;
+                part[cb] += tt[i] < ct[cb] ? 0.0f : p;
               }
           }
         }
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) sum[cb] += part[cb];
       }
     }
     if (next) store_tile(st ^ 1, tile + 1);

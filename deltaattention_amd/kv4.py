@@ -121,12 +121,12 @@ class KV4:
         _want(lengths, "lengths", (B, H), _I32, device)
         if mass is not None:
             _want(mass, "mass", rows, _F32, device)
-        kc, vc = k_codes.data_ptr(), v_codes.data_ptr()
-        if (kc | vc) % 16:
-            raise ValueError("k_codes and v_codes must be 16-byte aligned")
+        kc, vc, ks, vs = k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr()
+        if (kc | vc) % 16 or (ks | vs) % 4:
+            raise ValueError("codes must be 16-byte aligned, scales 4-byte")
         self._put(B, H, cap, D, device, Kv4Block(
-            kc, k_scales.data_ptr(), vc, v_scales.data_ptr(), counts.data_ptr(), timestamps.data_ptr(),
-            lengths.data_ptr(), None if mass is None else mass.data_ptr(), cap), None)
+            kc, ks, vc, vs, counts.data_ptr(), timestamps.data_ptr(), lengths.data_ptr(),
+            None if mass is None else mass.data_ptr(), cap), None)
         _set(self, "k_codes", k_codes)
         _set(self, "k_scales", k_scales)
         _set(self, "v_codes", v_codes)

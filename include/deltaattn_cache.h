@@ -28,7 +28,8 @@ extern "C" {
  *
  * All arrays are contiguous: codes [B, Hkv, capacity, 16 groups], exponents [B, Hkv,
  * capacity, groups], counts / timestamps / mass [B, Hkv, capacity], lengths [B, Hkv] (rows in
- * use; clamped into [0, capacity] where read).  Codes must be 16-byte aligned.  mass (the
+ * use; clamped into [0, capacity] where read).  Codes must be 16-byte
+ * aligned, exponents 4-byte.  mass (the
  * attention weight each row has received) may be null where a call does not use it.  At most
  * 2^26 rows a head and 65535 (sequence, head) pairs.
  */
