@@ -56,6 +56,7 @@ SIGNATURES = {
     "da_decode_step": (_I, [_P, _P]),
     # include/deltaattn_cache.h
     "da_kv4_quantize": (_I, [_P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _P, _P]),
+    "da_kv4_update": (_I, [_P, _P, _I, _L, _L, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _L, _L, _L, _F, _I, _P]),
     "da_kv4_dequantize": (_I, [_P, _L, _L, _L, _L, _P, _P, _I, _P]),
     "da_kv4_evict_workspace_size": (_L, [_L, _L, _L, _L]),
     "da_kv4_evict": (_I, [_P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _P]),

@@ -125,29 +125,39 @@ def delta_prefill_attention(query_states: torch.Tensor, key_states: torch.Tensor
                              num_packed_dev=packed.num_packed, out=out)
     timing.stop_event("time_delta_mm_pattern", ev)
     if past_key_value is not None and hasattr(past_key_value, "initialize_from_prefill"):
-        _handoff(past_key_value, layer_idx, packed, key_states, value_states)   # :762-773
+        _handoff(past_key_value, layer_idx, packed, key_states, value_states,   # :762-773
+                 query_states, scaling)
     return out
 
 
-def _handoff(cache, layer_idx, packed, key_states, value_states):
+def _handoff(cache, layer_idx, packed, key_states, value_states, query_states=None, scaling=None):
     """initialize_from_prefill with the P packed rows of every head and the last
-    min(N, W) prefill tokens (modeling_llama.py:762-773, 869-879)."""
+    min(N, W) prefill tokens (modeling_llama.py:762-773, 869-879).  A cache with a budget
+    (``FourBitCompressedCache``) also gets the attention weight that its ``observe`` last
+    queries gave each anchor."""
     q_len = key_states.shape[2]
     p = packed.trimmed()
     tail = min(q_len, cache.exact_window_size)
+    more = {}
+    if getattr(cache, "budget", None) is not None and query_states is not None:
+        n = min(cache.observe, query_states.shape[2])
+        more["mass"] = ops.attention_mass(
+            query_states[:, :, -n:], p.k_packed, counts=p.counts.contiguous(),
+            timestamps=p.timestamps.contiguous(), lengths=p.anchor_counts, q_start=q_len - n, scale=scaling)
     cache.initialize_from_prefill(
         layer_idx=layer_idx, k_packed=p.k_packed, v_packed=p.v_packed, counts=p.counts,
         timestamps=p.timestamps, k_exact=key_states[:, :, -tail:, :],
-        v_exact=value_states[:, :, -tail:, :], original_q_len=q_len)
+        v_exact=value_states[:, :, -tail:, :], original_q_len=q_len, **more)
 
 
 def delta_decode_handoff(key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
-                         past_key_value) -> None:
+                         past_key_value, query_states: Optional[torch.Tensor] = None,
+                         scaling: Optional[float] = None) -> None:
     """PATH 2's ``delta_decode`` tail (modeling_llama.py:805-879): after a dense prefill,
     delta-select and pack the post-RoPE keys with the globVR chunking, metric and
     threshold (always delta mode, whatever ``packing_mode`` says, as the reference
     launches chunked_eval_kernel directly), then hand the packed history and the exact
-    tail to the cache."""
+    tail to the cache.  ``query_states`` and ``scaling`` are for a cache with a budget."""
     fixed = getattr(globVR, "chunk_size", 0)                        # :809-816
     divide_to = getattr(globVR, "divide_to", 0)
     keep, _ = ops.select(key_states, getattr(globVR, "row_delta_threshold", 0.0),
@@ -156,7 +166,8 @@ def delta_decode_handoff(key_states: torch.Tensor, value_states: torch.Tensor, l
                          metric=getattr(globVR, "row_similarity_metric", "euclidean"),
                          arith=getattr(globVR, "row_delta_arith", "native"))
     packed = ops.pack(keep, key_states, value_states)               # :836-866
-    _handoff(past_key_value, layer_idx, packed, key_states, value_states)   # :868-879
+    _handoff(past_key_value, layer_idx, packed, key_states, value_states,   # :868-879
+             query_states, scaling)
 
 
 def dense_prefill_attention(query_states, key_states, value_states, scaling=None, out=None):

@@ -45,44 +45,6 @@ struct DecodeUpdateArgs {
   float thr;
 };
 
-// A lane's two elements (dims 2l and 2l + 1) of a cache row: one 32-bit word of a 16-bit
-// type, or two fp32 values (8 bytes).
-template <int DT>
-struct DecPair {
-  using Elem = uint16_t;
-  using Word = uint32_t;
-  static __device__ __forceinline__ float lo(Word w) { return E16<DT>::lo(w); }
-  static __device__ __forceinline__ float hi(Word w) { return E16<DT>::hi(w); }
-};
-template <>
-struct DecPair<DA_F32> {
-  using Elem = float;
-  using Word = u32x2;
-  static __device__ __forceinline__ float lo(Word w) { return __uint_as_float(w[0]); }
-  static __device__ __forceinline__ float hi(Word w) { return __uint_as_float(w[1]); }
-};
-
-// The update's test (deltaDecoding.py:61-77): does the evicted token (this lane's pair
-// ek, dims 2l and 2l + 1) merge into the last packed anchor (pair lk)?  Euclidean
-// dist^2 <= thr or cosine >= thr, with the selection's fixed fp32 tree; the same result
-// in every lane.
-template <bool COS, int DT>
-__device__ __forceinline__ bool evict_merges(typename DecPair<DT>::Word ek, typename DecPair<DT>::Word lk,
-                                             float thr) {
-#pragma clang fp contract(off)
-  using PT = DecPair<DT>;
-  const float e0 = PT::lo(ek), e1 = PT::hi(ek), l0 = PT::lo(lk), l1 = PT::hi(lk);
-  if (COS) {
-    const float eps = 1e-8f;
-    const float dot = wave_tree_sum(pair_dot(e0, e1, l0, l1));
-    const float ne = sqrt_rn(wave_tree_sum(pair_dot(e0, e1, e0, e1)) + eps);
-    const float nl = sqrt_rn(wave_tree_sum(pair_dot(l0, l1, l0, l1)) + eps);
-    return __fdiv_rn(dot, ne * nl) >= thr;
-  }
-  const float d0 = e0 - l0, d1 = e1 - l1;
-  return wave_tree_sum(pair_dot(d0, d1, d0, d1)) <= thr;
-}
-
 template <bool COS, int DT>
 __global__ __launch_bounds__(256) void decode_update_kernel(DecodeUpdateArgs a) {
 #pragma clang fp contract(off)

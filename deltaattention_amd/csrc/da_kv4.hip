@@ -217,6 +217,98 @@ __global__ __launch_bounds__(256) void dequantize4_kernel(Dequant4Args a) {
 }
 
 // ------------------------------------------------------------------------------------
+// one decode token
+// ------------------------------------------------------------------------------------
+struct Update4Args {
+  const void* new_k;
+  const void* new_v;
+  int64_t sn_b, sn_h;
+  void* kx;
+  void* vx;
+  int64_t sx_b, sx_h, sx_s;
+  DaKv4 kv;
+  void* k_last;  // [B, Hkv, D]
+  int64_t exact_len, total_len, window;
+  int B, H, D;
+  float thr;
+};
+
+// The largest magnitude (fp32 bits) of a lane's row of 16 lanes, which hold one group.
+__device__ __forceinline__ uint32_t row16_umax(uint32_t v) {
+  v = quad_umax(v);
+  uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppHalfMirror, 0xF, 0xF, false);
+  v = v > o ? v : o;
+  o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppMirror, 0xF, 0xF, false);
+  return v > o ? v : o;
+}
+
+// One wave a (sequence, KV head), lane l dims 2 l and 2 l + 1: decode_update_kernel's step with the
+// packed rows in 4 bits.  The test whether the evicted token merges looks at the last anchor's key as
+// it was, kept beside the rows, so the decisions are those of a cache at full width.
+template <bool COS, int DT>
+__global__ __launch_bounds__(256) void update4_kernel(Update4Args a) {
+  using PT = DecPair<DT>;
+  using E = typename PT::Elem;
+  using Word = typename PT::Word;
+  const int lane = threadIdx.x & 63;
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= a.B * a.H) return;
+  const int b = w / a.H, h = w - b * a.H;
+  const bool act = 2 * lane < a.D;
+  const int groups = (a.D + 31) / 32;
+  const int64_t widx = a.exact_len % a.window;
+  E* const ring_k = (E*)a.kx + b * a.sx_b + h * a.sx_h + widx * a.sx_s + 2 * lane;
+  E* const ring_v = (E*)a.vx + b * a.sx_b + h * a.sx_h + widx * a.sx_s + 2 * lane;
+  E* const last = (E*)a.k_last + (int64_t)w * a.D + 2 * lane;
+  if (a.exact_len >= a.window) {
+    const Word ek = act ? *(const Word*)ring_k : Word{};
+    const Word ev = act ? *(const Word*)ring_v : Word{};
+    int n = a.kv.lengths[w];
+    n = n < 0 ? 0 : (n > a.kv.capacity ? (int)a.kv.capacity : n);
+    const int64_t row0 = (int64_t)w * a.kv.capacity;
+    bool merge = false;
+    if (n > 0) {
+      const Word lk = act ? *(const Word*)last : Word{};
+      merge = evict_merges<COS, DT>(ek, lk, a.thr);
+    }
+    if (merge) {
+      if (lane == 0) a.kv.counts[row0 + n - 1] += 1;
+    } else if (n < a.kv.capacity) {
+      const int64_t row = row0 + n;
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const Word x = z == 0 ? ek : ev;
+        const float x0 = PT::lo(x), x1 = PT::hi(x);
+        const uint32_t m0 = __float_as_uint(x0) & 0x7fffffffu, m1 = __float_as_uint(x1) & 0x7fffffffu;
+        const uint32_t e = group_exponent(row16_umax(m0 > m1 ? m0 : m1));
+        uint32_t code = 0;
+        if (e != 255u) {
+          const float inv = __uint_as_float((254u - e) << 23);
+          code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x0 * inv, x1 * inv, 1.0f, 0);
+        }
+        uint8_t* const codes = z == 0 ? a.kv.k_codes : a.kv.v_codes;
+        uint8_t* const scales = z == 0 ? a.kv.k_scales : a.kv.v_scales;
+        if (lane < 16 * groups) codes[row * 16 * groups + lane] = (uint8_t)code;
+        if ((lane & 15) == 0 && lane < 16 * groups) scales[row * groups + (lane >> 4)] = (uint8_t)e;
+      }
+      if (act) *(Word*)last = ek;
+      if (lane == 0) {
+        a.kv.counts[row] = 1;
+        a.kv.timestamps[row] = (int32_t)(a.total_len - a.window);
+        if (a.kv.mass) a.kv.mass[row] = 0.0f;
+        a.kv.lengths[w] = n + 1;
+      }
+    }
+  }
+  if (act) {
+    const Word nk = *(const Word*)((const E*)a.new_k + b * a.sn_b + h * a.sn_h + 2 * lane);
+    const Word nv = *(const Word*)((const E*)a.new_v + b * a.sn_b + h * a.sn_h + 2 * lane);
+    *(Word*)ring_k = nk;
+    *(Word*)ring_v = nv;
+  }
+}
+
+// ------------------------------------------------------------------------------------
 // eviction: the rows kept
 // ------------------------------------------------------------------------------------
 struct HeavyArgs {
@@ -898,4 +990,39 @@ extern "C" int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t 
   DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   return launch_heavy(mass, lengths, B * Hkv, N, budget, sinks, recent, index, kept, workspace, (hipStream_t)stream,
                       who);
+}
+
+template <int DT>
+static void launch_update4(const Update4Args& a, bool cosine, hipStream_t st) {
+  const dim3 grid((unsigned)((a.B * a.H + 3) / 4));
+  if (cosine) hipLaunchKernelGGL((update4_kernel<true, DT>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((update4_kernel<false, DT>), grid, dim3(256), 0, st, a);
+}
+
+extern "C" int da_kv4_update(const void* new_k, const void* new_v, int dtype, int64_t B, int64_t Hkv, int64_t D,
+                             int64_t sn_b, int64_t sn_h, void* k_exact, void* v_exact, int64_t sx_b, int64_t sx_h,
+                             int64_t sx_s, const DaKv4* kv, void* k_last, int64_t exact_seq_len,
+                             int64_t total_seq_len, int64_t window, float threshold, int use_cosine, void* stream) {
+  const char* who = "da_kv4_update";
+  DA_REQUIRE(new_k && new_v && k_exact && v_exact && k_last, "%s: null pointer", who);
+  if (int rc = check_kv4(kv, B, Hkv, D, false, who)) return rc;
+  if (dtype != DA_BF16 && dtype != DA_F16 && dtype != DA_F32)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: rows must be bf16, fp16 or fp32", who);
+  DA_REQUIRE(window > 0 && exact_seq_len >= 0 && total_seq_len >= 0, "%s: bad lengths", who);
+  const uintptr_t pair_align = dtype == DA_F32 ? 7 : 3;
+  DA_REQUIRE(((sn_b | sn_h | sx_b | sx_h | sx_s) & 1) == 0 &&
+                 (((uintptr_t)new_k | (uintptr_t)new_v | (uintptr_t)k_exact | (uintptr_t)v_exact |
+                   (uintptr_t)k_last) & pair_align) == 0,
+             "%s: rows must be %d-byte aligned (even strides)", who, dtype == DA_F32 ? 8 : 4);
+  Update4Args a = {};
+  a.new_k = new_k; a.new_v = new_v; a.sn_b = sn_b; a.sn_h = sn_h;
+  a.kx = k_exact; a.vx = v_exact; a.sx_b = sx_b; a.sx_h = sx_h; a.sx_s = sx_s;
+  a.kv = *kv; a.k_last = k_last;
+  a.exact_len = exact_seq_len; a.total_len = total_seq_len; a.window = window;
+  a.B = (int)B; a.H = (int)Hkv; a.D = (int)D; a.thr = threshold;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DA_F32) launch_update4<DA_F32>(a, use_cosine != 0, st);
+  else if (dtype == DA_F16) launch_update4<DA_F16>(a, use_cosine != 0, st);
+  else launch_update4<DA_BF16>(a, use_cosine != 0, st);
+  return check_launch(who);
 }

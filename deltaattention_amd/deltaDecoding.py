@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 
-from . import globVR
+from . import globVR, kv4
 from ._launch import HALF, KernelLauncher, tensor, unit_stride
 from ._native import DecodeStep, check, current_stream, device_stream, dtype_code, lib
 
@@ -23,7 +23,7 @@ try:  # transformers' Cache base (the reference subclasses it, deltaDecoding.py:
 except Exception:  # pragma: no cover - transformers is optional for the kernels
     _CacheBase = object
 
-__all__ = ["HybridCompressedCache", "fused_hybrid_decode_update_kernel",
+__all__ = ["HybridCompressedCache", "FourBitCompressedCache", "fused_hybrid_decode_update_kernel",
            "fused_hybrid_decode_kernel", "decode_attention"]
 
 
@@ -335,10 +335,138 @@ class HybridCompressedCache(_CacheBase):
         return None
 
 
+class FourBitCompressedCache(HybridCompressedCache):
+    """The compressed cache with its packed anchors in 4 bits and, if wanted, bounded in number.
+
+    The prefill hand-off, ``update``, ``decode_step`` and the host-side trackers are
+    HybridCompressedCache's; the exact ring keeps its type.  The anchors of a layer are one
+    ``ops.KV4`` (``anchors[layer]``).  Whether an evicted token merges is decided on the last
+    anchor's key at full width (``k_last``), so counts, timestamps and lengths are those of
+    a HybridCompressedCache.  Unlike there, a head's rows are its own anchors without the zero
+    rows that pad it to the longest head.
+
+    With ``budget`` set every decode token adds the attention weight each anchor received to its
+    ``mass``, and a head keeps at most ``budget`` anchors: its first ``sinks``, its last ``recent``
+    and the heaviest of the others.  The hand-off cuts to the budget by the weights that the
+    prompt's last ``observe`` queries give (``attention.delta_prefill_attention`` computes
+    them); decoding cuts when ``slack`` anchors have been added.  A cut moves the layer's anchors
+    to new memory, so a captured graph of decode steps has to be captured again after one.
+    Without ``budget`` the cache grows as the reference's does (deltaDecoding.py:138-157).
+    """
+
+    def __init__(self, config, batch_size, dtype=torch.float16, exact_window_size=50,
+                 initial_capacity=1024, device="cuda", budget: Optional[int] = None, sinks: int = 4,
+                 recent: int = 64, slack: int = 256, observe: int = 64):
+        if _CacheBase is not object:
+            try:
+                _CacheBase.__init__(self, layers=[])
+            except TypeError:
+                _CacheBase.__init__(self)
+        if budget is not None and (sinks < 0 or recent < 1 or sinks + recent > budget or slack < 1 or observe < 1):
+            raise ValueError(f"a budget needs 1 <= recent, sinks + recent <= budget, slack and observe >= 1; got budget "
+                             f"{budget}, sinks {sinks}, recent {recent}, slack {slack}, observe {observe}")
+        self.exact_window_size = exact_window_size
+        self.head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
+        self.n_kv_heads = config.num_key_value_heads
+        self.bsz = batch_size
+        self.dtype = dtype
+        self.device = torch.device(device)
+        self.num_layers = config.num_hidden_layers
+        self.budget, self.sinks, self.recent, self.slack, self.observe = budget, sinks, recent, slack, observe
+        self.capacity = initial_capacity if budget is None else budget + slack
+        L, B, H, D, W = self.num_layers, self.bsz, self.n_kv_heads, self.head_dim, exact_window_size
+        self.anchors = [self._rows(self.capacity) for _ in range(L)]
+        self.k_last = torch.zeros((L, B, H, D), device=self.device, dtype=dtype)
+        self.k_exact = torch.zeros((L, B, H, W, D), device=self.device, dtype=dtype)
+        self.v_exact = torch.zeros_like(self.k_exact)
+        self.exact_seq_lens = [0 for _ in range(L)]
+        self.max_packed_len = [0 for _ in range(L)]
+        self.total_seq_lens = [0 for _ in range(L)]
+
+    def _rows(self, capacity):
+        kv = kv4.KV4.empty(self.bsz, self.n_kv_heads, capacity, self.head_dim, self.device)
+        kv.lengths.zero_()
+        return kv
+
+    @property
+    def packed_lengths(self):
+        """Anchors of every (sequence, KV head) of a layer, [B * Hkv] int32 each."""
+        return [kv.lengths.view(-1) for kv in self.anchors]
+
+    def initialize_from_prefill(self, layer_idx, k_packed, v_packed, counts, timestamps, k_exact,
+                                v_exact, original_q_len, mass=None):
+        """Prefill hand-off: the anchors (rows of count > 0, which come first) into 4 bits, the last
+        min(N, W) prefill tokens to the ring.  With a budget and more rows than it, ``mass`` ([B, Hkv,
+        P] float32, as ``ops.attention_mass`` gives it) says which stay."""
+        counts = counts.to(torch.int32).contiguous()
+        timestamps = timestamps.to(torch.int32).contiguous()
+        P = k_packed.shape[2]
+        lengths = (counts > 0).sum(-1, dtype=torch.int32)
+        last = (lengths - 1).clamp(min=0).long()[..., None, None].expand(-1, -1, 1, self.head_dim)
+        self.k_last[layer_idx] = torch.gather(k_packed, 2, last).squeeze(2)
+        index = None
+        if self.budget is not None and P > self.budget:
+            if mass is None:
+                raise ValueError(f"{P} anchors for a budget of {self.budget}: the hand-off needs their mass")
+            index, lengths = kv4.heavy_rows(mass, self.budget, self.sinks, self.recent, lengths)
+            P = self.budget
+        capacity = self.budget + self.slack if self.budget is not None else max(self.capacity, P + 1024)
+        self.anchors[layer_idx] = kv4.quantize_kv4(k_packed, v_packed, counts, timestamps, mass, lengths, index,
+                                                   capacity)
+        self.max_packed_len[layer_idx] = P
+        e_len = k_exact.shape[2]
+        self.k_exact[layer_idx, :, :, :e_len] = k_exact
+        self.v_exact[layer_idx, :, :, :e_len] = v_exact
+        self.exact_seq_lens[layer_idx] = e_len
+        self.total_seq_lens[layer_idx] = original_q_len
+
+    def _make_room(self, layer_idx):
+        """Before a token: a row for it in every head, by a cut to the budget or by growing."""
+        kv = self.anchors[layer_idx]
+        if self.max_packed_len[layer_idx] < kv.capacity:
+            return
+        if self.budget is None:
+            self.anchors[layer_idx] = kv4.evict_kv4(kv, kv.capacity, capacity=max(2 * kv.capacity, kv.capacity + 1024))
+        else:
+            self.anchors[layer_idx] = kv4.evict_kv4(kv, self.budget, self.sinks, self.recent, self.budget + self.slack)
+            self.max_packed_len[layer_idx] = self.budget
+
+    def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
+        """One decode token (``ops.decode_update_kv4``); prefill calls pass through."""
+        if key_states.shape[2] > 1:
+            return key_states, value_states
+        self._make_room(layer_idx)
+        threshold, use_cos = _metric_threshold()
+        kv4.decode_update_kv4(self.anchors[layer_idx], key_states, value_states, self.k_exact[layer_idx],
+                              self.v_exact[layer_idx], self.k_last[layer_idx], self.exact_seq_lens[layer_idx],
+                              self.total_seq_lens[layer_idx], float(threshold), use_cos)
+        if self.exact_seq_lens[layer_idx] >= self.exact_window_size:
+            self.max_packed_len[layer_idx] += 1
+            if self.total_seq_lens[layer_idx] % 256 == 0:  # reconcile with the device, as the base does
+                self.max_packed_len[layer_idx] = int(self.anchors[layer_idx].lengths.max().item())
+        self.exact_seq_lens[layer_idx] += 1
+        self.total_seq_lens[layer_idx] += 1
+        return key_states, value_states
+
+    def attend(self, query_states, layer_idx, scaling=None):
+        """q [B, Hq, 1, D] over the layer's anchors and ring; with a budget, the weights are added to
+        the anchors' mass."""
+        n = min(self.exact_seq_lens[layer_idx], self.exact_window_size)
+        return kv4.decode_attention_kv4(query_states, self.anchors[layer_idx], self.k_exact[layer_idx],
+                                        self.v_exact[layer_idx], n, scaling, accumulate=self.budget is not None)
+
+    def decode_step(self, query_states, key_states, value_states, layer_idx, scaling=None):
+        """``update`` then ``attend``: one decode token of one layer."""
+        self.update(key_states, value_states, layer_idx)
+        return self.attend(query_states, layer_idx, scaling)
+
+
 def decode_attention(q: torch.Tensor, cache: HybridCompressedCache, layer_idx: int,
                      scaling: Optional[float] = None) -> torch.Tensor:
     """q [B, Hq, 1, D] -> [B, Hq, 1, D] over the layer's compressed cache; restates
     LlamaAttention._forward_fused_hybrid_decode (modeling_llama.py:453-518)."""
+    if isinstance(cache, FourBitCompressedCache):
+        return cache.attend(q, layer_idx, scaling)
     B, Hq, _, D = q.shape
     q2 = q.squeeze(2).contiguous()
     kp, vp = cache.k_packed[layer_idx], cache.v_packed[layer_idx]

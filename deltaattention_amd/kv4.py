@@ -18,7 +18,7 @@ import torch
 from ._native import Kv4Block, call_on, check, dtype_code, lib
 
 __all__ = ["KV4", "attention_mass", "heavy_rows", "quantize_kv4", "dequantize_kv4", "evict_kv4",
-           "decode_attention_kv4"]
+           "decode_update_kv4", "decode_attention_kv4"]
 
 _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
@@ -354,6 +354,36 @@ def evict_kv4(kv: KV4, budget: int, sinks: int = 0, recent: int = 0, capacity: O
     rc = call_on(device, lib().da_kv4_evict, kv._ref, B, H, D, budget, sinks, recent, out._ref, None, ws.data_ptr(), n)
     check(rc, "da_kv4_evict")
     return out
+
+
+def decode_update_kv4(kv: KV4, key: torch.Tensor, value: torch.Tensor, k_exact: torch.Tensor, v_exact: torch.Tensor,
+                      k_last: torch.Tensor, exact_seq_len: int, total_seq_len: int, threshold: float,
+                      use_cosine: bool = False) -> None:
+    """One decode token into the ring k_exact, v_exact [B, Hkv, W, D] (slot exact_seq_len % W).  Where
+    the ring was full, the token that leaves it merges into its head's last 4-bit row (count + 1) or
+    becomes a new one, by the test of ``da_decode_update`` against that row's key as it was
+    (k_last [B, Hkv, D], kept up to date).  ``threshold`` is squared for the Euclidean test.  key, value
+    [B, Hkv, 1, D], ring and k_last share one type."""
+    B, H, D, device = kv.batch, kv.kv_heads, kv.head_dim, kv.device
+    dt = dtype_code(key, value, k_exact, v_exact, k_last)
+    if key.shape != (B, H, 1, D) or value.shape != key.shape or key.device != device or value.device != device:
+        raise ValueError(f"key and value must be {[B, H, 1, D]} on {device}")
+    if k_exact.dim() != 4 or not k_exact.shape[2] or k_exact.device != device or v_exact.device != device:
+        raise ValueError(f"k_exact and v_exact must be [{B}, {H}, W, {D}] on {device}")
+    W = k_exact.shape[2]
+    for t, name in ((k_exact, "k_exact"), (v_exact, "v_exact")):
+        _want(t, name, (B, H, W, D), k_exact.dtype, device)
+    _want(k_last, "k_last", (B, H, D), k_exact.dtype, device)
+    if exact_seq_len < 0 or total_seq_len < 0:
+        raise ValueError("negative lengths")
+    key, value = _rows(key), _rows(value)
+    if _strides(key) != _strides(value):
+        key, value = key.contiguous(), value.contiguous()
+    sn = _strides(key)
+    rc = call_on(device, lib().da_kv4_update, key.data_ptr(), value.data_ptr(), dt, B, H, D, sn[0], sn[1],
+                 k_exact.data_ptr(), v_exact.data_ptr(), H * W * D, W * D, D, kv._ref, k_last.data_ptr(),
+                 int(exact_seq_len), int(total_seq_len), W, threshold, 1 if use_cosine else 0)
+    check(rc, "da_kv4_update")
 
 
 def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tensor] = None,

@@ -23,7 +23,8 @@ Two layers of the swap:
   :func:`delta_llama_attention_forward`, the reference's whole forward: PATH 1 / PATH 2
   prefill by the configured implementation, the prefill -> cache hand-off, and PATH 3
   decode over the compressed cache.  Without a ``HybridCompressedCache`` it runs the
-  stock flow through the registered implementation.
+  stock flow through the registered implementation.  A ``FourBitCompressedCache`` (anchors
+  in 4 bits, bounded by accumulated attention weight) takes the same way.
 """
 from __future__ import annotations
 
@@ -170,7 +171,9 @@ def delta_llama_attention_forward(self, hidden_states: torch.Tensor,
                 query_states, key_states, value_states, scaling=self.scaling, out=view),
                 query_states.is_cuda)
             if getattr(globVR, "delta_decode", False):               # :805-879
-                attention.delta_decode_handoff(key_states, value_states, self.layer_idx, cache)
+                # a cache with a budget asks the queries which anchors to keep
+                more = (query_states, self.scaling) if getattr(cache, "budget", None) is not None else ()
+                attention.delta_decode_handoff(key_states, value_states, self.layer_idx, cache, *more)
         else:                                                        # PATH 1
             _timed(lambda: attention.delta_prefill_attention(
                 query_states, key_states, value_states, layer_idx=self.layer_idx,

@@ -18,14 +18,14 @@ import torch
 
 from . import _native
 from ._native import DA_F32, DA_I32, DA_VARIANT, check, current_stream, dtype_code, lib, strides_array
-from .kv4 import (KV4, attention_mass, decode_attention_kv4, dequantize_kv4, evict_kv4, heavy_rows,
-                  quantize_kv4)
+from .kv4 import (KV4, attention_mass, decode_attention_kv4, decode_update_kv4, dequantize_kv4,
+                  evict_kv4, heavy_rows, quantize_kv4)
 
 __all__ = ["PackedKV", "chunking", "select", "pack", "hybrid_prefill", "dense_prefill",
            "delta_prefill", "VarlenBatch", "varlen_batch", "PackedVarlen", "select_varlen",
            "pack_varlen", "hybrid_prefill_varlen", "delta_prefill_varlen", "dense_prefill_varlen",
            "KV4", "attention_mass", "heavy_rows", "quantize_kv4", "dequantize_kv4", "evict_kv4",
-           "decode_attention_kv4"]
+           "decode_update_kv4", "decode_attention_kv4"]
 
 
 def _stream() -> ctypes.c_void_p:

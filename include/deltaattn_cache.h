@@ -82,6 +82,20 @@ int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, int64_t bud
                  const DaKv4* out, int32_t* index, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * One decode token, as da_decode_update over 16-bit rows: where the ring [B, Hkv, W, D] is full
+ * (exact_seq_len >= window) the token in slot exact_seq_len % window leaves it and merges into the
+ * last row (count + 1) if it is close enough to that row's key as it was, k_last [B, Hkv, D]
+ * (contiguous; Euclidean dist^2 <= threshold, cosine >= threshold), or else becomes a new row
+ * (count 1, timestamp total_seq_len - window, mass 0) and the new k_last; with the capacity used up
+ * it is dropped.  The new token takes the slot.  new_k, new_v [B, Hkv, 1, D] (strides sn_b, sn_h),
+ * ring and k_last share one type; even strides, rows 4-byte aligned (fp32: 8-byte).
+ */
+int da_kv4_update(const void* new_k, const void* new_v, int dtype, int64_t B, int64_t Hkv, int64_t D, int64_t sn_b,
+                  int64_t sn_h, void* k_exact, void* v_exact, int64_t sx_b, int64_t sx_h, int64_t sx_s,
+                  const DaKv4* kv, void* k_last, int64_t exact_seq_len, int64_t total_seq_len, int64_t window,
+                  float threshold, int use_cosine, void* stream);
+
+/*
  * Row choice alone: mass [B, Hkv, N] fp32 contiguous, lengths [B, Hkv] (null: N) -> index
  * [B, Hkv, budget] int32 (rows kept, ascending; -1 past them) and kept [B, Hkv] int32, by the
  * rule of da_kv4_evict.  workspace as there (capacity = N).

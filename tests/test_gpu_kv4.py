@@ -300,3 +300,98 @@ def test_attend_nan_is_seen(gpu):
     q = torch.randn(1, 4, 1, 64, generator=gen).bfloat16().to(gpu)
     announce("attend nan")
     assert torch.isnan(ops.decode_attention_kv4(q, kv)).all()
+
+
+# ---- streams and graphs -----------------------------------------------------------------------------
+
+
+def _chain(ops, s):
+    """The operators as a program runs them: the prompt's weights, the rows they leave in 4 bits, a
+    token over those, and a second cut."""
+    mass = ops.attention_mass(s["q"], s["k"])
+    index, kept = ops.heavy_rows(mass, 40, 2, 8)
+    kv = ops.quantize_kv4(s["k"], s["v"], mass=mass, index=index, lengths=kept)
+    out = ops.decode_attention_kv4(s["q"][:, :, -1:], kv, s["k"][:, :, -16:], s["v"][:, :, -16:], accumulate=True)
+    small = ops.evict_kv4(kv, 24, 2, 8)
+    k, v = ops.dequantize_kv4(small)
+    return [mass, index, kept, out, kv.mass, small.mass, small.timestamps, small.lengths, k, v]
+
+
+def _chain_inputs(gpu, seed, B=2, H=2, G=4, N=300, D=128):
+    gen = _gen(seed)
+    return {"q": torch.randn(B, H * G, 48, D, generator=gen).bfloat16().to(gpu),
+            "k": torch.randn(B, H, N, D, generator=gen).bfloat16().to(gpu),
+            "v": torch.randn(B, H, N, D, generator=gen).bfloat16().to(gpu)}
+
+
+def test_chain_stream_and_graph(gpu):
+    """The chain on a stream of its own and captured into a graph gives, replay after replay and with
+    eager work and other inputs between, what it gives eagerly."""
+    from deltaattention_amd import ops
+    announce("kv4 chain: eager, side stream, graph")
+    a, b = _chain_inputs(gpu, 1), _chain_inputs(gpu, 2)
+    want_a, want_b = ([t.clone() for t in _chain(ops, s)] for s in (a, b))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _chain(ops, a)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for x, y in zip(got, want_a):
+        assert torch.equal(x, y)
+    s = {n: t.clone() for n, t in a.items()}
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _chain(ops, s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _chain(ops, s)
+    for turn in range(4):
+        src, want = ((a, want_a), (b, want_b))[turn % 2]
+        for n, t in src.items():
+            s[n].copy_(t)
+        graph.replay()
+        for x, y in zip(held, want):
+            assert torch.equal(x, y), turn
+        for x, y in zip(_chain(ops, b), want_b):  # eager work between the replays
+            assert torch.equal(x, y)
+        torch.cuda.synchronize()
+
+
+def test_two_streams_at_once(gpu):
+    """Two programs with their own inputs on two streams do not disturb each other."""
+    from deltaattention_amd import ops
+    announce("kv4 two streams")
+    ins = [_chain_inputs(gpu, 3 + i, N=2000) for i in range(2)]
+    want = [[t.clone() for t in _chain(ops, s)] for s in ins]
+    streams = [torch.cuda.Stream() for _ in ins]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = _chain(ops, ins[i])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for x, y in zip(g, w):
+            assert torch.equal(x, y)
+
+
+def test_deterministic(gpu):
+    """The same call gives the same bits, splits and all."""
+    from deltaattention_amd import ops
+    gen = _gen(12)
+    q = torch.randn(1, 8, 700, 64, generator=gen).to(gpu)
+    k = torch.randn(1, 2, 5000, 64, generator=gen).to(gpu)
+    kv, _ = _cache(gpu, gen, 1, 2, 9000, 64, [9000, 8000])
+    mass = kv.mass.clone()
+    announce("kv4 deterministic")
+    first = None
+    for _ in range(3):
+        kv.mass.copy_(mass)
+        got = [ops.attention_mass(q, k), ops.decode_attention_kv4(q[:, :, :1], kv, accumulate=True), kv.mass.clone()]
+        if first is not None:
+            for x, y in zip(got, first):
+                assert torch.equal(x, y)
+        first = got
