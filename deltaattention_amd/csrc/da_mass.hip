@@ -75,6 +75,17 @@ __device__ __forceinline__ void cut_chunk(f32x4 x0, f32x4 x1, u32x4 (&w)[NP]) {
     }
 }
 
+// Scheduling of a 32-row step: the product's eight fragments and 16 MFMAs among the exponentials of
+// the rows before (8K prompt 697 us without, 675 with; 32K window 70 / 64).
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // a read of LDS
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);   // two MFMAs
+    __builtin_amdgcn_sched_group_barrier(0x402, 12, 0);  // VALU and transcendental
+  }
+}
+
 // What the columns pass needs of a query: its weights are 2^(s - max) / sum.  The maximum is kept
 // apart from the sum (not as one logarithm): s - max is small where the weight is large, so it
 // rounds finely there.
@@ -100,10 +111,11 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   constexpr int kPart = kTile * kMRow;        // LDS bytes of one part of a stage
   __shared__ __attribute__((aligned(16))) char s_y[2][NP * kPart];
   // per row: PASS 0 log2(count); PASS 1 -max and 1 / sum
-  __shared__ __attribute__((aligned(16))) float s_add[2][kTile];
-  __shared__ __attribute__((aligned(16))) float s_mul[2][PASS == 1 ? kTile : 4];
-  __shared__ __attribute__((aligned(16))) int s_t[2][kTile];
-  __shared__ int s_flag[2], s_ext[4];
+  // (three stages of them: a wave may still be at a tile's last half when others store two tiles on)
+  __shared__ __attribute__((aligned(16))) float s_add[3][kTile];
+  __shared__ __attribute__((aligned(16))) float s_mul[3][PASS == 1 ? kTile : 4];
+  __shared__ __attribute__((aligned(16))) int s_t[3][kTile];
+  __shared__ int s_flag[3], s_ext[4];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cl = lane & 31, hl = lane >> 5;
   const int nbh = a.B * a.Hkv, id = blockIdx.x / nbh;
@@ -198,7 +210,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   // An extreme time of the columns, to decide for whole tiles: rows pass, the earliest query (keys
   // at or before it need no mask); columns pass, the latest key.
   int ext = PASS == 0 ? mass_pos(a, query_of(a, c0)) : c_last;
-  auto store_tile = [&](int st, int tile) {
+  auto store_tile = [&](int st, int mt, int tile) {
     char* const at0 = s_y[st] + sr * kMRow + ((sc ^ sr) << 4);  // row % 16 is sr
     if (chunk) {
 #pragma unroll
@@ -218,13 +230,13 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
       // bit 0 (rows pass): a key has a weight other than 1; bit 1: a row that some column may not see
       const bool mine = lane < kTile;
       if (mine) {
-        s_add[st][lane] = m_add;
-        if (PASS == 1) s_mul[st][lane] = m_mul;
-        s_t[st][lane] = m_t;
+        s_add[mt][lane] = m_add;
+        if (PASS == 1) s_mul[mt][lane] = m_mul;
+        s_t[mt][lane] = m_t;
       }
       const uint64_t odd = __ballot(mine && !zero_bits(m_add));
       const uint64_t late = __ballot(mine && (PASS == 0 ? m_t > ext : m_t < ext));
-      if (lane == 0) s_flag[st] = (odd ? 1 : 0) | (late ? 2 : 0);
+      if (lane == 0) s_flag[mt] = (odd ? 1 : 0) | (late ? 2 : 0);
     }
   };
   if (!chunk) {
@@ -289,120 +301,147 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   }
   const float c2 = a.scale_log2;
 
-  if (t_begin < t_end) store_tile(0, t_begin);
-  __syncthreads();
-  for (int tile = t_begin; tile < t_end; ++tile) {
-    const int st = (tile - t_begin) & 1;
-    const bool next = tile + 1 < t_end;
-    if (next) load_tile(tile + 1);
-    const int flag = __builtin_amdgcn_readfirstlane(s_flag[st]);
-    const bool mask = (flag & 2) != 0;
+  // scores of 32 rows: rows half * 32 .. of stage st against the wave's columns
+  auto product = [&](int st, int half, f32x16 (&s)[NCB]) {
+    const char* const yb = s_y[st] + (32 * half + cl) * kMRow;
 #pragma unroll
-    for (int half = 0; half < kTile / 32; ++half) {
-      f32x16 s[NCB];
+    for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb)
+      for (int r = 0; r < 16; ++r) s[cb][r] = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[cb][r] = 0.0f;
-      const char* const yb = s_y[st] + (32 * half + cl) * kMRow;
+    for (int kk = 0; kk < KK; ++kk) {
+      u32x4 f[NP];
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        u32x4 f[NP];
+      for (int p = 0; p < NP; ++p) f[p] = *(const u32x4*)(yb + p * kPart + (((2 * kk + hl) ^ (cl & 15)) << 4));
 #pragma unroll
-        for (int p = 0; p < NP; ++p) f[p] = *(const u32x4*)(yb + p * kPart + (((2 * kk + hl) ^ (cl & 15)) << 4));
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-          if constexpr (NP == 1) {
-            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
-          } else {  // the smallest products first
-            s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
-            s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
-          }
+      for (int cb = 0; cb < NCB; ++cb) {
+        if constexpr (NP == 1) {
+          s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
+        } else {  // the smallest products first
+          s[cb] = E16<MT>::mfma(f[0], x[2][cb][kk], s[cb]);
+          s[cb] = E16<MT>::mfma(f[2], x[0][cb][kk], s[cb]);
+          s[cb] = E16<MT>::mfma(f[1], x[1][cb][kk], s[cb]);
+          s[cb] = E16<MT>::mfma(f[0], x[1][cb][kk], s[cb]);
+          s[cb] = E16<MT>::mfma(f[1], x[0][cb][kk], s[cb]);
+          s[cb] = E16<MT>::mfma(f[0], x[0][cb][kk], s[cb]);
         }
-      }
-      const float* const add_row = s_add[st] + 32 * half + 4 * hl;
-      const float* const mul_row = s_mul[st] + (PASS == 1 ? 32 * half + 4 * hl : 0);
-      const int* const t_row = s_t[st] + 32 * half + 4 * hl;
-      // register r of a block is row 8 (r / 4) + 4 hl + r % 4 of the half
-      if (PASS == 0) {
-        const bool plain = flag == 0;
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-          float p = 0.0f;
-          const float base = is_neg_inf(m_run[cb]) ? 0.0f : m_run[cb];
-          if (plain) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) p += mexp2(__builtin_fmaf(s[cb][r], c2, -base));
-          } else {
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-              const f32x4 add = *(const f32x4*)(add_row + 8 * r4);
-              const int4 t4 = *(const int4*)(t_row + 8 * r4);
-              const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float v = __builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]);
-                if (tt[i] > ct[cb]) v = -INFINITY;
-                s[cb][4 * r4 + i] = v;
-                p += mexp2(v - base);
-              }
-            }
-          }
-          if (__ballot(is_neg_inf(m_run[cb]) || p > kMLarge)) {
-            float mx = m_run[cb];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              if (plain) s[cb][r] *= c2;
-              mx = __builtin_fmaxf(mx, s[cb][r]);
-            }
-            const float top = is_neg_inf(mx) ? 0.0f : mx;
-            sum[cb] *= mexp2(m_run[cb] - top);
-            p = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) p += mexp2(s[cb][r] - top);
-            m_run[cb] = mx;
-          }
-          sum[cb] += p;
-        }
-      } else {
-        float part[NCB];  // a half's 16 rows by themselves: long sums lose less
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) part[cb] = 0.0f;
-        if (!mask) {
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 add = *(const f32x4*)(add_row + 8 * r4), mul = *(const f32x4*)(mul_row + 8 * r4);
-#pragma unroll
-            for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                part[cb] = __builtin_fmaf(mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])), mul[i], part[cb]);
-          }
-        } else {
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 add = *(const f32x4*)(add_row + 8 * r4), mul = *(const f32x4*)(mul_row + 8 * r4);
-            const int4 t4 = *(const int4*)(t_row + 8 * r4);
-            const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
-#pragma unroll
-            for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float p = mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])) * mul[i];
-                part[cb] += tt[i] < ct[cb] ? 0.0f : p;
-              }
-          }
-        }
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) sum[cb] += part[cb];
       }
     }
-    if (next) store_tile(st ^ 1, tile + 1);
-    __syncthreads();
+  };
+  // The exponentials of 32 rows' scores into the columns' sums, `next` (the following rows' product,
+  // if any) issued first: one MFMA to every few of these instructions, so that the matrix unit works
+  // under them.  Register r of a block is row 8 (r / 4) + 4 hl + r % 4 of the half.
+  auto reduce = [&](const f32x16 (&s)[NCB], int mt, int half, auto&& next) {
+    const int flag = __builtin_amdgcn_readfirstlane(s_flag[mt]);
+    const float* const add_row = s_add[mt] + 32 * half + 4 * hl;
+    const float* const mul_row = s_mul[mt] + (PASS == 1 ? 32 * half + 4 * hl : 0);
+    const int* const t_row = s_t[mt] + 32 * half + 4 * hl;
+    float part[NCB];  // of these rows alone: long sums lose less
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) part[cb] = 0.0f;
+    if (PASS == 0) {
+      // the 16 scores of the lane's query in log2 units, to f
+      auto each = [&](int cb, auto&& f) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 add = *(const f32x4*)(add_row + 8 * r4);
+          const int4 t4 = *(const int4*)(t_row + 8 * r4);
+          const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = __builtin_fmaf(s[cb][4 * r4 + i], c2, add[i]);
+            f(tt[i] > ct[cb] ? -INFINITY : v);
+          }
+        }
+      };
+      float base[NCB];
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) base[cb] = is_neg_inf(m_run[cb]) ? 0.0f : m_run[cb];
+      if (flag == 0) {
+        next();
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) part[cb] += mexp2(__builtin_fmaf(s[cb][r], c2, -base[cb]));
+        interleave();
+      } else {
+        next();
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) each(cb, [&](float v) { part[cb] += mexp2(v - base[cb]); });
+      }
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        if (__ballot(is_neg_inf(m_run[cb]) || part[cb] > kMLarge)) {
+          float mx = m_run[cb];
+          each(cb, [&](float v) { mx = __builtin_fmaxf(mx, v); });
+          const float top = is_neg_inf(mx) ? 0.0f : mx;
+          sum[cb] *= mexp2(m_run[cb] - top);
+          part[cb] = 0.0f;
+          each(cb, [&](float v) { part[cb] += mexp2(v - top); });
+          m_run[cb] = mx;
+        }
+        sum[cb] += part[cb];
+      }
+    } else {
+      if ((flag & 2) == 0) {
+        next();
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 add = *(const f32x4*)(add_row + 8 * r4), mul = *(const f32x4*)(mul_row + 8 * r4);
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              part[cb] = __builtin_fmaf(mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])), mul[i], part[cb]);
+        }
+        interleave();
+      } else {
+        next();
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 add = *(const f32x4*)(add_row + 8 * r4), mul = *(const f32x4*)(mul_row + 8 * r4);
+          const int4 t4 = *(const int4*)(t_row + 8 * r4);
+          const int tt[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = mexp2(__builtin_fmaf(s[cb][4 * r4 + i], c2, add[i])) * mul[i];
+              part[cb] += tt[i] < ct[cb] ? 0.0f : p;
+            }
+        }
+      }
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) sum[cb] += part[cb];
+    }
+  };
+
+  if (t_begin < t_end) store_tile(0, 0, t_begin);
+  __syncthreads();
+  constexpr int kHalves = kTile / 32;
+  f32x16 cur[NCB], nxt[NCB];
+  if (kHalves == 2 && t_begin < t_end) product(0, 0, cur);
+  int mt = 0;
+  for (int tile = t_begin; tile < t_end; ++tile) {
+    const int st = (tile - t_begin) & 1, mn = mt == 2 ? 0 : mt + 1;
+    const bool more = tile + 1 < t_end;
+    if (more) load_tile(tile + 1);
+    if constexpr (kHalves == 2) {
+      reduce(cur, mt, 0, [&] { product(st, 1, nxt); });
+      if (more) {
+        store_tile(st ^ 1, mn, tile + 1);
+        __syncthreads();
+        reduce(nxt, mt, 1, [&] { product(st ^ 1, 0, cur); });
+      } else {
+        reduce(nxt, mt, 1, [] {});
+      }
+    } else {
+      product(st, 0, cur);
+      reduce(cur, mt, 0, [] {});
+      if (more) store_tile(st ^ 1, mn, tile + 1);
+      __syncthreads();
+    }
+    mt = mn;
   }
 
   // ---- the two halves of a column, then out ----
@@ -465,12 +504,20 @@ __global__ __launch_bounds__(256) void mass_join_cols_kernel(const float* part, 
   mass[i] = v;
 }
 
-// Splits of the streamed rows: workgroups for every CU a few times over, and at least 128 rows
-// each.
+// Splits of the streamed rows.  Where pieces of 128 rows (two stages) do not fill the chip's 512
+// places, a call is latency and takes them all (64 queries over 2048 keys: 20.5 us, with pieces of 256
+// 25.6); else pieces of at least 256 rows, for 1024 workgroups, so that the longest end early (1024
+// tokens of 8 x 4 heads 38.6 us, with pieces of 128 51; 8192 tokens 674, for 512 workgroups 837).
 static int mass_split(int64_t blocks, int64_t streamed) {
-  int64_t want = (1024 + blocks - 1) / blocks;
-  const int64_t most = (streamed + 127) / 128;
-  if (want > most) want = most;
+  const int64_t pieces = (streamed + 127) / 128;
+  int64_t want;
+  if (blocks * pieces <= 512) {
+    want = pieces;
+  } else {
+    want = (1024 + blocks - 1) / blocks;
+    const int64_t most = (streamed + 255) / 256;
+    if (want > most) want = most;
+  }
   if (want > 64) want = 64;
   return (int)(want < 1 ? 1 : want);
 }
