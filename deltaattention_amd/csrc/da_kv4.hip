@@ -856,7 +856,8 @@ static int launch_heavy(const float* mass, const int32_t* lengths, int64_t BH, i
     hipLaunchKernelGGL(heavy_rows_kernel, dim3((unsigned)BH), dim3(kHeavyThreads), 0, st, a);
     return check_launch(who);
   }
-  DA_REQUIRE(BH * w.chunks < (1ll << 31), "%s: more than 2^31 workgroups", who);
+  // a launch holds fewer than 2^32 threads
+  if (BH * w.chunks >= (1ll << 22)) return set_error(DA_ERR_UNSUPPORTED, "%s: too many rows for one call", who);
   const dim3 all((unsigned)(BH * w.chunks)), heads((unsigned)BH);
   hipLaunchKernelGGL(heavy_hist_kernel, all, dim3(kHeavyThreads), 0, st, a, w);
   hipLaunchKernelGGL(heavy_bin_kernel, heads, dim3(kHeavyThreads), 0, st, a, w);
@@ -897,7 +898,8 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   a.N = N; a.M = M; a.capacity = out->capacity; a.B = (int)B; a.H = (int)Hkv; a.D = (int)D;
   const int groups = (int)((D + 31) / 32);
   const int64_t blocks = ((M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems) + 7) / 8 * 8;
-  DA_REQUIRE(blocks * B * Hkv < (1ll << 31), "%s: more than 2^31 workgroups", who);
+  // a launch holds fewer than 2^32 threads
+  if (blocks * B * Hkv >= (1ll << 24)) return set_error(DA_ERR_UNSUPPORTED, "%s: too many rows for one call", who);
   const dim3 grid((unsigned)(blocks * B * Hkv), 3);  // blocks: a multiple of eight
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) launch_quantize<DA_F32>(a, groups, grid, st);

@@ -68,7 +68,6 @@ constexpr int kA4Part = 128;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                  0, 0);
@@ -630,7 +629,8 @@ extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq,
   a.stat = a.part + n * kA4Part;
   a.score = a.stat + kv4_stat_floats(n);
   const unsigned long long blocks = (unsigned long long)(B * Hq) + (unsigned long long)(B * Hkv) * ((kv->capacity + kMassKeys - 1) / kMassKeys);
-  DA_REQUIRE(B * Hkv < (1ll << 31) && blocks < (1ull << 31), "%s: too many heads", who);
+  // a launch holds fewer than 2^32 threads
+  if (B * Hkv >= (1 << 20) || blocks >= (1ull << 24)) return set_error(DA_ERR_UNSUPPORTED, "%s: too many heads and rows for one call", who);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) return launch_attn4<DA_F32>(a, accumulate != 0, st, who);
   if (dtype == DA_F16) return launch_attn4<DA_F16>(a, accumulate != 0, st, who);

@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   // the rows' times and weights.
   const int sr = tid >> 4, sc = tid & 15;
   const bool chunk = 8 * sc < a.D;  // chunks past the head dimension stay zero
-  const bool stepped = PASS == 0 || a.gshift >= 0;
+  const bool stepped = PASS == 0 || (a.gshift >= 0 && kTile >> a.gshift != 0);
   const int64_t step = (PASS == 0 ? kTile * a.sk_n : (int64_t)(kTile >> (a.gshift >= 0 ? a.gshift : 0)) * a.sq_n) * es;
   auto row_src = [&](int row) {
     if (PASS == 0) return kb + row * a.sk_n * es;
@@ -611,8 +611,10 @@ extern "C" int da_attention_mass(const void* q, const void* k, int dtype, int64_
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
   DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   const MassPlan p = mass_plan(dtype, B, Hq, Hkv, Nq, Nk);
-  if (p.rows >= (1ll << 30) || B * Hkv * p.split0 * p.blocks0 >= (1ll << 31) || B * Hkv * p.split1 * p.blocks1 >= (1ll << 31))
-    return set_error(DA_ERR_UNSUPPORTED, "%s: more than 2^30 query rows a KV head, or 2^31 workgroups", who);
+  // a launch holds fewer than 2^32 threads
+  if (p.rows >= (1ll << 30) || B * Hkv * p.split0 * p.blocks0 >= (1ll << 24) ||
+      B * Hkv * p.split1 * p.blocks1 >= (1ll << 24) || B * Hkv * p.rows >= (1ll << 28) || B * Hkv * Nk >= (1ll << 32))
+    return set_error(DA_ERR_UNSUPPORTED, "%s: too many query rows or keys for one call", who);
   MassArgs a = {};
   a.q = q; a.k = k;
   a.sq_b = sq_b; a.sq_h = sq_h; a.sq_n = sq_n; a.sk_b = sk_b; a.sk_h = sk_h; a.sk_n = sk_n;

@@ -129,7 +129,7 @@ int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hk
  * that sees no key adds nothing.  q [B, Hq, Nq, D], k [B, Hkv, Nk, D] of one type (bf16, fp16
  * or fp32), rows 16-byte aligned; counts, timestamps [B, Hkv, Nk] int32 contiguous or null;
  * mass [B, Hkv, Nk] fp32 contiguous, 0 from the length on.  Deterministic.  Hq / Hkv <= 64,
- * Nq * Hq / Hkv < 2^30, Nq, Nk <= 2^24, B * Hkv <= 65535.  workspace: da_attention_mass_workspace_size() bytes.
+ * Nq * Hq / Hkv < 2^30, Nq, Nk <= 2^24, B * Hkv <= 65535 (and fewer than 2^32 threads a launch).  workspace: da_attention_mass_workspace_size() bytes.
  */
 int64_t da_attention_mass_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq, int64_t Nk);
 int da_attention_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq,
