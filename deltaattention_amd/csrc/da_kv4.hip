@@ -73,19 +73,13 @@ __device__ __forceinline__ uint32_t group_exponent(uint32_t top) {
 // A lane takes 8 dims: 16 bytes of a 16-bit row (32 of an fp32 one), 4 bytes of codes; the
 // four lanes of a quad are one group, whose largest magnitude is two quad permutes away.
 // Lanes per row: 4 NG.  Each thread takes kQuantItems of them, a block's width apart, with
-// all of its loads in flight.  blockIdx.y = key, value or the
-// rows' small fields.  Workgroups go to the XCDs in turn, so
-// eight row blocks are interleaved and the (sequence, head) pairs of one follow each other on one
-// XCD: where projections lay the heads of a token side by side, that XCD reads whole tokens (by
-// head, each L2 would see one 256-byte piece in 2 KiB, two of its 16 channels: 101 us a 64K-token
-// prompt against XXX).
+// all of its loads in flight (64K tokens of 8 heads of 128 bf16 dims, as projections lay them out:
+// 65 us, 5.3 TB/s; one item a thread 74, four 65).  blockIdx.z = key, value or the rows' small fields.
 constexpr int kQuantItems = 2;
 template <int DT, int NG>
 __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
   constexpr uint32_t kLpr = 4 * NG;
-  const uint32_t nbh = a.B * a.H, turn = blockIdx.x >> 3, eight = turn / nbh;
-  const uint32_t blk = 8 * eight + (blockIdx.x & 7);
-  const int bh = turn - eight * nbh, z = blockIdx.y;
+  const int bh = blockIdx.y, z = blockIdx.z;
   const int b = bh / a.H, h = bh - b * a.H;
   const uint32_t M = (uint32_t)a.M;
   uint32_t len = M;
@@ -94,7 +88,7 @@ __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
     len = n < 0 ? 0 : ((uint32_t)n > M ? M : (uint32_t)n);
   }
   if (z == 2) {  // the rows' small fields, a lane each
-    for (uint32_t m = blk * 256 + threadIdx.x; m < M; m += gridDim.x / nbh * 256) {
+    for (uint32_t m = blockIdx.x * 256 + threadIdx.x; m < M; m += gridDim.x * 256) {
       int s = m < len ? (a.index ? a.index[(int64_t)bh * M + m] : (int)m) : -1;
       const bool real = s >= 0 && s < a.N;
       const int64_t row = bh * a.capacity + m, from = bh * a.N + (real ? s : 0);
@@ -106,7 +100,7 @@ __global__ __launch_bounds__(256) void quantize4_kernel(Quant4Args a) {
     return;
   }
   const char* base = (const char*)a.x[z] + (b * a.s_b[z] + h * a.s_h[z]) * (DT == DA_F32 ? 4 : 2);
-  const uint32_t first = blk * 256 * kQuantItems + threadIdx.x;  // below 2^31: capacity <= 2^26
+  const uint32_t first = blockIdx.x * 256 * kQuantItems + threadIdx.x;  // below 2^31: capacity <= 2^26
   float x[kQuantItems][8];
   int src[kQuantItems];
 #pragma unroll
@@ -897,10 +891,8 @@ extern "C" int da_kv4_quantize(const void* k, const void* v, int dtype, int64_t 
   a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass; a.o_lengths = out->lengths;
   a.N = N; a.M = M; a.capacity = out->capacity; a.B = (int)B; a.H = (int)Hkv; a.D = (int)D;
   const int groups = (int)((D + 31) / 32);
-  const int64_t blocks = ((M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems) + 7) / 8 * 8;
-  // a launch holds fewer than 2^32 threads
-  if (blocks * B * Hkv >= (1ll << 24)) return set_error(DA_ERR_UNSUPPORTED, "%s: too many rows for one call", who);
-  const dim3 grid((unsigned)(blocks * B * Hkv), 3);  // blocks: a multiple of eight
+  const int64_t blocks = (M * 4 * groups + 256 * kQuantItems - 1) / (256 * kQuantItems);
+  const dim3 grid((unsigned)blocks, (unsigned)(B * Hkv), 3);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F32) launch_quantize<DA_F32>(a, groups, grid, st);
   else if (dtype == DA_F16) launch_quantize<DA_F16>(a, groups, grid, st);

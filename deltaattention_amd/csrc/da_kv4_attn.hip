@@ -579,7 +579,9 @@ static int64_t kv4_stat_floats(int64_t n) { return (2 * n + 3) / 4 * 4; }
 extern "C" int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t capacity,
                                                    int accumulate) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || capacity <= 0) return 0;
-  const int64_t n = B * Hq * kv4_splits(B, Hkv, Hq / Hkv, capacity);
+  const int splits = kv4_splits(B, Hkv, Hq / Hkv, capacity);
+  if (splits == 1 && !accumulate) return 0;  // one launch writes the output
+  const int64_t n = B * Hq * splits;
   const int64_t scores = accumulate ? B * Hq * kv4_score_cap(capacity) : 0;
   return (n * kA4Part + kv4_stat_floats(n) + scores) * (int64_t)sizeof(float);
 }
@@ -611,7 +613,7 @@ extern "C" int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq,
   DA_REQUIRE((((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) & 15) == 0, "%s: codes must be 16-byte aligned", who);
   DA_REQUIRE(scale > 0.0f, "%s: scale must be positive", who);
   const int64_t need = da_kv4_attention_workspace_size(B, Hq, Hkv, kv->capacity, accumulate);
-  if (!workspace || workspace_bytes < need)
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
   DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   Attn4Args a = {};

@@ -197,6 +197,18 @@ class KV4:
         _set(self, name, t)
         return t
 
+    def clone(self) -> "KV4":
+        """A copy in memory of its own (of the rows past the lengths too)."""
+        out = KV4.empty(self.batch, self.kv_heads, self.capacity, self.head_dim, self.device, self.mass is not None)
+        for name in _TENSORS:
+            t = getattr(self, name)
+            if t is not None:
+                getattr(out, name).copy_(t)
+        return out
+
+    def __deepcopy__(self, memo):
+        return self.clone()
+
 
 def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tensor] = None,
                    timestamps: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
@@ -439,9 +451,9 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
         raise ValueError("out must have q's shape and device and a contiguous head dimension")
     so = out.stride()
     n = _attention_bytes(B, Hq, H, kv.capacity, 1 if accumulate else 0)
-    ws = torch.empty((n,), dtype=_U8, device=device)
+    ws = torch.empty((n,), dtype=_U8, device=device) if n else None  # held until the call is on its stream
     rc = call_on(device, lib().da_kv4_attention, q.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, kx, vx, sx[0],
                  sx[1], sx[2], n_exact, D ** -0.5 if scale is None else scale, 1 if accumulate else 0, out.data_ptr(),
-                 so[0], so[1], ws.data_ptr(), n)
+                 so[0], so[1], ws.data_ptr() if n else None, n)
     check(rc, "da_kv4_attention")
     return out

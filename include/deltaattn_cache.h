@@ -28,10 +28,9 @@ extern "C" {
  *
  * All arrays are contiguous: codes [B, Hkv, capacity, 16 groups], exponents [B, Hkv,
  * capacity, groups], counts / timestamps / mass [B, Hkv, capacity], lengths [B, Hkv] (rows in
- * use; clamped into [0, capacity] where read).  Codes must be 16-byte
- * aligned, exponents 4-byte.  mass (the
- * attention weight each row has received) may be null where a call does not use it.  At most
- * 2^26 rows a head and 65535 (sequence, head) pairs.
+ * use; clamped into [0, capacity] where read).  Codes must be 16-byte aligned, exponents
+ * 4-byte.  mass (the attention weight each row has received) may be null where a call does not
+ * use it.  At most 2^26 rows a head and 65535 (sequence, head) pairs.
  */
 typedef struct DaKv4 {
   uint8_t* k_codes;
@@ -113,7 +112,7 @@ int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t B, int64_t 
  * The rows' values enter as they are (bf16 holds them exactly), q and the weights in two or
  * three 16-bit parts, sums in fp32.  accumulate: kv->mass[b, g, j] += the softmax weight of
  * row j, summed over the query heads of the group.  Hq / Hkv <= 64, capacity <= 2^24.
- * workspace: da_kv4_attention_workspace_size() bytes.
+ * workspace: da_kv4_attention_workspace_size() bytes (none, and null, for a short cache).
  */
 int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t capacity, int accumulate);
 int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t sq_b,
@@ -129,7 +128,8 @@ int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hk
  * that sees no key adds nothing.  q [B, Hq, Nq, D], k [B, Hkv, Nk, D] of one type (bf16, fp16
  * or fp32), rows 16-byte aligned; counts, timestamps [B, Hkv, Nk] int32 contiguous or null;
  * mass [B, Hkv, Nk] fp32 contiguous, 0 from the length on.  Deterministic.  Hq / Hkv <= 64,
- * Nq * Hq / Hkv < 2^30, Nq, Nk <= 2^24, B * Hkv <= 65535 (and fewer than 2^32 threads a launch).  workspace: da_attention_mass_workspace_size() bytes.
+ * Nq * Hq / Hkv < 2^30, Nq, Nk <= 2^24, B * Hkv <= 65535, fewer than 2^32 threads a launch.
+ * workspace: da_attention_mass_workspace_size() bytes.
  */
 int64_t da_attention_mass_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq, int64_t Nk);
 int da_attention_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq,

@@ -210,3 +210,28 @@ def test_model(gpu, knobs, impl):
     for layer in range(2):
         assert 0 < int(cache.packed_lengths[layer].max()) <= 104
         assert float(cache.anchors[layer].mass[:, :, :16].sum()) > 0
+
+
+def test_deepcopy(gpu, knobs):
+    """A prompt's cache can be copied and continued twice: the copies share nothing."""
+    import copy
+    from deltaattention_amd import attention
+    from deltaattention_amd.deltaDecoding import FourBitCompressedCache
+    knobs.row_delta_threshold, knobs.row_similarity_metric = 6.0, "euclidean"
+    Hkv, G, D, N, W = 2, 4, 64, 300, 16
+    q, k, v = (t.to(gpu) for t in _inputs(1, Hkv * G, Hkv, N + 30, D, "bf16", 3))
+    announce("four-bit deepcopy")
+    cache = FourBitCompressedCache(_config(Hkv * G, Hkv, D), 1, dtype=torch.bfloat16, exact_window_size=W, budget=64,
+                                   recent=16, slack=8)
+    attention.delta_prefill_attention(q[:, :, :N], k[:, :, :N], v[:, :, :N], 0, cache)
+    bare = cache.anchors[0]
+    twin = copy.deepcopy(cache)
+    outs = []
+    for c in (cache, twin):
+        before = bare.lengths.clone(), bare.mass.clone()
+        outs.append([c.decode_step(q[:, :, t:t + 1], k[:, :, t:t + 1], v[:, :, t:t + 1], 0) for t in range(N, N + 30)])
+        if c is twin:
+            assert torch.equal(bare.lengths, before[0]) and torch.equal(bare.mass, before[1])
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+    assert copy.deepcopy(bare).mass.data_ptr() != bare.mass.data_ptr()
