@@ -474,7 +474,7 @@ constexpr int kChunkPer = 4, kChunk = kHeavyThreads * kChunkPer;
 struct HeavyWork {      // per head and chunk, in the workspace
   uint32_t* hist;       // [bh][chunks][kHeavyBins]
   uint32_t* list;       // [bh][chunks][kChunk]: orders of the rows of the border's bin
-  uint32_t* count;      // [bh][chunks][4]: rows in the list; rows above and at the border before the chunk
+  uint32_t* count;      // [bh][chunks][4]: rows in the list; rows above (first: in higher bins) and at the border
   uint32_t* border;     // [bh][4]: bin, rows needed of it; border, equals needed
   int chunks;
 };
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_bin_kernel(HeavyArgs a, H
   if (n > a.budget && need > 0) {
     uint32_t c0 = 0, c1 = 0;
     const u32x2* h = (const u32x2*)(const void*)(w.hist + (int64_t)bh * w.chunks * kHeavyBins) + tid;
-#pragma unroll 8
+#pragma unroll 16
     for (int c = 0; c < w.chunks; ++c) {
       const u32x2 v = h[(int64_t)c * (kHeavyBins / 2)];
       c0 += v[0];
@@ -537,20 +537,22 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_bin_kernel(HeavyArgs a, H
 }
 
 __global__ __launch_bounds__(kHeavyThreads) void heavy_list_kernel(HeavyArgs a, HeavyWork w) {
-  __shared__ uint32_t s_fill;
+  __shared__ uint32_t s_fill, s_above;
   const int bh = blockIdx.x / w.chunks, c = blockIdx.x - bh * w.chunks, tid = threadIdx.x, lane = tid & 63;
   const int n = heavy_length(a, bh);
   if (n <= a.budget) return;
   const uint32_t bin = w.border[4 * bh];
-  if (tid == 0) s_fill = 0;
+  if (tid == 0) s_fill = s_above = 0;
   uint32_t u[kChunkPer];
   bool in[kChunkPer];
   chunk_masses(a, bh, c * kChunk, a.sinks, n - a.recent, u, in);
   __syncthreads();
   uint32_t* const list = w.list + (int64_t)blockIdx.x * kChunk;
+  uint32_t above = 0;  // of this wave
 #pragma unroll
   for (int j = 0; j < kChunkPer; ++j) {
     const bool hit = in[j] && (u[j] >> 21) == bin;
+    above += (uint32_t)__popcll(__ballot(in[j] && (u[j] >> 21) > bin));
     const uint64_t act = __ballot(hit);
     if (act) {
       uint32_t at = 0;
@@ -559,8 +561,12 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_list_kernel(HeavyArgs a, 
       if (hit) list[at] = u[j];
     }
   }
+  if (lane == 0 && above) atomicAdd(&s_above, above);
   __syncthreads();
-  if (tid == 0) w.count[4 * blockIdx.x] = s_fill;
+  if (tid == 0) {
+    w.count[4 * blockIdx.x] = s_fill;
+    w.count[4 * blockIdx.x + 1] = s_above;
+  }
 }
 
 __global__ __launch_bounds__(kHeavyThreads) void heavy_border_kernel(HeavyArgs a, HeavyWork w) {
@@ -585,9 +591,13 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_border_kernel(HeavyArgs a
       __syncthreads();
       for (int c = wid; c < w.chunks; c += kHeavyWaves) {
         const uint32_t fill = count[4 * c];
-        for (uint32_t i0 = 0; i0 < fill; i0 += 64) {
-          const uint32_t i = i0 + lane, v = i < fill ? list[(int64_t)c * kChunk + i] : 0;
-          count_bin(s_hist, i < fill && (v & mask) == prefix, (v >> shift) & bits, lane);
+        for (uint32_t i0 = 0; i0 < fill; i0 += 256) {
+          uint32_t v[4];
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) v[j] = i0 + 64 * j + lane < fill ? list[(int64_t)c * kChunk + i0 + 64 * j + lane] : 0;
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+            count_bin(s_hist, i0 + 64 * j + lane < fill && (v[j] & mask) == prefix, (v[j] >> shift) & bits, lane);
         }
       }
       __syncthreads();
@@ -601,14 +611,13 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_border_kernel(HeavyArgs a
     w.border[4 * bh + 2] = any ? prefix : 0xffffffffu;
     w.border[4 * bh + 3] = any ? need : 0;
   }
-  // rows of each chunk above the border (higher bins, and in the list) and at it
+  // rows of each chunk above the border (the list kernel counted those of higher bins) and at it
   for (int c = wid; c < w.chunks; c += kHeavyWaves) {
     uint32_t g = 0, e = 0;
     if (any) {
-      const uint32_t* const h = w.hist + ((int64_t)bh * w.chunks + c) * kHeavyBins;
-#pragma unroll 8
-      for (uint32_t i = bin + 1 + lane; i < kHeavyBins; i += 64) g += h[i];
       const uint32_t fill = count[4 * c];
+      g = lane == 0 ? count[4 * c + 1] : 0;
+#pragma unroll 4
       for (uint32_t i = lane; i < fill; i += 64) {
         const uint32_t v = list[(int64_t)c * kChunk + i];
         g += v > prefix ? 1 : 0;
