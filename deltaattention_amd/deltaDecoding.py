@@ -5,7 +5,8 @@
 counts / timestamps / lengths, and an exact ring [L, B, Hkv, W, D].  The decode update
 and decode attention run the gfx950 kernels of libdeltaattn.so; the kernel objects
 ``fused_hybrid_decode_update_kernel`` and ``fused_hybrid_decode_kernel`` accept the
-reference's ``kernel[grid](...)`` launch.  bf16 caches only.
+reference's ``kernel[grid](...)`` launch.  Caches are bf16, fp16 or fp32;
+:class:`FourBitCompressedCache` holds the anchors in 4 bits and bounds their number.
 """
 from __future__ import annotations
 
