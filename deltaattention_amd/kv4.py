@@ -83,6 +83,29 @@ _set = object.__setattr__
 _TENSORS = ("k_codes", "k_scales", "v_codes", "v_scales", "counts", "timestamps", "lengths", "mass")
 
 
+@functools.lru_cache(maxsize=1024)
+def _layout(B: int, H: int, cap: int, D: int, mass: bool):
+    """One allocation's bytes, its fields' offsets in Kv4Block's order, and each one's view."""
+    g, size, at, views = (D + 31) // 32, 0, [], {}
+    rows, row_stride = (B, H, cap), (H * cap, cap, 1)
+    for name, width, dtype in (("k_codes", 16 * g, _U8), ("k_scales", g, _U8), ("v_codes", 16 * g, _U8),
+                               ("v_scales", g, _U8), ("counts", 4, _I32), ("timestamps", 4, _I32),
+                               ("lengths", 4, _I32), ("mass", 4, _F32)):
+        if name == "mass" and not mass:
+            at.append(None)
+            views[name] = None
+            continue
+        at.append(size)
+        if dtype == _U8:
+            views[name] = dtype, rows + (width,), (H * cap * width, cap * width, width, 1), size
+        elif name == "lengths":
+            views[name] = dtype, (B, H), (H, 1), size // 4
+        else:
+            views[name] = dtype, rows, row_stride, size // 4
+        size += (B * H * (1 if name == "lengths" else cap) * width + 255) & ~255
+    return size, at, views
+
+
 class KV4:
     """Key and value rows of one layer in 4 bits, for every (sequence, KV head).
 
@@ -156,44 +179,28 @@ class KV4:
         B, H, cap, D = int(batch), int(kv_heads), int(capacity), int(head_dim)
         if not (B > 0 and H > 0 and cap > 0) or D <= 0 or D > 128 or D % 8:
             raise ValueError(f"no cache of {batch} sequences, {kv_heads} heads, {capacity} rows and head_dim {head_dim}")
-        n, g = B * H * cap, (D + 31) // 32
-        up = lambda x: (x + 255) & ~255  # noqa: E731
-        codes, scales, field, heads = up(16 * g * n), up(g * n), up(4 * n), up(4 * B * H)
-        at = {"k_codes": 0, "v_codes": codes, "k_scales": 2 * codes, "v_scales": 2 * codes + scales}
-        end = 2 * (codes + scales)
-        for name in ("counts", "timestamps", "mass") if mass else ("counts", "timestamps"):
-            at[name] = end
-            end += field
-        at["lengths"] = end
-        own = torch.empty((end + heads,), dtype=_U8, device=device)
+        size, at, views = _layout(B, H, cap, D, bool(mass))
+        own = torch.empty((size,), dtype=_U8, device=device)
         device, p = _gpu(own, "the cache"), own.data_ptr()
         self = cls.__new__(cls)
-        self._put(B, H, cap, D, device, Kv4Block(
-            p, p + 2 * codes, p + codes, p + 2 * codes + scales, p + at["counts"], p + at["timestamps"],
-            p + at["lengths"], p + at["mass"] if mass else None, cap), [at, own, None, None])
+        self._put(B, H, cap, D, device, Kv4Block(*[None if x is None else p + x for x in at], cap),
+                  (views, {_U8: own}))
         return self
 
     def __getattr__(self, name):
         # only for what is not there yet: a tensor of a cache that empty() made
         if name not in _TENSORS:
             raise AttributeError(name)
-        at, own, ints, floats = self._own
-        first = at.get(name)
-        B, H, cap, g = self.batch, self.kv_heads, self.capacity, (self.head_dim + 31) // 32
-        if first is None:  # a cache without mass
+        views, own = self._own
+        view = views[name]
+        if view is None:  # a cache without mass
             t = None
-        elif name in ("counts", "timestamps", "lengths"):
-            if ints is None:
-                ints = self._own[2] = own.view(_I32)
-            t = ints.as_strided((B, H), (H, 1), first // 4) if name == "lengths" else \
-                ints.as_strided((B, H, cap), (H * cap, cap, 1), first // 4)
-        elif name == "mass":
-            if floats is None:
-                floats = self._own[3] = own.view(_F32)
-            t = floats.as_strided((B, H, cap), (H * cap, cap, 1), first // 4)
         else:
-            w = 16 * g if name in ("k_codes", "v_codes") else g
-            t = own.as_strided((B, H, cap, w), (H * cap * w, cap * w, w, 1), first)
+            dtype, shape, stride, first = view
+            base = own.get(dtype)
+            if base is None:
+                base = own[dtype] = own[_U8].view(dtype)
+            t = base.as_strided(shape, stride, first)
         _set(self, name, t)
         return t
 
