@@ -495,31 +495,39 @@ __global__ __launch_bounds__(256) void mass_join_rows_kernel(const float* part, 
   if (l == 0 && i < rows) ((f32x2*)(void*)stats)[i] = row_stats(M, L);
 }
 
-// The splits' column sums, added in order.
+// The splits' column sums: 32 columns a workgroup, eight threads a column that take every eighth
+// split, joined in order.
 __global__ __launch_bounds__(256) void mass_join_cols_kernel(const float* part, float* mass, int64_t cols, int split) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= cols) return;
+  __shared__ float s_v[8][32];
+  const int c = threadIdx.x & 31, sg = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + c;
   float v = 0.0f;
-  for (int s = 0; s < split; ++s) v += part[(int64_t)s * cols + i];
-  mass[i] = v;
+  if (i < cols) {
+#pragma unroll 4
+    for (int s = sg; s < split; s += 8) v += part[(int64_t)s * cols + i];
+  }
+  s_v[sg][c] = v;
+  __syncthreads();
+  if (sg == 0 && i < cols) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += s_v[k][c];
+    mass[i] = v;
+  }
 }
 
 // Splits of the streamed rows.  Where pieces of 128 rows (two stages) do not fill the chip's 512
-// places, a call is latency and takes them all (64 queries over 2048 keys: 20.5 us, with pieces of 256
-// 25.6); else pieces of at least 256 rows, for 1024 workgroups, so that the longest end early (1024
-// tokens of 8 x 4 heads 38.6 us, with pieces of 128 51; 8192 tokens 674, for 512 workgroups 837).
+// places, a call is latency and takes them all, up to 128 (64 queries over 2048 keys: 20.5 us, with pieces
+// of 256 25.6; over 32768 keys of one head 28.9, with 64 of them 34.3, with 256 28.4 and twice the
+// workspace).  Else pieces of at least 256 rows, for 1024 workgroups, so that the longest end early (1024
+// tokens of 8 x 4 heads 34 us, with pieces of 128 51; 8192 tokens 648, for 512 workgroups 837), up to
+// 64 (1 query over 32768 keys of 8 heads: 43.7, with 128 48.9).
 static int mass_split(int64_t blocks, int64_t streamed) {
   const int64_t pieces = (streamed + 127) / 128;
-  int64_t want;
-  if (blocks * pieces <= 512) {
-    want = pieces;
-  } else {
-    want = (1024 + blocks - 1) / blocks;
-    const int64_t most = (streamed + 255) / 256;
-    if (want > most) want = most;
-  }
-  if (want > 64) want = 64;
-  return (int)(want < 1 ? 1 : want);
+  if (blocks * pieces <= 512) return (int)(pieces < 128 ? pieces : 128);
+  int64_t want = (1024 + blocks - 1) / blocks;
+  const int64_t most = (streamed + 255) / 256;
+  if (want > most) want = most;
+  return (int)(want > 64 ? 64 : want);
 }
 struct MassPlan {
   int cols, split0, split1;
@@ -565,7 +573,7 @@ static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char
   launch_pass<DT, 1>(a, st);
   if (p.split1 > 1) {
     const int64_t cols = bh * a.Nk;
-    hipLaunchKernelGGL(mass_join_cols_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, st, a.part, a.mass,
+    hipLaunchKernelGGL(mass_join_cols_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st, a.part, a.mass,
                        cols, p.split1);
   }
   return check_launch(who);
