@@ -534,18 +534,21 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
 }
 
 // Workgroups of the attention launch: three a CU run at once (its registers), and no split is
-// shorter than a tile a wave; 64 splits are the most that pay their joining (8297 rows x 8 heads:
-// 64 10.2 us, 32 11.8).  A short cache is one workgroup of eight waves a head, without a second
-// launch (8 heads, 500 rows: 8.1 against 9.2 us, 750: 9.7 / 9.3, 1000: 10.9 / 9.2; a launch is 3.4 us
-// of the caller's time as well); 256 heads fill the chip like that (1000 rows: 15.4 / 20.0).
+// shorter than a tile a wave.  64 splits, or of 512 rows as many as there are up to 256, are the most
+// that pay their joining (8 heads of 8297 rows: 64 10.2 us, 32 11.8, 96 12.7; one of 112207: 64 19.2,
+// 128 15.1, 256 15.7; one of 1000000: 64 109, 128 61, 256 43).  A short cache is one workgroup of
+// eight waves a head, without a second launch (8 heads, 500 rows: 8.1 against 9.2 us, 750: 9.7 / 9.3,
+// 1000: 10.9 / 9.2; a launch is 3.4 us of the caller's time as well); 256 heads fill the chip like that
+// (1000 rows: 15.4 / 20.0).
 static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
   const int64_t units = B * Hkv * ((G + kA4Cols - 1) / kA4Cols);
   if (capacity <= (units >= 256 ? 1024 : 768)) return 1;
   const int64_t most = (capacity + kA4Tile * kA4Waves - 1) / (kA4Tile * kA4Waves);
   int64_t want = (768 + units - 1) / units;
-  if (want > 64) want = 64;
+  const int64_t pay = capacity / 512 < 64 ? 64 : capacity / 512 > 256 ? 256 : capacity / 512;
+  if (want > pay) want = pay;
   if (want > most) want = most;
-  return (int)(want < 1 ? 1 : want);
+  return (int)want;
 }
 static int64_t kv4_score_cap(int64_t capacity) { return (capacity + kA4Tile - 1) / kA4Tile * kA4Tile; }
 

@@ -202,6 +202,7 @@ ATTEND = [  # B, H, G, D, cap, lengths, W, exact, dtype
     (2, 1, 8, 128, 777, [776, 5], 128, 128, "fp32"), (1, 2, 4, 24, 100, [100, 99], 0, 0, "fp32"),
     (1, 8, 4, 128, 4100, [4100, 4099, 4096, 3000, 2049, 128, 127, 0], 128, 128, "bf16"),
     (1, 1, 4, 128, 70001, [69999], 64, 64, "fp16"), (5, 3, 2, 56, 97, list(range(0, 98, 7)) + [97], 3, 2, "bf16"),
+    (1, 1, 4, 128, 140000, [139999], 64, 64, "bf16"), (1, 2, 2, 64, 140000, [0, 5], 16, 16, "fp32"),
 ]
 
 
