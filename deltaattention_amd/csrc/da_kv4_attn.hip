@@ -157,13 +157,15 @@ struct Tile4 {
 
 // One workgroup: (sequence, KV head) blockIdx.x, split blockIdx.y, heads 16 z .. of the group.
 // MODE kParts: `nsplit` workgroups a head leave their partials; kScores: and the scores; kWhole: one
-// workgroup of eight waves takes the head and writes the output itself.
-enum Mode4 : int { kParts = 0, kScores = 1, kWhole = 2 };
+// workgroup of eight waves takes the head and writes the output itself; kWholeMass: and adds the weights,
+// its scores in LDS.
+enum Mode4 : int { kParts = 0, kScores = 1, kWhole = 2, kWholeMass = 3 };
+constexpr int kWholeRows = 1024;  // most rows of a cache that one workgroup takes
 template <int DT, int NG, int MODE>
-__global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(
+__global__ __launch_bounds__(MODE >= kWhole ? 512 : 256, MODE >= kWhole || DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(
     Attn4Args a) {
-  constexpr bool MASS = MODE == kScores;
-  constexpr int NW = MODE == kWhole ? 8 : kA4Waves;
+  constexpr bool WHOLE = MODE >= kWhole;
+  constexpr int NW = WHOLE ? 8 : kA4Waves;
   constexpr int QP = DT == DA_BF16 ? 1 : DT == DA_F16 ? 2 : 3;
   constexpr int PP = DT == DA_F32 ? 3 : 2;
   constexpr int NJ = 2 * NG;  // output tiles of 16 dims
@@ -173,6 +175,8 @@ __global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT ==
   __shared__ __attribute__((aligned(16))) char s_v[NW][kTileBytes];
   __shared__ __attribute__((aligned(16))) float s_bias[NW][kA4Tile];
   __shared__ float s_ml[NW][2][kA4Cols];
+  __shared__ __attribute__((aligned(16))) float s_score[MODE == kWholeMass ? kWholeRows * kA4Cols : 4];
+  __shared__ float s_weight[2][kA4Cols];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, t = lane >> 4;
   // The workgroups of a CU are a whole number of rounds apart, which without a turn of the heads
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT ==
   const int nwave = a.nsplit * NW;
   const int rfirst = nwave - 1 - (split * NW + wid);
   const int64_t head_part = ((int64_t)bh * a.G + h0) * a.nsplit + split;  // of column 0; nsplit a column
-  if (MODE != kWhole && t_begin >= t_end && nwave - 1 - (split * NW + NW - 1) >= rtiles) {  // nothing to do
+  if (!WHOLE && t_begin >= t_end && nwave - 1 - (split * NW + NW - 1) >= rtiles) {  // nothing to do
     if (tid < cols) *(f32x2*)(void*)(a.stat + 2 * (head_part + (int64_t)tid * a.nsplit)) = f32x2{-INFINITY, 0.0f};
     return;
   }
@@ -321,7 +325,8 @@ __global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT ==
 
   // ---- the rows, 32 at a time, the next tile's loads under this one's work ----
   // one tile's scores of all heads lie together: the heads' rows would be a power of two apart
-  float* const score = MASS ? a.score + (int64_t)bh * a.score_cap * a.G + (h0 + (have ? r : 0)) * kA4Tile + 4 * t : nullptr;
+  const int score_at = (have ? r : 0) * kA4Tile + 4 * t;
+  float* const score = MODE == kScores ? a.score + (int64_t)bh * a.score_cap * a.G + h0 * kA4Tile + score_at : nullptr;
   for (int tile = t_begin + wid; tile < t_end; tile += NW) {
     const int j0 = tile * kA4Tile;
     Tile4 nxt;
@@ -360,10 +365,12 @@ __global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT ==
         mx = __builtin_fmaxf(mx, s[u][i]);
       }
     }
-    if (MASS) {
-      if (have)
+    if (have) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) *(f32x4*)(score + (int64_t)j0 * a.G + 16 * u) = s[u];
+      for (int u = 0; u < 2; ++u) {
+        if (MODE == kScores) *(f32x4*)(score + (int64_t)j0 * a.G + 16 * u) = s[u];
+        if (MODE == kWholeMass) *(f32x4*)(s_score + j0 * cols + score_at + 16 * u) = s[u];
+      }
     }
     const float base = raise(mx);
     u32x4 pf[PP];
@@ -424,12 +431,25 @@ __global__ __launch_bounds__(MODE == kWhole ? 512 : 256, MODE == kWhole || DT ==
       o += f * ((const float*)(const void*)s_v[w])[c * kRow + d];
       L += f * s_ml[w][1][c];
     }
-    if (MODE == kWhole) {
+    if (WHOLE) {
+      if (MODE == kWholeMass && d == 0) {
+        s_weight[0][c] = base;
+        s_weight[1][c] = zero_bits(L) ? 0.0f : 1.0f / L;
+      }
       if (d < a.D) store_out<DT>(a, b, g * a.G + h0 + c, d, o, L);
     } else {
       const int64_t to = head_part + (int64_t)c * a.nsplit;
       a.part[to * kA4Part + d] = o;
       if (d == 0) *(f32x2*)(void*)(a.stat + 2 * to) = f32x2{M, L};
+    }
+  }
+  if (MODE == kWholeMass) {
+    __syncthreads();
+    for (int j = tid; j < n; j += 64 * NW) {
+      const float* const at = s_score + (j & -kA4Tile) * cols + (j & (kA4Tile - 1));
+      float w = 0.0f;
+      for (int c = 0; c < cols; ++c) w += exp2_hw(at[c * kA4Tile] - s_weight[0][c]) * s_weight[1][c];
+      a.mass[row0 + j] += w;
     }
   }
 }
@@ -542,7 +562,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
 // (1000 rows: 15.4 / 20.0).
 static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
   const int64_t units = B * Hkv * ((G + kA4Cols - 1) / kA4Cols);
-  if (capacity <= (units >= 256 ? 1024 : 768)) return 1;
+  if (capacity <= (units >= 256 ? kWholeRows : 768)) return 1;
   const int64_t most = (capacity + kA4Tile * kA4Waves - 1) / (kA4Tile * kA4Waves);
   int64_t want = (768 + units - 1) / units;
   const int64_t pay = capacity / 512 < 64 ? 64 : capacity / 512 > 256 ? 256 : capacity / 512;
@@ -550,25 +570,30 @@ static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
   if (want > most) want = most;
   return (int)want;
 }
+// One launch for it all: a short cache; where weights are added, one workgroup has to see all heads of
+// the group (8 heads of 60 rows with weights: 6.7 us against 10.0, 750 rows: 10.9 / 14.6; 512 heads of
+// 750: 25.7 / 25.3).
+static bool kv4_whole(int nsplit, int64_t G, bool mass) { return nsplit == 1 && (!mass || G <= kA4Cols); }
 static int64_t kv4_score_cap(int64_t capacity) { return (capacity + kA4Tile - 1) / kA4Tile * kA4Tile; }
 
 template <int DT, int NG>
 static void launch_attn4_ng(const Attn4Args& a, dim3 grid, int mode, hipStream_t st) {
   if (mode == kWhole) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kWhole>), grid, dim3(512), 0, st, a);
+  else if (mode == kWholeMass) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kWholeMass>), grid, dim3(512), 0, st, a);
   else if (mode == kScores) hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kScores>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((kv4_attn_kernel<DT, NG, kParts>), grid, dim3(256), 0, st, a);
 }
 template <int DT>
 static int launch_attn4(const Attn4Args& a, bool mass, hipStream_t st, const char* who) {
   const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)a.nsplit, (unsigned)((a.G + kA4Cols - 1) / kA4Cols));
-  const int mode = mass ? kScores : a.nsplit == 1 ? kWhole : kParts;
+  const int mode = kv4_whole(a.nsplit, a.G, mass) ? (mass ? kWholeMass : kWhole) : mass ? kScores : kParts;
   switch ((a.D + 31) / 32) {
     case 1: launch_attn4_ng<DT, 1>(a, grid, mode, st); break;
     case 2: launch_attn4_ng<DT, 2>(a, grid, mode, st); break;
     case 3: launch_attn4_ng<DT, 3>(a, grid, mode, st); break;
     default: launch_attn4_ng<DT, 4>(a, grid, mode, st); break;
   }
-  if (mode == kWhole) return check_launch(who);
+  if (mode >= kWhole) return check_launch(who);
   const unsigned heads = (unsigned)(a.B * a.Hkv * a.G);
   if (mass) {
     const unsigned chunks = (unsigned)((a.capacity + kMassKeys - 1) / kMassKeys);
@@ -589,7 +614,7 @@ extern "C" int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_
                                                    int accumulate) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || capacity <= 0) return 0;
   const int splits = kv4_splits(B, Hkv, Hq / Hkv, capacity);
-  if (splits == 1 && !accumulate) return 0;  // one launch writes the output
+  if (kv4_whole(splits, Hq / Hkv, accumulate != 0)) return 0;
   const int64_t n = B * Hq * splits;
   const int64_t scores = accumulate ? B * Hq * kv4_score_cap(capacity) : 0;
   return (n * kA4Part + kv4_stat_floats(n) + scores) * (int64_t)sizeof(float);
