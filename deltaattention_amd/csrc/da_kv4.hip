@@ -374,14 +374,13 @@ __device__ __forceinline__ int heavy_length(const HeavyArgs& a, int bh) {
 // registers.  The border (the need-th largest mass between the protected ends) comes from three
 // histogram passes over 11, 11 and 10 bits of the order; then the rows above it are written, and as
 // many of its equals as still fit, lowest row first, in row order.
-__global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) {
+__device__ __forceinline__ void heavy_choose(const HeavyArgs& a, int32_t* out) {
   __shared__ uint32_t s_hist[kHeavyBins];
   __shared__ uint32_t s_wave[kHeavyWaves];
   __shared__ uint32_t s_cnt[2][kHeavyPer * kHeavyWaves];  // rows above / at the border, in row order
   __shared__ uint32_t s_pick[2];
   const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int n = heavy_length(a, bh);
-  int32_t* const out = a.index + (int64_t)bh * a.budget;
   if (tid == 0) a.kept[bh] = n < a.budget ? n : a.budget;
   if (n <= a.budget) {
     for (int i = tid; i < a.budget; i += kHeavyThreads) out[i] = i < n ? i : -1;
@@ -463,6 +462,10 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) 
     const bool gt = (bg[j] >> lane) & 1, eq = (be[j] >> lane) & 1;
     if (gt || (eq && e < need)) out[a.sinks + g + (e < need ? e : need)] = lo + j * kHeavyThreads + tid;
   }
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heavy_rows_kernel(HeavyArgs a) {
+  heavy_choose(a, a.index + (int64_t)blockIdx.x * a.budget);
 }
 
 // Longer heads in chunks of kChunk rows, a workgroup each, in five launches that take the chip:
@@ -736,6 +739,27 @@ __device__ __forceinline__ void store_scales(uint8_t* p, uint32_t v) {
   }
 }
 
+// Row m's exponents, count, timestamp and mass from row src, zero where there is none.
+template <int NG>
+__device__ __forceinline__ void move_fields(const Move4Args& a, int bh, int m, int src) {
+  const int64_t to = bh * a.o_capacity + m, from = bh * a.capacity + src;
+  uint32_t ks = 0, vs = 0;
+  int c = 0, t = 0;
+  float w = 0.0f;
+  if (src >= 0) {
+    ks = load_scales<NG>(a.scales[0] + from * NG);
+    vs = load_scales<NG>(a.scales[1] + from * NG);
+    c = a.counts[from];
+    t = a.ts[from];
+    w = a.mass[from];
+  }
+  store_scales<NG>(a.o_scales[0] + to * NG, ks);
+  store_scales<NG>(a.o_scales[1] + to * NG, vs);
+  a.o_counts[to] = c;
+  a.o_ts[to] = t;
+  a.o_mass[to] = w;
+}
+
 // blockIdx.z = 0: a lane moves 16 bytes of codes (2 NG lanes a row, keys then values), read once and
 // past the caches; z = 1: a lane moves a row's small fields.  (With the fields on the codes' lanes the
 // memory instructions a row were three times as many: 131072 rows x 8 heads to 32768
@@ -747,25 +771,8 @@ __global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
   const int bh = blockIdx.y;
   const int32_t* const index = a.index + (int64_t)bh * a.budget;
   if (blockIdx.z == 1) {
-    for (int m = blockIdx.x * 256 + threadIdx.x; m < a.budget; m += gridDim.x * 256) {
-      const int src = index[m];
-      const int64_t to = bh * a.o_capacity + m, from = bh * a.capacity + src;
-      uint32_t ks = 0, vs = 0;
-      int c = 0, t = 0;
-      float w = 0.0f;
-      if (src >= 0) {
-        ks = load_scales<NG>(a.scales[0] + from * NG);
-        vs = load_scales<NG>(a.scales[1] + from * NG);
-        c = a.counts[from];
-        t = a.ts[from];
-        w = a.mass[from];
-      }
-      store_scales<NG>(a.o_scales[0] + to * NG, ks);
-      store_scales<NG>(a.o_scales[1] + to * NG, vs);
-      a.o_counts[to] = c;
-      a.o_ts[to] = t;
-      a.o_mass[to] = w;
-    }
+    for (int m = blockIdx.x * 256 + threadIdx.x; m < a.budget; m += gridDim.x * 256)
+      move_fields<NG>(a, bh, m, index[m]);
     return;
   }
   const uint32_t first = blockIdx.x * 256 * kMoveItems + threadIdx.x;
@@ -789,6 +796,28 @@ __global__ __launch_bounds__(256) void move4_kernel(Move4Args a) {
     if (m >= (uint32_t)a.budget) continue;
     const int c = (int)(it - m * kLpr), z = c >= NG ? 1 : 0, cc = c - z * NG;
     *(u32x4*)(a.o_codes[z] + ((bh * a.o_capacity + m) * NG + cc) * 16) = w[u];
+  }
+}
+
+// A small budget's choice and move in one launch, the rows' numbers in LDS (8 heads of 60 rows to 40:
+// 12.1 us against 13.2, of 300 to 256 12.6 / 13.2, and 3.4 us less of the caller's time; of 600 to 512
+// 13.6 / 13.4, of 2111 to 2048 24.6 / 15.2: one workgroup a head moves slowly).
+constexpr int kSmallBudget = 256;
+template <int NG>
+__global__ __launch_bounds__(kHeavyThreads) void evict_small_kernel(HeavyArgs h, Move4Args a) {
+  __shared__ int32_t s_index[kSmallBudget];
+  const int bh = blockIdx.x, tid = threadIdx.x;
+  heavy_choose(h, s_index);
+  __syncthreads();
+  for (int m = tid; m < a.budget; m += kHeavyThreads) {
+    move_fields<NG>(a, bh, m, s_index[m]);
+    if (h.index) h.index[(int64_t)bh * a.budget + m] = s_index[m];
+  }
+  for (int it = tid; it < a.budget * 2 * NG; it += kHeavyThreads) {
+    const int m = it / (2 * NG), c = it - m * (2 * NG), z = c >= NG ? 1 : 0, cc = c - z * NG, src = s_index[m];
+    u32x4 w = u32x4{0, 0, 0, 0};
+    if (src >= 0) w = __builtin_nontemporal_load((const u32x4*)(a.codes[z] + ((bh * a.capacity + src) * NG + cc) * 16));
+    *(u32x4*)(a.o_codes[z] + ((bh * a.o_capacity + m) * NG + cc) * 16) = w;
   }
 }
 
@@ -832,6 +861,8 @@ static int check_budget(int64_t budget, int64_t sinks, int64_t recent, const cha
              "%s: needs sinks + recent <= budget, budget in [1, 2^26]", who);
   return DA_OK;
 }
+
+static bool evict_small(int64_t capacity, int64_t budget) { return capacity <= kHeavyShort && budget <= kSmallBudget; }
 
 // The choice's scratch for heads that may be longer than kHeavyShort rows, after `at`.
 static HeavyWork heavy_work(int64_t BH, int64_t capacity, uint32_t* at, int64_t* bytes) {
@@ -934,6 +965,7 @@ extern "C" int da_kv4_dequantize(const DaKv4* kv, int64_t B, int64_t Hkv, int64_
 // The choice's scratch, then the rows kept, [B, Hkv, budget].
 extern "C" int64_t da_kv4_evict_workspace_size(int64_t B, int64_t Hkv, int64_t capacity, int64_t budget) {
   if (B <= 0 || Hkv <= 0 || capacity <= 0 || budget <= 0) return 0;
+  if (evict_small(capacity, budget)) return 0;
   int64_t bytes;
   heavy_work(B * Hkv, capacity, nullptr, &bytes);
   return bytes + B * Hkv * budget * (int64_t)sizeof(int32_t);
@@ -951,16 +983,10 @@ extern "C" int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, 
                  kv->counts != out->counts && kv->lengths != out->lengths,
              "%s: the rows move to other memory", who);
   const int64_t need = da_kv4_evict_workspace_size(B, Hkv, kv->capacity, budget);
-  if (!workspace || workspace_bytes < need)
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
   DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
-  int64_t scratch;
-  heavy_work(B * Hkv, kv->capacity, nullptr, &scratch);
-  int32_t* rows = index ? index : (int32_t*)((char*)workspace + scratch);
   hipStream_t st = (hipStream_t)stream;
-  if (int rc = launch_heavy(kv->mass, kv->lengths, B * Hkv, kv->capacity, budget, sinks, recent, rows, out->lengths,
-                            workspace, st, who))
-    return rc;
   Move4Args a = {};
   a.codes[0] = kv->k_codes; a.codes[1] = kv->v_codes;
   a.scales[0] = kv->k_scales; a.scales[1] = kv->v_scales;
@@ -968,8 +994,26 @@ extern "C" int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, 
   a.o_scales[0] = out->k_scales; a.o_scales[1] = out->v_scales;
   a.counts = kv->counts; a.ts = kv->timestamps; a.mass = kv->mass;
   a.o_counts = out->counts; a.o_ts = out->timestamps; a.o_mass = out->mass;
-  a.index = rows; a.capacity = kv->capacity; a.o_capacity = out->capacity; a.budget = (int)budget;
+  a.capacity = kv->capacity; a.o_capacity = out->capacity; a.budget = (int)budget;
   const int groups = (int)((D + 31) / 32);
+  if (evict_small(kv->capacity, budget)) {
+    const HeavyArgs h = {kv->mass, kv->lengths, kv->capacity, (int)budget, (int)sinks, (int)recent, index, out->lengths};
+    const dim3 heads((unsigned)(B * Hkv));
+    switch (groups) {
+      case 1: hipLaunchKernelGGL((evict_small_kernel<1>), heads, dim3(kHeavyThreads), 0, st, h, a); break;
+      case 2: hipLaunchKernelGGL((evict_small_kernel<2>), heads, dim3(kHeavyThreads), 0, st, h, a); break;
+      case 3: hipLaunchKernelGGL((evict_small_kernel<3>), heads, dim3(kHeavyThreads), 0, st, h, a); break;
+      default: hipLaunchKernelGGL((evict_small_kernel<4>), heads, dim3(kHeavyThreads), 0, st, h, a); break;
+    }
+    return check_launch(who);
+  }
+  int64_t scratch;
+  heavy_work(B * Hkv, kv->capacity, nullptr, &scratch);
+  int32_t* rows = index ? index : (int32_t*)((char*)workspace + scratch);
+  if (int rc = launch_heavy(kv->mass, kv->lengths, B * Hkv, kv->capacity, budget, sinks, recent, rows, out->lengths,
+                            workspace, st, who))
+    return rc;
+  a.index = rows;
   const dim3 grid((unsigned)((budget * 2 * groups + 256 * kMoveItems - 1) / (256 * kMoveItems)), (unsigned)(B * Hkv), 2);
   switch (groups) {
     case 1: hipLaunchKernelGGL((move4_kernel<1>), grid, dim3(256), 0, st, a); break;
@@ -988,7 +1032,7 @@ extern "C" int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t 
   DA_REQUIRE(B > 0 && Hkv > 0 && N > 0 && N <= (1 << 26) && B * Hkv <= 65535, "%s: bad shape", who);
   if (int rc = check_budget(budget, sinks, recent, who)) return rc;
   const int64_t need = da_kv4_evict_workspace_size(B, Hkv, N, budget);
-  if (!workspace || workspace_bytes < need)
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %lld bytes required", who, (long long)need);
   DA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   return launch_heavy(mass, lengths, B * Hkv, N, budget, sinks, recent, index, kept, workspace, (hipStream_t)stream,

@@ -20,11 +20,12 @@
 // V^T comes from a bf16 copy of the tile in LDS through ds_read_b64_tr_b16 in the same order.
 //
 // Ring rows (bf16, fp16 or fp32, at most a few hundred) run on fp32 MFMA with values converted
-// exactly; it needs no transposed operand, so they go from memory to the matrix unit directly.
+// exactly, K from registers and V through LDS.
 //
 // The keys of a (sequence, KV head) are split over `nsplit` workgroups of four waves, tiles dealt
 // out by the device's own length, so that a short cache leaves no workgroup more than a tile;
-// a second launch joins the splits and adds the weights, which need the whole softmax.
+// a second launch joins the splits and adds the weights, which need the whole softmax.  A cache of
+// small capacity is one workgroup a head instead, which does all of it.
 #include "da_common.hpp"
 #include "../../include/deltaattn_cache.h"
 

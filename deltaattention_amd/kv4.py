@@ -285,9 +285,9 @@ def heavy_rows(mass: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
     index = torch.empty((B, H, budget), dtype=_I32, device=device)
     kept = torch.empty((B, H), dtype=_I32, device=device)
     n = _evict_bytes(B, H, N, budget)
-    ws = torch.empty((n,), dtype=_U8, device=device)
+    ws = torch.empty((n,), dtype=_U8, device=device) if n else None
     rc = call_on(device, lib().da_heavy_rows, mass.data_ptr(), _ptr(lengths), B, H, N, budget, sinks, recent,
-                 index.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
+                 index.data_ptr(), kept.data_ptr(), _ptr(ws), n)
     check(rc, "da_heavy_rows")
     return index, kept
 
@@ -369,8 +369,8 @@ def evict_kv4(kv: KV4, budget: int, sinks: int = 0, recent: int = 0, capacity: O
     B, H, cap, D, device = kv.batch, kv.kv_heads, kv.capacity, kv.head_dim, kv.device
     out = KV4.empty(B, H, capacity, D, device)
     n = _evict_bytes(B, H, cap, budget)
-    ws = torch.empty((n,), dtype=_U8, device=device)
-    rc = call_on(device, lib().da_kv4_evict, kv._ref, B, H, D, budget, sinks, recent, out._ref, None, ws.data_ptr(), n)
+    ws = torch.empty((n,), dtype=_U8, device=device) if n else None
+    rc = call_on(device, lib().da_kv4_evict, kv._ref, B, H, D, budget, sinks, recent, out._ref, None, _ptr(ws), n)
     check(rc, "da_kv4_evict")
     return out
 
@@ -461,6 +461,6 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
     ws = torch.empty((n,), dtype=_U8, device=device) if n else None  # held until the call is on its stream
     rc = call_on(device, lib().da_kv4_attention, q.data_ptr(), dt, B, Hq, H, D, sq[0], sq[1], kv._ref, kx, vx, sx[0],
                  sx[1], sx[2], n_exact, D ** -0.5 if scale is None else scale, 1 if accumulate else 0, out.data_ptr(),
-                 so[0], so[1], ws.data_ptr() if n else None, n)
+                 so[0], so[1], _ptr(ws), n)
     check(rc, "da_kv4_attention")
     return out

@@ -74,7 +74,7 @@ int da_kv4_dequantize(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t N, int64_
  * sinks + recent <= budget <= out->capacity.  Rows [kept, budget) of `out` are zero, rows from
  * budget on are not written; out->lengths receives the rows kept.  kv->mass and out->mass are
  * needed.  index, if not null ([B, Hkv, budget] int32), receives the rows kept, -1 past them.
- * workspace: da_kv4_evict_workspace_size() bytes.
+ * workspace: da_kv4_evict_workspace_size() bytes (none, and null, for a small budget).
  */
 int64_t da_kv4_evict_workspace_size(int64_t B, int64_t Hkv, int64_t capacity, int64_t budget);
 int da_kv4_evict(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t D, int64_t budget, int64_t sinks, int64_t recent,

@@ -168,7 +168,8 @@ def test_heavy_rows(gpu, N, lengths, budget, sinks, recent, kind):
 @pytest.mark.parametrize("D", [8, 64, 88, 128])
 @pytest.mark.parametrize("cap,lengths,budget,sinks,recent,room", [
     (9, [9, 0, 1, 8], 4, 1, 1, 4), (40, [40, 39, 12, 11], 12, 0, 3, 20), (700, [700, 699, 128, 0], 127, 4, 64, 127),
-    (33, [33, 2, 40, -1], 60, 4, 8, 64)])
+    (33, [33, 2, 40, -1], 60, 4, 8, 64), (600, [600, 599, 257, 0], 257, 4, 64, 300),
+    (5000, [5000, 4097, 256, 255], 256, 0, 1, 256), (17000, [17000, 100, 16999, 99], 99, 3, 4, 100)])
 def test_evict(gpu, D, cap, lengths, budget, sinks, recent, room):
     from deltaattention_amd import ops
     gen = _gen(cap + D)
@@ -189,6 +190,23 @@ def test_evict(gpu, D, cap, lengths, budget, sinks, recent, room):
                 got, src = getattr(new, name)[b, h].cpu(), getattr(kv, name)[b, h].cpu()
                 assert torch.equal(got[:len(rows)], src[at]), name
                 assert (got[len(rows):budget] == 0).all(), name
+
+
+@pytest.mark.parametrize("cap,budget", [(700, 200), (700, 400), (17000, 200)])
+def test_evict_index(gpu, cap, budget):
+    """The rows' numbers that the C entry point gives back are heavy_rows'."""
+    from deltaattention_amd import ops
+    from deltaattention_amd._native import call_on, lib
+    kv, _ = _cache(gpu, _gen(cap + budget), 1, 3, cap, 64, [cap, cap - 3, budget - 1])
+    want, kept = ops.heavy_rows(kv.mass, budget, 4, 16, lengths=kv.lengths)
+    out = ops.KV4.empty(1, 3, budget, 64, gpu)
+    index = torch.empty(1, 3, budget, dtype=torch.int32, device=gpu)
+    n = lib().da_kv4_evict_workspace_size(1, 3, cap, budget)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device=gpu)
+    announce(f"evict index cap={cap} budget={budget}")
+    assert call_on(out.device, lib().da_kv4_evict, kv._ref, 1, 3, 64, budget, 4, 16, out._ref, index.data_ptr(),
+                   ws.data_ptr() if n else None, n) == 0
+    assert torch.equal(index, want) and torch.equal(out.lengths, kept)
 
 
 # ---- decode attention ---------------------------------------------------------------------------

@@ -59,6 +59,7 @@ def test_dequantize_refuses():
 def test_evict_and_rows_refuse():
     lib = _native.lib()
     need = lib.da_kv4_evict_workspace_size(1, 2, 64, 16)
+    assert need == 0  # a small budget's choice stays on the chip
     other = dict(k_codes=1 << 22, v_codes=1 << 22, mass=1 << 22, counts=1 << 22, lengths=1 << 22)
 
     def evict(kv=None, out=None, budget=16, sinks=1, recent=1, ws=A, n=need):
@@ -70,14 +71,17 @@ def test_evict_and_rows_refuse():
     for bad in (dict(budget=0), dict(sinks=-1), dict(recent=-1), dict(sinks=10, recent=7), dict(sinks=1 << 62, recent=1 << 62)):
         _refused(evict(**bad), -1, "budget")
     _refused(evict(budget=65), -1, "capacity")
-    _refused(evict(n=need - 1), -4, "workspace")
-    _refused(evict(ws=None), -4, "workspace")
+    need = lib.da_kv4_evict_workspace_size(1, 2, 1024, 512)
+    assert need > 0
+    large = dict(kv=_kv(capacity=1024), out=_kv(**dict(other, capacity=1024)), budget=512)
+    _refused(evict(**large, n=need - 1), -4, "workspace")
+    _refused(evict(**large, ws=None, n=need), -4, "workspace")
     assert lib.da_kv4_evict_workspace_size(0, 2, 64, 16) == 0
     rows = lib.da_heavy_rows
     _refused(rows(None, None, 1, 2, 64, 16, 0, 0, A, A, A, need, None), -1, "null")
     _refused(rows(A, None, 1, 0, 64, 16, 0, 0, A, A, A, need, None), -1, "shape")
     _refused(rows(A, None, 1, 2, 64, 16, 9, 8, A, A, A, need, None), -1, "budget")
-    _refused(rows(A, None, 1, 2, 64, 16, 0, 0, A, A, None, 0, None), -4, "workspace")
+    _refused(rows(A, None, 1, 2, 1024, 512, 0, 0, A, A, None, 0, None), -4, "workspace")
     # a head longer than 16384 rows needs scratch for its chunks as well
     assert lib.da_kv4_evict_workspace_size(1, 2, 16385, 16) > lib.da_kv4_evict_workspace_size(1, 2, 16384, 16)
 
