@@ -100,7 +100,7 @@ __device__ __forceinline__ f32x2 row_stats(float M, float L) {
 // KK: k steps of 16 dims a score takes (2, 4, 6 or 8: the steps are not left to a run-time bound,
 // which costs a copy of the accumulators each).
 template <int DT, int PASS, int KK>
-__global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
+__device__ __forceinline__ void mass_pass(const MassArgs& a) {
   constexpr int NP = DT == DA_F32 ? 3 : 1;
   constexpr int NW = DT == DA_F32 ? 2 : 1;    // 16-byte loads of a chunk of 8 elements
   constexpr int NCB = DT == DA_F32 ? 1 : 2;   // column blocks of 32 a wave holds
@@ -472,6 +472,22 @@ __global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
   }
 }
 
+template <int DT, int PASS, int KK>
+__global__ __launch_bounds__(256, 2) void mass_kernel(MassArgs a) {
+  mass_pass<DT, PASS, KK>(a);
+}
+
+// Both passes of a head in one launch, where neither has splits (split and blocks are 1): 16 queries
+// over 64 keys, 8 groups of 4 heads, 11.1 us against 11.8, host-inclusive 13.3 / 15.7.  A pass that would
+// be split is better split (64 queries over 100 keys: 18.4 against 20.0).
+constexpr int kMassSmall = 128;  // query rows and keys
+template <int DT, int KK>
+__global__ __launch_bounds__(256, 1) void mass_small_kernel(MassArgs a) {
+  mass_pass<DT, 0, KK>(a);
+  __syncthreads();
+  mass_pass<DT, 1, KK>(a);
+}
+
 // A query's (max, sum) parts, kJoinLanes lanes a query.
 constexpr int kJoinLanes = 16;
 __global__ __launch_bounds__(256) void mass_join_rows_kernel(const float* part, float* stats, int64_t rows, int split) {
@@ -530,6 +546,7 @@ static int mass_split(int64_t blocks, int64_t streamed) {
   return (int)(want > 64 ? 64 : want);
 }
 struct MassPlan {
+  bool small;
   int cols, split0, split1;
   int64_t blocks0, blocks1, rows, part;
 };
@@ -539,6 +556,7 @@ static MassPlan mass_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t
   p.rows = Hq / Hkv * Nq;
   p.blocks0 = (p.rows + p.cols - 1) / p.cols;
   p.blocks1 = (Nk + p.cols - 1) / p.cols;
+  p.small = p.rows <= kMassSmall && Nk <= kMassSmall;
   p.split0 = mass_split(p.blocks0 * B * Hkv, Nk);
   p.split1 = mass_split(p.blocks1 * B * Hkv, p.rows);
   const int64_t p0 = p.split0 > 1 ? B * Hkv * p.rows * p.split0 * 2 : 0;
@@ -560,6 +578,16 @@ static void launch_pass(const MassArgs& a, hipStream_t st) {
 template <int DT>
 static int launch_mass(MassArgs a, const MassPlan& p, hipStream_t st, const char* who) {
   const int64_t bh = (int64_t)a.B * a.Hkv;
+  if (p.small) {
+    a.split = a.blocks = 1;
+    switch ((a.D + 31) / 32) {
+      case 1: hipLaunchKernelGGL((mass_small_kernel<DT, 2>), dim3((unsigned)bh), dim3(256), 0, st, a); break;
+      case 2: hipLaunchKernelGGL((mass_small_kernel<DT, 4>), dim3((unsigned)bh), dim3(256), 0, st, a); break;
+      case 3: hipLaunchKernelGGL((mass_small_kernel<DT, 6>), dim3((unsigned)bh), dim3(256), 0, st, a); break;
+      default: hipLaunchKernelGGL((mass_small_kernel<DT, 8>), dim3((unsigned)bh), dim3(256), 0, st, a); break;
+    }
+    return check_launch(who);
+  }
   a.split = p.split0;
   a.blocks = (int)p.blocks0;
   launch_pass<DT, 0>(a, st);

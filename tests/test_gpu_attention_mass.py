@@ -24,6 +24,9 @@ CASES = [  # B, H, G, D, Nq, Nk, lengths, start, anchors, dtype
     (1, 1, 64, 32, 40, 90, None, None, False, "fp32"), (1, 1, 48, 32, 40, 90, None, None, False, "fp32"),
     (1, 1, 64, 32, 40, 90, None, None, False, "bf16"), (1, 2, 3, 128, 90, 90, None, None, False, "bf16"),
     (1, 1, 4, 128, 6, 2049, None, 5000, False, "bf16"), (1, 1, 1, 128, 1, 40000, None, None, False, "bf16"),
+    # one launch for both passes, and just not; few keys under many queries
+    (2, 2, 4, 128, 32, 128, [128, 0, 1, 77], 200, True, "fp16"), (1, 2, 1, 96, 128, 128, None, None, False, "fp32"),
+    (1, 1, 43, 128, 3, 128, [100], 150, True, "bf16"), (1, 2, 8, 64, 3000, 45, [45, 31], 20, True, "fp32"),
 ]
 
 
