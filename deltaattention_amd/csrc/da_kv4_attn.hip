@@ -161,7 +161,7 @@ struct Tile4 {
 // workgroup of eight waves takes the head and writes the output itself; kWholeMass: and adds the weights,
 // its scores in LDS.
 enum Mode4 : int { kParts = 0, kScores = 1, kWhole = 2, kWholeMass = 3 };
-constexpr int kWholeRows = 1024;  // most rows of a cache that one workgroup takes
+constexpr int kWholeRows = 1024;  // most rows of a cache that kWhole and kWholeMass take (s_score holds as many)
 template <int DT, int NG, int MODE>
 __global__ __launch_bounds__(MODE >= kWhole ? 512 : 256, MODE >= kWhole || DT == DA_F32 ? 2 : 3) void kv4_attn_kernel(
     Attn4Args a) {
@@ -573,8 +573,12 @@ static int kv4_splits(int64_t B, int64_t Hkv, int64_t G, int64_t capacity) {
 }
 // One launch for it all: a short cache; where weights are added, one workgroup has to see all heads of
 // the group (8 heads of 60 rows with weights: 6.7 us against 10.0, 750 rows: 10.9 / 14.6; 512 heads of
-// 750: 25.7 / 25.3).
-static bool kv4_whole(int nsplit, int64_t G, bool mass) { return nsplit == 1 && (!mass || G <= kA4Cols); }
+// 750: 25.7 / 25.3).  768 heads and more leave one split at any capacity, which does not make the cache
+// short: past kWholeRows it takes the two launches, with which it is as fast or faster too (768 heads of
+// 2048 rows without weights: 50 us against 56 in one, of 4096 78 / 86, 2048 heads of 8192 339 / 365).
+static bool kv4_whole(int nsplit, int64_t G, int64_t capacity, bool mass) {
+  return nsplit == 1 && capacity <= kWholeRows && (!mass || G <= kA4Cols);
+}
 static int64_t kv4_score_cap(int64_t capacity) { return (capacity + kA4Tile - 1) / kA4Tile * kA4Tile; }
 
 template <int DT, int NG>
@@ -587,7 +591,7 @@ static void launch_attn4_ng(const Attn4Args& a, dim3 grid, int mode, hipStream_t
 template <int DT>
 static int launch_attn4(const Attn4Args& a, bool mass, hipStream_t st, const char* who) {
   const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)a.nsplit, (unsigned)((a.G + kA4Cols - 1) / kA4Cols));
-  const int mode = kv4_whole(a.nsplit, a.G, mass) ? (mass ? kWholeMass : kWhole) : mass ? kScores : kParts;
+  const int mode = kv4_whole(a.nsplit, a.G, a.capacity, mass) ? (mass ? kWholeMass : kWhole) : mass ? kScores : kParts;
   switch ((a.D + 31) / 32) {
     case 1: launch_attn4_ng<DT, 1>(a, grid, mode, st); break;
     case 2: launch_attn4_ng<DT, 2>(a, grid, mode, st); break;
@@ -615,7 +619,7 @@ extern "C" int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_
                                                    int accumulate) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || capacity <= 0) return 0;
   const int splits = kv4_splits(B, Hkv, Hq / Hkv, capacity);
-  if (kv4_whole(splits, Hq / Hkv, accumulate != 0)) return 0;
+  if (kv4_whole(splits, Hq / Hkv, capacity, accumulate != 0)) return 0;
   const int64_t n = B * Hq * splits;
   const int64_t scores = accumulate ? B * Hq * kv4_score_cap(capacity) : 0;
   return (n * kA4Part + kv4_stat_floats(n) + scores) * (int64_t)sizeof(float);
