@@ -191,7 +191,7 @@ __device__ __forceinline__ void mass_pass(const MassArgs& a) {
       const int row = tile * kTile + lane;
       m_add = -INFINITY;
       m_mul = 0.0f;
-      m_t = PASS == 0 ? -kNever : kNever;  // past the end: no weight, a time that asks for no mask
+      m_t = -kNever;  // past the end: no weight; as a query it is masked, a key may be anything
       if (row < nrow) {
         if (PASS == 0) {
           const int c = cnt ? cnt[row] : 1;
@@ -235,7 +235,9 @@ __device__ __forceinline__ void mass_pass(const MassArgs& a) {
         s_t[mt][lane] = m_t;
       }
       const uint64_t odd = __ballot(mine && !zero_bits(m_add));
-      const uint64_t late = __ballot(mine && (PASS == 0 ? m_t > ext : m_t < ext));
+      // queries past the end ask for no mask, but where there is one they are behind it: a key that no
+      // query sees may hold a NaN, whose product with a row of zeros is one
+      const uint64_t late = __ballot(mine && (PASS == 0 ? m_t > ext : m_t < ext && tile * kTile + lane < nrow));
       if (lane == 0) s_flag[mt] = (odd ? 1 : 0) | (late ? 2 : 0);
     }
   };
