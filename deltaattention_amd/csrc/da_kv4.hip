@@ -314,10 +314,11 @@ struct HeavyArgs {
   int32_t* kept;   // [bh]
 };
 
-// Masses in an order of unsigned integers (-0 as 0).
+// Masses in an order of unsigned integers (-0 as 0; every NaN, of either sign, as one largest).
 __device__ __forceinline__ uint32_t mass_order(float m) {
-  const uint32_t u = __float_as_uint(m);
+  const uint32_t u = opaque_bits(m);
   if ((u << 1) == 0) return 0x80000000u;
+  if ((u << 1) > 0xff000000u) return 0xffffffffu;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
