@@ -421,11 +421,14 @@ class FourBitCompressedCache(HybridCompressedCache):
         self.exact_seq_lens[layer_idx] = e_len
         self.total_seq_lens[layer_idx] = original_q_len
 
-    def _make_room(self, layer_idx):
-        """Before a token: a row for it in every head, by a cut to the budget or by growing."""
+    def _make_room(self, layer_idx, key_states, value_states):
+        """Before a token: a row for it in every head, by a cut to the budget or by growing (not for a
+        token that the update will refuse)."""
         kv = self.anchors[layer_idx]
         if self.max_packed_len[layer_idx] < kv.capacity:
             return
+        kv4._check_update(kv, key_states, value_states, self.k_exact[layer_idx], self.v_exact[layer_idx],
+                          self.k_last[layer_idx], self.exact_seq_lens[layer_idx], self.total_seq_lens[layer_idx])
         if self.budget is None:
             self.anchors[layer_idx] = kv4.evict_kv4(kv, kv.capacity, capacity=max(2 * kv.capacity, kv.capacity + 1024))
         else:
@@ -436,7 +439,7 @@ class FourBitCompressedCache(HybridCompressedCache):
         """One decode token (``ops.decode_update_kv4``); prefill calls pass through."""
         if key_states.shape[2] > 1:
             return key_states, value_states
-        self._make_room(layer_idx)
+        self._make_room(layer_idx, key_states, value_states)
         threshold, use_cos = _metric_threshold()
         kv4.decode_update_kv4(self.anchors[layer_idx], key_states, value_states, self.k_exact[layer_idx],
                               self.v_exact[layer_idx], self.k_last[layer_idx], self.exact_seq_lens[layer_idx],
@@ -457,7 +460,18 @@ class FourBitCompressedCache(HybridCompressedCache):
                                         self.v_exact[layer_idx], n, scaling, accumulate=self.budget is not None)
 
     def decode_step(self, query_states, key_states, value_states, layer_idx, scaling=None):
-        """``update`` then ``attend``: one decode token of one layer."""
+        """``update`` then ``attend``: one decode token of one layer.  What ``attend`` would refuse is
+        refused before ``update`` writes anything."""
+        kv = self.anchors[layer_idx]
+        B, Hq, D = kv4._check_query(query_states, kv)
+        if query_states.dtype != self.k_exact.dtype:
+            raise TypeError(f"decode_step: the query is {query_states.dtype}, the cache {self.k_exact.dtype}")
+        if Hq > 64 * kv.kv_heads:
+            raise ValueError(f"decode_step: {Hq} query heads over {kv.kv_heads} KV heads, at most 64 to one")
+        if scaling is not None and not scaling > 0:
+            raise ValueError(f"decode_step: scaling must be positive, got {scaling}")
+        if key_states.shape != (B, kv.kv_heads, 1, D):  # update passes a prompt's tokens through
+            raise ValueError(f"decode_step: expected key {[B, kv.kv_heads, 1, D]}, got {list(key_states.shape)}")
         self.update(key_states, value_states, layer_idx)
         return self.attend(query_states, layer_idx, scaling)
 

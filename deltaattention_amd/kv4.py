@@ -375,14 +375,8 @@ def evict_kv4(kv: KV4, budget: int, sinks: int = 0, recent: int = 0, capacity: O
     return out
 
 
-def decode_update_kv4(kv: KV4, key: torch.Tensor, value: torch.Tensor, k_exact: torch.Tensor, v_exact: torch.Tensor,
-                      k_last: torch.Tensor, exact_seq_len: int, total_seq_len: int, threshold: float,
-                      use_cosine: bool = False) -> None:
-    """One decode token into the ring k_exact, v_exact [B, Hkv, W, D] (slot exact_seq_len % W).  Where
-    the ring was full, the token that leaves it merges into its head's last 4-bit row (count + 1) or
-    becomes a new one, by the test of ``da_decode_update`` against that row's key as it was
-    (k_last [B, Hkv, D], kept up to date).  ``threshold`` is squared for the Euclidean test.  key, value
-    [B, Hkv, 1, D], ring and k_last share one type."""
+def _check_update(kv: KV4, key, value, k_exact, v_exact, k_last, exact_seq_len, total_seq_len) -> int:
+    """The type code of ``decode_update_kv4``'s rows, or what it refuses."""
     B, H, D, device = kv.batch, kv.kv_heads, kv.head_dim, kv.device
     dt = dtype_code(key, value, k_exact, v_exact, k_last)
     if key.shape != (B, H, 1, D) or value.shape != key.shape or key.device != device or value.device != device:
@@ -395,14 +389,43 @@ def decode_update_kv4(kv: KV4, key: torch.Tensor, value: torch.Tensor, k_exact: 
     _want(k_last, "k_last", (B, H, D), k_exact.dtype, device)
     if exact_seq_len < 0 or total_seq_len < 0:
         raise ValueError("negative lengths")
+    return dt
+
+
+def decode_update_kv4(kv: KV4, key: torch.Tensor, value: torch.Tensor, k_exact: torch.Tensor, v_exact: torch.Tensor,
+                      k_last: torch.Tensor, exact_seq_len: int, total_seq_len: int, threshold: float,
+                      use_cosine: bool = False) -> None:
+    """One decode token into the ring k_exact, v_exact [B, Hkv, W, D] (slot exact_seq_len % W).  Where
+    the ring was full, the token that leaves it merges into its head's last 4-bit row (count + 1) or
+    becomes a new one, by the test of ``da_decode_update`` against that row's key as it was
+    (k_last [B, Hkv, D], kept up to date).  ``threshold`` is squared for the Euclidean test.  key, value
+    [B, Hkv, 1, D], ring and k_last share one type."""
+    dt = _check_update(kv, key, value, k_exact, v_exact, k_last, exact_seq_len, total_seq_len)
+    B, H, W, D = k_exact.shape
     key, value = _rows(key), _rows(value)
     if _strides(key) != _strides(value):
         key, value = key.contiguous(), value.contiguous()
     sn = _strides(key)
-    rc = call_on(device, lib().da_kv4_update, key.data_ptr(), value.data_ptr(), dt, B, H, D, sn[0], sn[1],
+    rc = call_on(kv.device, lib().da_kv4_update, key.data_ptr(), value.data_ptr(), dt, B, H, D, sn[0], sn[1],
                  k_exact.data_ptr(), v_exact.data_ptr(), H * W * D, W * D, D, kv._ref, k_last.data_ptr(),
                  int(exact_seq_len), int(total_seq_len), W, threshold, 1 if use_cosine else 0)
     check(rc, "da_kv4_update")
+
+
+def _check_query(q: torch.Tensor, kv: KV4) -> Tuple[int, int, int]:
+    """(B, Hq, D) of one token's queries over ``kv``."""
+    device, H = kv.device, kv.kv_heads
+    shape = q.shape
+    if len(shape) == 4 and shape[2] == 1:
+        B, Hq, _, D = shape
+    elif len(shape) == 3:
+        B, Hq, D = shape
+    else:
+        raise ValueError("q is [B, Hq, 1, D] or [B, Hq, D]")
+    if q.device != device or B != kv.batch or D != kv.head_dim or Hq % H or not Hq:
+        raise ValueError(f"q {list(shape)} on {q.device} does not fit a cache of {kv.batch} sequences, {H} KV heads "
+                         f"and head_dim {kv.head_dim} on {device}")
+    return B, Hq, D
 
 
 def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tensor] = None,
@@ -417,17 +440,8 @@ def decode_attention_kv4(q: torch.Tensor, kv: KV4, k_exact: Optional[torch.Tenso
     ``kv.mass``.  A head without any key gives zeros.  Query head h reads KV head
     h // (Hq // Hkv).
     """
-    device, H = kv.device, kv.kv_heads
-    shape = q.shape
-    if len(shape) == 4 and shape[2] == 1:
-        B, Hq, _, D = shape
-    elif len(shape) == 3:
-        B, Hq, D = shape
-    else:
-        raise ValueError("q is [B, Hq, 1, D] or [B, Hq, D]")
-    if q.device != device or B != kv.batch or D != kv.head_dim or Hq % H or not Hq:
-        raise ValueError(f"q {list(shape)} on {q.device} does not fit a cache of {kv.batch} sequences, {H} KV heads "
-                         f"and head_dim {kv.head_dim} on {device}")
+    B, Hq, D = _check_query(q, kv)
+    device, H, shape = kv.device, kv.kv_heads, q.shape
     if (k_exact is None) != (v_exact is None):
         raise ValueError("k_exact and v_exact come together")
     if accumulate and kv.mass is None:
