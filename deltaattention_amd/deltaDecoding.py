@@ -389,6 +389,12 @@ class FourBitCompressedCache(HybridCompressedCache):
         kv.lengths.zero_()
         return kv
 
+    def _replace(self, layer_idx, kv):
+        """The layer's anchors from here on.  Those before may have been made on another stream than this
+        one, whose work still reads them: their memory stays until that is done."""
+        self.anchors[layer_idx].record_stream(torch.cuda.current_stream(kv.device))
+        self.anchors[layer_idx] = kv
+
     @property
     def packed_lengths(self):
         """Anchors of every (sequence, KV head) of a layer, [B * Hkv] int32 each."""
@@ -412,8 +418,8 @@ class FourBitCompressedCache(HybridCompressedCache):
             index, lengths = kv4.heavy_rows(mass, self.budget, self.sinks, self.recent, lengths)
             P = self.budget
         capacity = self.budget + self.slack if self.budget is not None else max(self.capacity, P + 1024)
-        self.anchors[layer_idx] = kv4.quantize_kv4(k_packed, v_packed, counts, timestamps, mass, lengths, index,
-                                                   capacity)
+        self._replace(layer_idx, kv4.quantize_kv4(k_packed, v_packed, counts, timestamps, mass, lengths, index,
+                                                  capacity))
         self.max_packed_len[layer_idx] = P
         e_len = k_exact.shape[2]
         self.k_exact[layer_idx, :, :, :e_len] = k_exact
@@ -430,9 +436,9 @@ class FourBitCompressedCache(HybridCompressedCache):
         kv4._check_update(kv, key_states, value_states, self.k_exact[layer_idx], self.v_exact[layer_idx],
                           self.k_last[layer_idx], self.exact_seq_lens[layer_idx], self.total_seq_lens[layer_idx])
         if self.budget is None:
-            self.anchors[layer_idx] = kv4.evict_kv4(kv, kv.capacity, capacity=max(2 * kv.capacity, kv.capacity + 1024))
+            self._replace(layer_idx, kv4.evict_kv4(kv, kv.capacity, capacity=max(2 * kv.capacity, kv.capacity + 1024)))
         else:
-            self.anchors[layer_idx] = kv4.evict_kv4(kv, self.budget, self.sinks, self.recent, self.budget + self.slack)
+            self._replace(layer_idx, kv4.evict_kv4(kv, self.budget, self.sinks, self.recent, self.budget + self.slack))
             self.max_packed_len[layer_idx] = self.budget
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):

@@ -216,6 +216,13 @@ class KV4:
     def __deepcopy__(self, memo):
         return self.clone()
 
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """``torch.Tensor.record_stream`` of the cache's memory: once the object is gone, it is not
+        given out again before what ``stream`` has been given by then is done."""
+        for t in [self._own[1][_U8]] if self._own else [getattr(self, name) for name in _TENSORS]:
+            if t is not None:
+                t.record_stream(stream)
+
 
 def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tensor] = None,
                    timestamps: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
