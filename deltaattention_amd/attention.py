@@ -132,14 +132,15 @@ def delta_prefill_attention(query_states: torch.Tensor, key_states: torch.Tensor
 
 def _handoff(cache, layer_idx, packed, key_states, value_states, query_states=None, scaling=None):
     """initialize_from_prefill with the P packed rows of every head and the last
-    min(N, W) prefill tokens (modeling_llama.py:762-773, 869-879).  A cache with a budget
-    (``FourBitCompressedCache``) also gets the attention weight that its ``observe`` last
-    queries gave each anchor."""
+    min(N, W) prefill tokens (modeling_llama.py:762-773, 869-879).  A
+    ``FourBitCompressedCache`` with a budget also gets the attention weight that its
+    ``observe`` last queries gave each anchor."""
+    from .deltaDecoding import FourBitCompressedCache
     q_len = key_states.shape[2]
     p = packed.trimmed()
     tail = min(q_len, cache.exact_window_size)
     more = {}
-    if getattr(cache, "budget", None) is not None and query_states is not None:
+    if query_states is not None and isinstance(cache, FourBitCompressedCache) and cache.budget is not None:
         n = min(cache.observe, query_states.shape[2])
         more["mass"] = ops.attention_mass(
             query_states[:, :, -n:], p.k_packed, counts=p.counts.contiguous(),
@@ -157,7 +158,8 @@ def delta_decode_handoff(key_states: torch.Tensor, value_states: torch.Tensor, l
     delta-select and pack the post-RoPE keys with the globVR chunking, metric and
     threshold (always delta mode, whatever ``packing_mode`` says, as the reference
     launches chunked_eval_kernel directly), then hand the packed history and the exact
-    tail to the cache.  ``query_states`` and ``scaling`` are for a cache with a budget."""
+    tail to the cache.  ``query_states`` and ``scaling`` are for a FourBitCompressedCache
+    with a budget."""
     fixed = getattr(globVR, "chunk_size", 0)                        # :809-816
     divide_to = getattr(globVR, "divide_to", 0)
     keep, _ = ops.select(key_states, getattr(globVR, "row_delta_threshold", 0.0),

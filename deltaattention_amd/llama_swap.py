@@ -171,8 +171,8 @@ def delta_llama_attention_forward(self, hidden_states: torch.Tensor,
                 query_states, key_states, value_states, scaling=self.scaling, out=view),
                 query_states.is_cuda)
             if getattr(globVR, "delta_decode", False):               # :805-879
-                # a cache with a budget asks the queries which anchors to keep
-                more = (query_states, self.scaling) if getattr(cache, "budget", None) is not None else ()
+                # the bounded cache asks the queries which anchors to keep
+                more = (query_states, self.scaling) if isinstance(cache, deltaDecoding.FourBitCompressedCache) else ()
                 attention.delta_decode_handoff(key_states, value_states, self.layer_idx, cache, *more)
         else:                                                        # PATH 1
             _timed(lambda: attention.delta_prefill_attention(
