@@ -179,9 +179,16 @@ class KV4:
         B, H, cap, D = int(batch), int(kv_heads), int(capacity), int(head_dim)
         if not (B > 0 and H > 0 and cap > 0) or D <= 0 or D > 128 or D % 8:
             raise ValueError(f"no cache of {batch} sequences, {kv_heads} heads, {capacity} rows and head_dim {head_dim}")
-        size, at, views = _layout(B, H, cap, D, bool(mass))
-        own = torch.empty((size,), dtype=_U8, device=device)
+        return cls._over(torch.empty((_layout(B, H, cap, D, bool(mass))[0],), dtype=_U8, device=device), B, H, cap, D,
+                         bool(mass))
+
+    @classmethod
+    def _over(cls, own, B, H, cap, D, mass):
+        """The cache whose fields lie in the bytes ``own`` (_layout)."""
+        size, at, views = _layout(B, H, cap, D, mass)
         device, p = _gpu(own, "the cache"), own.data_ptr()
+        if own.shape != (size,) or p % 256:
+            raise ValueError(f"{size} bytes at a multiple of 256 expected, got {list(own.shape)}")
         self = cls.__new__(cls)
         self._put(B, H, cap, D, device, Kv4Block(*[None if x is None else p + x for x in at], cap),
                   (views, {_U8: own}))
@@ -215,6 +222,14 @@ class KV4:
 
     def __deepcopy__(self, memo):
         return self.clone()
+
+    def __reduce__(self):
+        # copy.copy: another KV4 of the same tensors; pickling: of the tensors as torch pickles them
+        if self._own:  # one allocation: its bytes, not eight views of them
+            return KV4._over, (self._own[1][_U8], self.batch, self.kv_heads, self.capacity, self.head_dim,
+                               self._own[0]["mass"] is not None)
+        return KV4, (self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.counts, self.timestamps, self.lengths,
+                     self.head_dim, self.mass)
 
     def record_stream(self, stream: torch.cuda.Stream) -> None:
         """``torch.Tensor.record_stream`` of the cache's memory: once the object is gone, it is not
