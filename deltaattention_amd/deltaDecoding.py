@@ -405,12 +405,21 @@ class FourBitCompressedCache(HybridCompressedCache):
         """Prefill hand-off: the anchors (rows of count > 0, which come first) into 4 bits, the last
         min(N, W) prefill tokens to the ring.  With a budget and more rows than it, ``mass`` ([B, Hkv,
         P] float32, as ``ops.attention_mass`` gives it) says which stay."""
+        B, H, D = self.bsz, self.n_kv_heads, self.head_dim
+        P, e_len = k_packed.shape[2], k_exact.shape[2]
+        for t, name, want in ((k_packed, "k_packed", (B, H, P, D)), (v_packed, "v_packed", (B, H, P, D)),
+                              (counts, "counts", (B, H, P)), (timestamps, "timestamps", (B, H, P)),
+                              (k_exact, "k_exact", (B, H, e_len, D)), (v_exact, "v_exact", (B, H, e_len, D))):
+            if t.shape != want:
+                raise ValueError(f"{name} must have shape {list(want)}, got {list(t.shape)}")
+        if e_len > self.exact_window_size:
+            raise ValueError(f"{e_len} exact tokens for a window of {self.exact_window_size}")
+        # everything that can be refused comes before the first write
         counts = counts.to(torch.int32).contiguous()
         timestamps = timestamps.to(torch.int32).contiguous()
-        P = k_packed.shape[2]
         lengths = (counts > 0).sum(-1, dtype=torch.int32)
-        last = (lengths - 1).clamp(min=0).long()[..., None, None].expand(-1, -1, 1, self.head_dim)
-        self.k_last[layer_idx] = torch.gather(k_packed, 2, last).squeeze(2)
+        last = (lengths - 1).clamp(min=0).long()[..., None, None].expand(-1, -1, 1, D)
+        last = torch.gather(k_packed, 2, last).squeeze(2)
         index = None
         if self.budget is not None and P > self.budget:
             if mass is None:
@@ -420,8 +429,8 @@ class FourBitCompressedCache(HybridCompressedCache):
         capacity = self.budget + self.slack if self.budget is not None else max(self.capacity, P + 1024)
         self._replace(layer_idx, kv4.quantize_kv4(k_packed, v_packed, counts, timestamps, mass, lengths, index,
                                                   capacity))
+        self.k_last[layer_idx] = last
         self.max_packed_len[layer_idx] = P
-        e_len = k_exact.shape[2]
         self.k_exact[layer_idx, :, :, :e_len] = k_exact
         self.v_exact[layer_idx, :, :, :e_len] = v_exact
         self.exact_seq_lens[layer_idx] = e_len
