@@ -25,7 +25,8 @@
 // The keys of a (sequence, KV head) are split over `nsplit` workgroups of four waves, tiles dealt
 // out by the device's own length, so that a short cache leaves no workgroup more than a tile;
 // a second launch joins the splits and adds the weights, which need the whole softmax.  A cache of
-// small capacity is one workgroup a head instead, which does all of it.
+// at most 768 rows, or 1024 where the heads fill the chip, is one workgroup a head instead, which does
+// all of it.
 #include "da_common.hpp"
 #include "../../include/deltaattn_cache.h"
 
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(MODE >= kWhole ? 512 : 256, MODE >= kWhole || DT ==
     cur = nxt;
   }
 
-  // ---- join the four waves; the V tiles' LDS holds their sums ----
+  // ---- join the workgroup's waves; the V tiles' LDS holds their sums ----
   l_run = cols_sum(l_run);
   if (t == 0) {
     s_ml[wid][0][r] = m_run;
@@ -554,8 +555,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn4Args a) {
   }
 }
 
-// Workgroups of the attention launch: three a CU run at once (its registers), and no split is
-// shorter than a tile a wave.  64 splits, or of 512 rows as many as there are up to 256, are the most
+// Workgroups of the attention launch: three a CU run at once (the registers of the 16-bit types' kernels:
+// 124 to 171 VGPRs; fp32's 192 to 216 leave room for two, and the number was not measured for it apart),
+// and no split is shorter than a tile a wave.  64 splits, or of 512 rows as many as there are up to 256, are the most
 // that pay their joining (8 heads of 8297 rows: 64 10.2 us, 32 11.8, 96 12.7; one of 112207: 64 19.2,
 // 128 15.1, 256 15.7; one of 1000000: 64 109, 128 61, 256 43).  A short cache is one workgroup of
 // eight waves a head, without a second launch (8 heads, 500 rows: 8.1 against 9.2 us, 750: 9.7 / 9.3,

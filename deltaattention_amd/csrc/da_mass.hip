@@ -11,15 +11,21 @@
 //   columns  S = Q K^T, keys as columns: sum of 2^(s - lse) over the queries, in the lane that
 //            owns the key.
 //
-// They are one kernel with the operands swapped: a wave holds its 64 columns' operand in
-// registers for the whole run and the rows stream through LDS, 32 at a time, shared by the four
-// waves of a workgroup, so that each fragment read from LDS feeds two MFMAs.  Per score there is
+// They are one kernel with the operands swapped: a wave holds its columns' operand (64 columns of a
+// 16-bit type, 32 of fp32) in registers for the whole run and the rows stream through LDS in
+// double-buffered stages of 64 (fp32: 32) that the four waves of a workgroup share, worked on 32 rows
+// at a time, so that each fragment read from LDS feeds two MFMAs.  Per score there is
 // one fused multiply-add, one exp2 and one addition; the maximum is looked at only where a sum
 // leaves fp32's comfortable range.  Queries of a group are interleaved (row = query G + head),
 // so a tile's positions are close together and whole tiles are either visible or not.
 //
 // Both passes split their streamed axis where there are too few columns to fill the chip; the
-// parts are joined by small launches in a fixed order.
+// parts are joined by small launches in a fixed order.  Up to 128 query rows and keys a head, both
+// passes are one launch of one workgroup a head.
+//
+// What bounds it: 8192 queries of 8 x 4 heads (305 + 333 us) keep the matrix unit busy for 40 and 36% of
+// the cycles and the VALU for 62 and 53%.  Neither is full, and the sums are near all of it: at 246 to
+// 254 VGPRs two waves a SIMD are what fits, and the two units take turns more than they overlap.
 //
 // fp32 tensors: each operand is cut into three bf16 parts, and the six products of weight
 // 2^-16 and above are kept (error about 2^-24 of |q||k|, as an fp32 product's own rounding).

@@ -351,7 +351,12 @@ class FourBitCompressedCache(HybridCompressedCache):
     and the heaviest of the others.  The hand-off cuts to the budget by the weights that the
     prompt's last ``observe`` queries give (``attention.delta_prefill_attention`` computes
     them); decoding cuts when ``slack`` anchors have been added.  A cut moves the layer's anchors
-    to new memory, so a captured graph of decode steps has to be captured again after one.
+    to new memory, so a captured ``attend`` has to be captured again after one (a captured
+    ``update`` repeats one ring slot: slot and position are host numbers, as in the base class).
+
+    A call that is refused changes nothing.  ``decode_step`` is ``update`` and ``attend`` in turn, two
+    library calls where the full-width cache makes one: 29.5 us of a caller's time against 18.5 at 8297
+    anchors of 8 heads.
     Without ``budget`` the cache grows as the reference's does (deltaDecoding.py:138-157).
     """
 

@@ -250,8 +250,9 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, counts: Optional[torch.Tens
     Query i is at position ``q_start + i`` (default Nk - Nq, the last ones; needed with
     ``timestamps``) and sees key j if j is below the head's ``lengths`` and its position
     ``timestamps[b, g, j]`` (default j) is not past the query's.  ``counts`` adds log(count) to
-    the scores, as packed anchors have it; a count <= 0 hides the key.  A query that sees
-    nothing adds nothing; keys past the length get 0.
+    the scores, as packed anchors have it; a count <= 0 hides the key, a timestamp of 2^31 - 1
+    too.  A query that sees nothing adds nothing; keys that no query sees, and those past the
+    length, get 0, whatever they hold.
     """
     device = _gpu(q, "q")
     if q.dim() != 4 or k.dim() != 4:
@@ -294,7 +295,7 @@ def heavy_rows(mass: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
 
     A head with at most ``budget`` rows (``lengths``, default N) keeps all.  A longer one keeps
     its first ``sinks`` rows, its last ``recent`` rows, and of those between the
-    budget - sinks - recent with the largest mass, ties to the lower row.
+    budget - sinks - recent with the largest mass (a NaN is the largest), ties to the lower row.
     """
     device = _gpu(mass, "mass")
     if mass.dim() != 3:

@@ -70,7 +70,7 @@ int da_kv4_dequantize(const DaKv4* kv, int64_t B, int64_t Hkv, int64_t N, int64_
  * The rows of `kv` that a budget leaves, in their order, moved to `out` (other memory).  A
  * head with at most `budget` rows keeps all.  A longer one keeps its first `sinks` rows, its
  * last `recent` rows, and of those between the budget - sinks - recent with the largest mass
- * (compared as numbers, -0 = 0, a NaN as the largest; ties go to the lower row).
+ * (compared as numbers, -0 = 0, a NaN of either sign as the largest; ties go to the lower row).
  * sinks + recent <= budget <= out->capacity.  Rows [kept, budget) of `out` are zero, rows from
  * budget on are not written; out->lengths receives the rows kept.  kv->mass and out->mass are
  * needed.  index, if not null ([B, Hkv, budget] int32), receives the rows kept, -1 past them.
@@ -112,7 +112,8 @@ int da_heavy_rows(const float* mass, const int32_t* lengths, int64_t B, int64_t 
  * The rows' values enter as they are (bf16 holds them exactly), q and the weights in two or
  * three 16-bit parts, sums in fp32.  accumulate: kv->mass[b, g, j] += the softmax weight of
  * row j, summed over the query heads of the group.  Hq / Hkv <= 64, capacity <= 2^24.
- * workspace: da_kv4_attention_workspace_size() bytes (none, and null, for a short cache).
+ * workspace: da_kv4_attention_workspace_size() bytes (none, and null, for a cache of up to 768
+ * rows a head, or 1024 of many heads, that one workgroup a head takes).
  */
 int64_t da_kv4_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t capacity, int accumulate);
 int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t sq_b,
@@ -124,8 +125,9 @@ int da_kv4_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hk
  * The attention weight that every key receives from a run of queries: mass[b, g, j] = sum over
  * the query heads h of group g and the queries i of softmax_j(scale q[b, h, i] . k[b, g, j] +
  * log counts[b, g, j]) over the keys that query i sees: j < lengths[b, g] (null: Nk) and
- * timestamps[b, g, j] <= q_start + i (null timestamps: j; a count <= 0 hides the key).  A query
- * that sees no key adds nothing.  q [B, Hq, Nq, D], k [B, Hkv, Nk, D] of one type (bf16, fp16
+ * timestamps[b, g, j] <= q_start + i (null timestamps: j; a count <= 0 hides the key).  Positions
+ * q_start + i are taken as the nearest in [-(2^31 - 2), 2^31 - 2], so a key at 2^31 - 1 is never
+ * seen.  A query that sees no key adds nothing, a key that no query sees gets 0, whatever they hold.  q [B, Hq, Nq, D], k [B, Hkv, Nk, D] of one type (bf16, fp16
  * or fp32), rows 16-byte aligned; counts, timestamps [B, Hkv, Nk] int32 contiguous or null;
  * mass [B, Hkv, Nk] fp32 contiguous, 0 from the length on.  Deterministic.  Hq / Hkv <= 64,
  * Nq * Hq / Hkv < 2^30, Nq, Nk <= 2^24, B * Hkv <= 65535, fewer than 2^32 threads a launch.
