@@ -23,7 +23,8 @@ DA_SELECT_COSINE = 1
 DA_SELECT_ARITH16 = 2
 DA_NUM_STRIDES = 24
 
-# (name, restype, argtypes) for every symbol of include/deltaattn.h and deltaattn_cache.h
+# (name, restype, argtypes) for every symbol of include/deltaattn.h, deltaattn_cache.h and
+# deltaattn_paged.h
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 SIGNATURES = {
     "da_last_error": (ctypes.c_char_p, []),
@@ -67,6 +68,11 @@ SIGNATURES = {
     "da_attention_mass_workspace_size": (_L, [_L, _L, _L, _L, _L]),
     "da_attention_mass": (_I, [_P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _F, _P, _P,
                                _L, _P]),
+    # include/deltaattn_paged.h
+    "da_paged_append": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L,
+                             _I, _I, _P, _P, _P]),
+    "da_paged_attention_workspace_size": (_L, [_I, _L, _L, _L, _L, _P, _P, _P]),
+    "da_paged_attention": (_I, [_P, _L, _L, _P, _L, _L, _I, _L, _L, _L, _L, _F, _P, _P, _P, _P, _L, _P]),
 }
 
 
@@ -91,6 +97,18 @@ class Kv4Block(ctypes.Structure):
     """struct DaKv4 of include/deltaattn_cache.h (field for field)."""
     _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("counts", _P),
                 ("timestamps", _P), ("lengths", _P), ("mass", _P), ("capacity", _L)]
+
+
+class PagedKVBlock(ctypes.Structure):
+    """struct DaPagedKV of include/deltaattn_paged.h (field for field)."""
+    _fields_ = [("k", _P), ("v", _P), ("num_pages", _L), ("page_size", _L), ("sk_p", _L), ("sk_h", _L), ("sk_n", _L),
+                ("sv_p", _L), ("sv_h", _L), ("sv_n", _L)]
+
+
+class PagedBatchBlock(ctypes.Structure):
+    """struct DaPagedBatch of include/deltaattn_paged.h (field for field)."""
+    _fields_ = [("table", _P), ("lengths", _P), ("cu", _P), ("start", _P), ("B", _L), ("width", _L),
+                ("table_stride", _L), ("max_seqlen", _L)]
 
 
 DA_DECODE_SCRATCH_BYTES = 32 << 20
