@@ -25,6 +25,7 @@ constexpr int kWave = 64;
 // ------------------------------------------------------------------------------------
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
+int cu_count();  // compute units of the current device
 
 #define DA_REQUIRE(cond, ...)                                   \
   do {                                                          \

@@ -61,8 +61,43 @@ __device__ __forceinline__ int sequence_of(const PageBatch& s, int t, int lane) 
   return -1;
 }
 
+// A call of paged attention.  A list is the batch's own sequences or the groups of a shared prefix;
+// an item is the queries that one list entry brings to one KV head, its rows are (token, query head of
+// the group) in that order.  Entries of up to kStreamRows rows are `short`: their items' keys go as one
+// stream over the chip (da_paged_stream.hip).
+constexpr int kStreamRows = 32;
+
+struct PagedAttnArgs {
+  const char* q;
+  char* out;
+  int64_t sq_t, sq_h, so_t, so_h;
+  int Hq, Hkv, G, D;
+  float scale_log2;  // softmax scale * log2(e)
+  Pages pages;
+  PageBatch seq, prefix;  // prefix.B = 0: none
+  // stream
+  int workers;       // workgroups of the stream
+  int whole;         // 1: no item is split
+  int slot_rows;     // rows of a slot
+  uint32_t* begin;   // [1 + entries]: tiles a worker, the entries' first tiles
+  float* slots;      // [2 workers][slot_rows][kState]: parts of items, two a worker
+  float* states;     // [2 lists][T][Hq][kState], with a prefix: results of unsplit items
+};
+// a row's result before it is joined: D sums padded to 128, the maximum (log2 units), the sum of weights
+constexpr int kState = 132;
+constexpr int kStreamTile = 128;  // keys
+
+__device__ __forceinline__ bool is_short(int tokens, int G) { return tokens * G <= kStreamRows; }
+// tiles of an item of the stream; a sequence that sees nothing has one, which writes its zeros
+__device__ __forceinline__ int stream_tiles(int tokens, int keys, int G, bool own) {
+  if (tokens == 0 || !is_short(tokens, G)) return 0;
+  const int n = (keys + kStreamTile - 1) / kStreamTile;
+  return own && n == 0 ? 1 : n;
+}
+
 // Host: checks and the kernels' forms of the ABI's blocks.
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who);
+int launch_paged_stream(const PagedAttnArgs& a, int dtype, hipStream_t st);
 int fill_batch(PageBatch& s, const DaPagedBatch* b, const Pages& p, int64_t T, const char* who);
 
 }  // namespace da
