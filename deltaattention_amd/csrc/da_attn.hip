@@ -37,6 +37,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "da_paged.hpp"
 #include "da_tile.hpp"
 
 namespace da {
@@ -44,7 +45,8 @@ namespace da {
 constexpr int kD = 128;
 constexpr int kBlock = 128;  // logical block of the reference schedule
 
-enum Variant : int { kHybrid = 0, kSanity = 1, kPure = 2, kDense = 3 };
+// kPaged: the queries of a paged batch (include/deltaattn_paged.h) over pages, one phase.
+enum Variant : int { kHybrid = 0, kSanity = 1, kPure = 2, kDense = 3, kPaged = 4 };
 
 // ts, cnt, their strides, no_count and cnt_is_float are the schedule kernel's: the attention
 // kernels do not read them, but without them in the block run 0.6 % slower (32768 tokens, hybrid
@@ -88,6 +90,16 @@ struct AttnArgs {
   int units;        // B * Hkv * (G / hpw)
   int slots;        // workgroups an XCD runs at once, two a CU
   int* queue;       // 8 work-queue counters (persistent attn_w64_kernel grid) or null
+};
+
+// kPaged: q and out are [T, heads, D] (s*_b and s*_n their token strides, seq.cu the list's), the keys
+// of a row group are cut into `splits` equal runs of tiles, unit (g, b, heads, split).
+struct PagedRowsArgs : AttnArgs {
+  Pages pages;
+  PageBatch list;
+  int splits;
+  int short_rows;  // entries of up to so many rows are left to the stream
+  float* parts;    // [splits][T][Hq][kState], or null: the result goes to out
 };
 
 // Phase-1 extent of a query block (deltaFlashAttention.py:58-80): n_safe = the number of
@@ -238,8 +250,8 @@ __device__ __forceinline__ void item_at(int k, int units, int n_rg, int slots, i
 // head) over 128 NCB / hpw rows.  Ends with every LDS read of the window loop done (its last
 // barrier) and every load landed; the finalize uses only the wave's own Q region, so the next
 // item may start staging at once.
-template <int VARIANT, int DT, int NCB, bool LAZY>
-__device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit, const int rg) {
+template <int VARIANT, int DT, int NCB, bool LAZY, class Args>
+__device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_split, const int rg) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* const kst0 = smem;
   char* const vst0 = smem + 2 * kWKBytes;
@@ -254,6 +266,11 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
   // wrote (the K fragment layout), so the 32 registers it would take stay free
   char* const qs = meta0 + 4 * kWMetaSlot + wid * kWQBytes;
   const int hl = lane >> 5, ql = lane & 31;
+  int unit = unit_split, split = 0;
+  if constexpr (VARIANT == kPaged) {
+    unit = unit_split / a.splits;
+    split = unit_split - unit * a.splits;
+  }
   const int hsh = a.hpw >> 1;  // log2 of the query heads a workgroup takes
   const int hunits = a.G >> hsh;
   const int gb = unit / hunits;  // g * B + b
@@ -263,8 +280,16 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
   const int h = g * a.G + (hu << hsh) + (wid & ((1 << hsh) - 1));
   const int wg_rows = (128 * NCB) >> hsh;
   const int R0 = rg * wg_rows;
-  const int Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
-  const int Nk = a.seq.cu ? a.seq.len(b) : a.Nk;
+  int Nq, Nk, off = 0;  // row r sees the keys up to r + off
+  if constexpr (VARIANT == kPaged) {
+    Nq = a.list.tokens(b);
+    Nk = a.list.keys(b);
+    off = a.causal ? Nk - Nq : 0;
+    if (Nq * a.G <= a.short_rows) return;
+  } else {
+    Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
+    Nk = a.seq.cu ? a.seq.len(b) : a.Nk;
+  }
   if (R0 >= Nq) return;  // a row group past the end of a shorter sequence (whole workgroup)
   // first row of this wave; column block cb holds r0w + 32 cb + ql
   const int r0w = R0 + 32 * NCB * (wid >> hsh);
@@ -313,6 +338,14 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
     n1 = min(n1 * (kBlock / kWTK), (P + kWTK - 1) / kWTK);
     kend = 0;
   }
+  if constexpr (VARIANT == kPaged) {
+    // this split's run of the row group's tiles
+    const int all = a.causal ? min(Nk, off + wg_end) : Nk;
+    const int tiles = all > 0 ? (all + kWTK - 1) / kWTK : 0;
+    const int per = (tiles + a.splits - 1) / a.splits;
+    ds = dsw = split * per * kWTK;
+    kend = min(all, ds + per * kWTK);
+  }
   n1 = __builtin_amdgcn_readfirstlane(n1);
   ds = __builtin_amdgcn_readfirstlane(ds);
   const int n2 = kend > ds ? (kend - ds + kWTK - 1) / kWTK : 0;
@@ -331,7 +364,7 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
   // causal: a Phase-2 tile whose first key is past the wave's last row is skipped
   int t_skip = INT_MAX;
   if (a.causal) {
-    const int d = r0w + 32 * NCB - 1 - ds;
+    const int d = off + r0w + 32 * NCB - 1 - ds;
     t_skip = __builtin_amdgcn_readfirstlane(d < 0 ? n1 : n1 + d / kWTK + 1);
   }
   if (kPureV) t_skip = __builtin_amdgcn_readfirstlane(n1w);
@@ -408,7 +441,51 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
                                                mlane * 4, 0, 0, 0);
     }
   };
+  // Pages: the wave's eight rows of a tile lie in one page (pages begin at multiples of 16 rows).  Its
+  // number is a scalar load made a window before the tile's K is asked for, and kept for V.
+  int kpage = 0, vpage = 0;
+  auto page_of = [&](int t_raw) {
+    if constexpr (VARIANT == kPaged) {
+      const int key = ds + min(t_raw, T - 1) * kWTK + 8 * wid_s;
+      const int at = min(key, a.list.max_keys - 1) >> a.pages.shift;
+      const auto* table = (const __attribute__((address_space(4))) int32_t*)uniform_ptr(
+          a.list.table + (int64_t)b * a.list.table_stride);
+      return table[__builtin_amdgcn_readfirstlane(at)];
+    } else {
+      return 0;
+    }
+  };
+  auto dma_paged = [&](bool isK, int t_raw, int page, unsigned st) {
+    if constexpr (VARIANT == kPaged) {
+      const int key = ds + min(t_raw, T - 1) * kWTK + 8 * wid_s;
+      const bool there = (unsigned)page < (unsigned)a.pages.num_pages;
+      const int64_t in = key & ((1 << a.pages.shift) - 1), id = there ? page : 0;
+      const int64_t at = isK ? id * a.pages.sk_p + g * a.pages.sk_h + in * a.pages.sk_n
+                             : id * a.pages.sv_p + g * a.pages.sv_h + in * a.pages.sv_n;
+      const int snb = (int)(2 * (isK ? a.pages.sk_n : a.pages.sv_n));
+      const int range = there ? clamp0_uniform(Nk - key, 8) * snb : 0;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<void*>(uniform_ptr((isK ? a.pages.k : a.pages.v) + 2 * at)), (short)0, range, kBufferDword3);
+      char* dst = isK ? kst0 + st : vst0 + st;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = 4 * j + (lane >> 4);  // of the eight
+        const int rowt = 8 * wid_s + row;
+        const int chunk = (lane & 15) ^ (isK ? (rowt & 15) : 4 * (rowt & 3));
+        const int voff = (int)__umul24((unsigned)row, (unsigned)snb) + chunk * 16 + (chunk * 8 < a.D ? 0 : range);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void*)(dst + (2 * wid_s + j) * 1024), 16, voff, 0, 0, 0);
+      }
+    }
+  };
   auto dma_issue = [&](int tk, int tv, unsigned kst, unsigned vst) {
+    if constexpr (VARIANT == kPaged) {
+      dma_paged(true, tk, kpage, kst);
+      dma_paged(false, tv, vpage, vst);
+      vpage = kpage;
+      kpage = page_of(tk + 1);
+      return;
+    }
     dma_rows(true, tk, kst);
     dma_rows(false, tv, vst);
     if (wid_s == 0) dma_meta(tk);
@@ -440,7 +517,13 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
 
   unsigned stA = 0, stB = kWKBytes;
   if (T > 0) {
-    dma_rows(true, 0, stA);
+    if constexpr (VARIANT == kPaged) {
+      vpage = page_of(0);
+      kpage = page_of(1);
+      dma_paged(true, 0, vpage, stA);
+    } else {
+      dma_rows(true, 0, stA);
+    }
     if (wid_s == 0) dma_meta(0);
     dma_issue(1, 0, stB, stA);  // V of tile w - 1 is read in stage stB of window w
   }
@@ -595,8 +678,8 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
       if (kPureV) {
         mask_pure32(s[cb], (const int*)(ms + kWTs), row, hl);
       } else if (t >= n1) {
-        if ((a.causal && key0 + kWTK - 1 > r0w + 32 * cb) || key0 + kWTK > Nk)
-          mask_dense32(s[cb], key0, row, hl, Nk, a.causal);
+        if ((a.causal && key0 + kWTK - 1 > off + r0w + 32 * cb) || key0 + kWTK > Nk)
+          mask_dense32(s[cb], key0, row + off, hl, Nk, a.causal);
       }
     }
     // p against the current maximum first; only where a lane's sum of its 16 p
@@ -704,9 +787,27 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
     const float l_tot = halves_sum(l_i[cb]);
+    if constexpr (VARIANT == kPaged) {
+      if (a.parts) {  // sums, maximum and sum of weights as they are, to be joined
+        const int row = r0w + 32 * cb + ql;
+        if (row < Nq) {
+          float* st = a.parts + (((int64_t)split * a.list.T + a.list.first(b) + row) * a.Hq + h) * kState;
+#pragma unroll
+          for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *(f32x4*)(st + 32 * db + 8 * j + 4 * hl) = f32x4{o[cb][db][4 * j], o[cb][db][4 * j + 1],
+                                                               o[cb][db][4 * j + 2], o[cb][db][4 * j + 3]};
+          if (hl == 0) *(f32x2*)(st + 128) = f32x2{mc[cb], l_tot};
+        }
+        continue;
+      }
+    }
     float inv;
     if (VARIANT == kPure)
       inv = l_tot > 0.0f ? 1.0f / l_tot : 1.0f;  // deltaFlashAttention.py:353-354
+    else if (VARIANT == kPaged)
+      inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;  // a query that sees no key
     else
       inv = 1.0f / l_tot;
 #pragma unroll
@@ -752,14 +853,14 @@ __device__ __forceinline__ void attn_w64_item(const AttnArgs& a, const int unit,
 // the others, so the XCDs, whose clocks differ by several per cent, finish together,
 // and no dispatch gap lies between two items on a CU.  Every counter only grows, so each
 // workgroup's loop ends after at most 8 empty takes; workgroups never wait on each other.
-template <int VARIANT, int DT, int NCB, bool LAZY>
+template <int VARIANT, int DT, int NCB, bool LAZY, class Args = AttnArgs>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void attn_w64_kernel(AttnArgs a) {
+void attn_w64_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int* const slot = (int*)(smem + kWItemSlot);
   const int tid = threadIdx.x;
   const int n_rg = a.n_row_groups;
-  const bool persistent = a.queue != nullptr;
+  const bool persistent = VARIANT != kPaged && a.queue != nullptr;
   unsigned xcc = 0;
   if (persistent) {
     asm volatile("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
@@ -813,10 +914,10 @@ void attn_w64_kernel(AttnArgs a) {
     // opaque per item: its fields are loaded inside each item instead of being held in
     // scalar registers across the loop (the block is the kernel's only argument, at
     // offset 0)
-    const __attribute__((address_space(4))) AttnArgs* ap =
-        (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    const __attribute__((address_space(4))) Args* ap =
+        (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(ap));
-    const AttnArgs ai = *ap;
+    const Args ai = *ap;
     attn_w64_item<VARIANT, DT, NCB, LAZY>(ai, unit, rg);
 #else
     attn_w64_item<VARIANT, DT, NCB, LAZY>(a, unit, rg);
@@ -1011,9 +1112,12 @@ struct F32Frags {
   static constexpr int R = VARIANT == kPure && DB == 4 ? 2 : F % 4 == 0 ? 4 : F;
 };
 
-template <int VARIANT, int DB>
+// What an entry of a table that names no page reads (kPaged).
+__device__ const float kZeroRow[kD] = {};
+
+template <int VARIANT, int DB, class Args = AttnArgs>
 __global__ __launch_bounds__(64 * kFWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void attn_f32_kernel(AttnArgs a, int paired) {
+void attn_f32_kernel(Args a, int paired) {
   constexpr int NW = kFWaves;
   using FR = F32Frags<VARIANT, DB>;
   __shared__ float s_o[NW * 16 * DB * 64];  // the waves' O, [wave][r][db][lane]
@@ -1030,7 +1134,9 @@ void attn_f32_kernel(AttnArgs a, int paired) {
   // shortest up, so that every CU gets about the same work (2048 tokens x 8 heads of 64 dims:
   // 63 us, 80 with the longest first throughout) ----
   const int nrb = (a.Nq + kFRows - 1) / kFRows;
-  const int units = a.B * a.Hq;
+  int splits = 1, split = 0;
+  if constexpr (VARIANT == kPaged) splits = a.splits;
+  const int units = a.B * a.Hq * splits;
   const bool whole = (units & 7) == 0 && (!a.seq.cu || (a.Hq & 7) == 0);
   int unit, j;  // j: row blocks from the last one
   if (paired) {
@@ -1052,11 +1158,22 @@ void attn_f32_kernel(AttnArgs a, int paired) {
   // of units does that by itself)
   if (a.seq.cu && !whole && !(units & 1)) unit = (unit + j) % units;
   const int rb = nrb - 1 - j;
+  if constexpr (VARIANT == kPaged) {
+    split = unit % splits;
+    unit /= splits;
+  }
   const int h = unit / a.B, b = unit % a.B;
   const int g = h / a.G;
   const int bg = b * a.Hkv + g;
-  const int Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
-  const int Nk = a.seq.cu ? a.seq.len(b) : a.Nk;
+  int Nq, Nk, off = 0;  // row r sees the keys up to r + off
+  if constexpr (VARIANT == kPaged) {
+    Nq = a.list.tokens(b);
+    Nk = a.list.keys(b);
+    off = a.causal ? Nk - Nq : 0;
+  } else {
+    Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
+    Nk = a.seq.cu ? a.seq.len(b) : a.Nk;
+  }
   const int R0 = rb * kFRows;
   if (R0 >= Nq) return;  // a row block past the end of a shorter sequence (whole workgroup)
   const int D = a.D;
@@ -1088,6 +1205,14 @@ void attn_f32_kernel(AttnArgs a, int paired) {
     n1 = min(n1 * kBlock, P);
     kend = 0;
   }
+  if constexpr (VARIANT == kPaged) {
+    // this split's run of the row block's tiles
+    const int all = a.causal ? min(Nk, off + R0 + kFRows) : Nk;
+    const int tiles = all > 0 ? (all + kFTile - 1) / kFTile : 0;
+    const int per = (tiles + splits - 1) / splits;
+    ds = split * per * kFTile;
+    kend = min(all, ds + per * kFTile);
+  }
   const int t1 = (n1 + kFTile - 1) / kFTile;
   const int t2 = kend > ds ? (kend - ds + kFTile - 1) / kFTile : 0;
   const int T = t1 + t2;
@@ -1112,6 +1237,70 @@ void attn_f32_kernel(AttnArgs a, int paired) {
   // Fragment f of tile t.  Keys past the source's end repeat its last row (a row of the
   // same tile) and get no weight; dims past D are zero (K) or never stored (V).  A row is a
   // scalar tile base plus a 32-bit lane offset (below 32 rows of less than 2^25 bytes).
+  // Pages: rows 0 .. 15 and 16 .. 31 of a tile each lie in one; a half without keys, or whose entry
+  // names no page, reads a row of zeros with stride 0.
+  struct Halves {
+    const float* p[2][2];  // [K, V][half]
+    unsigned sn[2][2];
+  };
+  auto halves_of = [&](const int t) {
+    Halves x = {};
+    if constexpr (VARIANT == kPaged) {
+      const auto* table = (const __attribute__((address_space(4))) int32_t*)uniform_ptr(
+          a.list.table + (int64_t)b * a.list.table_stride);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int key = __builtin_amdgcn_readfirstlane(ds + t * kFTile + 16 * half);
+        const int page = table[min(key, a.list.max_keys - 1) >> a.pages.shift];
+        const bool there = key < Nk && (unsigned)page < (unsigned)a.pages.num_pages;
+        const int64_t in = key & ((1 << a.pages.shift) - 1), id = there ? page : 0;
+        const float* k = (const float*)a.pages.k + id * a.pages.sk_p + g * a.pages.sk_h + in * a.pages.sk_n;
+        const float* v = (const float*)a.pages.v + id * a.pages.sv_p + g * a.pages.sv_h + in * a.pages.sv_n;
+        x.p[0][half] = there ? k : kZeroRow;
+        x.p[1][half] = there ? v : kZeroRow;
+        x.sn[0][half] = there ? (unsigned)a.pages.sk_n : 0u;
+        x.sn[1][half] = there ? (unsigned)a.pages.sv_n : 0u;
+      }
+    }
+    return x;
+  };
+  Halves at_now, at_next;
+  auto load_paged = [&](auto FC, const Halves& at, const int t, float (&x)[16]) {
+    constexpr int f = decltype(FC)::value;
+    // rows past the last key of a half repeat it
+    const int last = Nk - 1 - (ds + t * kFTile);
+    int ql = lane & 31, hl = lane >> 5;
+    asm volatile("" : "+v"(ql), "+v"(hl));
+    if constexpr (f < DB) {
+      const float* base = ql & 16 ? at.p[0][1] : at.p[0][0];
+      const unsigned sn = ql & 16 ? at.sn[0][1] : at.sn[0][0];
+      base += (unsigned)min(ql & 15, ql & 16 ? max(last - 16, 0) : last) * sn + 4 * hl;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int m = 4 * f + u;
+        const f32x4 w = 8 * m < D ? *(const f32x4*)(base + 8 * m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * u + e] = w[e];
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < FR::NR; ++u) {
+        const int r = (f - DB) * FR::NR + u;
+        const int half = r >> 3;  // of the tile: r < 8 are rows 0 .. 15
+        const float* base = at.p[1][half];
+        const unsigned off = (unsigned)min(8 * ((r >> 2) & 1) + 4 * hl + (r & 3), half ? max(last - 16, 0) : last) * at.sn[1][half];
+        struct __attribute__((packed, aligned(4))) Row { float v[DB]; };
+        if (D == 32 * DB) {
+          const Row w = *(const Row*)(base + off + DB * ql);
+#pragma unroll
+          for (int e = 0; e < DB; ++e) x[DB * u + e] = w.v[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < DB; ++e) x[DB * u + e] = base[off + min(DB * ql + e, D - 1)];
+        }
+      }
+    }
+  };
   auto load = [&](auto FC, const int t, float (&x)[16]) {
     constexpr int f = decltype(FC)::value;
     const bool ph1 = t < t1;
@@ -1156,16 +1345,27 @@ void attn_f32_kernel(AttnArgs a, int paired) {
   float ring[FR::R][16];
 
   int t = wid;
-  if (t < T)
-    static_for<FR::R - 1>([&](auto FC) { load(FC, t, ring[decltype(FC)::value]); });
+  if (t < T) {
+    if constexpr (VARIANT == kPaged) at_next = halves_of(t);
+    static_for<FR::R - 1>([&](auto FC) {
+      if constexpr (VARIANT == kPaged) load_paged(FC, at_next, t, ring[decltype(FC)::value]);
+      else load(FC, t, ring[decltype(FC)::value]);
+    });
+  }
   for (; t < T; t += NW) {
     const bool ph1 = t < t1;
     const int key0 = ph1 ? t * kFTile : ds + (t - t1) * kFTile;
     const int tn = min(t + NW, T - 1);  // past the last tile: loaded again, never used
+    if constexpr (VARIANT == kPaged) {
+      at_now = at_next;
+      at_next = halves_of(tn);
+    }
     // fragment f + R - 1 goes out before fragment f is used
     auto ahead = [&](auto FC) {
       constexpr int n = decltype(FC)::value + FR::R - 1;
-      load(std::integral_constant<int, n % FR::F>{}, n < FR::F ? t : tn, ring[n % FR::R]);
+      constexpr std::integral_constant<int, n % FR::F> NC{};
+      if constexpr (VARIANT == kPaged) load_paged(NC, n < FR::F ? at_now : at_next, n < FR::F ? t : tn, ring[n % FR::R]);
+      else load(NC, n < FR::F ? t : tn, ring[n % FR::R]);
       __builtin_amdgcn_sched_barrier(0);
     };
     f32x16 s = f32x16{};
@@ -1188,7 +1388,7 @@ void attn_f32_kernel(AttnArgs a, int paired) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         bool ok = bias[e] != -INFINITY;
-        if (!ph1) ok = ok && kl + e < kend && (!a.causal || kl + e <= row);     // deltaFlashAttention.py:126-130
+        if (!ph1) ok = ok && kl + e < kend && (!a.causal || kl + e <= row + off);     // deltaFlashAttention.py:126-130
         if (VARIANT == kPure) ok = ok && (e == 0 ? ts.x : e == 1 ? ts.y : e == 2 ? ts.z : ts.w) <= row;  // :338-341
         s[4 * r4 + e] = ok ? (s[4 * r4 + e] + bias[e]) * c : -INFINITY;
         mt = __builtin_fmaxf(mt, s[4 * r4 + e]);
@@ -1242,7 +1442,9 @@ void attn_f32_kernel(AttnArgs a, int paired) {
     L += s_ml[w][1][lane] * f[w];
   }
   // a row without any key (pure Phase 1) stays zero, deltaFlashAttention.py:353-354
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  if constexpr (VARIANT == kPaged)
+    if (a.parts) inv = 1.0f;  // sums, maximum and sum of weights as they are, to be joined
   float x[kOwn * DB];
 #pragma unroll
   for (int i = 0; i < kOwn * DB; ++i) {
@@ -1254,6 +1456,11 @@ void attn_f32_kernel(AttnArgs a, int paired) {
   if (row >= Nq) return;
   const int r0 = kOwn * wid, d0 = DB * (8 * (r0 >> 2) + 4 * hl + (r0 & 3));
   float* orow = (float*)a.out + a.seq.base(b, a.so_b, a.so_n) + (int64_t)h * a.so_h + (int64_t)row * a.so_n;
+  if constexpr (VARIANT == kPaged)
+    if (a.parts) {
+      orow = a.parts + (((int64_t)split * a.list.T + a.list.first(b) + row) * a.Hq + h) * kState;
+      if (wid == 0 && hl == 0) *(f32x2*)(orow + 128) = f32x2{M, L};
+    }
 #pragma unroll
   for (int i = 0; i < kOwn * DB; i += 2)  // D is even: two dims are both in or both out
     if (d0 + i < D) *(f32x2*)(orow + d0 + i) = f32x2{x[i], x[i + 1]};
@@ -1360,6 +1567,75 @@ static int launch_attn_f32(const AttnArgs& a, hipStream_t st) {
     case 3: return launch_attn_f32_t<V, 3>(a, st);
     default: return launch_attn_f32_t<V, 4>(a, st);
   }
+}
+
+// ---- paged batches (da_paged_attn.hip plans them) ----
+template <int DT, int NCB, bool LAZY>
+static int launch_rows_t(const PagedRowsArgs& a, unsigned grid, hipStream_t st) {
+  static int done = 0;
+  if (!done) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, LAZY, PagedRowsArgs>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
+    if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+    done = 1;
+  }
+  hipLaunchKernelGGL((attn_w64_kernel<kPaged, DT, NCB, LAZY, PagedRowsArgs>), dim3(grid), dim3(256), kWLds, st, a);
+  return check_launch("paged attention (rows)");
+}
+
+template <int DB>
+static int launch_rows_f32(const PagedRowsArgs& a, unsigned grid, hipStream_t st) {
+  hipLaunchKernelGGL((attn_f32_kernel<kPaged, DB, PagedRowsArgs>), dim3(grid), dim3(64 * kFWaves), 0, st, a,
+                     grid <= 2u * cu_count() ? 1 : 0);
+  return check_launch("paged attention (rows, fp32)");
+}
+
+RowsShape paged_rows_shape(int dtype, int G) {
+  if (dtype == DA_F32) return RowsShape{1, kFRows, kFRows};
+  const int hpw = G % 4 == 0 ? 4 : (G % 2 == 0 ? 2 : 1);
+  return RowsShape{hpw, 128 / hpw, 256 / hpw};
+}
+
+int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts, int dtype,
+                      hipStream_t st) {
+  const RowsShape shape = paged_rows_shape(dtype, p.G);
+  PagedRowsArgs a = {};
+  a.q = (const uint16_t*)p.q; a.out = (uint16_t*)p.out;
+  a.sq_b = a.sq_n = p.sq_t; a.sq_h = p.sq_h;
+  a.so_b = a.so_n = p.so_t; a.so_h = p.so_h;
+  a.B = list.B; a.Hq = p.Hq; a.Hkv = p.Hkv; a.G = p.G; a.D = p.D;
+  a.Nq = list.max_len;
+  a.seq = SeqMap{list.cu, list.T, list.max_len};
+  a.scale_log2 = p.scale_log2;
+  a.causal = own ? 1 : 0;
+  a.hpw = shape.hpw;
+  a.pages = p.pages;
+  a.list = list;
+  a.splits = splits;
+  a.short_rows = p.short_rows[own];
+  a.parts = parts;
+  const int rows = wide ? shape.wide : shape.narrow;
+  a.n_row_groups = (list.max_len + rows - 1) / rows;
+  a.units = list.B * (p.Hq / shape.hpw) * splits;
+  a.slots = 2 * cu_count() / 8;
+  const int64_t grid = (int64_t)a.units * a.n_row_groups;
+  if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
+  if (dtype == DA_F32) {
+    switch ((p.D + 31) / 32) {
+      case 1: return launch_rows_f32<1>(a, (unsigned)grid, st);
+      case 2: return launch_rows_f32<2>(a, (unsigned)grid, st);
+      case 3: return launch_rows_f32<3>(a, (unsigned)grid, st);
+      default: return launch_rows_f32<4>(a, (unsigned)grid, st);
+    }
+  }
+  const unsigned n = (unsigned)grid;
+  const bool lazy = shape.hpw == 4;
+  if (dtype == DA_F16) {
+    if (wide) return lazy ? launch_rows_t<DA_F16, 2, true>(a, n, st) : launch_rows_t<DA_F16, 2, false>(a, n, st);
+    return lazy ? launch_rows_t<DA_F16, 1, true>(a, n, st) : launch_rows_t<DA_F16, 1, false>(a, n, st);
+  }
+  if (wide) return lazy ? launch_rows_t<DA_BF16, 2, true>(a, n, st) : launch_rows_t<DA_BF16, 2, false>(a, n, st);
+  return lazy ? launch_rows_t<DA_BF16, 1, true>(a, n, st) : launch_rows_t<DA_BF16, 1, false>(a, n, st);
 }
 
 static int launch_attn(int variant, int dtype, AttnArgs& a, hipStream_t st) {

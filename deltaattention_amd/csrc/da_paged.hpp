@@ -75,6 +75,8 @@ struct PagedAttnArgs {
   float scale_log2;  // softmax scale * log2(e)
   Pages pages;
   PageBatch seq, prefix;  // prefix.B = 0: none
+  int short_rows[2];  // of both lists ([0] the prefix, [1] the sequences): entries of up to so many
+                      // rows are the stream's
   // stream
   int workers;       // workgroups of the stream
   int whole;         // 1: no item is split
@@ -82,21 +84,32 @@ struct PagedAttnArgs {
   uint32_t* begin;   // [1 + entries]: tiles a worker, the entries' first tiles
   float* slots;      // [2 workers][slot_rows][kState]: parts of items, two a worker
   float* states;     // [2 lists][T][Hq][kState], with a prefix: results of unsplit items
+  // entries with more rows: their items' keys in so many parts, by list
+  int splits[2];
+  float* parts[2];   // [splits][T][Hq][kState], or null: the result is in out
 };
 // a row's result before it is joined: D sums padded to 128, the maximum (log2 units), the sum of weights
 constexpr int kState = 132;
 constexpr int kStreamTile = 128;  // keys
 
-__device__ __forceinline__ bool is_short(int tokens, int G) { return tokens * G <= kStreamRows; }
 // tiles of an item of the stream; a sequence that sees nothing has one, which writes its zeros
-__device__ __forceinline__ int stream_tiles(int tokens, int keys, int G, bool own) {
-  if (tokens == 0 || !is_short(tokens, G)) return 0;
+__device__ __forceinline__ int stream_tiles(const PagedAttnArgs& a, int tokens, int keys, bool own) {
+  if (tokens == 0 || tokens * a.G > a.short_rows[own]) return 0;
   const int n = (keys + kStreamTile - 1) / kStreamTile;
   return own && n == 0 ? 1 : n;
 }
 
 // Host: checks and the kernels' forms of the ABI's blocks.
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who);
+// Rows of one query head that a workgroup of the row kernels takes (with its query heads): half-size
+// and full-size groups.
+struct RowsShape {
+  int hpw, narrow, wide;
+};
+RowsShape paged_rows_shape(int dtype, int G);
+// The entries of `list` with more than short_rows rows.
+int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts, int dtype,
+                      hipStream_t st);
 int launch_paged_stream(const PagedAttnArgs& a, int dtype, hipStream_t st);
 int fill_batch(PageBatch& s, const DaPagedBatch* b, const Pages& p, int64_t T, const char* who);
 

@@ -98,7 +98,7 @@ void paged_stream_kernel(PagedAttnArgs a) {
   const int E = a.prefix.B + a.seq.B;
   // units of the share: tiles, or items where none is split
   auto units_of = [&](int tokens, int keys, bool own) {
-    const int n = stream_tiles(tokens, keys, a.G, own);
+    const int n = stream_tiles(a, tokens, keys, own);
     return (uint32_t)(a.whole ? min(n, 1) : n) * (uint32_t)a.Hkv;
   };
 
@@ -175,7 +175,7 @@ void paged_stream_kernel(PagedAttnArgs a) {
     f = __builtin_amdgcn_readfirstlane(f);
     nt = __builtin_amdgcn_readfirstlane(nt);
     nk = __builtin_amdgcn_readfirstlane(nk);
-    const int tiles = stream_tiles(nt, nk, a.G, own);
+    const int tiles = stream_tiles(a, nt, nk, own);
     if (tiles == 0) {
       ++e;
       continue;
@@ -372,56 +372,6 @@ void paged_stream_kernel(PagedAttnArgs a) {
   }
 }
 
-// ---- the parts of a row joined: a wave a (token, query head), two dims a lane ----
-template <int DT>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int t = blockIdx.x, h = blockIdx.y * 4 + wid;
-  if (h >= a.Hq) return;
-  const int b = sequence_of(a.seq, t, lane);
-  if (b < 0) return;
-  const int g = h / a.G;
-  float M = -INFINITY, L = 0.0f, y0 = 0.0f, y1 = 0.0f;
-  // a part's state: the running result takes it in
-  auto take = [&](const float* st) {
-    const f32x2 ml = *(const f32x2*)(st + 128), z = *(const f32x2*)(st + 2 * lane);
-    const float mn = __builtin_fmaxf(M, ml[0]), ref = mn == -INFINITY ? 0.0f : mn;
-    const float fo = exp2_fast(M - ref), fn = exp2_fast(ml[0] - ref);
-    y0 = y0 * fo + z[0] * fn;
-    y1 = y1 * fo + z[1] * fn;
-    L = L * fo + ml[1] * fn;
-    M = mn;
-  };
-  for (int list = a.prefix.B ? 0 : 1; list < 2; ++list) {
-    const PageBatch& s = list ? a.seq : a.prefix;
-    const int e = list ? b : sequence_of(s, t, lane);
-    if (e < 0) continue;
-    const int tokens = s.tokens(e), i = t - s.first(e);
-    if (i >= tokens) {
-      if (list) return;
-      continue;
-    }
-    const int tiles = stream_tiles(tokens, s.keys(e), a.G, list);
-    if (tiles == 0) continue;
-    const uint32_t per = a.whole ? 1 : a.begin[0];
-    const uint32_t U = a.whole ? 0 : a.begin[1 + (list ? a.prefix.B : 0) + e] + g * tiles;
-    const uint32_t w0 = U / per, w1 = a.whole ? w0 : (U + tiles - 1) / per;
-    if (w0 == w1) {
-      if (a.prefix.B == 0) return;  // written where it was computed
-      take(a.states + (((int64_t)list * a.seq.T + t) * a.Hq + h) * kState);
-      continue;
-    }
-    const int r = i * a.G + h - g * a.G;
-    for (uint32_t w = w0; w <= w1; ++w)
-      take(a.slots + ((int64_t)(2 * w + (w == w0 && U != w0 * per ? 1 : 0)) * a.slot_rows + r) * kState);
-  }
-  if (2 * lane >= a.D) return;
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-  char* row = a.out + 2 * (t * a.so_t + h * a.so_h);
-  *(uint32_t*)(row + 4 * lane) = E16<DT>::pack(y0 * inv, y1 * inv);
-}
-
 template <int DT>
 static int launch_stream_t(const PagedAttnArgs& a, hipStream_t st) {
   static int done = 0;
@@ -432,10 +382,7 @@ static int launch_stream_t(const PagedAttnArgs& a, hipStream_t st) {
     done = 1;
   }
   hipLaunchKernelGGL(paged_stream_kernel<DT>, dim3((unsigned)a.workers), dim3(256), kStreamLds, st, a);
-  if (int rc = check_launch("paged attention (stream)")) return rc;
-  if (a.whole && a.prefix.B == 0) return DA_OK;
-  hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((unsigned)a.seq.T, (unsigned)((a.Hq + 3) / 4)), dim3(256), 0, st, a);
-  return check_launch("paged attention (join)");
+  return check_launch("paged attention (stream)");
 }
 
 int launch_paged_stream(const PagedAttnArgs& a, int dtype, hipStream_t st) {
