@@ -93,7 +93,7 @@ struct AttnArgs {
 };
 
 // kPaged: q and out are [T, heads, D] (s*_b and s*_n their token strides, seq.cu the list's), the keys
-// of a row group are cut into `splits` equal runs of tiles, unit (g, b, heads, split).
+// of a row group are cut into `splits` equal runs of tiles, unit (g, heads, b, split).
 struct PagedRowsArgs : AttnArgs {
   Pages pages;
   PageBatch list;
@@ -273,9 +273,19 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   }
   const int hsh = a.hpw >> 1;  // log2 of the query heads a workgroup takes
   const int hunits = a.G >> hsh;
-  const int gb = unit / hunits;  // g * B + b
-  const int hu = unit - gb * hunits;
-  const int g = gb / a.B, b = gb - (gb / a.B) * a.B;
+  int g, b, hu;
+  if constexpr (VARIANT == kPaged) {
+    // (g, hu) by b: an XCD's units are some heads of every sequence, whatever the sequences' lengths
+    const int head = unit / a.B;
+    b = unit - head * a.B;
+    g = head / hunits;
+    hu = head - g * hunits;
+  } else {
+    const int gb = unit / hunits;  // g * B + b
+    hu = unit - gb * hunits;
+    g = gb / a.B;
+    b = gb - (gb / a.B) * a.B;
+  }
   const int bg = b * a.Hkv + g;
   const int h = g * a.G + (hu << hsh) + (wid & ((1 << hsh) - 1));
   const int wg_rows = (128 * NCB) >> hsh;
@@ -1570,16 +1580,16 @@ static int launch_attn_f32(const AttnArgs& a, hipStream_t st) {
 }
 
 // ---- paged batches (da_paged_attn.hip plans them) ----
-template <int DT, int NCB, bool LAZY>
+template <int DT, int NCB>
 static int launch_rows_t(const PagedRowsArgs& a, unsigned grid, hipStream_t st) {
   static int done = 0;
   if (!done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, LAZY, PagedRowsArgs>),
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
     if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
     done = 1;
   }
-  hipLaunchKernelGGL((attn_w64_kernel<kPaged, DT, NCB, LAZY, PagedRowsArgs>), dim3(grid), dim3(256), kWLds, st, a);
+  hipLaunchKernelGGL((attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>), dim3(grid), dim3(256), kWLds, st, a);
   return check_launch("paged attention (rows)");
 }
 
@@ -1629,13 +1639,8 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
     }
   }
   const unsigned n = (unsigned)grid;
-  const bool lazy = shape.hpw == 4;
-  if (dtype == DA_F16) {
-    if (wide) return lazy ? launch_rows_t<DA_F16, 2, true>(a, n, st) : launch_rows_t<DA_F16, 2, false>(a, n, st);
-    return lazy ? launch_rows_t<DA_F16, 1, true>(a, n, st) : launch_rows_t<DA_F16, 1, false>(a, n, st);
-  }
-  if (wide) return lazy ? launch_rows_t<DA_BF16, 2, true>(a, n, st) : launch_rows_t<DA_BF16, 2, false>(a, n, st);
-  return lazy ? launch_rows_t<DA_BF16, 1, true>(a, n, st) : launch_rows_t<DA_BF16, 1, false>(a, n, st);
+  if (dtype == DA_F16) return wide ? launch_rows_t<DA_F16, 2>(a, n, st) : launch_rows_t<DA_F16, 1>(a, n, st);
+  return wide ? launch_rows_t<DA_BF16, 2>(a, n, st) : launch_rows_t<DA_BF16, 1>(a, n, st);
 }
 
 static int launch_attn(int variant, int dtype, AttnArgs& a, hipStream_t st) {

@@ -67,6 +67,12 @@ __device__ __forceinline__ int sequence_of(const PageBatch& s, int t, int lane) 
 // stream over the chip (da_paged_stream.hip).
 constexpr int kStreamRows = 32;
 
+// An item that several workers of the stream share, kept by the one with its first part.
+struct StreamRecord {
+  int first, tokens, head;  // the entry's first token and its tokens, the KV head
+  int slot, others;         // the first part's slot; the parts after it, each in the next worker's first slot
+};
+
 struct PagedAttnArgs {
   const char* q;
   char* out;
@@ -81,7 +87,8 @@ struct PagedAttnArgs {
   int workers;       // workgroups of the stream
   int whole;         // 1: no item is split
   int slot_rows;     // rows of a slot
-  uint32_t* begin;   // [1 + entries]: tiles a worker, the entries' first tiles
+  uint32_t* begin;   // [2 + entries]: tiles a worker, the entries' first tiles, all tiles
+  StreamRecord* records;  // [workers], where the stream's items are joined by themselves, or null
   float* slots;      // [2 workers][slot_rows][kState]: parts of items, two a worker
   float* states;     // [2 lists][T][Hq][kState], with a prefix: results of unsplit items
   // entries with more rows: their items' keys in so many parts, by list
@@ -98,6 +105,45 @@ __device__ __forceinline__ int stream_tiles(const PagedAttnArgs& a, int tokens, 
   const int n = (keys + kStreamTile - 1) / kStreamTile;
   return own && n == 0 ? 1 : n;
 }
+
+// Four dims d .. d + 3 of a row's sums, and the row's maximum and sum of weights, over parts.
+struct RowSum {
+  float M = -INFINITY, L = 0.0f;
+  f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+  __device__ __forceinline__ void add(f32x2 ml, f32x4 z) {
+    const float mn = __builtin_fmaxf(M, ml[0]), ref = mn == -INFINITY ? 0.0f : mn;
+    const float fo = __builtin_amdgcn_exp2f(M - ref), fn = __builtin_amdgcn_exp2f(ml[0] - ref);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = y[i] * fo + z[i] * fn;
+    L = L * fo + ml[1] * fn;
+    M = mn;
+  }
+  __device__ __forceinline__ void take(const float* state, int d) { add(*(const f32x2*)(state + 128), *(const f32x4*)(state + d)); }
+  // n states `step` floats apart, four in flight
+  __device__ __forceinline__ void take_all(const float* state, int64_t step, int n, int d) {
+    for (int i = 0; i < n; i += 4) {
+      f32x2 ml[4];
+      f32x4 z[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // past the last: read again, left out
+        const float* p = state + min(i + j, n - 1) * step;
+        ml[j] = *(const f32x2*)(p + 128);
+        z[j] = *(const f32x4*)(p + d);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) add(ml[j], z[j]);
+    }
+  }
+  template <int DT>
+  __device__ __forceinline__ void store(const PagedAttnArgs& a, int token, int head, int d) const {
+    if (d >= a.D) return;
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const int64_t at = token * a.so_t + head * a.so_h + d;
+    if constexpr (DT == DA_F32) *(f32x4*)(a.out + 4 * at) = f32x4{y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+    else *(u32x2*)(a.out + 2 * at) = u32x2{E16<DT>::pack(y[0] * inv, y[1] * inv), E16<DT>::pack(y[2] * inv, y[3] * inv)};
+  }
+};
 
 // Host: checks and the kernels' forms of the ABI's blocks.
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who);

@@ -7,77 +7,123 @@
 // A prefix is a list of its own, seen whole by all rows of a group at once: its keys are read once for
 // the group, and each row's result is joined with that of its own sequence.
 #include <algorithm>
+#include <cmath>
 
 #include "da_paged.hpp"
 #include "da_tile.hpp"
 
 namespace da {
 
-// The parts of a row joined: a wave a (token, query head), two dims a lane.
-template <int DT>
+// The parts of every row joined: a row's 128 dims over 32 lanes, eight rows of a token a workgroup; or,
+// with WIDE, where rows are few, one row, whose parts eight half-waves share.
+template <int DT, bool WIDE>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int t = blockIdx.x, h = blockIdx.y * 4 + wid;
-  if (h >= a.Hq) return;
-  const int b = sequence_of(a.seq, t, lane);
-  if (b < 0) return;
+  __shared__ float s_sum[WIDE ? 8 : 1][kState];
+  const int lane = threadIdx.x & 63, t = blockIdx.x, d = 4 * (threadIdx.x & 31), half = threadIdx.x >> 5;
+  const int h = WIDE ? blockIdx.y : blockIdx.y * 8 + half;
+  const int entry[2] = {a.prefix.B ? sequence_of(a.prefix, t, lane) : -1, sequence_of(a.seq, t, lane)};
+  if (entry[1] < 0 || h >= a.Hq) return;
   const int g = h / a.G;
-  float M = -INFINITY, L = 0.0f, y0 = 0.0f, y1 = 0.0f;
-  // a part's state: the running result takes it in
-  auto take = [&](const float* st) {
-    const f32x2 ml = *(const f32x2*)(st + 128), z = *(const f32x2*)(st + 2 * lane);
-    const float mn = __builtin_fmaxf(M, ml[0]), ref = mn == -INFINITY ? 0.0f : mn;
-    const float fo = exp2_fast(M - ref), fn = exp2_fast(ml[0] - ref);
-    y0 = y0 * fo + z[0] * fn;
-    y1 = y1 * fo + z[1] * fn;
-    L = L * fo + ml[1] * fn;
-    M = mn;
-  };
-  for (int list = a.prefix.B ? 0 : 1; list < 2; ++list) {
+  const int first = WIDE ? half : 0, by = WIDE ? 8 : 1;  // this half-wave's parts
+  RowSum sum;
+  for (int list = 0; list < 2; ++list) {
     const PageBatch& s = list ? a.seq : a.prefix;
-    const int e = list ? b : sequence_of(s, t, lane);
+    const int e = entry[list];
     if (e < 0) continue;
     const int tokens = s.tokens(e), i = t - s.first(e);
     if (i >= tokens) {
       if (list) return;
       continue;
     }
+    const float* state;
+    int64_t step = 0;
+    int n = 1;
     if (tokens * a.G > a.short_rows[list]) {  // the row kernels'
       if (!a.parts[list]) return;
-      for (int p = 0; p < a.splits[list]; ++p) take(a.parts[list] + (((int64_t)p * s.T + t) * a.Hq + h) * kState);
-      continue;
+      state = a.parts[list] + ((int64_t)t * a.Hq + h) * kState;
+      step = (int64_t)s.T * a.Hq * kState;
+      n = a.splits[list];
+    } else {
+      const int tiles = stream_tiles(a, tokens, s.keys(e), list);
+      if (tiles == 0) continue;
+      const uint32_t per = a.whole ? 1 : a.begin[0];
+      const uint32_t U = a.whole ? 0 : a.begin[1 + (list ? a.prefix.B : 0) + e] + g * tiles;
+      const uint32_t w0 = U / per, w1 = a.whole ? w0 : (U + tiles - 1) / per;
+      if (w0 == w1) {
+        if (a.prefix.B == 0) return;  // written where it was computed
+        state = a.states + (((int64_t)list * a.seq.T + t) * a.Hq + h) * kState;
+      } else {
+        // the first part may be its worker's last segment; the others are their workers' first
+        const int r = i * a.G + h - g * a.G;
+        if (first == 0) sum.take(a.slots + ((int64_t)(2 * w0 + (U != w0 * per ? 1 : 0)) * a.slot_rows + r) * kState, d);
+        state = a.slots + (2 * ((int64_t)w0 + 1) * a.slot_rows + r) * kState;
+        step = 2 * (int64_t)a.slot_rows * kState;
+        n = w1 - w0;
+      }
     }
-    const int tiles = stream_tiles(a, tokens, s.keys(e), list);
-    if (tiles == 0) continue;
-    const uint32_t per = a.whole ? 1 : a.begin[0];
-    const uint32_t U = a.whole ? 0 : a.begin[1 + (list ? a.prefix.B : 0) + e] + g * tiles;
-    const uint32_t w0 = U / per, w1 = a.whole ? w0 : (U + tiles - 1) / per;
-    if (w0 == w1) {
-      if (a.prefix.B == 0) return;  // written where it was computed
-      take(a.states + (((int64_t)list * a.seq.T + t) * a.Hq + h) * kState);
-      continue;
-    }
-    const int r = i * a.G + h - g * a.G;
-    for (uint32_t w = w0; w <= w1; ++w)
-      take(a.slots + ((int64_t)(2 * w + (w == w0 && U != w0 * per ? 1 : 0)) * a.slot_rows + r) * kState);
+    if (first < n) sum.take_all(state + first * step, by * step, (n - first + by - 1) / by, d);
   }
-  if (2 * lane >= a.D) return;
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-  if constexpr (DT == DA_F32)
-    *(f32x2*)(a.out + 4 * (t * a.so_t + h * a.so_h) + 8 * lane) = f32x2{y0 * inv, y1 * inv};
-  else
-    *(uint32_t*)(a.out + 2 * (t * a.so_t + h * a.so_h) + 4 * lane) = E16<DT>::pack(y0 * inv, y1 * inv);
+  if constexpr (WIDE) {
+    *(f32x4*)(&s_sum[half][d]) = sum.y;
+    if (d == 0) *(f32x2*)(&s_sum[half][128]) = f32x2{sum.M, sum.L};
+    __syncthreads();
+    if (half > 0) return;
+    for (int i = 1; i < 8; ++i) sum.take(s_sum[i], d);
+  }
+  sum.template store<DT>(a, t, h, d);
 }
 
-// Items of up to kWholeTiles tiles are not split: one launch.
-constexpr int kWholeTiles = 8;
-// A part of a row kernel's item has at least so many keys.
-constexpr int kPartKeys = 1024;
+template <int DT>
+static int launch_join(const PagedAttnArgs& a, hipStream_t st) {
+  const int T = a.seq.T;
+  if ((int64_t)T * a.Hq <= 8 * cu_count())
+    hipLaunchKernelGGL((paged_join_kernel<DT, true>), dim3((unsigned)T, (unsigned)a.Hq), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((paged_join_kernel<DT, false>), dim3((unsigned)T, (unsigned)((a.Hq + 7) / 8)), dim3(256), 0, st, a);
+  return check_launch("paged attention (join)");
+}
+
+// The stream's items are not split (one launch, a workgroup an item) up to 6 tiles, and up to 16 where
+// the items fill half the CUs.  One sequence of 8 heads: 400 keys 12.1 us against 11.8 split, 600 13.4 / 12.3,
+// 1000 17.2 / 12.9, where a second launch costs the caller 4; 16 sequences: 600 keys 15.7 / 20.9, 2000
+// 28.7 / 32.2; 64: 2000 96.5 / 98.4.
+static bool stream_whole(int64_t items, int keys) {
+  const int tiles = (keys + kStreamTile - 1) / kStreamTile;
+  return tiles <= 6 || (tiles <= 16 && 2 * items >= cu_count());
+}
+
+// Rows of a head that a workgroup of the row kernels takes, and into how many runs it cuts the keys:
+// the least of an estimate.  A run's time is its 32-key tiles times a tile's (us, measured with up to
+// one workgroup a CU and with two); parts cost their writing and reading, 3.5 TB/s, and a launch.
+// 512 tokens of 32 heads after 5000: narrow 1 part 141 us, 4 parts 72, 8 82, wide 8 75; 2048 after 30011:
+// narrow 998, wide 1204, 2 parts 903, 4 924; 512 at a sequence's start: 1 part 21, 2 31.
+static void shape_rows(PagedAttnArgs& a, int list, bool& wide, int dtype) {
+  const PageBatch& s = list ? a.seq : a.prefix;
+  const RowsShape shape = paged_rows_shape(dtype, a.G);
+  const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = 2.0 * cu_count();
+  const int tiles = (s.max_keys + 31) / 32;
+  double best = 0.0;
+  for (int w = 0; w < (shape.wide > shape.narrow && s.max_len > shape.narrow ? 2 : 1); ++w) {
+    const int rows = w ? shape.wide : shape.narrow;
+    // items: those of the longest entry, and of the others if their mean is not the stream's
+    const int64_t longest = (s.max_len + rows - 1) / rows, others = s.B - 1, rest = s.T - s.max_len;
+    int64_t items = longest;
+    if (others > 0 && rest * a.G > others * a.short_rows[list]) items += std::min(others * longest, rest / rows + others);
+    items *= a.Hq / shape.hpw;
+    for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (n > 1 && n > tiles) break;
+      const double all = (double)items * n, rounds = all <= slots ? 1.0 : all / slots + 0.3;
+      const bool two = 2 * all > slots;
+      const double tile = dtype == DA_F32 ? (two ? 1.75 : 0.9) * ((a.D + 31) / 32) / 4 : w ? (two ? 1.75 : 1.22) : (two ? 1.0 : 0.78);
+      const double time = rounds * ((tiles + n - 1) / n) * tile + (n > 1 || a.prefix.B ? n * part + (n > 1 ? 5 : 0) : 0.0);
+      if ((w == 0 && n == 1) || time < best) best = time, wide = w, a.splits[list] = n;
+    }
+  }
+}
 
 struct PagedPlan {
   bool stream, rows[2], wide[2], join;
-  int64_t slots, states, parts[2], total;  // byte offsets in the workspace
+  int64_t records, slots, states, parts[2], total;  // byte offsets in the workspace
 };
 static int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -105,25 +151,17 @@ static PagedPlan plan(PagedAttnArgs& a, int dtype) {
     }
     p.rows[i] = most > a.short_rows[i];
     if (!p.rows[i]) continue;
-    const RowsShape shape = paged_rows_shape(dtype, a.G);
-    auto items = [&](int rows) {
-      const int64_t all = (int64_t)s.B * ((s.max_len + rows - 1) / rows);
-      return std::min<int64_t>(all, s.T / rows + s.B) * (a.Hq / shape.hpw);
-    };
-    const int64_t slots = 2 * cu_count();
-    p.wide[i] = s.max_len > shape.narrow;
-    const int64_t n = items(p.wide[i] ? shape.wide : shape.narrow);
-    a.splits[i] = (int)std::max<int64_t>(1, std::min<int64_t>((slots + n - 1) / n, s.max_keys / kPartKeys));
-    if (a.splits[i] == 1 && n < slots) p.wide[i] = false;
+    shape_rows(a, i, p.wide[i], dtype);
     if (a.splits[i] > 1 || a.prefix.B) parts |= 1 << i;
   }
-  a.whole = keys <= kWholeTiles * kStreamTile;
+  a.whole = stream_whole((int64_t)E * a.Hkv, keys);
   a.workers = a.whole ? E * a.Hkv : 2 * cu_count();
   a.slot_rows = (int)slot_rows;
   const bool cut = p.stream && !a.whole;
-  p.join = a.prefix.B || cut || parts;
+  p.join = a.prefix.B || parts;  // else the stream joins its own parts
   const int64_t state = (int64_t)a.seq.T * a.Hq * kState * 4;
-  p.slots = cut ? round256(4 * (1 + (int64_t)E)) : 0;
+  p.records = cut ? round256(4 * (2 + (int64_t)E)) : 0;
+  p.slots = p.records + (cut && !p.join ? round256(a.workers * (int64_t)sizeof(StreamRecord)) : 0);
   p.states = p.slots + (cut ? round256(2 * (int64_t)a.workers * slot_rows * kState * 4) : 0);
   p.parts[0] = p.states + (p.stream && a.prefix.B ? 2 * round256(state) : 0);
   p.parts[1] = p.parts[0] + (parts & 1 ? round256(a.splits[0] * state) : 0);
@@ -187,6 +225,7 @@ extern "C" int da_paged_attention(const void* q, int64_t sq_t, int64_t sq_h, voi
   DA_REQUIRE(((uintptr_t)workspace & 255) == 0, "%s: the workspace must be 256-byte aligned", who);
   char* ws = (char*)workspace;
   a.begin = (uint32_t*)ws;
+  a.records = p.join || a.whole ? nullptr : (StreamRecord*)(ws + p.records);
   a.slots = (float*)(ws + p.slots);
   a.states = (float*)(ws + p.states);
   for (int i = 0; i < 2; ++i) a.parts[i] = p.parts[i] < 0 ? nullptr : (float*)(ws + p.parts[i]);
@@ -197,11 +236,5 @@ extern "C" int da_paged_attention(const void* q, int64_t sq_t, int64_t sq_h, voi
     if (p.rows[i])
       if (int rc = launch_paged_rows(a, i ? a.seq : a.prefix, i == 1, p.wide[i], a.splits[i], a.parts[i], dtype, st)) return rc;
   if (!p.join) return DA_OK;
-  const dim3 grid((unsigned)T, (unsigned)((Hq + 3) / 4));
-  switch (dtype) {
-    case DA_BF16: hipLaunchKernelGGL(paged_join_kernel<DA_BF16>, grid, dim3(256), 0, st, a); break;
-    case DA_F16: hipLaunchKernelGGL(paged_join_kernel<DA_F16>, grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL(paged_join_kernel<DA_F32>, grid, dim3(256), 0, st, a);
-  }
-  return check_launch("paged attention (join)");
+  return dtype == DA_BF16 ? launch_join<DA_BF16>(a, st) : dtype == DA_F16 ? launch_join<DA_F16>(a, st) : launch_join<DA_F32>(a, st);
 }

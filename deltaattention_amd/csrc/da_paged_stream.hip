@@ -17,7 +17,7 @@
 
 namespace da {
 
-constexpr int kWaveLds = 16384;  // a wave's K and V tiles; its rows' sums at the end
+constexpr int kStageLds = 16384;  // a wave's K and V tiles; its rows' sums at the end
 constexpr int kStreamEntries = 256;
 struct StreamShared {
   float ml[4][2][32];
@@ -25,35 +25,38 @@ struct StreamShared {
   uint32_t waves[4], total;
   int entry;
   uint32_t offset;
+  StreamRecord record;
 };
-constexpr int kStreamLds = 4 * kWaveLds + (int)sizeof(StreamShared);
+constexpr int stream_lds(int stages) { return 4 * stages * kStageLds + (int)sizeof(StreamShared); }
 
-// Waits for all but the last N loads, then for the eight 16-byte reads at a ^ 32 j.
+// Waits for all but the wave's last N loads.
 template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+// The eight 16-byte reads at a ^ 32 j, waited for.
 __device__ __forceinline__ void read_keys(u32x4 (&k)[8], uint32_t a) {
   asm volatile(
-      "s_waitcnt vmcnt(%16)\n\t"
       "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
       "ds_read_b128 %4, %12\n\tds_read_b128 %5, %13\n\tds_read_b128 %6, %14\n\tds_read_b128 %7, %15\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(k[4]), "=&v"(k[5]), "=&v"(k[6]), "=&v"(k[7])
-      : "v"(a), "v"(a ^ 32u), "v"(a ^ 64u), "v"(a ^ 96u), "v"(a ^ 128u), "v"(a ^ 160u), "v"(a ^ 192u), "v"(a ^ 224u), "i"(N)
+      : "v"(a), "v"(a ^ 32u), "v"(a ^ 64u), "v"(a ^ 96u), "v"(a ^ 128u), "v"(a ^ 160u), "v"(a ^ 192u), "v"(a ^ 224u)
       : "memory");
 }
 // The V^T fragments of 16 keys (OFF: their byte offset): four blocks of 32 dims at a ^ 64 db, two
 // transposing reads each.
-template <int OFF, int N>
+template <int OFF>
 __device__ __forceinline__ void read_values(u32x4 (&v)[4], uint32_t a) {
   i16x4 lo[4], hi[4];
   asm volatile(
-      "s_waitcnt vmcnt(%14)\n\t"
       "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
       "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
       "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
       "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-      : "v"(a), "v"(a ^ 64u), "v"(a ^ 128u), "v"(a ^ 192u), "i"(OFF), "i"(OFF + 2048), "i"(N)
+      : "v"(a), "v"(a ^ 64u), "v"(a ^ 128u), "v"(a ^ 192u), "i"(OFF), "i"(OFF + 2048)
       : "memory");
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -87,65 +90,89 @@ __device__ __forceinline__ uint32_t workgroup_sum(uint32_t x, StreamShared& sh, 
   return incl - x + (wid > 0 ? w0 : 0) + (wid > 1 ? w1 : 0) + (wid > 2 ? w2 : 0);
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// A worker's run of tiles: from tile `offset` (head by head) of entry `entry` on.  Entries chunk ..
+// chunk + 255 are in sh.
+struct Share {
+  int entry, chunk;
+  uint32_t offset, tiles, per;
+};
+
+// Workgroup-uniform; false if there is nothing to do.  Where no item is split, worker w has item w (offset
+// is its head, tiles 1).
+__device__ __forceinline__ bool share_of(const PagedAttnArgs& a, StreamShared& sh, Share& share) {
+  const int tid = threadIdx.x, E = a.prefix.B + a.seq.B;
+  int first = 0, tokens = 0, keys = 0;
+  if (a.whole) {
+    const int e = blockIdx.x / a.Hkv;
+    entry_of(a, e, first, tokens, keys);
+    if (stream_tiles(a, tokens, keys, e >= a.prefix.B) == 0) return false;
+    if (tid == 0) sh.first[0] = first, sh.tokens[0] = tokens, sh.keys[0] = keys;
+    __syncthreads();
+    share = Share{e, e, (uint32_t)(blockIdx.x - e * a.Hkv), 1, 1};
+    return true;
+  }
+  // the entries' tiles summed in order, 256 entries at a time
+  auto tiles_of = [&](int i) { return (uint32_t)stream_tiles(a, tokens, keys, i >= a.prefix.B) * (uint32_t)a.Hkv; };
+  if (tid < E) entry_of(a, tid, first, tokens, keys);
+  uint32_t mine = tiles_of(tid), sum, rest = 0;
+  uint32_t before = workgroup_sum(mine, sh, sum);
+  if (E > kStreamEntries) {
+    const int f = first, t = tokens, k = keys;
+    uint32_t x = 0;
+    for (int i = tid + kStreamEntries; i < E; i += kStreamEntries) {
+      entry_of(a, i, first, tokens, keys);
+      x += tiles_of(i);
+    }
+    workgroup_sum(x, sh, rest);
+    first = f, tokens = t, keys = k;
+  }
+  const uint32_t total = sum + rest;
+  const uint32_t per = max((total + a.workers - 1) / a.workers, 1u);
+  const uint32_t u = blockIdx.x * per;
+  if (blockIdx.x == 0 && tid == 0) a.begin[0] = per, a.begin[1 + E] = total;
+  int chunk = 0;
+  for (uint32_t base = 0;;) {
+    const int i = chunk + tid;
+    sh.first[tid] = first, sh.tokens[tid] = tokens, sh.keys[tid] = keys;
+    if (blockIdx.x == 0 && i < E) a.begin[1 + i] = base + before;
+    if (u >= base + before && u < base + before + mine) sh.entry = i, sh.offset = u - base - before;
+    base += sum;
+    // worker 0 goes through all entries, for `begin`
+    if ((blockIdx.x != 0 && (u < base || u >= total)) || chunk + kStreamEntries >= E) break;
+    chunk += kStreamEntries;
+    first = tokens = keys = 0;
+    if (chunk + tid < E) entry_of(a, chunk + tid, first, tokens, keys);
+    mine = tiles_of(chunk + tid);
+    before = workgroup_sum(mine, sh, sum);
+  }
+  if (u >= total) return false;
+  if (tid == 0) sh.record.others = 0;
+  __syncthreads();
+  share = Share{__builtin_amdgcn_readfirstlane(sh.entry), chunk, (uint32_t)__builtin_amdgcn_readfirstlane(sh.offset),
+                min(per, total - u), per};
+  return true;
+}
+
+// STAGES tiles of a wave in LDS: 1, with two workgroups a CU; 2 where there is no more than one
+// workgroup a CU anyway, whose next tile's loads are then under way a tile earlier.
+template <int DT, int STAGES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3 - STAGES, 3 - STAGES)))
 void paged_stream_kernel(PagedAttnArgs a) {
+  constexpr int kWaveLds = STAGES * kStageLds;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   StreamShared& sh = *(StreamShared*)(smem + 4 * kWaveLds);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, ql = lane & 31;
-  const int E = a.prefix.B + a.seq.B;
-  // units of the share: tiles, or items where none is split
-  auto units_of = [&](int tokens, int keys, bool own) {
-    const int n = stream_tiles(a, tokens, keys, own);
-    return (uint32_t)(a.whole ? min(n, 1) : n) * (uint32_t)a.Hkv;
-  };
-
-  // ---- this worker's share: the entries' units summed in order, 256 entries at a time ----
-  int first = 0, tokens = 0, keys = 0;
-  if (tid < E) entry_of(a, tid, first, tokens, keys);
-  uint32_t mine = units_of(tokens, keys, tid >= a.prefix.B), sum, rest = 0;
-  uint32_t before = workgroup_sum(mine, sh, sum);
-  if (E > kStreamEntries) {
-    for (int i = tid + kStreamEntries; i < E; i += kStreamEntries) {
-      int f, t, k;
-      entry_of(a, i, f, t, k);
-      rest += units_of(t, k, i >= a.prefix.B);
-    }
-    uint32_t all;
-    workgroup_sum(rest, sh, all);
-    rest = all;
-  }
-  const uint32_t total = sum + rest;
-  const uint32_t per = max((total + a.workers - 1) / a.workers, 1u);
-  uint32_t u = blockIdx.x * per;
-  if (blockIdx.x == 0 && tid == 0 && !a.whole) a.begin[0] = per;
-  int chunk = 0;
-  for (uint32_t base = 0;;) {
-    const int i = chunk + tid;
-    sh.first[tid] = first, sh.tokens[tid] = tokens, sh.keys[tid] = keys;
-    if (blockIdx.x == 0 && i < E && !a.whole) a.begin[1 + i] = base + before;
-    if (u >= base + before && u < base + before + mine) sh.entry = i, sh.offset = u - base - before;
-    base += sum;
-    // worker 0, which starts in the first chunk that has units, goes through all of them for `begin`
-    if ((blockIdx.x != 0 && (u < base || u >= total)) || chunk + kStreamEntries >= E) break;
-    chunk += kStreamEntries;
-    first = tokens = keys = 0;
-    if (i + kStreamEntries < E) entry_of(a, i + kStreamEntries, first, tokens, keys);
-    mine = units_of(tokens, keys, i + kStreamEntries >= a.prefix.B);
-    before = workgroup_sum(mine, sh, sum);
-  }
-  if (u >= total) return;
-  __syncthreads();
-  int e = __builtin_amdgcn_readfirstlane(sh.entry);
-  uint32_t off = __builtin_amdgcn_readfirstlane(sh.offset);
-  uint32_t left = min(per, total - u);
+  Share share;
+  if (!share_of(a, sh, share)) return;
+  int e = share.entry;
+  uint32_t off = share.offset, left = share.tiles;
   int part = 0;  // the segment's number
 
-  const uint32_t kb = lds_addr(smem) + wid * kWaveLds, vb = kb + kWaveLds / 2;
+  const uint32_t kb = lds_addr(smem) + wid * kWaveLds, vb = kb + kStageLds / 2;
   char* const kl = smem + wid * kWaveLds;
-  char* const vl = kl + kWaveLds / 2;
+  char* const vl = kl + kStageLds / 2;
   // K: rows of 256 bytes, chunk c of row r at c ^ (r & 15), the lane reads chunks 2 j + hl of row ql;
   // V: chunk c of row r at c ^ 4 (r & 3), read transposed
   const uint32_t ka = kb + ql * 256 + (((hl ^ ql) & 1) << 4) + ((ql & 14) << 4);
@@ -170,7 +197,8 @@ void paged_stream_kernel(PagedAttnArgs a) {
   while (left > 0) {
     const bool own = e >= a.prefix.B;
     int f, nt, nk;
-    if ((unsigned)(e - chunk) < kStreamEntries) f = sh.first[e - chunk], nt = sh.tokens[e - chunk], nk = sh.keys[e - chunk];
+    const int at = e - share.chunk;
+    if ((unsigned)at < kStreamEntries) f = sh.first[at], nt = sh.tokens[at], nk = sh.keys[at];
     else entry_of(a, e, f, nt, nk);
     f = __builtin_amdgcn_readfirstlane(f);
     nt = __builtin_amdgcn_readfirstlane(nt);
@@ -214,7 +242,7 @@ void paged_stream_kernel(PagedAttnArgs a) {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<void*>(uniform_ptr((isK ? a.pages.k : a.pages.v) + 2 * at)), (short)0,
             valid * (int)(isK ? skb : svb), kBufferDword3);
-        char* dst = (isK ? kl : vl) + 4096 * half;
+        char* dst = (isK ? kl : vl) + (STAGES == 2 ? (i & 1) * kStageLds : 0) + 4096 * half;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + 1024 * j), 16,
@@ -244,23 +272,31 @@ void paged_stream_kernel(PagedAttnArgs a) {
       load_ids(0);
       load_rows(true, 0);
       load_rows(false, 0);
+      if (STAGES == 2 && m > 1) {
+        load_rows(true, 1);
+        load_rows(false, 1);
+      }
     }
 #pragma nounroll
     for (int i = 0; i < m; ++i) {
-      const bool more = i + 1 < m;
+      // in flight, eight loads each: K and V of this tile, with two stages those of the next too
+      const bool more = i + STAGES < m;
+      const uint32_t stage = STAGES == 2 ? (i & 1) * kStageLds : 0;
       f32x16 x;
       {
         u32x4 k[8];
-        read_keys<8>(k, ka);
+        if (STAGES == 2 && i + 1 < m) wait_loads<24>();
+        else wait_loads<8>();
+        read_keys(k, ka + stage);
         x = E16<DT>::mfma(k[0], qw[0], f32x16{});
 #pragma unroll
         for (int j = 1; j < 8; ++j) x = E16<DT>::mfma(k[j], qw[j], x);
       }
       const int key0 = key_first + i * kStreamTile;
-      // V of this tile needs the same pages as K did: new ones are read after it has been asked for
+      // V of the tiles before has been asked for: their pages are done with
       if (more) {
-        if (((i + 1) & 31) == 0) load_ids(i + 1);
-        load_rows(true, i + 1);
+        if (((i + STAGES) & 31) == 0) load_ids(i + STAGES);
+        load_rows(true, i + STAGES);
       }
       if (key0 + 32 > least) {
 #pragma unroll
@@ -292,21 +328,23 @@ void paged_stream_kernel(PagedAttnArgs a) {
         l *= alpha;
       }
       l += ps;
-      if (!more) __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      if (more) wait_loads<STAGES == 2 ? 24 : 8>();
+      else if (STAGES == 2 && i + 1 < m) wait_loads<16>();
+      else wait_loads<0>();
       u32x4 v[4];
-      read_values<0, 8>(v, va);
+      read_values<0>(v, va + stage);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
         o[db] = E16<DT>::mfma(v[db], hi[0], o[db]);
         o[db] = E16<DT>::mfma(v[db], lo[0], o[db]);
       }
-      read_values<4096, 8>(v, va);
+      read_values<4096>(v, va + stage);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
         o[db] = E16<DT>::mfma(v[db], hi[1], o[db]);
         o[db] = E16<DT>::mfma(v[db], lo[1], o[db]);
       }
-      if (more) load_rows(false, i + 1);
+      if (more) load_rows(false, i + STAGES);
     }
 
     // ---- the four waves' results joined: each leaves its rows in its own LDS, 16-byte chunk c of row
@@ -363,6 +401,10 @@ void paged_stream_kernel(PagedAttnArgs a) {
         if (d0 == 0) *(f32x2*)(state + 128) = f32x2{M, L};
       }
     }
+    // an item that goes on in the next worker's share is joined by whoever has its first part
+    if (!a.whole && a.records && tid == 0 && n < tiles) {
+      if (t0 == 0) sh.record = StreamRecord{f, nt, h, (int)(2 * blockIdx.x + min(part, 1)), (int)((tiles - n + share.per - 1) / share.per)};
+    }
     ++part;
     const uint32_t used = a.whole ? 1 : n;
     off += used;
@@ -370,23 +412,45 @@ void paged_stream_kernel(PagedAttnArgs a) {
     if (off == (uint32_t)(a.whole ? 1 : tiles) * a.Hkv) ++e, off = 0;
     if (left > 0) __syncthreads();  // the sums are read before the next tiles arrive in their place
   }
+  if (!a.whole && a.records && tid == 0) a.records[blockIdx.x] = sh.record;
 }
 
+// The parts of the stream's items joined, by the worker that has the first: a row's 128 dims over 32
+// lanes, eight rows at a time.
 template <int DT>
+__global__ __launch_bounds__(256) void paged_stream_join_kernel(PagedAttnArgs a) {
+  const StreamRecord rec = a.records[blockIdx.x];
+  if (blockIdx.x * a.begin[0] >= a.begin[1 + a.prefix.B + a.seq.B] || rec.others == 0) return;
+  const int d = 4 * (threadIdx.x & 31);
+  for (int r = threadIdx.x >> 5; r < rec.tokens * a.G; r += 8) {
+    RowSum sum;
+    sum.take(a.slots + ((int64_t)rec.slot * a.slot_rows + r) * kState, d);
+    const float* next = a.slots + (2 * ((int64_t)blockIdx.x + 1) * a.slot_rows + r) * kState;
+    sum.take_all(next, 2 * (int64_t)a.slot_rows * kState, rec.others, d);
+    sum.template store<DT>(a, rec.first + r / a.G, rec.head * a.G + r % a.G, d);
+  }
+}
+
+template <int DT, int STAGES>
 static int launch_stream_t(const PagedAttnArgs& a, hipStream_t st) {
   static int done = 0;
   if (!done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_stream_kernel<DT>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, kStreamLds);
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_stream_kernel<DT, STAGES>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, stream_lds(STAGES));
     if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
     done = 1;
   }
-  hipLaunchKernelGGL(paged_stream_kernel<DT>, dim3((unsigned)a.workers), dim3(256), kStreamLds, st, a);
-  return check_launch("paged attention (stream)");
+  hipLaunchKernelGGL((paged_stream_kernel<DT, STAGES>), dim3((unsigned)a.workers), dim3(256), stream_lds(STAGES), st, a);
+  if (int rc = check_launch("paged attention (stream)")) return rc;
+  if (!a.records) return DA_OK;
+  hipLaunchKernelGGL(paged_stream_join_kernel<DT>, dim3((unsigned)a.workers), dim3(256), 0, st, a);
+  return check_launch("paged attention (stream, join)");
 }
 
 int launch_paged_stream(const PagedAttnArgs& a, int dtype, hipStream_t st) {
-  return dtype == DA_F16 ? launch_stream_t<DA_F16>(a, st) : launch_stream_t<DA_BF16>(a, st);
+  const bool two = a.whole && a.workers <= cu_count();
+  if (dtype == DA_F16) return two ? launch_stream_t<DA_F16, 2>(a, st) : launch_stream_t<DA_F16, 1>(a, st);
+  return two ? launch_stream_t<DA_BF16, 2>(a, st) : launch_stream_t<DA_BF16, 1>(a, st);
 }
 
 }  // namespace da

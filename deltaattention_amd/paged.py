@@ -14,8 +14,8 @@ from typing import Optional
 
 import torch
 
-from ._native import PagedBatchBlock, PagedKVBlock, call_on, check, dtype_code, lib
-from .kv4 import _gpu, _rows
+from ._native import DA_F32, PagedBatchBlock, PagedKVBlock, call_on, check, dtype_code, lib
+from .kv4 import _gpu
 
 __all__ = ["PagedKV", "PagedBatch", "append_paged", "paged_attention", "shared_prefix_attention"]
 
@@ -99,18 +99,24 @@ class PagedBatch:
         self._ref = ctypes.byref(self._block)
 
 
-def _tokens(t: torch.Tensor, name: str, kv: PagedKV) -> torch.Tensor:
-    """A [T, heads, D] tensor that fits the pages, with 16-byte aligned rows."""
-    if t.dim() != 3 or t.shape[2] != kv.head_dim or t.device != kv.device or t.dtype != kv.dtype:
+def _tokens(t: torch.Tensor, name: str, kv: PagedKV):
+    """(t, its shape, its strides) of a [T, heads, D] tensor that fits the pages; a copy where its rows do
+    not begin at multiples of 16 bytes."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != kv.head_dim or t.dtype is not kv.dtype or t.device != kv.device:
         raise ValueError(f"{name} must be [tokens, heads, {kv.head_dim}] {kv.dtype} on {kv.device}, got "
-                         f"{list(t.shape)} {t.dtype} on {t.device}")
-    return _rows(t)
+                         f"{list(shape)} {t.dtype} on {t.device}")
+    s = t.stride()
+    if s[2] != 1 or (s[0] | s[1]) & 7 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = t.stride()
+    return t, shape, s
 
 
-def _output(out: Optional[torch.Tensor], q: torch.Tensor, name: str) -> torch.Tensor:
+def _output(out: Optional[torch.Tensor], q: torch.Tensor, shape, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() % 16:
+        return q.new_empty(shape)
+    if out.shape != shape or out.dtype is not q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() & 15:
         raise ValueError(f"{name} must have q's shape, type and device, a contiguous head dimension and 16-byte alignment")
     return out
 
@@ -134,18 +140,20 @@ def append_paged(kv: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Tenso
     stay.  A position past the rows takes the last one.  Without cos and sin nothing is rotated.
     Tokens past the batch's last and places past its table are not written.
     """
-    k, v = _tokens(k, "k", kv), _tokens(v, "v", kv)
-    T = k.shape[0]
-    if k.shape[1] != kv.kv_heads or v.shape != k.shape or not T:
-        raise ValueError(f"k and v must be [tokens, {kv.kv_heads}, {kv.head_dim}], got {list(k.shape)} and {list(v.shape)}")
+    k, shape, sk = _tokens(k, "k", kv)
+    v, of_v, sv = _tokens(v, "v", kv)
+    T, H, D = shape
+    if H != kv.kv_heads or of_v != shape or not T:
+        raise ValueError(f"k and v must be [tokens, {kv.kv_heads}, {D}], got {list(shape)} and {list(of_v)}")
     _batch(batch, kv, T)
-    sk, sv, sq, so, Hq, qp, op = k.stride(), v.stride(), (0, 0), (0, 0), 0, None, None
+    sq, so, Hq, qp, op = (0, 0), (0, 0), 0, None, None
     if q is not None:
-        src = _tokens(q, "q", kv)
-        if q.shape[0] != T or not q.shape[1]:
-            raise ValueError(f"q {list(q.shape)} must hold the {T} tokens of k")
-        out = _output(out, q, "out")
-        Hq, sq, so, qp, op = q.shape[1], src.stride(), out.stride(), src.data_ptr(), out.data_ptr()
+        src, of_q, sq = _tokens(q, "q", kv)
+        Hq = of_q[1]
+        if of_q[0] != T or not Hq:
+            raise ValueError(f"q {list(of_q)} must hold the {T} tokens of k")
+        out = _output(out, q, of_q, "out")
+        so, qp, op = out.stride(), src.data_ptr(), out.data_ptr()
     elif out is not None:
         raise ValueError("out is for the rotated queries: it needs q")
     rows = s_rot = rot = 0
@@ -153,37 +161,42 @@ def append_paged(kv: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Tenso
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     if cos is not None:
-        if cos.dim() != 2 or sin.shape != cos.shape or sin.dtype != cos.dtype or cos.device != kv.device \
-                or sin.device != kv.device or cos.stride(1) != 1 or sin.stride() != cos.stride():
+        table, s = cos.shape, cos.stride()
+        if len(table) != 2 or sin.shape != table or sin.dtype is not cos.dtype or cos.device != kv.device \
+                or sin.device != kv.device or s[1] != 1 or sin.stride() != s:
             raise ValueError("cos and sin must be [rows, R / 2] of one shape, type and stride on the pages' device")
-        rows, rot, s_rot = cos.shape[0], 2 * cos.shape[1], cos.stride(0)
-        if cos.dtype not in (torch.float32, kv.dtype):
+        rows, rot, s_rot = table[0], 2 * table[1], s[0]
+        if cos.dtype is torch.float32:
+            code = DA_F32
+        elif cos.dtype is not kv.dtype:
             raise TypeError(f"cos and sin must be torch.float32 or {kv.dtype}, got {cos.dtype}")
-        if not rows or not rot or rot % 4 or rot > kv.head_dim:
-            raise ValueError(f"cos and sin of {list(cos.shape)} do not fit a head_dim of {kv.head_dim}: R is a multiple of 4")
+        if not rows or not rot or rot % 4 or rot > D:
+            raise ValueError(f"cos and sin of {list(table)} do not fit a head_dim of {D}: R is a multiple of 4")
         if per_token and rows < T:
             raise ValueError(f"{rows} rows of cos and sin for {T} tokens")
-        code, cp, sp = dtype_code(cos), cos.data_ptr(), sin.data_ptr()
+        cp, sp = cos.data_ptr(), sin.data_ptr()
     rc = call_on(kv.device, lib().da_paged_append, k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], qp, sq[0], sq[1],
-                 op, so[0], so[1], kv._code, T, Hq, kv.kv_heads, kv.head_dim, cp, sp, code, rows, s_rot, rot,
-                 1 if interleaved else 0, 1 if per_token else 0, kv._ref, batch._ref)
+                 op, so[0], so[1], kv._code, T, Hq, H, D, cp, sp, code, rows, s_rot, rot, 1 if interleaved else 0,
+                 1 if per_token else 0, kv._ref, batch._ref)
     check(rc, "da_paged_append")
     return out
 
 
 def _attention(q, kv, batch, prefix, scale, out):
-    src = _tokens(q, "q", kv)
-    T, Hq, D = src.shape
-    if not T or not Hq or Hq % kv.kv_heads:
-        raise ValueError(f"{T} tokens of {Hq} query heads over {kv.kv_heads} KV heads")
+    src, shape, sq = _tokens(q, "q", kv)
+    T, Hq, D = shape
+    H = kv.kv_heads
+    if not T or not Hq or Hq % H:
+        raise ValueError(f"{T} tokens of {Hq} query heads over {H} KV heads")
     _batch(batch, kv, T)
-    out = _output(out, q, "out")
-    sq, so = src.stride(), out.stride()
+    out = _output(out, q, shape, "out")
+    so = out.stride()
     common = None if prefix is None else prefix._ref
-    n = lib().da_paged_attention_workspace_size(kv._code, T, Hq, kv.kv_heads, D, kv._ref, batch._ref, common)
+    native = lib()
+    n = native.da_paged_attention_workspace_size(kv._code, T, Hq, H, D, kv._ref, batch._ref, common)
     ws = torch.empty((n,), dtype=_U8, device=kv.device) if n > 0 else None  # held until the call is on its stream
-    rc = call_on(kv.device, lib().da_paged_attention, src.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], kv._code, T,
-                 Hq, kv.kv_heads, D, D ** -0.5 if scale is None else scale, kv._ref, batch._ref, common,
+    rc = call_on(kv.device, native.da_paged_attention, src.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], kv._code,
+                 T, Hq, H, D, D ** -0.5 if scale is None else scale, kv._ref, batch._ref, common,
                  None if ws is None else ws.data_ptr(), n)
     check(rc, "da_paged_attention")
     return out
