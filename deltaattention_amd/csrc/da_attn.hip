@@ -1143,10 +1143,15 @@ void attn_f32_kernel(Args a, int paired) {
   // CU taking one of the first half and one of the second: there the second half runs from the
   // shortest up, so that every CU gets about the same work (2048 tokens x 8 heads of 64 dims:
   // 63 us, 80 with the longest first throughout) ----
-  const int nrb = (a.Nq + kFRows - 1) / kFRows;
-  int splits = 1, split = 0;
-  if constexpr (VARIANT == kPaged) splits = a.splits;
-  const int units = a.B * a.Hq * splits;
+  // kPaged: a block's rows are (token, query head of one KV head), so that the keys of a decode step
+  // are read once for the group; units are KV heads
+  int nrb = (a.Nq + kFRows - 1) / kFRows;
+  int units = a.B * a.Hq, splits = 1, split = 0;
+  if constexpr (VARIANT == kPaged) {
+    splits = a.splits;
+    nrb = (a.Nq * a.G + kFRows - 1) / kFRows;
+    units = a.B * a.Hkv * splits;
+  }
   const bool whole = (units & 7) == 0 && (!a.seq.cu || (a.Hq & 7) == 0);
   int unit, j;  // j: row blocks from the last one
   if (paired) {
@@ -1173,7 +1178,7 @@ void attn_f32_kernel(Args a, int paired) {
     unit /= splits;
   }
   const int h = unit / a.B, b = unit % a.B;
-  const int g = h / a.G;
+  const int g = VARIANT == kPaged ? h : h / a.G;
   const int bg = b * a.Hkv + g;
   int Nq, Nk, off = 0;  // row r sees the keys up to r + off
   if constexpr (VARIANT == kPaged) {
@@ -1185,7 +1190,7 @@ void attn_f32_kernel(Args a, int paired) {
     Nk = a.seq.cu ? a.seq.len(b) : a.Nk;
   }
   const int R0 = rb * kFRows;
-  if (R0 >= Nq) return;  // a row block past the end of a shorter sequence (whole workgroup)
+  if (R0 >= (VARIANT == kPaged ? Nq * a.G : Nq)) return;  // a row block past the end of a shorter sequence (whole workgroup)
   const int D = a.D;
   const float c = a.scale_log2;
 
@@ -1217,7 +1222,7 @@ void attn_f32_kernel(Args a, int paired) {
   }
   if constexpr (VARIANT == kPaged) {
     // this split's run of the row block's tiles
-    const int all = a.causal ? min(Nk, off + R0 + kFRows) : Nk;
+    const int all = a.causal ? min(Nk, off + (R0 + kFRows - 1) / a.G + 1) : Nk;
     const int tiles = all > 0 ? (all + kFTile - 1) / kFTile : 0;
     const int per = (tiles + splits - 1) / splits;
     ds = split * per * kFTile;
@@ -1236,7 +1241,12 @@ void attn_f32_kernel(Args a, int paired) {
   const int32_t* tsrow = a.tsw ? a.tsw + (int64_t)bg * a.wcap : nullptr;
 
   // ---- Q^T: dims 8 m + 4 hl .. + 3 of query R0 + ql (rows past Nq and dims past D zero) ----
-  const int row = R0 + ql;
+  int row = R0 + ql, hr = h;
+  if constexpr (VARIANT == kPaged) {
+    hr = g * a.G + row % a.G;
+    row = row / a.G;
+    qg = (const float*)a.q + a.seq.base(b, a.sq_b, a.sq_n) + (int64_t)hr * a.sq_h;
+  }
   f32x4 qf[4 * DB];
 #pragma unroll
   for (int m = 0; m < 4 * DB; ++m) {
@@ -1465,10 +1475,10 @@ void attn_f32_kernel(Args a, int paired) {
   }
   if (row >= Nq) return;
   const int r0 = kOwn * wid, d0 = DB * (8 * (r0 >> 2) + 4 * hl + (r0 & 3));
-  float* orow = (float*)a.out + a.seq.base(b, a.so_b, a.so_n) + (int64_t)h * a.so_h + (int64_t)row * a.so_n;
+  float* orow = (float*)a.out + a.seq.base(b, a.so_b, a.so_n) + (int64_t)hr * a.so_h + (int64_t)row * a.so_n;
   if constexpr (VARIANT == kPaged)
     if (a.parts) {
-      orow = a.parts + (((int64_t)split * a.list.T + a.list.first(b) + row) * a.Hq + h) * kState;
+      orow = a.parts + (((int64_t)split * a.list.T + a.list.first(b) + row) * a.Hq + hr) * kState;
       if (wid == 0 && hl == 0) *(f32x2*)(orow + 128) = f32x2{M, L};
     }
 #pragma unroll
@@ -1601,9 +1611,9 @@ static int launch_rows_f32(const PagedRowsArgs& a, unsigned grid, hipStream_t st
 }
 
 RowsShape paged_rows_shape(int dtype, int G) {
-  if (dtype == DA_F32) return RowsShape{1, kFRows, kFRows};
+  if (dtype == DA_F32) return RowsShape{G, G, kFRows, kFRows};
   const int hpw = G % 4 == 0 ? 4 : (G % 2 == 0 ? 2 : 1);
-  return RowsShape{hpw, 128 / hpw, 256 / hpw};
+  return RowsShape{1, hpw, 128 / hpw, 256 / hpw};
 }
 
 int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts, int dtype,
@@ -1618,15 +1628,15 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
   a.seq = SeqMap{list.cu, list.T, list.max_len};
   a.scale_log2 = p.scale_log2;
   a.causal = own ? 1 : 0;
-  a.hpw = shape.hpw;
+  a.hpw = dtype == DA_F32 ? 1 : shape.heads;
   a.pages = p.pages;
   a.list = list;
   a.splits = splits;
   a.short_rows = p.short_rows[own];
   a.parts = parts;
   const int rows = wide ? shape.wide : shape.narrow;
-  a.n_row_groups = (list.max_len + rows - 1) / rows;
-  a.units = list.B * (p.Hq / shape.hpw) * splits;
+  a.n_row_groups = (list.max_len * shape.pack + rows - 1) / rows;
+  a.units = list.B * (p.Hq / shape.heads) * splits;
   a.slots = 2 * cu_count() / 8;
   const int64_t grid = (int64_t)a.units * a.n_row_groups;
   if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");

@@ -147,10 +147,10 @@ struct RowSum {
 
 // Host: checks and the kernels' forms of the ABI's blocks.
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who);
-// Rows of one query head that a workgroup of the row kernels takes (with its query heads): half-size
-// and full-size groups.
+// What a workgroup of the row kernels takes: `heads` query heads of a KV head and, of their rows (pack of
+// them a token), a half-size or full-size group.
 struct RowsShape {
-  int hpw, narrow, wide;
+  int pack, heads, narrow, wide;
 };
 RowsShape paged_rows_shape(int dtype, int G);
 // The entries of `list` with more than short_rows rows.

@@ -103,13 +103,15 @@ static void shape_rows(PagedAttnArgs& a, int list, bool& wide, int dtype) {
   const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = 2.0 * cu_count();
   const int tiles = (s.max_keys + 31) / 32;
   double best = 0.0;
-  for (int w = 0; w < (shape.wide > shape.narrow && s.max_len > shape.narrow ? 2 : 1); ++w) {
+  const int64_t most = (int64_t)s.max_len * shape.pack, others = s.B - 1, rest = s.T - s.max_len;
+  for (int w = 0; w < (shape.wide > shape.narrow && most > shape.narrow ? 2 : 1); ++w) {
     const int rows = w ? shape.wide : shape.narrow;
     // items: those of the longest entry, and of the others if their mean is not the stream's
-    const int64_t longest = (s.max_len + rows - 1) / rows, others = s.B - 1, rest = s.T - s.max_len;
+    const int64_t longest = (most + rows - 1) / rows;
     int64_t items = longest;
-    if (others > 0 && rest * a.G > others * a.short_rows[list]) items += std::min(others * longest, rest / rows + others);
-    items *= a.Hq / shape.hpw;
+    if (others > 0 && rest * a.G > others * a.short_rows[list])
+      items += std::min(others * longest, rest * shape.pack / rows + others);
+    items *= a.Hq / shape.heads;
     for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (n > 1 && n > tiles) break;
       const double all = (double)items * n, rounds = all <= slots ? 1.0 : all / slots + 0.3;
