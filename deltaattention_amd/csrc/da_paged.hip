@@ -245,7 +245,7 @@ extern "C" int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const 
   if (rot) {
     DA_REQUIRE(cos && sin && rows > 0, "%s: rotation needs cos and sin", who);
     DA_REQUIRE(rot_dtype == DA_F32 || rot_dtype == dtype, "%s: cos and sin must be fp32 or of the pages' type", who);
-    DA_REQUIRE(s_rot >= rot / 2 || rows == 1, "%s: rows of cos and sin overlap", who);
+    DA_REQUIRE(s_rot >= rot / 2 || s_rot == 0 || rows == 1, "%s: rows of cos and sin overlap", who);
     DA_REQUIRE(!per_token || rows >= T, "%s: a row of cos and sin for every token is needed", who);
   }
   DA_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out) & 15) == 0, "%s: tensors must be 16-byte aligned",

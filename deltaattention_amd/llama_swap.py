@@ -24,7 +24,10 @@ Two layers of the swap:
   prefill by the configured implementation, the prefill -> cache hand-off, and PATH 3
   decode over the compressed cache.  Without a ``HybridCompressedCache`` it runs the
   stock flow through the registered implementation.  A ``FourBitCompressedCache`` (anchors
-  in 4 bits, bounded by accumulated attention weight) takes the same way.
+  in 4 bits, bounded by accumulated attention weight) takes the same way.  A ``PagedCache``
+  (every token at full width, in pages) takes keys and queries before RoPE, which is applied as
+  they are written, and continues a sequence with any number of tokens: dense attention over
+  its pages, or PATH 1 for a prompt that begins it.
 """
 from __future__ import annotations
 
@@ -53,8 +56,8 @@ def _check(query, key, kwargs):
     if query.shape[2] != key.shape[2]:
         raise NotImplementedError(
             "the deltaattention implementations are prefill paths (query length == key "
-            "length); decode through deltaDecoding.HybridCompressedCache with "
-            "llama_swap.install(model)")
+            "length); decode through deltaDecoding.HybridCompressedCache or paged_cache.PagedCache "
+            "with llama_swap.install(model)")
     pos = kwargs.get("position_ids")
     if isinstance(pos, torch.Tensor) and pos.numel() > 0 and int(pos.reshape(-1)[0]) != 0:
         # a continuation whose cache returned only the new tokens (a HybridCompressedCache
@@ -109,6 +112,25 @@ def _is_compressed_cache(cache) -> bool:
     return isinstance(cache, HybridCompressedCache)
 
 
+def _paged_attention(self, cache, query_states, key_states, value_states, cos, sin):
+    """One layer's step over a PagedCache: [B, N, Hq, D].  The states are those before RoPE."""
+    N = query_states.shape[2]
+    if self.config._attn_implementation == DELTA and N > 1 and cache.get_seq_length(self.layer_idx) == 0:
+        # PATH 1 selects among the rotated keys of the whole prompt, which go to the pages as they are
+        from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
+        query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
+        cache.append(key_states, value_states, self.layer_idx)
+        out, view = _out_view(query_states)
+        _timed(lambda: attention.delta_prefill_attention(
+            query_states, key_states, value_states, layer_idx=self.layer_idx, scaling=self.scaling,
+            track_sparsity=_track_sparsity(), out=view), query_states.is_cuda)
+        return out
+    query = cache.append(key_states, value_states, self.layer_idx, query_states, cos, sin)
+    if N == 1:
+        return cache.attend(query, self.layer_idx, self.scaling)
+    return _timed(lambda: cache.attend(query, self.layer_idx, self.scaling), query.is_cuda)
+
+
 def _kv_size_sample(cache) -> None:
     """Layer-0 KV-size tracker of the decode steps (modeling_llama.py:572-595): every
     ``kv_log_interval`` tokens, the memory saved against an uncompressed cache."""
@@ -134,9 +156,11 @@ def delta_llama_attention_forward(self, hidden_states: torch.Tensor,
     single-token step runs PATH 3: ``cache.update`` (merge or append of the evicted
     token, ring write, :565-567) then the compressed decode attention (:453-518).  Any
     other cache (or none) takes the stock flow: ``update`` then the registered
-    attention implementation.  Returns (attn_output, None)."""
+    attention implementation.  A PagedCache takes any number of tokens at any point of the
+    sequence (:func:`_paged_attention`).  Returns (attn_output, None)."""
     from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
     from . import deltaDecoding
+    from .paged_cache import PagedCache
 
     cache = past_key_values if past_key_values is not None else kwargs.pop("past_key_value", None)
     input_shape = hidden_states.shape[:-1]
@@ -148,9 +172,13 @@ def delta_llama_attention_forward(self, hidden_states: torch.Tensor,
     key_states = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
     value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
     cos, sin = position_embeddings
-    query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
+    paged = isinstance(cache, PagedCache)
+    if not paged:
+        query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
 
-    if not _is_compressed_cache(cache):
+    if paged:
+        attn_output = _paged_attention(self, cache, query_states, key_states, value_states, cos, sin)
+    elif not _is_compressed_cache(cache):
         if cache is not None:
             key_states, value_states = cache.update(key_states, value_states, self.layer_idx)
         fn = {DELTA: delta_attention_forward, DENSE: dense_attention_forward}.get(

@@ -55,7 +55,8 @@ typedef struct DaPagedBatch {
  * aligned), of the pages' type (bf16, fp16 or fp32).  q_out may be q.  Rotation: dims d and
  * d + rot / 2 (interleaved: 2 d and 2 d + 1), d < rot / 2, become x cos - y sin and y cos + x sin, in
  * fp32, rounded once; dims from rot on stay.  cos, sin [rows, rot / 2] fp32 or of the pages' type
- * (rot_dtype), rows s_rot apart; row p is for position p, or with per_token for token p (rows >= T).
+ * (rot_dtype), rows s_rot apart (0: one row for all); row p is for position p, or with per_token for
+ * token p (rows >= T).
  * A position outside the rows takes the nearest row.  rot = 0: no rotation.
  */
 int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_t, int64_t sv_h,

@@ -84,7 +84,8 @@ def test_append_refuses():
     _refused(_append(cos=None), -1, "cos and sin")
     _refused(_append(rows=0), -1, "cos and sin")
     _refused(_append(rt=2), -1, "pages' type")
-    _refused(_append(s_rot=63), -1, "overlap")
+    for s in (63, 1, -64):
+        _refused(_append(s_rot=s), -1, "overlap")
     _refused(_append(tok=1, rows=7), -1, "every token")
 
 
