@@ -37,7 +37,7 @@
 #include <cstring>
 #include <type_traits>
 
-#include "da_paged.hpp"
+#include "da_paged_stream.hpp"
 #include "da_tile.hpp"
 
 namespace da {
@@ -93,13 +93,15 @@ struct AttnArgs {
 };
 
 // kPaged: q and out are [T, heads, D] (s*_b and s*_n their token strides, seq.cu the list's), the keys
-// of a row group are cut into `splits` equal runs of tiles, unit (g, heads, b, split).
+// of a row group are cut into `splits` equal runs of tiles, unit (g, b, split).  A row is a (token, query
+// head of the group): entry b has tokens(b) * G of them.
 struct PagedRowsArgs : AttnArgs {
   Pages pages;
   PageBatch list;
   int splits;
   int short_rows;  // entries of up to so many rows are left to the stream
   float* parts;    // [splits][T][Hq][kState], or null: the result goes to out
+  int spread;      // the order of the items, see paged_item_at
 };
 
 // Phase-1 extent of a query block (deltaFlashAttention.py:58-80): n_safe = the number of
@@ -246,6 +248,23 @@ __device__ __forceinline__ void item_at(int k, int units, int n_rg, int slots, i
   }
 }
 
+// Item of workgroup wg, the longest row groups first.  Whole units an XCD where they split evenly (an
+// XCD's L2 then has one unit's K and V at a time), or, `spread`, all units' row groups in turn over the
+// XCDs, which evens out a ragged batch.
+__device__ __forceinline__ void paged_item_at(const PagedRowsArgs& a, int wg, int& unit, int& rg) {
+  if (a.spread) {
+    const int j = wg / a.units;
+    unit = (wg + j) % a.units;
+    rg = a.n_row_groups - 1 - j;
+  } else if ((a.units & 7) == 0) {
+    const int upx = a.units >> 3;
+    item_at(wg >> 3, upx, a.n_row_groups, a.slots, unit, rg);
+    unit += (wg & 7) * upx;
+  } else {
+    item_at(wg, a.units, a.n_row_groups, 8 * a.slots, unit, rg);
+  }
+}
+
 // One (unit, row group) of attn_w64_kernel: a.hpw (4, 2 or 1) query heads of one (batch, KV
 // head) over 128 NCB / hpw rows.  Ends with every LDS read of the window loop done (its last
 // barrier) and every load landed; the finalize uses only the wave's own Q region, so the next
@@ -271,31 +290,29 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     unit = unit_split / a.splits;
     split = unit_split - unit * a.splits;
   }
-  const int hsh = a.hpw >> 1;  // log2 of the query heads a workgroup takes
-  const int hunits = a.G >> hsh;
-  int g, b, hu;
+  const int hsh = VARIANT == kPaged ? 0 : a.hpw >> 1;  // log2 of the query heads a workgroup takes
+  int g, b, h;
   if constexpr (VARIANT == kPaged) {
-    // (g, hu) by b: an XCD's units are some heads of every sequence, whatever the sequences' lengths
-    const int head = unit / a.B;
-    b = unit - head * a.B;
-    g = head / hunits;
-    hu = head - g * hunits;
+    g = unit / a.B;
+    b = unit - g * a.B;
+    h = 0;  // the rows are (token, query head of the group)
   } else {
+    const int hunits = a.G >> hsh;
     const int gb = unit / hunits;  // g * B + b
-    hu = unit - gb * hunits;
+    const int hu = unit - gb * hunits;
     g = gb / a.B;
     b = gb - (gb / a.B) * a.B;
+    h = g * a.G + (hu << hsh) + (wid & ((1 << hsh) - 1));
   }
   const int bg = b * a.Hkv + g;
-  const int h = g * a.G + (hu << hsh) + (wid & ((1 << hsh) - 1));
   const int wg_rows = (128 * NCB) >> hsh;
   const int R0 = rg * wg_rows;
-  int Nq, Nk, off = 0;  // row r sees the keys up to r + off
+  int Nq, Nk, off = 0;  // a row of token i sees the keys up to i + off
   if constexpr (VARIANT == kPaged) {
-    Nq = a.list.tokens(b);
+    Nq = a.list.tokens(b) * a.G;
     Nk = a.list.keys(b);
-    off = a.causal ? Nk - Nq : 0;
-    if (Nq * a.G <= a.short_rows) return;
+    off = a.causal ? Nk - a.list.tokens(b) : 0;
+    if (Nq <= a.short_rows) return;
   } else {
     Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
     Nk = a.seq.cu ? a.seq.len(b) : a.Nk;
@@ -304,6 +321,12 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   // first row of this wave; column block cb holds r0w + 32 cb + ql
   const int r0w = R0 + 32 * NCB * (wid >> hsh);
   const int wg_end = R0 + wg_rows;
+  // kPaged: the token of a row, and its place in q and out
+  auto token = [&](int row) { return VARIANT == kPaged ? row / a.G : row; };
+  auto place = [&](int row, int64_t s_h, int64_t s_n) {
+    const int t = row / a.G;
+    return (int64_t)(g * a.G + row - t * a.G) * s_h + (int64_t)t * s_n;
+  };
 
   // ---- schedule: packed tiles 0 .. n1 - 1, then exact tiles from key ds on.  A workgroup's
   // rows lie in one logical 128-row block, except where one head takes 256 rows (hpw
@@ -350,7 +373,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   }
   if constexpr (VARIANT == kPaged) {
     // this split's run of the row group's tiles
-    const int all = a.causal ? min(Nk, off + wg_end) : Nk;
+    const int all = a.causal ? min(Nk, off + token(wg_end - 1) + 1) : Nk;
     const int tiles = all > 0 ? (all + kWTK - 1) / kWTK : 0;
     const int per = (tiles + a.splits - 1) / a.splits;
     ds = dsw = split * per * kWTK;
@@ -374,7 +397,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   // causal: a Phase-2 tile whose first key is past the wave's last row is skipped
   int t_skip = INT_MAX;
   if (a.causal) {
-    const int d = off + r0w + 32 * NCB - 1 - ds;
+    const int d = off + token(r0w + 32 * NCB - 1) - ds;
     t_skip = __builtin_amdgcn_readfirstlane(d < 0 ? n1 : n1 + d / kWTK + 1);
   }
   if (kPureV) t_skip = __builtin_amdgcn_readfirstlane(n1w);
@@ -524,6 +547,15 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) mc[cb] = -__FLT_MAX__, l_i[cb] = 0.0f;
   const float c = a.scale_log2;
+  // kPaged: the last key that the lane's row, and that the column block's first row, sees
+  int seen[NCB], least[NCB];
+  if constexpr (VARIANT == kPaged) {
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      seen[cb] = off + token(r0w + 32 * cb + ql);
+      least[cb] = __builtin_amdgcn_readfirstlane(off + token(r0w + 32 * cb));
+    }
+  }
 
   unsigned stA = 0, stB = kWKBytes;
   if (T > 0) {
@@ -547,6 +579,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     for (int cb = 0; cb < NCB; ++cb) {
       const int row = r0w + 32 * cb + ql;
       const uint16_t* qrow = a.q + a.seq.base(b, a.sq_b, a.sq_n) + (int64_t)h * a.sq_h + (int64_t)min(row, Nq - 1) * a.sq_n;
+      if constexpr (VARIANT == kPaged) qrow = a.q + a.seq.base(b, a.sq_b, a.sq_n) + place(min(row, Nq - 1), a.sq_h, a.sq_n);
 #pragma unroll
       for (int t = 0; t < kD / 16; ++t) {
         const int d0 = 16 * t + 8 * hl;
@@ -684,12 +717,12 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     const int key0 = key0_of(t);
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      const int row = r0w + 32 * cb + ql;
+      const int row = VARIANT == kPaged ? seen[cb] : r0w + 32 * cb + ql;
       if (kPureV) {
         mask_pure32(s[cb], (const int*)(ms + kWTs), row, hl);
       } else if (t >= n1) {
-        if ((a.causal && key0 + kWTK - 1 > off + r0w + 32 * cb) || key0 + kWTK > Nk)
-          mask_dense32(s[cb], key0, row + off, hl, Nk, a.causal);
+        if ((a.causal && key0 + kWTK - 1 > (VARIANT == kPaged ? least[cb] : r0w + 32 * cb)) || key0 + kWTK > Nk)
+          mask_dense32(s[cb], key0, row, hl, Nk, a.causal);
       }
     }
     // p against the current maximum first; only where a lane's sum of its 16 p
@@ -793,7 +826,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   // ---- finalize: each column block goes through the wave's own Q region of LDS (its
   // last Q.K is done), 16-byte chunk c of row r at position c ^ (r & 15), and leaves as
   // whole rows, four per store instruction, instead of 16 bytes of 32 rows ----
-  uint16_t* const obase = a.out + a.seq.base(b, a.so_b, a.so_n) + (int64_t)h * a.so_h;
+  uint16_t* const obase = a.out + a.seq.base(b, a.so_b, a.so_n) + (int64_t)h * a.so_h;  // kPaged: h = 0
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
     const float l_tot = halves_sum(l_i[cb]);
@@ -801,7 +834,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
       if (a.parts) {  // sums, maximum and sum of weights as they are, to be joined
         const int row = r0w + 32 * cb + ql;
         if (row < Nq) {
-          float* st = a.parts + (((int64_t)split * a.list.T + a.list.first(b) + row) * a.Hq + h) * kState;
+          float* st = a.parts + ((int64_t)split * a.list.T + a.list.first(b)) * a.Hq * kState + place(row, kState, (int64_t)a.Hq * kState);
 #pragma unroll
           for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -843,7 +876,11 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
       const int row = r0w + 32 * cb + 4 * it + (lane >> 4);
-      if (row < Nq && cq * 8 < a.D) *(u32x4*)(obase + (int64_t)row * a.so_n + cq * 8) = rw[it];
+      if constexpr (VARIANT == kPaged) {
+        if (row < Nq && cq * 8 < a.D) *(u32x4*)(obase + place(row, a.so_h, a.so_n) + cq * 8) = rw[it];
+      } else {
+        if (row < Nq && cq * 8 < a.D) *(u32x4*)(obase + (int64_t)row * a.so_n + cq * 8) = rw[it];
+      }
     }
     // the reads of this block are done before the next block overwrites the region
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
@@ -881,7 +918,9 @@ void attn_w64_kernel(Args a) {
     if (!persistent) {
       if (!first) break;
       const int wg = blockIdx.x;
-      if ((a.units & 7) == 0) {
+      if constexpr (VARIANT == kPaged) {
+        paged_item_at(a, wg, unit, rg);
+      } else if ((a.units & 7) == 0) {
         const int xcd = wg & 7, upx = a.units >> 3;
         item_at(wg >> 3, upx, n_rg, a.slots, unit, rg);
         unit += xcd * upx;
@@ -933,6 +972,41 @@ void attn_w64_kernel(Args a) {
     attn_w64_item<VARIANT, DT, NCB, LAZY>(a, unit, rg);
 #endif
   }
+}
+
+// The stream (bound by memory) and a list's row groups (bound by the matrix units) in one launch, in
+// turns of a workgroup a CU each, so that a CU, which takes two, has one of either.
+struct PagedPairArgs {
+  PagedAttnArgs s;
+  PagedRowsArgs r;
+  int turn, items, row_turns, stream_turns;  // workgroups a turn; row groups; turns of either
+};
+template <int DT, int NCB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_pair_kernel(PagedPairArgs p) {
+  const int j = blockIdx.x / p.turn, at = blockIdx.x - j * p.turn, n = p.row_turns + p.stream_turns;
+  // the row groups' turns spread evenly over all, the first of all among them
+  const int before = (int)(((int64_t)j * p.row_turns + n - 1) / n), after = (int)(((int64_t)(j + 1) * p.row_turns + n - 1) / n);
+  const bool rows = after > before;
+  const int wg = p.turn * (rows ? before : j - before) + at;
+  if (wg >= (rows ? p.items : p.s.workers)) return;
+#if defined(__HIP_DEVICE_COMPILE__)
+  // each side reads its arguments by itself, from the kernel-argument segment (the block is the kernel's
+  // only argument, at offset 0): what both hold would otherwise be in scalar registers at once
+  const __attribute__((address_space(4))) PagedPairArgs* ap =
+      (const __attribute__((address_space(4))) PagedPairArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  if (rows) {
+    asm volatile("" : "+s"(ap));
+    const PagedRowsArgs r = ap->r;
+    int unit, rg;
+    paged_item_at(r, wg, unit, rg);
+    attn_w64_item<kPaged, DT, NCB, true>(r, unit, rg);
+  } else {
+    asm volatile("" : "+s"(ap));
+    const PagedAttnArgs s = ap->s;
+    stream_worker<DT, 1>(s, wg);
+  }
+#endif
 }
 
 // Per (batch, kv head): maxima of packed blocks of 128 timestamps (lanes at or
@@ -1603,6 +1677,22 @@ static int launch_rows_t(const PagedRowsArgs& a, unsigned grid, hipStream_t st) 
   return check_launch("paged attention (rows)");
 }
 
+template <int DT, int NCB>
+static int launch_pair_t(const PagedPairArgs& p, hipStream_t st) {
+  constexpr int lds = kWLds > stream_lds(1) ? kWLds : stream_lds(1);
+  static int done = 0;
+  if (!done) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_pair_kernel<DT, NCB>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+    done = 1;
+  }
+  const int64_t grid = (int64_t)p.turn * (p.row_turns + p.stream_turns);
+  if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
+  hipLaunchKernelGGL((paged_pair_kernel<DT, NCB>), dim3((unsigned)grid), dim3(256), lds, st, p);
+  return check_launch("paged attention (rows and stream)");
+}
+
 template <int DB>
 static int launch_rows_f32(const PagedRowsArgs& a, unsigned grid, hipStream_t st) {
   hipLaunchKernelGGL((attn_f32_kernel<kPaged, DB, PagedRowsArgs>), dim3(grid), dim3(64 * kFWaves), 0, st, a,
@@ -1610,15 +1700,14 @@ static int launch_rows_f32(const PagedRowsArgs& a, unsigned grid, hipStream_t st
   return check_launch("paged attention (rows, fp32)");
 }
 
-RowsShape paged_rows_shape(int dtype, int G) {
-  if (dtype == DA_F32) return RowsShape{G, G, kFRows, kFRows};
-  const int hpw = G % 4 == 0 ? 4 : (G % 2 == 0 ? 2 : 1);
-  return RowsShape{1, hpw, 128 / hpw, 256 / hpw};
+RowsShape paged_rows_shape(int dtype) {
+  if (dtype == DA_F32) return RowsShape{kFRows, kFRows};
+  return RowsShape{128, 256};
 }
 
-int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts, int dtype,
-                      hipStream_t st) {
-  const RowsShape shape = paged_rows_shape(dtype, p.G);
+int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts,
+                      bool with_stream, int dtype, hipStream_t st) {
+  const RowsShape shape = paged_rows_shape(dtype);
   PagedRowsArgs a = {};
   a.q = (const uint16_t*)p.q; a.out = (uint16_t*)p.out;
   a.sq_b = a.sq_n = p.sq_t; a.sq_h = p.sq_h;
@@ -1628,15 +1717,18 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
   a.seq = SeqMap{list.cu, list.T, list.max_len};
   a.scale_log2 = p.scale_log2;
   a.causal = own ? 1 : 0;
-  a.hpw = dtype == DA_F32 ? 1 : shape.heads;
+  a.hpw = 1;
   a.pages = p.pages;
   a.list = list;
   a.splits = splits;
   a.short_rows = p.short_rows[own];
   a.parts = parts;
+  // 6 prompts of 1250 to 3001 tokens, 4 KV heads: 237 us spread, 294 by units; 8 of 4569 to 28485, 2 KV heads
+  // 4.2 / 7.7 ms, 8 KV heads 15.1 / 13.8
+  a.spread = (p.Hkv & 7) != 0;
   const int rows = wide ? shape.wide : shape.narrow;
-  a.n_row_groups = (list.max_len * shape.pack + rows - 1) / rows;
-  a.units = list.B * (p.Hq / shape.heads) * splits;
+  a.n_row_groups = (int)(((int64_t)list.max_len * p.G + rows - 1) / rows);
+  a.units = list.B * p.Hkv * splits;
   a.slots = 2 * cu_count() / 8;
   const int64_t grid = (int64_t)a.units * a.n_row_groups;
   if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
@@ -1649,6 +1741,12 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
     }
   }
   const unsigned n = (unsigned)grid;
+  if (with_stream) {
+    const int turn = cu_count() & ~7;  // XCD x has the workgroups x mod 8 of a turn
+    const PagedPairArgs pair = {p, a, turn, (int)grid, (int)((grid + turn - 1) / turn), (p.workers + turn - 1) / turn};
+    if (dtype == DA_F16) return wide ? launch_pair_t<DA_F16, 2>(pair, st) : launch_pair_t<DA_F16, 1>(pair, st);
+    return wide ? launch_pair_t<DA_BF16, 2>(pair, st) : launch_pair_t<DA_BF16, 1>(pair, st);
+  }
   if (dtype == DA_F16) return wide ? launch_rows_t<DA_F16, 2>(a, n, st) : launch_rows_t<DA_F16, 1>(a, n, st);
   return wide ? launch_rows_t<DA_BF16, 2>(a, n, st) : launch_rows_t<DA_BF16, 1>(a, n, st);
 }

@@ -64,7 +64,7 @@ __device__ __forceinline__ int sequence_of(const PageBatch& s, int t, int lane) 
 // A call of paged attention.  A list is the batch's own sequences or the groups of a shared prefix;
 // an item is the queries that one list entry brings to one KV head, its rows are (token, query head of
 // the group) in that order.  Entries of up to kStreamRows rows are `short`: their items' keys go as one
-// stream over the chip (da_paged_stream.hip).
+// stream over the chip (da_paged_stream.hpp).
 constexpr int kStreamRows = 32;
 
 // An item that several workers of the stream share, kept by the one with its first part.
@@ -99,9 +99,18 @@ struct PagedAttnArgs {
 constexpr int kState = 132;
 constexpr int kStreamTile = 128;  // keys
 
+// The sequences or the prefix's groups, field by field (a reference to either would put the kernel's
+// arguments into memory).
+__device__ __forceinline__ PageBatch list_of(const PagedAttnArgs& a, bool own) {
+  const PageBatch &x = a.seq, &y = a.prefix;
+  return PageBatch{own ? x.table : y.table, own ? x.lengths : y.lengths, own ? x.cu : y.cu, own ? x.start : y.start,
+                   own ? x.table_stride : y.table_stride, own ? x.B : y.B, own ? x.T : y.T, own ? x.max_len : y.max_len,
+                   own ? x.max_keys : y.max_keys};
+}
+
 // tiles of an item of the stream; a sequence that sees nothing has one, which writes its zeros
 __device__ __forceinline__ int stream_tiles(const PagedAttnArgs& a, int tokens, int keys, bool own) {
-  if (tokens == 0 || tokens * a.G > a.short_rows[own]) return 0;
+  if (tokens == 0 || tokens * a.G > (own ? a.short_rows[1] : a.short_rows[0])) return 0;
   const int n = (keys + kStreamTile - 1) / kStreamTile;
   return own && n == 0 ? 1 : n;
 }
@@ -147,15 +156,16 @@ struct RowSum {
 
 // Host: checks and the kernels' forms of the ABI's blocks.
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who);
-// What a workgroup of the row kernels takes: `heads` query heads of a KV head and, of their rows (pack of
-// them a token), a half-size or full-size group.
+// Rows of a KV head, (token, query head of the group), that a workgroup of the row kernels takes: a
+// half-size or full-size group.
 struct RowsShape {
-  int pack, heads, narrow, wide;
+  int narrow, wide;
 };
-RowsShape paged_rows_shape(int dtype, int G);
-// The entries of `list` with more than short_rows rows.
-int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts, int dtype,
-                      hipStream_t st);
+RowsShape paged_rows_shape(int dtype);
+// The entries of `list` with more than short_rows rows; with_stream (not for fp32): and the stream.
+int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, bool wide, int splits, float* parts,
+                      bool with_stream, int dtype, hipStream_t st);
+int launch_paged_stream_join(const PagedAttnArgs& a, int dtype, hipStream_t st);
 int launch_paged_stream(const PagedAttnArgs& a, int dtype, hipStream_t st);
 int fill_batch(PageBatch& s, const DaPagedBatch* b, const Pages& p, int64_t T, const char* who);
 

@@ -2,7 +2,7 @@
 // entries, and the parts of a result joined.
 //
 // An entry (a sequence, or a group behind a prefix) of up to kStreamRows rows goes to the stream
-// (da_paged_stream.hip); one with more rows, and all of fp32, to the row kernels (da_attn.hip's, over
+// (da_paged_stream.hpp); one with more rows, and all of fp32, to the row kernels (da_attn.hip's, over
 // pages), whose items are blocks of rows and, where those do not fill the chip, runs of keys.
 // A prefix is a list of its own, seen whole by all rows of a group at once: its keys are read once for
 // the group, and each row's result is joined with that of its own sequence.
@@ -99,19 +99,19 @@ static bool stream_whole(int64_t items, int keys) {
 // narrow 998, wide 1204, 2 parts 903, 4 924; 512 at a sequence's start: 1 part 21, 2 31.
 static void shape_rows(PagedAttnArgs& a, int list, bool& wide, int dtype) {
   const PageBatch& s = list ? a.seq : a.prefix;
-  const RowsShape shape = paged_rows_shape(dtype, a.G);
+  const RowsShape shape = paged_rows_shape(dtype);
   const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = 2.0 * cu_count();
   const int tiles = (s.max_keys + 31) / 32;
   double best = 0.0;
-  const int64_t most = (int64_t)s.max_len * shape.pack, others = s.B - 1, rest = s.T - s.max_len;
+  const int64_t most = (int64_t)s.max_len * a.G, others = s.B - 1, rest = s.T - s.max_len;
   for (int w = 0; w < (shape.wide > shape.narrow && most > shape.narrow ? 2 : 1); ++w) {
     const int rows = w ? shape.wide : shape.narrow;
     // items: those of the longest entry, and of the others if their mean is not the stream's
     const int64_t longest = (most + rows - 1) / rows;
     int64_t items = longest;
     if (others > 0 && rest * a.G > others * a.short_rows[list])
-      items += std::min(others * longest, rest * shape.pack / rows + others);
-    items *= a.Hq / shape.heads;
+      items += std::min(others * longest, rest * a.G / rows + others);
+    items *= a.Hkv;
     for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (n > 1 && n > tiles) break;
       const double all = (double)items * n, rounds = all <= slots ? 1.0 : all / slots + 0.3;
@@ -227,16 +227,23 @@ extern "C" int da_paged_attention(const void* q, int64_t sq_t, int64_t sq_h, voi
   DA_REQUIRE(((uintptr_t)workspace & 255) == 0, "%s: the workspace must be 256-byte aligned", who);
   char* ws = (char*)workspace;
   a.begin = (uint32_t*)ws;
-  a.records = p.join || a.whole ? nullptr : (StreamRecord*)(ws + p.records);
+  a.records = p.join || !p.stream || a.whole ? nullptr : (StreamRecord*)(ws + p.records);
   a.slots = (float*)(ws + p.slots);
   a.states = (float*)(ws + p.states);
   for (int i = 0; i < 2; ++i) a.parts[i] = p.parts[i] < 0 ? nullptr : (float*)(ws + p.parts[i]);
   hipStream_t st = (hipStream_t)stream;
-  if (p.stream)
+  // the rows of a prefix and the stream in one launch: both wait for memory most of the time (16 sequences
+  // behind 32768 tokens 43.8 us, apart 48.4).  A prompt's rows want both workgroups of a CU to themselves
+  // (512 tokens beside 15 decoding sequences 131 us together, 117 apart)
+  const bool pair = p.stream && p.rows[0];
+  if (p.stream && !pair)
     if (int rc = launch_paged_stream(a, dtype, st)) return rc;
   for (int i = 0; i < 2; ++i)
     if (p.rows[i])
-      if (int rc = launch_paged_rows(a, i ? a.seq : a.prefix, i == 1, p.wide[i], a.splits[i], a.parts[i], dtype, st)) return rc;
+      if (int rc = launch_paged_rows(a, i ? a.seq : a.prefix, i == 1, p.wide[i], a.splits[i], a.parts[i], pair && i == 0, dtype,
+                                     st))
+        return rc;
+  if (a.records) return launch_paged_stream_join(a, dtype, st);
   if (!p.join) return DA_OK;
   return dtype == DA_BF16 ? launch_join<DA_BF16>(a, st) : dtype == DA_F16 ? launch_join<DA_F16>(a, st) : launch_join<DA_F32>(a, st);
 }

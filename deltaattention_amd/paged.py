@@ -55,6 +55,13 @@ class PagedKV:
         self._ref = ctypes.byref(self._block)
 
 
+def _ints(t: torch.Tensor, name: str, n: int, device: torch.device) -> int:
+    """The address of an int32 tensor of n values."""
+    if t.dtype is not _I32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values on {device}")
+    return t.data_ptr()
+
+
 class PagedBatch:
     """The sequences of a call, on the device.
 
@@ -72,9 +79,10 @@ class PagedBatch:
     def __init__(self, table: torch.Tensor, lengths: torch.Tensor, cu_seqlens=None, max_seqlen: Optional[int] = None,
                  start: Optional[torch.Tensor] = None):
         device = _gpu(table, "table")
-        if table.dim() != 2 or table.stride(1) != 1 or table.dtype != _I32 or not table.numel():
+        shape, stride = table.shape, table.stride()
+        if len(shape) != 2 or stride[1] != 1 or table.dtype is not _I32 or 0 in shape:
             raise ValueError("table must be int32 [B, width] with contiguous rows")
-        B, width = table.shape
+        B, width = shape
         cu = cu_seqlens
         if cu is not None and not (isinstance(cu, torch.Tensor) and cu.device.type == "cuda"):
             host = [int(x) for x in (cu.tolist() if isinstance(cu, torch.Tensor) else cu)]
@@ -83,19 +91,17 @@ class PagedBatch:
             longest = max(1, max(y - x for x, y in zip(host, host[1:])))
             max_seqlen = longest if max_seqlen is None else max(longest, int(max_seqlen))
             cu = torch.tensor(host, dtype=_I32, device=device)
-        for t, name, n in ((lengths, "lengths", B), (cu, "cu_seqlens", B + 1), (start, "start", B)):
-            if t is not None and (t.dtype != _I32 or t.dim() != 1 or t.shape[0] != n or t.device != device
-                                  or (n > 1 and t.stride(0) != 1)):
-                raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values on {device}")
         if cu is None:
-            max_seqlen = 1
-        elif max_seqlen is None or max_seqlen <= 0:
-            raise ValueError("max_seqlen (the most tokens a sequence brings) is needed with cu_seqlens on the device")
+            at_cu, max_seqlen = None, 1
+        else:
+            at_cu = _ints(cu, "cu_seqlens", B + 1, device)
+            if max_seqlen is None or max_seqlen <= 0:
+                raise ValueError("max_seqlen (the most tokens a sequence brings) is needed with cu_seqlens on the device")
         self.table, self.lengths, self.cu, self.start = table, lengths, cu, start
         self.batch, self.max_seqlen, self.device = B, int(max_seqlen), device
-        self._block = PagedBatchBlock(table.data_ptr(), lengths.data_ptr(), None if cu is None else cu.data_ptr(),
-                                   None if start is None else start.data_ptr(), B, width, table.stride(0),
-                                   self.max_seqlen)
+        self._block = PagedBatchBlock(table.data_ptr(), _ints(lengths, "lengths", B, device), at_cu,
+                                      None if start is None else _ints(start, "start", B, device), B, width, stride[0],
+                                      self.max_seqlen)
         self._ref = ctypes.byref(self._block)
 
 
