@@ -392,11 +392,15 @@ class FourBitCompressedCache(HybridCompressedCache):
     def _rows(self, capacity):
         kv = kv4.KV4.empty(self.bsz, self.n_kv_heads, capacity, self.head_dim, self.device)
         kv.lengths.zero_()
+        kv.mass.zero_()
         return kv
 
-    def _replace(self, layer_idx, kv):
-        """The layer's anchors from here on.  Those before may have been made on another stream than this
-        one, whose work still reads them: their memory stays until that is done."""
+    def _replace(self, layer_idx, kv, rows):
+        """The layer's anchors from here on, the first ``rows`` of them written: the mass of the others is 0
+        until a token takes them.  The anchors before may have been made on another stream than this one, whose
+        work still reads them: their memory stays until that is done."""
+        if rows < kv.capacity:
+            kv.mass[:, :, rows:].zero_()
         self.anchors[layer_idx].record_stream(torch.cuda.current_stream(kv.device))
         self.anchors[layer_idx] = kv
 
@@ -433,7 +437,7 @@ class FourBitCompressedCache(HybridCompressedCache):
             P = self.budget
         capacity = self.budget + self.slack if self.budget is not None else max(self.capacity, P + 1024)
         self._replace(layer_idx, kv4.quantize_kv4(k_packed, v_packed, counts, timestamps, mass, lengths, index,
-                                                  capacity))
+                                                  capacity), P)
         self.k_last[layer_idx] = last
         self.max_packed_len[layer_idx] = P
         self.k_exact[layer_idx, :, :, :e_len] = k_exact
@@ -450,9 +454,11 @@ class FourBitCompressedCache(HybridCompressedCache):
         kv4._check_update(kv, key_states, value_states, self.k_exact[layer_idx], self.v_exact[layer_idx],
                           self.k_last[layer_idx], self.exact_seq_lens[layer_idx], self.total_seq_lens[layer_idx])
         if self.budget is None:
-            self._replace(layer_idx, kv4.evict_kv4(kv, kv.capacity, capacity=max(2 * kv.capacity, kv.capacity + 1024)))
+            self._replace(layer_idx, kv4.evict_kv4(kv, kv.capacity, capacity=max(2 * kv.capacity, kv.capacity + 1024)),
+                          kv.capacity)
         else:
-            self._replace(layer_idx, kv4.evict_kv4(kv, self.budget, self.sinks, self.recent, self.budget + self.slack))
+            self._replace(layer_idx, kv4.evict_kv4(kv, self.budget, self.sinks, self.recent, self.budget + self.slack),
+                          self.budget)
             self.max_packed_len[layer_idx] = self.budget
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
