@@ -93,7 +93,7 @@ struct AttnArgs {
 };
 
 // kPaged: q and out are [T, heads, D] (s*_b and s*_n their token strides, seq.cu the list's), the keys
-// of a row group are cut into `splits` equal runs of tiles, unit (g, b, split).  A row is a (token, query
+// of a row group are cut into `splits` equal runs of tiles, unit (g, split).  A row is a (token, query
 // head of the group): entry b has tokens(b) * G of them.
 struct PagedRowsArgs : AttnArgs {
   Pages pages;
@@ -103,6 +103,28 @@ struct PagedRowsArgs : AttnArgs {
   float* parts;    // [splits][T][Hq][kState], or null: the result goes to out
   int spread;      // the order of the items, see paged_item_at
 };
+
+// Row group `at` of a list whose entries have tokens * G rows, in groups of `rows`: entry b has the
+// places from first(b) * G / rows + b on, which holds its groups whatever the entries before have (a place
+// or two an entry is left over); its last group, of a causal entry the longest, comes first.  For a whole
+// wave; false for a place without one.
+__device__ __forceinline__ bool group_at(const PagedRowsArgs& a, int rows, int at, int lane, int& b, int& rg) {
+  auto begin = [&](int e) { return a.list.first(e) * a.G / rows + e; };
+  int lo = 0, n = a.list.B;
+  while (n > 1) {  // the last entry that begins at or before `at` is in [lo, lo + n)
+    const int step = (n + 63) >> 6;
+    const bool before = lane * step < n && begin(lo + lane * step) <= at;
+    const int c = __popcll(__ballot(before));
+    if (c == 0) return false;
+    const int next = lo + (c - 1) * step;
+    n = min(step, lo + n - next);
+    lo = next;
+  }
+  b = __builtin_amdgcn_readfirstlane(lo);
+  const int groups = (a.list.tokens(b) * a.G + rows - 1) / rows;
+  rg = __builtin_amdgcn_readfirstlane(groups - 1 - (at - begin(b)));
+  return rg >= 0 && rg < groups;
+}
 
 // Phase-1 extent of a query block (deltaFlashAttention.py:58-80): n_safe = the number of
 // packed blocks whose prefix maximum timestamp is below thr -- the prefix maxima do not
@@ -248,20 +270,19 @@ __device__ __forceinline__ void item_at(int k, int units, int n_rg, int slots, i
   }
 }
 
-// Item of workgroup wg, the longest row groups first.  Whole units an XCD where they split evenly (an
-// XCD's L2 then has one unit's K and V at a time), or, `spread`, all units' row groups in turn over the
+// Item of workgroup wg: unit (KV head, run of keys) and row group.  Whole units an XCD where they split evenly
+// (an XCD's L2 then has one unit's K and V at a time), or, `spread`, all units' row groups in turn over the
 // XCDs, which evens out a ragged batch.
-__device__ __forceinline__ void paged_item_at(const PagedRowsArgs& a, int wg, int& unit, int& rg) {
+__device__ __forceinline__ void paged_item_at(const PagedRowsArgs& a, int wg, int& unit, int& group) {
   if (a.spread) {
-    const int j = wg / a.units;
-    unit = (wg + j) % a.units;
-    rg = a.n_row_groups - 1 - j;
-  } else if ((a.units & 7) == 0) {
+    group = wg / a.units;
+    unit = (wg + group) % a.units;
+  } else {
     const int upx = a.units >> 3;
+    int rg;
     item_at(wg >> 3, upx, a.n_row_groups, a.slots, unit, rg);
     unit += (wg & 7) * upx;
-  } else {
-    item_at(wg, a.units, a.n_row_groups, 8 * a.slots, unit, rg);
+    group = a.n_row_groups - 1 - rg;
   }
 }
 
@@ -270,7 +291,7 @@ __device__ __forceinline__ void paged_item_at(const PagedRowsArgs& a, int wg, in
 // barrier) and every load landed; the finalize uses only the wave's own Q region, so the next
 // item may start staging at once.
 template <int VARIANT, int DT, int NCB, bool LAZY, class Args>
-__device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_split, const int rg) {
+__device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_split, const int rg_item) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* const kst0 = smem;
   char* const vst0 = smem + 2 * kWKBytes;
@@ -285,17 +306,15 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   // wrote (the K fragment layout), so the 32 registers it would take stay free
   char* const qs = meta0 + 4 * kWMetaSlot + wid * kWQBytes;
   const int hl = lane >> 5, ql = lane & 31;
-  int unit = unit_split, split = 0;
-  if constexpr (VARIANT == kPaged) {
-    unit = unit_split / a.splits;
-    split = unit_split - unit * a.splits;
-  }
+  const int unit = unit_split;
+  int split = 0;
   const int hsh = VARIANT == kPaged ? 0 : a.hpw >> 1;  // log2 of the query heads a workgroup takes
-  int g, b, h;
+  int g, b, h, rg = rg_item;
   if constexpr (VARIANT == kPaged) {
-    g = unit / a.B;
-    b = unit - g * a.B;
+    g = unit / a.splits;
+    split = unit - g * a.splits;
     h = 0;  // the rows are (token, query head of the group)
+    if (!group_at(a, 128 * NCB, rg_item, lane, b, rg)) return;
   } else {
     const int hunits = a.G >> hsh;
     const int gb = unit / hunits;  // g * B + b
@@ -1191,7 +1210,8 @@ template <int VARIANT, int DB>
 struct F32Frags {
   static constexpr int NV = DB <= 2 ? DB : 4;      // value fragments of a tile
   static constexpr int NR = 16 / NV;               // S^T registers (key pairs) a value fragment serves
-  static constexpr int F = DB + NV;                // fragments of a tile
+  // fragments of a tile (pages, 96 dims: an empty one more, so that a ring of 4 does: registers)
+  static constexpr int F = DB + NV + (VARIANT == kPaged && DB == 3);
   // ring size; F % R == 0 keeps its slots static (pure Phase 1 at 128 dims has registers for two)
   static constexpr int R = VARIANT == kPure && DB == 4 ? 2 : F % 4 == 0 ? 4 : F;
 };
@@ -1223,10 +1243,10 @@ void attn_f32_kernel(Args a, int paired) {
   int units = a.B * a.Hq, splits = 1, split = 0;
   if constexpr (VARIANT == kPaged) {
     splits = a.splits;
-    nrb = (a.Nq * a.G + kFRows - 1) / kFRows;
-    units = a.B * a.Hkv * splits;
+    nrb = a.n_row_groups;
+    units = a.units;
   }
-  const bool whole = (units & 7) == 0 && (!a.seq.cu || (a.Hq & 7) == 0);
+  const bool whole = (units & 7) == 0 && (VARIANT == kPaged || !a.seq.cu || (a.Hq & 7) == 0);
   int unit, j;  // j: row blocks from the last one
   if (paired) {
     const int nx = whole ? 8 : 1;
@@ -1246,12 +1266,13 @@ void attn_f32_kernel(Args a, int paired) {
   // without whole heads per XCD a long sequence's row blocks go round the XCDs (an odd number
   // of units does that by itself)
   if (a.seq.cu && !whole && !(units & 1)) unit = (unit + j) % units;
-  const int rb = nrb - 1 - j;
+  int rb = nrb - 1 - j;
+  int h = unit / a.B, b = unit % a.B;
   if constexpr (VARIANT == kPaged) {
-    split = unit % splits;
-    unit /= splits;
+    h = unit / splits;
+    split = unit - h * splits;
+    if (!group_at(a, kFRows, j, lane, b, rb)) return;
   }
-  const int h = unit / a.B, b = unit % a.B;
   const int g = VARIANT == kPaged ? h : h / a.G;
   const int bg = b * a.Hkv + g;
   int Nq, Nk, off = 0;  // row r sees the keys up to r + off
@@ -1361,6 +1382,7 @@ void attn_f32_kernel(Args a, int paired) {
   Halves at_now, at_next;
   auto load_paged = [&](auto FC, const Halves& at, const int t, float (&x)[16]) {
     constexpr int f = decltype(FC)::value;
+    if constexpr (f >= DB + FR::NV) return;
     // rows past the last key of a half repeat it
     const int last = Nk - 1 - (ds + t * kFTile);
     int ql = lane & 31, hl = lane >> 5;
@@ -1515,6 +1537,7 @@ void attn_f32_kernel(Args a, int paired) {
           o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(ring[(DB + fv) % FR::R][DB * u + db], s[fv * FR::NR + u],
                                                        o[db], 0, 0, 0);
     });
+    if constexpr (FR::F > DB + FR::NV) ahead(std::integral_constant<int, DB + FR::NV>{});
   }
 
   // ---- merge: wave w adds up registers kOwn w .. + kOwn - 1 (kOwn DB consecutive dims
@@ -1666,13 +1689,8 @@ static int launch_attn_f32(const AttnArgs& a, hipStream_t st) {
 // ---- paged batches (da_paged_attn.hip plans them) ----
 template <int DT, int NCB>
 static int launch_rows_t(const PagedRowsArgs& a, unsigned grid, hipStream_t st) {
-  static int done = 0;
-  if (!done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
-    if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
-    done = 1;
-  }
+  static bool done[kMaxDevices] = {};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>), kWLds, done)) return rc;
   hipLaunchKernelGGL((attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>), dim3(grid), dim3(256), kWLds, st, a);
   return check_launch("paged attention (rows)");
 }
@@ -1680,13 +1698,8 @@ static int launch_rows_t(const PagedRowsArgs& a, unsigned grid, hipStream_t st) 
 template <int DT, int NCB>
 static int launch_pair_t(const PagedPairArgs& p, hipStream_t st) {
   constexpr int lds = kWLds > stream_lds(1) ? kWLds : stream_lds(1);
-  static int done = 0;
-  if (!done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_pair_kernel<DT, NCB>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
-    done = 1;
-  }
+  static bool done[kMaxDevices] = {};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&paged_pair_kernel<DT, NCB>), lds, done)) return rc;
   const int64_t grid = (int64_t)p.turn * (p.row_turns + p.stream_turns);
   if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
   hipLaunchKernelGGL((paged_pair_kernel<DT, NCB>), dim3((unsigned)grid), dim3(256), lds, st, p);
@@ -1727,8 +1740,8 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
   // 4.2 / 7.7 ms, 8 KV heads 15.1 / 13.8
   a.spread = (p.Hkv & 7) != 0;
   const int rows = wide ? shape.wide : shape.narrow;
-  a.n_row_groups = (int)(((int64_t)list.max_len * p.G + rows - 1) / rows);
-  a.units = list.B * p.Hkv * splits;
+  a.n_row_groups = (int)((int64_t)list.T * p.G / rows) + list.B;  // the places of group_at
+  a.units = p.Hkv * splits;
   a.slots = 2 * cu_count() / 8;
   const int64_t grid = (int64_t)a.units * a.n_row_groups;
   if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");

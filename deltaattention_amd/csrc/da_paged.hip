@@ -181,6 +181,17 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
 }
 
+int allow_lds(const void* kernel, int bytes, bool (&done)[kMaxDevices]) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const bool known = dev >= 0 && dev < kMaxDevices;
+  if (e == hipSuccess && known && done[dev]) return DA_OK;
+  if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  if (known) done[dev] = true;
+  return DA_OK;
+}
+
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who) {
   DA_REQUIRE(kv && kv->k && kv->v, "%s: null pages", who);
   DA_REQUIRE(kv->num_pages > 0 && kv->num_pages < (1ll << 31), "%s: no pages", who);

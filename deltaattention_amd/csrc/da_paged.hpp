@@ -154,6 +154,9 @@ struct RowSum {
   }
 };
 
+// Lets a kernel use more than 64 KiB of dynamic LDS on the current device (once a device).
+constexpr int kMaxDevices = 64;
+int allow_lds(const void* kernel, int bytes, bool (&done)[kMaxDevices]);
 // Host: checks and the kernels' forms of the ABI's blocks.
 int fill_pages(Pages& p, const DaPagedKV* kv, int64_t D, const char* who);
 // Rows of a KV head, (token, query head of the group), that a workgroup of the row kernels takes: a

@@ -181,6 +181,7 @@ static int fill_attention(PagedAttnArgs& a, int dtype, int64_t T, int64_t Hq, in
     return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128] (got %lld)", who, (long long)D);
   DA_REQUIRE(T > 0 && T < (1ll << 28) && Hq > 0 && Hkv > 0 && Hq < (1 << 16), "%s: empty shape", who);
   DA_REQUIRE(Hq % Hkv == 0, "%s: Hq (%lld) must be a multiple of Hkv (%lld)", who, (long long)Hq, (long long)Hkv);
+  DA_REQUIRE(T * Hq < (1ll << 31), "%s: more than 2^31 rows", who);
   if (int rc = fill_pages(a.pages, kv, D, who)) return rc;
   if (int rc = fill_batch(a.seq, batch, a.pages, T, who)) return rc;
   if (prefix) {

@@ -27,13 +27,8 @@ __global__ __launch_bounds__(256) void paged_stream_join_kernel(PagedAttnArgs a)
 
 template <int DT, int STAGES>
 static int launch_stream_t(const PagedAttnArgs& a, hipStream_t st) {
-  static int done = 0;
-  if (!done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_stream_kernel<DT, STAGES>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, stream_lds(STAGES));
-    if (e != hipSuccess) return set_error(DA_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
-    done = 1;
-  }
+  static bool done[kMaxDevices] = {};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&paged_stream_kernel<DT, STAGES>), stream_lds(STAGES), done)) return rc;
   hipLaunchKernelGGL((paged_stream_kernel<DT, STAGES>), dim3((unsigned)a.workers), dim3(256), stream_lds(STAGES), st, a);
   return check_launch("paged attention (stream)");
 }

@@ -86,6 +86,47 @@ def test_decode(gpu, Hq, Hkv, dtype):
     w.check(w.call(ops))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("Hq,Hkv", [(64, 1), (33, 1), (66, 2), (32, 1)])
+def test_many_heads_to_one(gpu, Hq, Hkv, dtype):
+    """Groups of 32 query heads and more: a token alone is more rows than the stream takes."""
+    from deltaattention_amd import ops
+    announce(f"paged attention {Hq}/{Hkv} {dtype}")
+    w = World([1, 3, 0, 1], [700, 40, 9, 0], Hq, Hkv, 64, 16, dtype, prefix=[(2, 90), (2, 17)])
+    w.check(w.call(ops))
+    w.prefix = None
+    w.check(w.call(ops))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("B,long", [(300, 0), (700, 3), (257, 1)])
+def test_many_sequences(gpu, B, long, wide):
+    """More sequences than a workgroup has threads, some of them long or without tokens; a table with room
+    for long ones (`wide`) has the keys of all go as one stream."""
+    from deltaattention_amd import ops
+    announce(f"paged attention of {B} sequences, {long} long, wide={wide}")
+    new = [0 if b % 50 == 7 else 1 for b in range(B)]
+    past = [(b * 7) % 60 + (3000 if b % 90 == 5 and b // 90 < long else 0) for b in range(B)]
+    new[B // 2] = 45 if long else 1
+    w = World(new, past, 8, 2, 64, 16, "bf16")
+    if wide:
+        w.table = torch.cat([w.table, torch.full((B, 300), -1, dtype=torch.int32)], 1)
+    w.check(w.call(ops))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_more_tokens_than_max_seqlen(gpu, dtype):
+    """A sequence with more tokens than max_seqlen is cut to it; the others are as they should be."""
+    from deltaattention_amd import ops
+    announce(f"paged attention, max_seqlen too small {dtype}")
+    w = World([5, 300, 1, 40], [10, 20, 400, 7], 8, 2, 64, 16, dtype)
+    got = ops.paged_attention(w.q.cuda(), ops.PagedKV(w.k.cuda(), w.v.cuda()),
+                              ops.PagedBatch(w.table.cuda(), _i(w.lengths), _i(w.cu), 40)).double().cpu()
+    want, tol = w.want()
+    for a, b in ((0, 5), (305, 306), (306, 346)):
+        assert ((got[a:b] - want[a:b]).abs() <= tol[a:b]).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("D", [8, 40, 64, 80, 96, 120])
 def test_head_dims(gpu, D, dtype):
