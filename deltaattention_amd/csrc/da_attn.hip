@@ -102,13 +102,21 @@ struct PagedRowsArgs : AttnArgs {
   int short_rows;  // entries of up to so many rows are left to the stream
   float* parts;    // [splits][T][Hq][kState], or null: the result goes to out
   int spread;      // the order of the items, see paged_item_at
+  int ranked;      // the places of row groups, see group_at: 0, or the most groups an entry has
 };
 
-// Row group `at` of a list whose entries have tokens * G rows, in groups of `rows`: entry b has the
+// Row group `at` of a list whose entries have tokens * G rows, in groups of `rows`.  Entry b has the
 // places from first(b) * G / rows + b on, which holds its groups whatever the entries before have (a place
-// or two an entry is left over); its last group, of a causal entry the longest, comes first.  For a whole
-// wave; false for a place without one.
+// or two an entry is left over); its last group, of a causal entry the longest, comes first.  Or, `ranked`,
+// all entries' longest possible groups come first, then all those one shorter.  For a whole wave; false for
+// a place without a group.
 __device__ __forceinline__ bool group_at(const PagedRowsArgs& a, int rows, int at, int lane, int& b, int& rg) {
+  if (a.ranked) {
+    const int k = at / a.list.B;
+    b = at - k * a.list.B;
+    rg = a.ranked - 1 - k;
+    return rg >= 0 && rg * rows < a.list.tokens(b) * a.G;
+  }
   auto begin = [&](int e) { return a.list.first(e) * a.G / rows + e; };
   int lo = 0, n = a.list.B;
   while (n > 1) {  // the last entry that begins at or before `at` is in [lo, lo + n)
@@ -275,8 +283,9 @@ __device__ __forceinline__ void item_at(int k, int units, int n_rg, int slots, i
 // XCDs, which evens out a ragged batch.
 __device__ __forceinline__ void paged_item_at(const PagedRowsArgs& a, int wg, int& unit, int& group) {
   if (a.spread) {
-    group = wg / a.units;
-    unit = (wg + group) % a.units;
+    const int item = (wg & ~7) + ((wg + (wg >> 3)) & 7);  // every XCD gets every place of an eight in turn
+    group = item / a.units;
+    unit = item - group * a.units;
   } else {
     const int upx = a.units >> 3;
     int rg;
@@ -1740,10 +1749,15 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
   // 4.2 / 7.7 ms, 8 KV heads 15.1 / 13.8
   a.spread = (p.Hkv & 7) != 0;
   const int rows = wide ? shape.wide : shape.narrow;
-  a.n_row_groups = (int)((int64_t)list.T * p.G / rows) + list.B;  // the places of group_at
+  // the places of group_at; ranked where that leaves at most half of them empty (6 prompts of 1250 to 3001
+  // tokens, 4 KV heads, 237 us against 250) and no XCD has units of its own, which want a sequence at a time
+  const int64_t places = (int64_t)list.T * p.G / rows + list.B, most = ((int64_t)list.max_len * p.G + rows - 1) / rows;
+  a.ranked = (p.Hkv & 7) != 0 && list.B > 1 && most * list.B <= 2 * places ? (int)most : 0;
+  a.n_row_groups = (int)(a.ranked ? most * list.B : places);
   a.units = p.Hkv * splits;
   a.slots = 2 * cu_count() / 8;
-  const int64_t grid = (int64_t)a.units * a.n_row_groups;
+  int64_t grid = (int64_t)a.units * a.n_row_groups;
+  if (dtype != DA_F32) grid = (grid + 7) & ~7ll;  // paged_item_at turns within eights, group_at knows no more places
   if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
   if (dtype == DA_F32) {
     switch ((p.D + 31) / 32) {

@@ -95,12 +95,12 @@ static bool stream_whole(int64_t items, int keys) {
 // Rows of a head that a workgroup of the row kernels takes, and into how many runs it cuts the keys:
 // the least of an estimate.  A run's time is its 32-key tiles times a tile's (us, measured with up to
 // one workgroup a CU and with two); parts cost their writing and reading, 3.5 TB/s, and a launch.
-// 512 tokens of 32 heads after 5000: narrow 1 part 141 us, 4 parts 72, 8 82, wide 8 75; 2048 after 30011:
+// `paired`: a CU's other workgroup is the stream's.  512 tokens of 32 heads after 5000: narrow 1 part 141 us, 4 parts 72, 8 82, wide 8 75; 2048 after 30011:
 // narrow 998, wide 1204, 2 parts 903, 4 924; 512 at a sequence's start: 1 part 21, 2 31.
-static void shape_rows(PagedAttnArgs& a, int list, bool& wide, int dtype) {
+static void shape_rows(PagedAttnArgs& a, int list, bool& wide, bool paired, int dtype) {
   const PageBatch& s = list ? a.seq : a.prefix;
   const RowsShape shape = paged_rows_shape(dtype);
-  const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = 2.0 * cu_count();
+  const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = (paired ? 1.0 : 2.0) * cu_count();
   const int tiles = (s.max_keys + 31) / 32;
   double best = 0.0;
   const int64_t most = (int64_t)s.max_len * a.G, others = s.B - 1, rest = s.T - s.max_len;
@@ -115,7 +115,7 @@ static void shape_rows(PagedAttnArgs& a, int list, bool& wide, int dtype) {
     for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (n > 1 && n > tiles) break;
       const double all = (double)items * n, rounds = all <= slots ? 1.0 : all / slots + 0.3;
-      const bool two = 2 * all > slots;
+      const bool two = !paired && 2 * all > slots;
       const double tile = dtype == DA_F32 ? (two ? 1.75 : 0.9) * ((a.D + 31) / 32) / 4 : w ? (two ? 1.75 : 1.22) : (two ? 1.0 : 0.78);
       const double time = rounds * ((tiles + n - 1) / n) * tile + (n > 1 || a.prefix.B ? n * part + (n > 1 ? 5 : 0) : 0.0);
       if ((w == 0 && n == 1) || time < best) best = time, wide = w, a.splits[list] = n;
@@ -127,6 +127,10 @@ struct PagedPlan {
   bool stream, rows[2], wide[2], join;
   int64_t records, slots, states, parts[2], total;  // byte offsets in the workspace
 };
+// The rows of a prefix and the stream run in one launch: both wait for memory most of the time (16 sequences
+// behind 32768 tokens 43.8 us, apart 48.4).  A prompt's rows want both workgroups of a CU to themselves (512
+// tokens beside 15 decoding sequences 131 us together, 117 apart).
+static bool paired_rows(const PagedPlan& p, int list) { return list == 0 && p.stream; }
 static int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 // How a call runs, by what the host knows of it.
@@ -152,8 +156,10 @@ static PagedPlan plan(PagedAttnArgs& a, int dtype) {
       slot_rows = std::max(slot_rows, std::min<int64_t>(most, kStreamRows));
     }
     p.rows[i] = most > a.short_rows[i];
+  }
+  for (int i = 0; i < 2; ++i) {
     if (!p.rows[i]) continue;
-    shape_rows(a, i, p.wide[i], dtype);
+    shape_rows(a, i, p.wide[i], paired_rows(p, i), dtype);
     if (a.splits[i] > 1 || a.prefix.B) parts |= 1 << i;
   }
   a.whole = stream_whole((int64_t)E * a.Hkv, keys);
@@ -233,10 +239,7 @@ extern "C" int da_paged_attention(const void* q, int64_t sq_t, int64_t sq_h, voi
   a.states = (float*)(ws + p.states);
   for (int i = 0; i < 2; ++i) a.parts[i] = p.parts[i] < 0 ? nullptr : (float*)(ws + p.parts[i]);
   hipStream_t st = (hipStream_t)stream;
-  // the rows of a prefix and the stream in one launch: both wait for memory most of the time (16 sequences
-  // behind 32768 tokens 43.8 us, apart 48.4).  A prompt's rows want both workgroups of a CU to themselves
-  // (512 tokens beside 15 decoding sequences 131 us together, 117 apart)
-  const bool pair = p.stream && p.rows[0];
+  const bool pair = p.rows[0] && paired_rows(p, 0);
   if (p.stream && !pair)
     if (int rc = launch_paged_stream(a, dtype, st)) return rc;
   for (int i = 0; i < 2; ++i)

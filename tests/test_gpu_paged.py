@@ -456,6 +456,75 @@ def test_captured_steps(gpu, prefix, dtype):
         lengths += 1
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("new,past,prefix", [([70, 1, 33], [5000, 900, 3], ()), ([1] * 40, [30] * 40, [(25, 2000), (15, 90)]),
+                                             ([3] * 12, [10] * 12, [(12, 700)]), ([300], [0], ())])
+def test_captured_attention(gpu, new, past, prefix, dtype):
+    """Every kernel's launches captured and replayed on other queries, with eager calls between."""
+    from deltaattention_amd import ops
+    announce(f"paged attention captured {new[:3]} {prefix} {dtype}")
+    w = World(new, past, 8, 2, 64, 16, dtype, prefix=prefix)
+    kv, batch = ops.PagedKV(w.k.cuda(), w.v.cuda()), w.batch(ops)
+    pre = None if not prefix else ops.PagedBatch(w.prefix[0].cuda(), _i(w.prefix[1]), w.prefix[2])
+
+    def call(q):
+        return ops.shared_prefix_attention(q, kv, batch, pre) if prefix else ops.paged_attention(q, kv, batch)
+    gen = torch.Generator().manual_seed(8)
+    qs = [torch.randn(w.q.shape, generator=gen).to(w.dtype).cuda() for _ in range(4)]
+    eager = [call(q) for q in qs]
+    still = qs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(still)
+    for q, want in zip(qs, eager):
+        still.copy_(q)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(call(q), want)
+    w.q = qs[-1].cpu()
+    w.check(out)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_outside_every_group(gpu, new, dtype):
+    """Tokens before the first group and after the last see their own sequence alone."""
+    from deltaattention_amd import ops
+    announce(f"shared prefix, sequences outside the groups, {new} tokens {dtype}")
+    w = World([new] * 6, [3 * b for b in range(6)], 8, 2, 64, 16, dtype, prefix=[(2, 100), (3, 55), (1, 9)])
+    t, n, cu = w.prefix
+    w.prefix = (t[:2], n[:2], [2 * new, 4 * new, 5 * new])
+    pre = ops.PagedBatch(w.prefix[0].cuda(), _i(w.prefix[1]), _i(w.prefix[2]), 2 * new)
+    w.check(ops.shared_prefix_attention(w.q.cuda(), ops.PagedKV(w.k.cuda(), w.v.cuda()), w.batch(ops), pre))
+
+
+def test_two_streams_at_once(gpu):
+    """Calls of every kernel in flight on two streams: no memory is shared between calls."""
+    from deltaattention_amd import ops
+    announce("paged attention on two streams at once")
+    worlds = [World([1] * 9, [4000 + 7 * b for b in range(9)], 8, 2, 64, 16, "bf16"),
+              World([200, 1, 3], [900, 5000, 0], 8, 2, 64, 16, "bf16"),
+              World([1] * 30, [20] * 30, 8, 2, 64, 16, "bf16", prefix=[(30, 3000)])]
+    calls = []
+    for w in worlds:
+        kv, batch, q = ops.PagedKV(w.k.cuda(), w.v.cuda()), w.batch(ops), w.q.cuda()
+        pre = None if w.prefix is None else ops.PagedBatch(w.prefix[0].cuda(), _i(w.prefix[1]), w.prefix[2])
+        calls.append((lambda q=q, kv=kv, batch=batch: ops.paged_attention(q, kv, batch)) if pre is None else
+                     (lambda q=q, kv=kv, batch=batch, pre=pre: ops.shared_prefix_attention(q, kv, batch, pre)))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 3, calls[i % 3]()))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert torch.equal(g, want[i])
+
+
 def test_other_stream(gpu):
     from deltaattention_amd import ops
     announce("paged attention on another stream")
