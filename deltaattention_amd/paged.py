@@ -28,12 +28,12 @@ class PagedKV:
     dimension (a view of [num_pages, page_size, Hkv, D] too); ``page_size`` a power of two from 16
     on, D a multiple of 8 up to 128.  The tensors of an object are fixed, their contents are not."""
 
-    __slots__ = ("k_pages", "v_pages", "num_pages", "kv_heads", "page_size", "head_dim", "dtype", "device", "_code",
-                 "_block", "_ref")
+    __slots__ = ("k_pages", "v_pages", "num_pages", "kv_heads", "page_size", "head_dim", "dtype", "device", "_index",
+                 "_code", "_block", "_ref")
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
-        shape, device = k_pages.shape, _gpu(k_pages, "k_pages")
-        if len(shape) != 4 or v_pages.shape != shape or v_pages.device != device:
+        shape, device, index = k_pages.shape, _gpu(k_pages, "k_pages"), k_pages.get_device()
+        if len(shape) != 4 or v_pages.shape != shape or v_pages.get_device() != index:
             raise ValueError("k_pages and v_pages are [num_pages, Hkv, page_size, D] of one shape on one device")
         code = dtype_code(k_pages, v_pages)
         P, H, S, D = shape
@@ -50,15 +50,15 @@ class PagedKV:
                              "16-byte alignment")
         self.k_pages, self.v_pages = k_pages, v_pages
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = P, H, S, D
-        self.dtype, self.device, self._code = k_pages.dtype, device, code
+        self.dtype, self.device, self._index, self._code = k_pages.dtype, device, index, code
         self._block = PagedKVBlock(kp, vp, P, S, sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
         self._ref = ctypes.byref(self._block)
 
 
-def _ints(t: torch.Tensor, name: str, n: int, device: torch.device) -> int:
-    """The address of an int32 tensor of n values."""
-    if t.dtype is not _I32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values on {device}")
+def _ints(t: torch.Tensor, name: str, n: int, index: int) -> int:
+    """The address of an int32 tensor of n values on GPU ``index``."""
+    if t.dtype is not _I32 or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values on cuda:{index}")
     return t.data_ptr()
 
 
@@ -74,11 +74,11 @@ class PagedBatch:
     a CPU tensor of cu_seqlens is checked, copied to the device and gives ``max_seqlen``.  The tensors
     are fixed, their contents are not."""
 
-    __slots__ = ("table", "lengths", "cu", "start", "batch", "max_seqlen", "device", "_block", "_ref")
+    __slots__ = ("table", "lengths", "cu", "start", "batch", "max_seqlen", "device", "_index", "_block", "_ref")
 
     def __init__(self, table: torch.Tensor, lengths: torch.Tensor, cu_seqlens=None, max_seqlen: Optional[int] = None,
                  start: Optional[torch.Tensor] = None):
-        device = _gpu(table, "table")
+        device, index = _gpu(table, "table"), table.get_device()
         shape, stride = table.shape, table.stride()
         if len(shape) != 2 or stride[1] != 1 or table.dtype is not _I32 or 0 in shape:
             raise ValueError("table must be int32 [B, width] with contiguous rows")
@@ -94,13 +94,13 @@ class PagedBatch:
         if cu is None:
             at_cu, max_seqlen = None, 1
         else:
-            at_cu = _ints(cu, "cu_seqlens", B + 1, device)
+            at_cu = _ints(cu, "cu_seqlens", B + 1, index)
             if max_seqlen is None or max_seqlen <= 0:
                 raise ValueError("max_seqlen (the most tokens a sequence brings) is needed with cu_seqlens on the device")
         self.table, self.lengths, self.cu, self.start = table, lengths, cu, start
-        self.batch, self.max_seqlen, self.device = B, int(max_seqlen), device
-        self._block = PagedBatchBlock(table.data_ptr(), _ints(lengths, "lengths", B, device), at_cu,
-                                      None if start is None else _ints(start, "start", B, device), B, width, stride[0],
+        self.batch, self.max_seqlen, self.device, self._index = B, int(max_seqlen), device, index
+        self._block = PagedBatchBlock(table.data_ptr(), _ints(lengths, "lengths", B, index), at_cu,
+                                      None if start is None else _ints(start, "start", B, index), B, width, stride[0],
                                       self.max_seqlen)
         self._ref = ctypes.byref(self._block)
 
@@ -109,7 +109,7 @@ def _tokens(t: torch.Tensor, name: str, kv: PagedKV):
     """(t, its shape, its strides) of a [T, heads, D] tensor that fits the pages; a copy where its rows do
     not begin at multiples of 16 bytes."""
     shape = t.shape
-    if len(shape) != 3 or shape[2] != kv.head_dim or t.dtype is not kv.dtype or t.device != kv.device:
+    if len(shape) != 3 or shape[2] != kv.head_dim or t.dtype is not kv.dtype or t.get_device() != kv._index:
         raise ValueError(f"{name} must be [tokens, heads, {kv.head_dim}] {kv.dtype} on {kv.device}, got "
                          f"{list(shape)} {t.dtype} on {t.device}")
     s = t.stride()
@@ -122,13 +122,13 @@ def _tokens(t: torch.Tensor, name: str, kv: PagedKV):
 def _output(out: Optional[torch.Tensor], q: torch.Tensor, shape, name: str) -> torch.Tensor:
     if out is None:
         return q.new_empty(shape)
-    if out.shape != shape or out.dtype is not q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() & 15:
+    if out.shape != shape or out.dtype is not q.dtype or out.get_device() != q.get_device() or out.stride(2) != 1 or out.data_ptr() & 15:
         raise ValueError(f"{name} must have q's shape, type and device, a contiguous head dimension and 16-byte alignment")
     return out
 
 
 def _batch(batch: PagedBatch, kv: PagedKV, T: int) -> None:
-    if batch.device != kv.device:
+    if batch._index != kv._index:
         raise ValueError(f"the batch is on {batch.device}, the pages on {kv.device}")
     if batch.cu is None and batch.batch > T:
         raise ValueError(f"{T} tokens for {batch.batch} sequences of one each")
@@ -168,8 +168,8 @@ def append_paged(kv: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Tenso
         raise ValueError("cos and sin come together")
     if cos is not None:
         table, s = cos.shape, cos.stride()
-        if len(table) != 2 or sin.shape != table or sin.dtype is not cos.dtype or cos.device != kv.device \
-                or sin.device != kv.device or s[1] != 1 or sin.stride() != s:
+        if len(table) != 2 or sin.shape != table or sin.dtype is not cos.dtype or cos.get_device() != kv._index \
+                or sin.get_device() != kv._index or s[1] != 1 or sin.stride() != s:
             raise ValueError("cos and sin must be [rows, R / 2] of one shape, type and stride on the pages' device")
         rows, rot, s_rot = table[0], 2 * table[1], s[0]
         if cos.dtype is torch.float32:
@@ -227,6 +227,6 @@ def shared_prefix_attention(q: torch.Tensor, kv: PagedKV, batch: PagedBatch, pre
     The prefix's keys and values are read once for the group, not once for each sequence."""
     if prefix.cu is None:
         raise ValueError("prefix needs cu_seqlens: which of q's tokens belong to which group")
-    if prefix.device != kv.device:
+    if prefix._index != kv._index:
         raise ValueError(f"the prefix is on {prefix.device}, the pages on {kv.device}")
     return _attention(q, kv, batch, prefix, scale, out)
