@@ -94,14 +94,15 @@ static bool stream_whole(int64_t items, int keys) {
 
 // Rows of a head that a workgroup of the row kernels takes, and into how many runs it cuts the keys:
 // the least of an estimate.  A run's time is its 32-key tiles times a tile's (us, measured with up to
-// one workgroup a CU and with two); parts cost their writing and reading, 3.5 TB/s, and a launch.
+// one workgroup a CU and with two), and 3 us to begin and end; parts cost their writing and reading, 3.5 TB/s,
+// and a launch.
 // `paired`: a CU's other workgroup is the stream's.  512 tokens of 32 heads after 5000: narrow 1 part 141 us, 4 parts 72, 8 82, wide 8 75; 2048 after 30011:
 // narrow 998, wide 1204, 2 parts 903, 4 924; 512 at a sequence's start: 1 part 21, 2 31.
 static void shape_rows(PagedAttnArgs& a, int list, bool& wide, bool paired, int dtype) {
   const PageBatch& s = list ? a.seq : a.prefix;
   const RowsShape shape = paged_rows_shape(dtype);
   const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = (paired ? 1.0 : 2.0) * cu_count();
-  const int tiles = (s.max_keys + 31) / 32;
+  const int tiles = (s.max_keys + 31) / 32, dims = (a.D + 31) / 32;
   double best = 0.0;
   const int64_t most = (int64_t)s.max_len * a.G, others = s.B - 1, rest = s.T - s.max_len;
   for (int w = 0; w < (shape.wide > shape.narrow && most > shape.narrow ? 2 : 1); ++w) {
@@ -116,8 +117,9 @@ static void shape_rows(PagedAttnArgs& a, int list, bool& wide, bool paired, int 
       if (n > 1 && n > tiles) break;
       const double all = (double)items * n, rounds = all <= slots ? 1.0 : all / slots + 0.3;
       const bool two = !paired && 2 * all > slots;
-      const double tile = dtype == DA_F32 ? (two ? 1.75 : 0.9) * ((a.D + 31) / 32) / 4 : w ? (two ? 1.75 : 1.22) : (two ? 1.0 : 0.78);
-      const double time = rounds * ((tiles + n - 1) / n) * tile + (n > 1 || a.prefix.B ? n * part + (n > 1 ? 5 : 0) : 0.0);
+      const double tile = dtype == DA_F32 ? (two ? 0.4 + 0.75 * dims : 0.25 + 0.39 * dims)
+                                          : w ? (two ? 1.75 : 1.22) : (two ? 1.0 : 0.78);
+      const double time = rounds * ((tiles + n - 1) / n * tile + 3.0) + (n > 1 || a.prefix.B ? n * part + (n > 1 ? 5 : 0) : 0.0);
       if ((w == 0 && n == 1) || time < best) best = time, wide = w, a.splits[list] = n;
     }
   }
