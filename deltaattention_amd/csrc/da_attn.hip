@@ -299,9 +299,11 @@ __device__ __forceinline__ void paged_item_at(const PagedRowsArgs& a, int wg, in
 // head) over 128 NCB / hpw rows.  Ends with every LDS read of the window loop done (its last
 // barrier) and every load landed; the finalize uses only the wave's own Q region, so the next
 // item may start staging at once.
-template <int VARIANT, int DT, int NCB, bool LAZY, class Args>
+// DIM: head dimensions that the products cover (64 for kPaged with no more than that).
+template <int VARIANT, int DT, int NCB, bool LAZY, int DIM, class Args>
 __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_split, const int rg_item) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int DB = DIM / 32;  // blocks of 32 dims
   char* const kst0 = smem;
   char* const vst0 = smem + 2 * kWKBytes;
   char* const meta0 = smem + 2 * (kWKBytes + kWVBytes);
@@ -561,11 +563,11 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   int v_lane = (4 * ((lane >> 4) >> 1) + ((lane & 15) >> 2)) * 256 +
                ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + 8 * (lane & 1) + 64 * ((lane & 15) >> 2);
 
-  f32x16 o[NCB][4];
+  f32x16 o[NCB][DB];
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[cb][i] = f32x16{};
+    for (int i = 0; i < DB; ++i) o[cb][i] = f32x16{};
   f32x16 s[NCB];
   u32x4 pw[NCB][2];
   // mc: the running maximum times c, the reference point of p = 2^(s c - mc).  Until a
@@ -599,17 +601,17 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   }
   // ---- Q^T of both column blocks in registers, loaded while the first tiles are in
   // flight; rows past Nq load row Nq - 1 and dims past D dims 0..7, zeroed after ----
-  u32x4 qreg[kD / 16];
+  u32x4 qreg[DIM / 16];
   {
     // both column blocks requested before either is used: one round trip, not two
-    u32x4 w[NCB][kD / 16];
+    u32x4 w[NCB][DIM / 16];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
       const int row = r0w + 32 * cb + ql;
       const uint16_t* qrow = a.q + a.seq.base(b, a.sq_b, a.sq_n) + (int64_t)h * a.sq_h + (int64_t)min(row, Nq - 1) * a.sq_n;
       if constexpr (VARIANT == kPaged) qrow = a.q + a.seq.base(b, a.sq_b, a.sq_n) + place(min(row, Nq - 1), a.sq_h, a.sq_n);
 #pragma unroll
-      for (int t = 0; t < kD / 16; ++t) {
+      for (int t = 0; t < DIM / 16; ++t) {
         const int d0 = 16 * t + 8 * hl;
         w[cb][t] = *(const u32x4*)(qrow + (d0 < a.D ? d0 : 0));
       }
@@ -620,7 +622,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     for (int cb = 0; cb < NCB; ++cb) {
       const int row = r0w + 32 * cb + ql;
 #pragma unroll
-      for (int t = 0; t < kD / 16; ++t) {
+      for (int t = 0; t < DIM / 16; ++t) {
         asm volatile("" : "+v"(w[cb][t]));
         const u32x4 qv = (row < Nq && 16 * t + 8 * hl < a.D) ? w[cb][t] : u32x4{0, 0, 0, 0};
         if (cb == 0)
@@ -648,7 +650,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   auto matrix_block = [&](const int t, auto PVC, auto QKC) __attribute__((always_inline)) {
     constexpr bool PV = decltype(PVC)::value, QK = decltype(QKC)::value;
     constexpr bool BIAS = QK && kWeights;
-    constexpr int NPV = PV ? 8 : 0, NQK = QK ? kD / 16 : 0;
+    constexpr int NPV = PV ? 2 * DB : 0, NQK = QK ? DIM / 16 : 0;
     constexpr int EBIAS = NPV;                   // stream index of the bias reads
     constexpr int EQK = NPV + (BIAS ? 1 : 0);    // stream index of (K, Q) pair 0
     constexpr int E = EQK + NQK;                 // stream length
@@ -676,7 +678,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
       asm volatile("" : "+v"(v_lane));
       const uint32_t vl = vb + v_lane;
 #pragma unroll
-      for (int db = 0; db < 4; ++db) va[db] = vl ^ (64u * db);
+      for (int db = 0; db < DB; ++db) va[db] = vl ^ (64u * db);
     }
     uint32_t kla = 0, qla = 0, bla = 0;
     if constexpr (QK) {
@@ -685,13 +687,13 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
       if constexpr (NCB == 2) qla = lds_addr(qs) + k_lane;
       bla = lds_addr(meta_of(t) + kWCnt) + 16 * hl;
     }
-    i16x4 vlo[8], vhi[8];
-    u32x4 kw[kD / 16], qw[NCB == 2 ? kD / 16 : 1], bw[4];
+    i16x4 vlo[2 * DB], vhi[2 * DB];
+    u32x4 kw[DIM / 16], qw[NCB == 2 ? DIM / 16 : 1], bw[4];
     auto read = [&](auto EC) {
       constexpr int e = decltype(EC)::value;
       if constexpr (e < NPV) {
-        vlo[e] = ds_read_tr16<(e >> 2) * 4096>(va[e & 3]);
-        vhi[e] = ds_read_tr16<(e >> 2) * 4096 + 2048>(va[e & 3]);
+        vlo[e] = ds_read_tr16<(e / DB) * 4096>(va[e % DB]);
+        vhi[e] = ds_read_tr16<(e / DB) * 4096 + 2048>(va[e % DB]);
       } else if constexpr (BIAS && e == EBIAS) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) bw[r] = ds_read_b128_asm(bla + 32 * r);
@@ -707,8 +709,8 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
       if constexpr (i < NPV) {
         lgkm_wait<pending(i)>(vlo[i], vhi[i]);
         const u32x4 vw = __builtin_bit_cast(u32x4, __builtin_shufflevector(vlo[i], vhi[i], 0, 1, 2, 3, 4, 5, 6, 7));
-        o[0][i & 3] = E16<DT>::mfma(vw, pw[0][i >> 2], o[0][i & 3]);
-        if constexpr (NCB == 2) o[1][i & 3] = E16<DT>::mfma(vw, pw[1][i >> 2], o[1][i & 3]);
+        o[0][i % DB] = E16<DT>::mfma(vw, pw[0][i / DB], o[0][i % DB]);
+        if constexpr (NCB == 2) o[1][i % DB] = E16<DT>::mfma(vw, pw[1][i / DB], o[1][i % DB]);
       } else {
         constexpr int j = i - NPV;
         if constexpr (NCB == 2) lgkm_wait<pending(i)>(kw[j], qw[j]);
@@ -787,7 +789,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
         const float alpha = upd ? exp2_fast(mc[cb] - m_new) : 1.0f;
         if (LAZY || __builtin_amdgcn_ballot_w64(upd)) {
 #pragma unroll
-          for (int db = 0; db < 4; ++db)
+          for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[cb][db][r] *= alpha;
         }
@@ -864,7 +866,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
         if (row < Nq) {
           float* st = a.parts + ((int64_t)split * a.list.T + a.list.first(b)) * a.Hq * kState + place(row, kState, (int64_t)a.Hq * kState);
 #pragma unroll
-          for (int db = 0; db < 4; ++db)
+          for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *(f32x4*)(st + 32 * db + 8 * j + 4 * hl) = f32x4{o[cb][db][4 * j], o[cb][db][4 * j + 1],
@@ -882,7 +884,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     else
       inv = 1.0f / l_tot;
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         u32x2 w;
@@ -928,7 +930,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
 // the others, so the XCDs, whose clocks differ by several per cent, finish together,
 // and no dispatch gap lies between two items on a CU.  Every counter only grows, so each
 // workgroup's loop ends after at most 8 empty takes; workgroups never wait on each other.
-template <int VARIANT, int DT, int NCB, bool LAZY, class Args = AttnArgs>
+template <int VARIANT, int DT, int NCB, bool LAZY, int DIM = kD, class Args = AttnArgs>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void attn_w64_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -995,9 +997,9 @@ void attn_w64_kernel(Args a) {
         (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(ap));
     const Args ai = *ap;
-    attn_w64_item<VARIANT, DT, NCB, LAZY>(ai, unit, rg);
+    attn_w64_item<VARIANT, DT, NCB, LAZY, DIM>(ai, unit, rg);
 #else
-    attn_w64_item<VARIANT, DT, NCB, LAZY>(a, unit, rg);
+    attn_w64_item<VARIANT, DT, NCB, LAZY, DIM>(a, unit, rg);
 #endif
   }
 }
@@ -1009,7 +1011,7 @@ struct PagedPairArgs {
   PagedRowsArgs r;
   int turn, items, row_turns, stream_turns;  // workgroups a turn; row groups; turns of either
 };
-template <int DT, int NCB>
+template <int DT, int NCB, int DIM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_pair_kernel(PagedPairArgs p) {
   const int j = blockIdx.x / p.turn, at = blockIdx.x - j * p.turn, n = p.row_turns + p.stream_turns;
@@ -1028,7 +1030,7 @@ void paged_pair_kernel(PagedPairArgs p) {
     const PagedRowsArgs r = ap->r;
     int unit, rg;
     paged_item_at(r, wg, unit, rg);
-    attn_w64_item<kPaged, DT, NCB, true>(r, unit, rg);
+    attn_w64_item<kPaged, DT, NCB, true, DIM>(r, unit, rg);
   } else {
     asm volatile("" : "+s"(ap));
     const PagedAttnArgs s = ap->s;
@@ -1467,6 +1469,8 @@ void attn_f32_kernel(Args a, int paired) {
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x16{};
   float m_i = -INFINITY, l_i = 0.0f;
+  // the hardware's 2^x is off by 1 ulp, and by the weights below 2^-126 that exp2f keeps; kPaged takes it
+  auto power = [](float x) { return VARIANT == kPaged ? exp2_fast(x) : exp2f(x); };
   float ring[FR::R][16];
 
   int t = wid;
@@ -1520,11 +1524,11 @@ void attn_f32_kernel(Args a, int paired) {
       }
     }
     const float mn = __builtin_fmaxf(m_i, halves_max(mt));
-    const float alpha = mn == -INFINITY ? 1.0f : exp2f(m_i - mn);
+    const float alpha = mn == -INFINITY ? 1.0f : power(m_i - mn);
     float ps = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[r] = mn == -INFINITY ? 0.0f : exp2f(s[r] - mn);
+      s[r] = mn == -INFINITY ? 0.0f : power(s[r] - mn);
       ps += s[r];
     }
     l_i = l_i * alpha + ps;
@@ -1564,7 +1568,7 @@ void attn_f32_kernel(Args a, int paired) {
   for (int w = 0; w < NW; ++w) M = __builtin_fmaxf(M, s_ml[w][0][lane]);
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    f[w] = M == -INFINITY ? 0.0f : exp2f(s_ml[w][0][lane] - M);
+    f[w] = M == -INFINITY ? 0.0f : power(s_ml[w][0][lane] - M);
     L += s_ml[w][1][lane] * f[w];
   }
   // a row without any key (pure Phase 1) stays zero, deltaFlashAttention.py:353-354
@@ -1696,23 +1700,31 @@ static int launch_attn_f32(const AttnArgs& a, hipStream_t st) {
 }
 
 // ---- paged batches (da_paged_attn.hip plans them) ----
-template <int DT, int NCB>
+template <int DT, int NCB, int DIM>
 static int launch_rows_t(const PagedRowsArgs& a, unsigned grid, hipStream_t st) {
   static bool done[kMaxDevices] = {};
-  if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>), kWLds, done)) return rc;
-  hipLaunchKernelGGL((attn_w64_kernel<kPaged, DT, NCB, true, PagedRowsArgs>), dim3(grid), dim3(256), kWLds, st, a);
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&attn_w64_kernel<kPaged, DT, NCB, true, DIM, PagedRowsArgs>), kWLds, done))
+    return rc;
+  hipLaunchKernelGGL((attn_w64_kernel<kPaged, DT, NCB, true, DIM, PagedRowsArgs>), dim3(grid), dim3(256), kWLds, st, a);
   return check_launch("paged attention (rows)");
 }
 
-template <int DT, int NCB>
+template <int DT, int NCB, int DIM>
 static int launch_pair_t(const PagedPairArgs& p, hipStream_t st) {
   constexpr int lds = kWLds > stream_lds(1) ? kWLds : stream_lds(1);
   static bool done[kMaxDevices] = {};
-  if (int rc = allow_lds(reinterpret_cast<const void*>(&paged_pair_kernel<DT, NCB>), lds, done)) return rc;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&paged_pair_kernel<DT, NCB, DIM>), lds, done)) return rc;
   const int64_t grid = (int64_t)p.turn * (p.row_turns + p.stream_turns);
   if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
-  hipLaunchKernelGGL((paged_pair_kernel<DT, NCB>), dim3((unsigned)grid), dim3(256), lds, st, p);
+  hipLaunchKernelGGL((paged_pair_kernel<DT, NCB, DIM>), dim3((unsigned)grid), dim3(256), lds, st, p);
   return check_launch("paged attention (rows and stream)");
+}
+
+// pair: with the stream, or null
+template <int DT, int NCB>
+static int launch_rows_dim(const PagedRowsArgs& a, unsigned grid, const PagedPairArgs* pair, hipStream_t st) {
+  if (a.D <= 64) return pair ? launch_pair_t<DT, NCB, 64>(*pair, st) : launch_rows_t<DT, NCB, 64>(a, grid, st);
+  return pair ? launch_pair_t<DT, NCB, kD>(*pair, st) : launch_rows_t<DT, NCB, kD>(a, grid, st);
 }
 
 template <int DB>
@@ -1769,14 +1781,11 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
     }
   }
   const unsigned n = (unsigned)grid;
-  if (with_stream) {
-    const int turn = cu_count() & ~7;  // XCD x has the workgroups x mod 8 of a turn
-    const PagedPairArgs pair = {p, a, turn, (int)grid, (int)((grid + turn - 1) / turn), (p.workers + turn - 1) / turn};
-    if (dtype == DA_F16) return wide ? launch_pair_t<DA_F16, 2>(pair, st) : launch_pair_t<DA_F16, 1>(pair, st);
-    return wide ? launch_pair_t<DA_BF16, 2>(pair, st) : launch_pair_t<DA_BF16, 1>(pair, st);
-  }
-  if (dtype == DA_F16) return wide ? launch_rows_t<DA_F16, 2>(a, n, st) : launch_rows_t<DA_F16, 1>(a, n, st);
-  return wide ? launch_rows_t<DA_BF16, 2>(a, n, st) : launch_rows_t<DA_BF16, 1>(a, n, st);
+  const int turn = cu_count() & ~7;  // XCD x has the workgroups x mod 8 of a turn
+  const PagedPairArgs both = {p, a, turn, (int)grid, (int)((grid + turn - 1) / turn), (p.workers + turn - 1) / turn};
+  const PagedPairArgs* pair = with_stream ? &both : nullptr;
+  if (dtype == DA_F16) return wide ? launch_rows_dim<DA_F16, 2>(a, n, pair, st) : launch_rows_dim<DA_F16, 1>(a, n, pair, st);
+  return wide ? launch_rows_dim<DA_BF16, 2>(a, n, pair, st) : launch_rows_dim<DA_BF16, 1>(a, n, pair, st);
 }
 
 static int launch_attn(int variant, int dtype, AttnArgs& a, hipStream_t st) {
