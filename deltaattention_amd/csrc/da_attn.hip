@@ -1715,7 +1715,7 @@ static int launch_pair_t(const PagedPairArgs& p, hipStream_t st) {
   static bool done[kMaxDevices] = {};
   if (int rc = allow_lds(reinterpret_cast<const void*>(&paged_pair_kernel<DT, NCB, DIM>), lds, done)) return rc;
   const int64_t grid = (int64_t)p.turn * (p.row_turns + p.stream_turns);
-  if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
+  if (grid >= (1ll << 24)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
   hipLaunchKernelGGL((paged_pair_kernel<DT, NCB, DIM>), dim3((unsigned)grid), dim3(256), lds, st, p);
   return check_launch("paged attention (rows and stream)");
 }
@@ -1771,7 +1771,7 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
   a.slots = 2 * cu_count() / 8;
   int64_t grid = (int64_t)a.units * a.n_row_groups;
   if (dtype != DA_F32) grid = (grid + 7) & ~7ll;  // paged_item_at turns within eights, group_at knows no more places
-  if (grid >= (1ll << 31)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
+  if (grid >= (1ll << 24)) return set_error(DA_ERR_INVALID, "paged attention: grid too large");
   if (dtype == DA_F32) {
     switch ((p.D + 31) / 32) {
       case 1: return launch_rows_f32<1>(a, (unsigned)grid, st);

@@ -48,7 +48,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
       if (tiles == 0) continue;
       const uint32_t per = a.whole ? 1 : a.begin[0];
       const uint32_t U = a.whole ? 0 : a.begin[1 + (list ? a.prefix.B : 0) + e] + g * tiles;
-      const uint32_t w0 = U / per, w1 = a.whole ? w0 : (U + tiles - 1) / per;
+      const uint32_t last = a.whole ? 0 : a.workers - 1;
+      const uint32_t w0 = min(U / per, last), w1 = min((U + tiles - 1) / per, last);
       if (w0 == w1) {
         if (a.prefix.B == 0) return;  // written where it was computed
         state = a.states + (((int64_t)list * a.seq.T + t) * a.Hq + h) * kState;
@@ -190,6 +191,7 @@ static int fill_attention(PagedAttnArgs& a, int dtype, int64_t T, int64_t Hq, in
   DA_REQUIRE(T > 0 && T < (1ll << 28) && Hq > 0 && Hkv > 0 && Hq < (1 << 16), "%s: empty shape", who);
   DA_REQUIRE(Hq % Hkv == 0, "%s: Hq (%lld) must be a multiple of Hkv (%lld)", who, (long long)Hq, (long long)Hkv);
   DA_REQUIRE(T * Hq < (1ll << 31), "%s: more than 2^31 rows", who);
+  DA_REQUIRE(T < (1ll << 24), "%s: more than 2^24 tokens", who);  // a launch has less than 2^32 threads
   if (int rc = fill_pages(a.pages, kv, D, who)) return rc;
   if (int rc = fill_batch(a.seq, batch, a.pages, T, who)) return rc;
   if (prefix) {

@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void paged_stream_join_kernel(PagedAttnArgs a)
     RowSum sum;
     sum.take(a.slots + ((int64_t)rec.slot * a.slot_rows + r) * kState, d);
     const float* next = a.slots + (2 * ((int64_t)blockIdx.x + 1) * a.slot_rows + r) * kState;
-    sum.take_all(next, 2 * (int64_t)a.slot_rows * kState, rec.others, d);
+    sum.take_all(next, 2 * (int64_t)a.slot_rows * kState, min(rec.others, a.workers - 1 - (int)blockIdx.x), d);
     sum.template store<DT>(a, rec.first + r / a.G, rec.head * a.G + r % a.G, d);
   }
 }

@@ -24,7 +24,7 @@ constexpr int kStreamEntries = 256;
 struct StreamShared {
   float ml[4][2][32];
   int first[kStreamEntries], tokens[kStreamEntries], keys[kStreamEntries];
-  uint32_t waves[4], total;
+  uint32_t waves[4];
   int entry;
   uint32_t offset;
   StreamRecord record;
@@ -148,7 +148,10 @@ __device__ __forceinline__ bool share_of(const PagedAttnArgs& a, const int worke
     before = workgroup_sum(mine, sh, sum);
   }
   if (u >= total) return false;
-  if (tid == 0) sh.record.others = 0;
+  if (tid == 0) {
+    sh.record.others = 0;
+    if (a.records) a.records[worker].others = 0;
+  }
   __syncthreads();
   share = Share{__builtin_amdgcn_readfirstlane(sh.entry), chunk, (uint32_t)__builtin_amdgcn_readfirstlane(sh.offset),
                 min(per, total - u), per};
@@ -198,13 +201,16 @@ __device__ __forceinline__ void stream_worker(const PagedAttnArgs& a, const int 
 
   while (left > 0) {
     const bool own = e >= a.prefix.B;
-    int f, nt, nk;
-    const int at = e - share.chunk;
-    if ((unsigned)at < kStreamEntries) f = sh.first[at], nt = sh.tokens[at], nk = sh.keys[at];
-    else entry_of(a, e, f, nt, nk);
-    f = __builtin_amdgcn_readfirstlane(f);
-    nt = __builtin_amdgcn_readfirstlane(nt);
-    nk = __builtin_amdgcn_readfirstlane(nk);
+    if (e >= a.prefix.B + a.seq.B) return;  // lengths that changed under the call
+    if ((unsigned)(e - share.chunk) >= kStreamEntries) {  // the next entries
+      share.chunk = e;
+      __syncthreads();
+      if (e + tid < a.prefix.B + a.seq.B) entry_of(a, e + tid, sh.first[tid], sh.tokens[tid], sh.keys[tid]);
+      __syncthreads();
+    }
+    const int f = __builtin_amdgcn_readfirstlane(sh.first[e - share.chunk]);
+    const int nt = __builtin_amdgcn_readfirstlane(sh.tokens[e - share.chunk]);
+    const int nk = __builtin_amdgcn_readfirstlane(sh.keys[e - share.chunk]);
     const int tiles = stream_tiles(a, nt, nk, own);
     if (tiles == 0) {
       ++e;
@@ -248,7 +254,7 @@ __device__ __forceinline__ void stream_worker(const PagedAttnArgs& a, const int 
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + 1024 * j), 16,
-                                                   isK ? (int)ko[j] : (int)vo, isK ? 0 : (int)(4 * j * svb), 0, 0);
+                                                   isK ? (int)ko[j] : (int)(vo + 4 * j * svb), 0, 0, 0);
       }
     };
 

@@ -144,7 +144,8 @@ def append_paged(kv: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Tenso
     D): row p is for position p, with ``per_token`` row t for token t.  Dims d and d + R / 2 (with
     ``interleaved`` 2 d and 2 d + 1) are a pair, turned in float32 and rounded once; dims from R on
     stay.  A position past the rows takes the last one.  Without cos and sin nothing is rotated.
-    Tokens past the batch's last and places past its table are not written.
+    Tokens past the batch's last and places past its table are not written; two tokens meant for one
+    place leave either of them there.
     """
     k, shape, sk = _tokens(k, "k", kv)
     v, of_v, sv = _tokens(v, "v", kv)

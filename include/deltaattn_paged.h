@@ -56,8 +56,8 @@ typedef struct DaPagedBatch {
  * d + rot / 2 (interleaved: 2 d and 2 d + 1), d < rot / 2, become x cos - y sin and y cos + x sin, in
  * fp32, rounded once; dims from rot on stay.  cos, sin [rows, rot / 2] fp32 or of the pages' type
  * (rot_dtype), rows s_rot apart (0: one row for all); row p is for position p, or with per_token for
- * token p (rows >= T).
- * A position outside the rows takes the nearest row.  rot = 0: no rotation.
+ * token p (rows >= T).  A position outside the rows takes the nearest row.  rot = 0: no rotation.
+ * Two tokens meant for one place (tables with a page in common) leave either of them there.
  */
 int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_t, int64_t sv_h,
                     const void* q, int64_t sq_t, int64_t sq_h, void* q_out, int64_t so_t, int64_t so_h, int dtype,
@@ -73,8 +73,9 @@ int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, in
  * before its own (prefix->start is not read, prefix->max_seqlen is the most tokens of a group).
  * q, out [T, Hq, D] (strides *_t, *_h; rows 16-byte aligned) of the pages' type; query head h reads
  * KV head h / (Hq / Hkv).  A query that sees no key gives zeros.  Scores, maxima, sums and partial
- * results are fp32.  Deterministic.  workspace: da_paged_attention_workspace_size() bytes of the
- * same arguments (none, and null, where it returns 0), 256-byte aligned.
+ * results are fp32.  Deterministic.  T is less than 2^24.  What batch and prefix point to must not
+ * change while the call runs.  workspace: da_paged_attention_workspace_size() bytes of the same
+ * arguments (none, and null, where it returns 0), 256-byte aligned.
  */
 int64_t da_paged_attention_workspace_size(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                           const DaPagedKV* kv, const DaPagedBatch* batch,

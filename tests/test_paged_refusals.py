@@ -93,6 +93,7 @@ def test_attention_refuses():
     _refused(_attend(out=None), -1, "null")
     _refused(_attend(Hq=3), -1, "multiple of Hkv")
     _refused(_attend(T=1 << 27, Hq=32, Hkv=8), -1, "2^31 rows")
+    _refused(_attend(T=1 << 24, Hq=32, Hkv=8), -1, "2^24 tokens")
     _refused(_attend(scale=0.0), -1, "scale")
     _refused(_attend(prefix=_batch(cu=None, B=3)), -1, "cu")
     _refused(_attend(prefix=_batch(width=0)), -1, "empty")
