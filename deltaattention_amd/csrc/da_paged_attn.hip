@@ -95,14 +95,17 @@ static bool stream_whole(int64_t items, int keys) {
 
 // Rows of a head that a workgroup of the row kernels takes, and into how many runs it cuts the keys:
 // the least of an estimate.  A run's time is its 32-key tiles times a tile's (us, measured with up to
-// one workgroup a CU and with two), and 3 us to begin and end; parts cost their writing and reading, 3.5 TB/s,
-// and a launch.
-// `paired`: a CU's other workgroup is the stream's.  512 tokens of 32 heads after 5000: narrow 1 part 141 us, 4 parts 72, 8 82, wide 8 75; 2048 after 30011:
-// narrow 998, wide 1204, 2 parts 903, 4 924; 512 at a sequence's start: 1 part 21, 2 31.
+// one workgroup a CU and with two), and 3 us to begin and end; parts cost their writing and reading,
+// 3.5 TB/s, and a launch.  512 tokens of 32 heads after 5000: narrow 1 part 141 us, 4 parts 72, 8 82, wide 8 75;
+// 2048 after 30011: narrow 998, wide 1204, 2 parts 903, 4 924; 512 at a sequence's start: 1 part 21, 2 31.
+// `paired`: beside the stream, whose loads slow a tile and the parts' writing (1.5 TB/s).  Over 188 batches
+// (16 to 300 sequences of 60 to 3000 keys behind 700 to 100000, five sets of heads) the choice costs 2%
+// more than the best, 17% at most: 130 sequences of 60 keys behind 100000, 64 heads: narrow 6 parts 523 us,
+// wide 24 473, wide 6 672.
 static void shape_rows(PagedAttnArgs& a, int list, bool& wide, bool paired, int dtype) {
   const PageBatch& s = list ? a.seq : a.prefix;
   const RowsShape shape = paged_rows_shape(dtype);
-  const double part = (double)s.T * a.Hq * kState * 8 / 3.5e6, slots = (paired ? 1.0 : 2.0) * cu_count();
+  const double part = (double)s.T * a.Hq * kState * 8 / (paired ? 1.5e6 : 3.5e6), slots = 2.0 * cu_count();
   const int tiles = (s.max_keys + 31) / 32, dims = (a.D + 31) / 32;
   double best = 0.0;
   const int64_t most = (int64_t)s.max_len * a.G, others = s.B - 1, rest = s.T - s.max_len;
@@ -117,9 +120,10 @@ static void shape_rows(PagedAttnArgs& a, int list, bool& wide, bool paired, int 
     for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (n > 1 && n > tiles) break;
       const double all = (double)items * n, rounds = all <= slots ? 1.0 : all / slots + 0.3;
-      const bool two = !paired && 2 * all > slots;
+      const bool two = 2 * all > slots;
       const double tile = dtype == DA_F32 ? (two ? 0.4 + 0.75 * dims : 0.25 + 0.39 * dims)
-                                          : w ? (two ? 1.75 : 1.22) : (two ? 1.0 : 0.78);
+                          : paired         ? (w ? 1.2 : 0.9) * (two ? 1.5 : 1.0)
+                                           : w ? (two ? 1.75 : 1.22) : (two ? 1.0 : 0.78);
       const double time = rounds * ((tiles + n - 1) / n * tile + 3.0) + (n > 1 || a.prefix.B ? n * part + (n > 1 ? 5 : 0) : 0.0);
       if ((w == 0 && n == 1) || time < best) best = time, wide = w, a.splits[list] = n;
     }
