@@ -1761,11 +1761,12 @@ int launch_paged_rows(const PagedAttnArgs& p, const PageBatch& list, bool own, b
   // 4.2 / 7.7 ms, 8 KV heads 15.1 / 13.8
   a.spread = (p.Hkv & 7) != 0;
   const int rows = wide ? shape.wide : shape.narrow;
-  // the places of group_at; ranked where that leaves at most half of them empty (6 prompts of 1250 to 3001
-  // tokens, 4 KV heads, 237 us against 250) and no XCD has units of its own, which want a sequence at a time
+  // the places of group_at; ranked where that needs no more of them, for one empty place among few can
+  // leave a CU without its second workgroup (256 tokens of 16 heads after 60000, 16 runs: 171 us, with an empty
+  // place a unit 238); or where it leaves at most half of them empty (6 prompts of 1250 to 3001 tokens, 4 KV
+  // heads, 237 us against 250) and no XCD has units of its own, which want a sequence at a time
   const int64_t places = (int64_t)list.T * p.G / rows + list.B, most = ((int64_t)list.max_len * p.G + rows - 1) / rows;
-  // (or where it needs no more places)
-  a.ranked = list.B > 1 && most * list.B <= ((p.Hkv & 7) != 0 ? 2 : 1) * places ? (int)most : 0;
+  a.ranked = most * list.B <= ((p.Hkv & 7) != 0 ? 2 : 1) * places ? (int)most : 0;
   a.n_row_groups = (int)(a.ranked ? most * list.B : places);
   a.units = p.Hkv * splits;
   a.slots = 2 * cu_count() / 8;
