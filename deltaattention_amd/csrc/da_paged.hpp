@@ -43,7 +43,8 @@ struct PageBatch {
 };
 
 // The sequence of token t, for a whole wave (t uniform): the last b with cu[b] <= t, -1 for a token
-// before cu[0] or from cu[B] on.  Each round a wave looks at 64 places of the range that is left.
+// before cu[0] or from cu[B] on.  Each round a wave looks at 64 places of the range that is left.  Of a cu that
+// does not rise it may be another one or -1, but never one that begins after t.
 __device__ __forceinline__ int sequence_of(const PageBatch& s, int t, int lane) {
   if (!s.cu) return t < s.B ? t : -1;
   int lo = 0, n = s.B + 1;  // cu[lo .. lo + n) holds the border
@@ -51,10 +52,11 @@ __device__ __forceinline__ int sequence_of(const PageBatch& s, int t, int lane) 
     const int step = (n + 63) >> 6;
     const int i = lo + lane * step;
     const bool before = lane * step < n && s.cu[i] <= t;
-    const int c = __popcll(__ballot(before));
+    const uint64_t all = __ballot(before);
+    const int c = __popcll(all);
     if (c == 0) return -1;
     const int at = lo + (c - 1) * step;
-    if (step == 1) return at < s.B ? at : -1;
+    if (step == 1) return at < s.B && (all >> (c - 1) & 1) ? at : -1;
     n = min(step, lo + n - at);
     lo = at;
   }
