@@ -93,14 +93,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   if (t >= a.seq.T) return;
   const int b = sequence_of(a.seq, t, lane);
   if (b < 0) return;
-  const int n = a.seq.tokens(b), i = t - a.seq.first(b);
-  if (i >= n) return;
-  // the token's place, and the row of cos and sin
-  const int slot = a.seq.keys(b) - n + i;
-  int64_t row = a.per_token ? t : (int64_t)slot + (a.seq.start ? a.seq.start[b] : 0);
+  if (a.seq.cu && t >= a.seq.cu[b + 1]) return;
+  // the token's place (max_seqlen does not move it), and the row of cos and sin
+  const int64_t slot = a.seq.slot(b, t);
+  int64_t row = a.per_token ? t : slot + (a.seq.start ? a.seq.start[b] : 0);
   row = row < 0 ? 0 : row >= a.rows ? a.rows - 1 : row;
   int page = -1;
-  if (slot >= 0) page = a.seq.table[(int64_t)b * a.seq.table_stride + (slot >> a.pages.shift)];
+  if (slot >= 0 && slot < a.seq.max_keys) page = a.seq.table[(int64_t)b * a.seq.table_stride + (slot >> a.pages.shift)];
   const bool kept = page >= 0 && page < a.pages.num_pages;
   const int64_t in = slot & ((1 << a.pages.shift) - 1);
   char* const kd = const_cast<char*>(a.pages.k) + ES * (page * a.pages.sk_p + in * a.pages.sk_n);

@@ -14,7 +14,8 @@ struct Pages {
   int num_pages, shift;  // page size 1 << shift
 };
 
-// The sequences of a call; everything read from memory is clamped to what the tensors hold.
+// The sequences of a call; everything read from memory is clamped to what the tensors hold, but for the slot
+// of a token, which is what lengths and cu say, in the table or not.
 struct PageBatch {
   const int32_t* table;
   const int32_t* lengths;
@@ -39,6 +40,10 @@ struct PageBatch {
   __device__ __forceinline__ int keys(int b) const {
     const int n = lengths[b];
     return n < 0 ? 0 : (n > max_keys ? max_keys : n);
+  }
+  // the slot of token t of sequence b: its new tokens are the last of all it has
+  __device__ __forceinline__ int64_t slot(int b, int t) const {
+    return (int64_t)lengths[b] + t - (cu ? (int64_t)cu[b + 1] : b + 1);
   }
 };
 

@@ -143,9 +143,9 @@ def append_paged(kv: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Tenso
     cos, sin [rows, R / 2] (float32 or the pages' type, contiguous along R / 2; R a multiple of 4 up to
     D): row p is for position p, with ``per_token`` row t for token t.  Dims d and d + R / 2 (with
     ``interleaved`` 2 d and 2 d + 1) are a pair, turned in float32 and rounded once; dims from R on
-    stay.  A position past the rows takes the last one.  Without cos and sin nothing is rotated.
-    Tokens past the batch's last and places past its table are not written; two tokens meant for one
-    place leave either of them there.
+    stay.  A position outside the rows takes the nearest one.  Without cos and sin nothing is rotated.
+    Tokens past the batch's last are left alone, and a token whose place is not in the table is not written
+    (its query is rotated); two tokens meant for one place leave either of them there.
     """
     k, shape, sk = _tokens(k, "k", kv)
     v, of_v, sv = _tokens(v, "v", kv)

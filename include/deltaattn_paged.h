@@ -34,12 +34,14 @@ typedef struct DaPagedKV {
  * The sequences of a call.  Sequence b has lengths[b] tokens in its pages (those that this call
  * brings included, and last), token j in row j % page_size of page table[b][j / page_size].  It
  * brings the tokens cu[b] .. cu[b + 1] - 1 of q, k, v [T, heads, D] (null cu: token b alone), of which
- * no sequence has more than max_seqlen.  The position of token j is start[b] + j (null: j).
+ * no sequence has more than max_seqlen (which the append does not read).  Token t is its token
+ * j = lengths[b] - cu[b + 1] + t, whose position is start[b] + j (null: j).
  * Rows past cu[B] are left as they are.  What the arrays hold is clamped on the device: cu into
  * [0, T] and to max_seqlen tokens, lengths into [0, width * page_size]; a page outside
  * [0, num_pages) is never touched (its tokens' keys and values count as zeros, a token meant for
- * it is not written).  A token whose sequence is shorter than what it brings (its place would be
- * before row 0) is not written and attends to nothing.
+ * it is not written).  A token whose place j is not in the table (before row 0, as in a sequence that
+ * is shorter than what it brings, or from width * page_size on) is not written; before row 0 it attends
+ * to nothing.  With a cu that does not rise no row outside the batch is touched.
  */
 typedef struct DaPagedBatch {
   const int32_t* table; /* [B, width], rows table_stride apart */
