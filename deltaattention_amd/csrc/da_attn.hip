@@ -341,7 +341,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
   if constexpr (VARIANT == kPaged) {
     Nq = a.list.tokens(b) * a.G;
     Nk = a.list.keys(b);
-    off = a.causal ? Nk - a.list.tokens(b) : 0;
+    off = a.causal ? a.list.before(b) : 0;
     if (Nq <= a.short_rows) return;
   } else {
     Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
@@ -1290,7 +1290,7 @@ void attn_f32_kernel(Args a, int paired) {
   if constexpr (VARIANT == kPaged) {
     Nq = a.list.tokens(b);
     Nk = a.list.keys(b);
-    off = a.causal ? Nk - Nq : 0;
+    off = a.causal ? a.list.before(b) : 0;
   } else {
     Nq = a.seq.cu ? a.seq.len(b) : a.Nq;
     Nk = a.seq.cu ? a.seq.len(b) : a.Nk;

@@ -45,6 +45,11 @@ struct PageBatch {
   __device__ __forceinline__ int64_t slot(int b, int t) const {
     return (int64_t)lengths[b] + t - (cu ? (int64_t)cu[b + 1] : b + 1);
   }
+  // that of its first token, within 2^30 to either side, which is farther than any key
+  __device__ __forceinline__ int before(int b) const {
+    const int64_t n = slot(b, first(b));
+    return n < -(1 << 30) ? -(1 << 30) : n > (1 << 30) ? 1 << 30 : (int)n;
+  }
 };
 
 // The sequence of token t, for a whole wave (t uniform): the last b with cu[b] <= t, -1 for a token

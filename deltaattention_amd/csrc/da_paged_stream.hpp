@@ -23,7 +23,7 @@ constexpr int kStageLds = 16384;  // a wave's K and V tiles; its rows' sums at t
 constexpr int kStreamEntries = 256;
 struct StreamShared {
   float ml[4][2][32];
-  int first[kStreamEntries], tokens[kStreamEntries], keys[kStreamEntries];
+  int first[kStreamEntries], tokens[kStreamEntries], keys[kStreamEntries], before[kStreamEntries];
   uint32_t waves[4];
   int entry;
   uint32_t offset;
@@ -65,14 +65,15 @@ __device__ __forceinline__ void read_values(u32x4 (&v)[4], uint32_t a) {
     v[i] = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// tokens, keys and first token of list entry e: the prefix's groups, then the sequences
-__device__ __forceinline__ void entry_of(const PagedAttnArgs& a, int e, int& first, int& tokens, int& keys) {
+// first token, tokens, keys and the first token's slot of list entry e: the prefix's groups, then the sequences
+__device__ __forceinline__ void entry_of(const PagedAttnArgs& a, int e, int& first, int& tokens, int& keys, int& before) {
   const bool own = e >= a.prefix.B;
   const PageBatch s = list_of(a, own);
   const int b = own ? e - a.prefix.B : e;
   first = s.first(b);
   tokens = s.tokens(b);
   keys = s.keys(b);
+  before = s.before(b);
 }
 
 // Exclusive sum over the workgroup's threads; all threads get the total too.
@@ -103,30 +104,30 @@ struct Share {
 // is its head, tiles 1).
 __device__ __forceinline__ bool share_of(const PagedAttnArgs& a, const int worker, StreamShared& sh, Share& share) {
   const int tid = threadIdx.x, E = a.prefix.B + a.seq.B;
-  int first = 0, tokens = 0, keys = 0;
+  int first = 0, tokens = 0, keys = 0, at = 0;
   if (a.whole) {
     const int e = worker / a.Hkv;
-    entry_of(a, e, first, tokens, keys);
+    entry_of(a, e, first, tokens, keys, at);
     if (stream_tiles(a, tokens, keys, e >= a.prefix.B) == 0) return false;
-    if (tid == 0) sh.first[0] = first, sh.tokens[0] = tokens, sh.keys[0] = keys;
+    if (tid == 0) sh.first[0] = first, sh.tokens[0] = tokens, sh.keys[0] = keys, sh.before[0] = at;
     __syncthreads();
     share = Share{e, e, (uint32_t)(worker - e * a.Hkv), 1, 1};
     return true;
   }
   // the entries' tiles summed in order, 256 entries at a time
   auto tiles_of = [&](int i) { return (uint32_t)stream_tiles(a, tokens, keys, i >= a.prefix.B) * (uint32_t)a.Hkv; };
-  if (tid < E) entry_of(a, tid, first, tokens, keys);
+  if (tid < E) entry_of(a, tid, first, tokens, keys, at);
   uint32_t mine = tiles_of(tid), sum, rest = 0;
   uint32_t before = workgroup_sum(mine, sh, sum);
   if (E > kStreamEntries) {
-    const int f = first, t = tokens, k = keys;
+    const int f = first, t = tokens, k = keys, s = at;
     uint32_t x = 0;
     for (int i = tid + kStreamEntries; i < E; i += kStreamEntries) {
-      entry_of(a, i, first, tokens, keys);
+      entry_of(a, i, first, tokens, keys, at);
       x += tiles_of(i);
     }
     workgroup_sum(x, sh, rest);
-    first = f, tokens = t, keys = k;
+    first = f, tokens = t, keys = k, at = s;
   }
   const uint32_t total = sum + rest;
   const uint32_t per = max((total + a.workers - 1) / a.workers, 1u);
@@ -135,7 +136,7 @@ __device__ __forceinline__ bool share_of(const PagedAttnArgs& a, const int worke
   int chunk = 0;
   for (uint32_t base = 0;;) {
     const int i = chunk + tid;
-    sh.first[tid] = first, sh.tokens[tid] = tokens, sh.keys[tid] = keys;
+    sh.first[tid] = first, sh.tokens[tid] = tokens, sh.keys[tid] = keys, sh.before[tid] = at;
     if (worker == 0 && i < E) a.begin[1 + i] = base + before;
     if (u >= base + before && u < base + before + mine) sh.entry = i, sh.offset = u - base - before;
     base += sum;
@@ -143,7 +144,7 @@ __device__ __forceinline__ bool share_of(const PagedAttnArgs& a, const int worke
     if ((worker != 0 && (u < base || u >= total)) || chunk + kStreamEntries >= E) break;
     chunk += kStreamEntries;
     first = tokens = keys = 0;
-    if (chunk + tid < E) entry_of(a, chunk + tid, first, tokens, keys);
+    if (chunk + tid < E) entry_of(a, chunk + tid, first, tokens, keys, at);
     mine = tiles_of(chunk + tid);
     before = workgroup_sum(mine, sh, sum);
   }
@@ -205,12 +206,13 @@ __device__ __forceinline__ void stream_worker(const PagedAttnArgs& a, const int 
     if ((unsigned)(e - share.chunk) >= kStreamEntries) {  // the next entries
       share.chunk = e;
       __syncthreads();
-      if (e + tid < a.prefix.B + a.seq.B) entry_of(a, e + tid, sh.first[tid], sh.tokens[tid], sh.keys[tid]);
+      if (e + tid < a.prefix.B + a.seq.B) entry_of(a, e + tid, sh.first[tid], sh.tokens[tid], sh.keys[tid], sh.before[tid]);
       __syncthreads();
     }
     const int f = __builtin_amdgcn_readfirstlane(sh.first[e - share.chunk]);
     const int nt = __builtin_amdgcn_readfirstlane(sh.tokens[e - share.chunk]);
     const int nk = __builtin_amdgcn_readfirstlane(sh.keys[e - share.chunk]);
+    const int before = __builtin_amdgcn_readfirstlane(sh.before[e - share.chunk]);
     const int tiles = stream_tiles(a, nt, nk, own);
     if (tiles == 0) {
       ++e;
@@ -220,10 +222,10 @@ __device__ __forceinline__ void stream_worker(const PagedAttnArgs& a, const int 
     const int t0 = a.whole ? 0 : off - h * tiles;
     const int n = a.whole ? tiles : min((uint32_t)(tiles - t0), left);
     const int rows = nt * a.G;
-    // keys that row ql sees; row 0 sees the fewest
+    // keys that row ql sees, of those that are there; row 0 sees the fewest
     const int tok = ql / a.G;
-    const int seen = own ? nk - nt + 1 + tok : nk;
-    const int least = own ? nk - nt + 1 : nk;
+    const int seen = own ? min(nk, before + 1 + tok) : nk;
+    const int least = own ? min(nk, before + 1) : nk;
 
     // ---- this wave's tiles: 32 keys from 128 t + 32 wid on, while there are any ----
     const int key_first = t0 * kStreamTile + 32 * wid;

@@ -215,7 +215,8 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: PagedBatch, scale: Opti
     in the pages): query token i of the n that sequence b brings sees the keys of slots 0 ..
     lengths[b] - n + i.  One token a sequence is a decode step; many are a prompt, or the next part of one;
     both may come in one batch.  Query head h reads KV head h // (Hq // Hkv).  A query without any key
-    gives zeros; rows of tokens past the batch's last are left as ``out`` has them."""
+    gives zeros; rows of tokens past the batch's last, or past a sequence's ``max_seqlen``, are left as
+    ``out`` has them."""
     return _attention(q, kv, batch, None, scale, out)
 
 

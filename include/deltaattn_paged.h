@@ -40,8 +40,9 @@ typedef struct DaPagedKV {
  * [0, T] and to max_seqlen tokens, lengths into [0, width * page_size]; a page outside
  * [0, num_pages) is never touched (its tokens' keys and values count as zeros, a token meant for
  * it is not written).  A token whose place j is not in the table (before row 0, as in a sequence that
- * is shorter than what it brings, or from width * page_size on) is not written; before row 0 it attends
- * to nothing.  With a cu that does not rise no row outside the batch is touched.
+ * is shorter than what it brings, or from width * page_size on) is not written, and attends to the
+ * places before its own that are there.  Attention leaves the tokens of a sequence past max_seqlen as they
+ * are.  With a cu that does not rise no row outside the batch is touched.
  */
 typedef struct DaPagedBatch {
   const int32_t* table; /* [B, width], rows table_stride apart */
@@ -68,8 +69,8 @@ int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, in
                     const DaPagedBatch* batch, void* stream);
 
 /*
- * Attention of the new tokens, which are in their pages already: query token i of n of sequence b
- * over the keys 0 .. lengths[b] - n + i of its sequence.  With `prefix`, the batch's tokens are cut
+ * Attention of the new tokens, which are in their pages already: query token t of sequence b over
+ * the keys 0 .. lengths[b] - cu[b + 1] + t of its sequence that its table holds.  With `prefix`, the batch's tokens are cut
  * into prefix->B groups (prefix->cu, in tokens; each sequence inside one group), and every query of
  * group g also sees all prefix->lengths[g] keys in the pages prefix->table[g], as if they stood
  * before its own (prefix->start is not read, prefix->max_seqlen is the most tokens of a group).
