@@ -185,7 +185,19 @@ constexpr float kLazyLog2 = 8.0f;
 // 16 * 2^8: below that bound every p is at most 2^8 * 16, and a rescale is not needed
 // (p stays far from fp32's range and keeps bf16's relative precision).
 constexpr float kLazySum = 16.0f * 256.0f;
-// That (LAZY) is for GQA groups that are a multiple of 4.  The others take every tile's maximum:
+// kPaged in fp16 keeps its weights 2^11 times as large: mc, their reference point, is the maximum less 11.
+// fp16 ends at 2^-24, and thousands of keys below 2^-25 of the best would vanish (4000 at 2^-25.3 whose values are
+// the result came out at 0); now each is off by 2^-36 of the best at most.  A lane's sum above 1.125 * 2^15 has
+// the maximum taken: no weight passes that before (fp16 holds 65504), and one of the 16 is then above 1.125 * 2^11,
+// so the maximum has risen.
+template <int VARIANT, int DT>
+struct LazyRule {
+  static constexpr bool kRaised = VARIANT == kPaged && DT == DA_F16;
+  static constexpr float bias = kRaised ? 11.0f : 0.0f;
+  static constexpr float sum = kRaised ? 1.125f * 32768.0f : kLazySum;
+  static constexpr float step = kRaised ? 0.0f : kLazyLog2;
+};
+// That (LAZY) is for GQA groups that are a multiple of 4, and for kPaged.  The others take every tile's maximum:
 // the largest p of a row is then 1, which 16 bits hold exactly, and their error against 64
 // bits stays what it was (fp16, 8 heads x 1067 tokens: 2.58e-4; 4 % more with the lazy rule).
 
@@ -742,6 +754,7 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     });
   };
   // ---- softmax of tile t: the two column blocks one after the other, one check each ----
+  using Rule = LazyRule<VARIANT, DT>;
   auto softmax_tile = [&](const int t) __attribute__((always_inline)) {
     const char* ms = meta_of(t);
     const int key0 = key0_of(t);
@@ -778,13 +791,13 @@ __device__ __forceinline__ void attn_w64_item(const Args& a, const int unit_spli
     for (int cb = 0; cb < NCB; ++cb) {
       float ps = LAZY ? exps(cb, -mc[cb]) : 0.0f;
       // the bound also catches an infinite sum
-      if (!LAZY || __builtin_amdgcn_ballot_w64(ps > kLazySum)) {
+      if (!LAZY || __builtin_amdgcn_ballot_w64(ps > Rule::sum)) {
         float m = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) m = __builtin_fmaxf(m, __builtin_fmaxf(s[cb][r], s[cb][r + 1]));
-        const float mxc = halves_max(m) * c;
+        const float mxc = halves_max(m) * c - Rule::bias;
         // alpha = 1 exactly where a lane keeps its maximum (also where it has none yet)
-        const bool upd = mxc > mc[cb] + (LAZY ? kLazyLog2 : 0.0f);
+        const bool upd = mxc > mc[cb] + (LAZY ? Rule::step : 0.0f);
         const float m_new = upd ? mxc : mc[cb];
         const float alpha = upd ? exp2_fast(mc[cb] - m_new) : 1.0f;
         if (LAZY || __builtin_amdgcn_ballot_w64(upd)) {

@@ -11,7 +11,9 @@
 // scores, V while on the next one's, with exact vmcnt waits and no barrier.  Two workgroups a CU keep
 // 8 waves' loads in flight, about 128 KiB a CU.  S^T = K Q^T and O^T += V^T P^T on
 // v_mfma_f32_32x32x16: a lane holds one row and 16 keys.  The weights enter in two 16-bit parts (the
-// matrix unit is idle most of the time here), so the one rounding that matters is the output's.
+// matrix unit is idle most of the time here), so the one rounding that matters is the output's.  In fp16
+// they are 2^15 times as large, with the maximum less 15 as their reference point: fp16 ends at 2^-24,
+// and thousands of keys below 2^-25 of the best would vanish.
 #pragma once
 
 #include "da_paged.hpp"
@@ -316,7 +318,7 @@ __device__ __forceinline__ void stream_worker(const PagedAttnArgs& a, const int 
       float top = x[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = __builtin_fmaxf(top, x[r]);
-      const float mn = __builtin_fmaxf(mx, halves_max(top) * c);
+      const float mn = __builtin_fmaxf(mx, halves_max(top) * c - (DT == DA_F16 ? 15.0f : 0.0f));
       const float ref = mn == -INFINITY ? 0.0f : mn;
       const float alpha = exp2_fast(mx - ref);
       mx = mn;
