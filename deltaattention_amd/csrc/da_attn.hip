@@ -187,14 +187,14 @@ constexpr float kLazyLog2 = 8.0f;
 constexpr float kLazySum = 16.0f * 256.0f;
 // kPaged in fp16 keeps its weights 2^11 times as large: mc, their reference point, is the maximum less 11.
 // fp16 ends at 2^-24, and thousands of keys below 2^-25 of the best would vanish (4000 at 2^-25.3 whose values are
-// the result came out at 0); now each is off by 2^-36 of the best at most.  A lane's sum above 1.125 * 2^15 has
-// the maximum taken: no weight passes that before (fp16 holds 65504), and one of the 16 is then above 1.125 * 2^11,
+// the result came out at 0); now each is off by 2^-36 of the best at most.  A lane's sum above 1.875 * 2^15 has
+// the maximum taken: no weight passes that before (fp16 holds 65504), and one of the 16 is then above 1.875 * 2^11,
 // so the maximum has risen.
 template <int VARIANT, int DT>
 struct LazyRule {
   static constexpr bool kRaised = VARIANT == kPaged && DT == DA_F16;
   static constexpr float bias = kRaised ? 11.0f : 0.0f;
-  static constexpr float sum = kRaised ? 1.125f * 32768.0f : kLazySum;
+  static constexpr float sum = kRaised ? 1.875f * 32768.0f : kLazySum;
   static constexpr float step = kRaised ? 0.0f : kLazyLog2;
 };
 // That (LAZY) is for GQA groups that are a multiple of 4, and for kPaged.  The others take every tile's maximum:
