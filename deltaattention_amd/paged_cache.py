@@ -134,17 +134,17 @@ class PagedCache(_CacheBase):
         if any(x != self._total for x in self._seen):
             raise RuntimeError(f"layer {layer_idx} brings {n} tokens to {self._seen[layer_idx]}, but the layers of one step "
                                f"have to bring the same ({self._total} in all)")
-        more = -(-want // self.page_size) - len(self._pages[0])
+        have = len(self._pages[0])
+        more = -(-want // self.page_size) - have
         if more > 0:
             taken = self._pool.take(more * self.bsz)
-            have = len(self._pages[0])
+            rows = [taken[b * more:(b + 1) * more] for b in range(self.bsz)]
+            for mine, new in zip(self._pages, rows):
+                mine.extend(new)
             if have + more > self._table.shape[1]:
                 wide = torch.zeros((self.bsz, max(2 * self._table.shape[1], have + more)), dtype=torch.int32, device=self.device)
                 wide[:, :have] = self._table[:, :have]
                 self._table = wide
-            rows = [taken[b * more:(b + 1) * more] for b in range(self.bsz)]
-            for mine, new in zip(self._pages, rows):
-                mine.extend(new)
             self._table[:, have:have + more] = torch.tensor(rows, dtype=torch.int32).to(self.device)
         self._lengths.fill_(want)
         self._total = want
@@ -155,6 +155,18 @@ class PagedCache(_CacheBase):
             group = self._copies * n
             self._prefix = paged.PagedBatch(self._prefix_table, self._prefix_lengths,
                                             self._starts(self.bsz // self._copies, group), group)
+
+    def _step(self):
+        """What a step changes before its first kernel runs, for ``_back``."""
+        return self._total, self._batch, self._prefix, len(self._pages[0])
+
+    def _back(self, step) -> None:
+        """To what ``_step`` gave: the pages taken since go back, the lengths on the device are those before."""
+        self._total, self._batch, self._prefix, have = step
+        for mine in self._pages:
+            self._pool.drop(mine[have:])
+            del mine[have:]
+        self._lengths.fill_(self._total)
 
     def fork(self, copies: int) -> "PagedCache":
         """A cache of ``copies`` sequences for each one here, in order, all behind this cache's tokens as
@@ -193,20 +205,32 @@ class PagedCache(_CacheBase):
 
     def append(self, key: torch.Tensor, value: torch.Tensor, layer_idx: int, query: Optional[torch.Tensor] = None,
                cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
-        """A step's key, value [B, Hkv, N, D] into the layer's pages.  With cos and sin [B or 1, N, R] (or R / 2;
-        a model's position embeddings, both halves alike) keys, and query [B, Hq, N, D], are rotated.
-        Returns the query as [B * N, Hq, D], rotated or as it was."""
+        """A step's key, value [B, Hkv, N, D] into the layer's pages.  With cos and sin [B or 1, N, R] (a model's
+        position embeddings, whose two halves are alike: the first is read) keys, and query [B, Hq, N, D], are
+        rotated.  Returns the query as [B * N, Hq, D], rotated or as it was."""
         k, v = self._tokens(key, "key", self.n_kv_heads), self._tokens(value, "value", self.n_kv_heads)
         n = key.shape[2]
         if value.shape[2] != n or (query is not None and query.shape[2] != n):
             raise ValueError(f"key, value and query bring {n}, {value.shape[2]} and "
                              f"{None if query is None else query.shape[2]} tokens")
         q = None if query is None else self._tokens(query, "query")
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin come together")
         if cos is not None:
             cos, sin = (self._rows(t, n) for t in (cos, sin))
-        self._begin(layer_idx, n)
-        got = paged.append_paged(self._pool.layers[layer_idx], self._batch, k, v, q=None if cos is None else q, cos=cos,
-                                 sin=sin, per_token=True)
+            if cos.shape != sin.shape or cos.dtype != sin.dtype:
+                raise ValueError(f"cos {list(cos.shape)} {cos.dtype} and sin {list(sin.shape)} {sin.dtype} differ")
+            if cos.stride() != sin.stride() or cos.stride(1) != 1:
+                cos, sin = cos.contiguous(), sin.contiguous()
+        before = self._step()
+        try:
+            self._begin(layer_idx, n)
+            got = paged.append_paged(self._pool.layers[layer_idx], self._batch, k, v, q=None if cos is None else q, cos=cos,
+                                     sin=sin, per_token=True)
+        except BaseException:
+            if before != self._step():
+                self._back(before)
+            raise
         self._seen[layer_idx] += n
         return q if cos is None else got
 
