@@ -35,17 +35,23 @@ class _Pool:
         self._views()
 
     def _views(self):
-        self.layers = [paged.PagedKV(k, v) for k, v in zip(self.k, self.v)]
+        n = len(self.holders)
+        self.layers = [paged.PagedKV(k[:n], v[:n]) for k, v in zip(self.k, self.v)]
 
     def grow(self, pages):
-        """To ``pages`` pages, contents kept.  The memory before may be read on another stream than this one."""
-        old = self.k.shape[1]
+        """To ``pages`` pages, contents kept.  Where memory for v is short after k has its own, k stays the larger
+        one and all else as it was.  The memory before may be read on another stream than this one."""
+        old = len(self.holders)
         for name in ("k", "v"):
             t = getattr(self, name)
+            if t.shape[1] >= pages:
+                continue
             new = torch.empty((t.shape[0], pages, *t.shape[2:]), dtype=t.dtype, device=t.device)
-            new[:, :old] = t
-            t.record_stream(torch.cuda.current_stream(t.device))
+            new[:, :old] = t[:, :old]
+            if t.is_cuda:
+                t.record_stream(torch.cuda.current_stream(t.device))
             setattr(self, name, new)
+            self._views()
         self.holders += [0] * (pages - old)
         self.free = list(range(pages - 1, old - 1, -1)) + self.free
         self._views()
