@@ -252,8 +252,11 @@ class PagedCache(_CacheBase):
 
     def attend(self, query: torch.Tensor, layer_idx: int, scaling: Optional[float] = None) -> torch.Tensor:
         """The step's queries [B * N, Hq, D] (as ``append`` returns them) over the layer: [B, N, Hq, D]."""
-        if self._batch is None or self._seen[layer_idx] != self._total or query.dim() != 3 or query.shape[0] % self.bsz:
+        if self._batch is None or self._seen[layer_idx] != self._total:
             raise RuntimeError("attend follows the append of the same step and layer")
+        n = self._batch.max_seqlen
+        if query.dim() != 3 or query.shape[0] != self.bsz * n:
+            raise ValueError(f"query must hold the step's {n} tokens of {self.bsz} sequences, got {list(query.shape)}")
         kv = self._pool.layers[layer_idx]
         if self._prefix is None:
             out = paged.paged_attention(query, kv, self._batch, scale=scaling)
