@@ -22,6 +22,12 @@ except Exception:  # pragma: no cover - transformers is optional for the kernels
 __all__ = ["PagedCache"]
 
 
+def _indexed(device) -> torch.device:
+    """``device`` with its index: "cuda" is the device that is current now, whichever is later."""
+    device = torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+
+
 class _Pool:
     """Pages of every layer, k and v [L, pages, Hkv, page_size, D], how many hold each page, and which
     are free."""
@@ -92,7 +98,7 @@ class PagedCache(_CacheBase):
                 super().__init__(layers=[])
             except TypeError:
                 super().__init__()
-        self.bsz, self.dtype, self.device = int(batch_size), dtype, torch.device(device)
+        self.bsz, self.dtype, self.device = int(batch_size), dtype, _indexed(device)
         if self.bsz <= 0 or page_size <= 0:
             raise ValueError(f"{batch_size} sequences, pages of {page_size} tokens")
         self.prefix_length, self._copies, self._common = 0, _copies, None
