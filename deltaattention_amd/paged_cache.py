@@ -13,6 +13,7 @@ from typing import List, Optional
 import torch
 
 from . import paged
+from ._native import _raw_stream
 
 try:
     from transformers import Cache as _CacheBase
@@ -28,9 +29,22 @@ def _indexed(device) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
 
 
+def _stream_of(device: torch.device) -> int:
+    """The handle of the device's current stream."""
+    return _raw_stream(device.index) if device.type == "cuda" else 0
+
+
+def _keep(tensors, stream) -> None:
+    """Their memory stays until what ``stream`` has been given by the time they go is done."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
 class _Pool:
     """Pages of every layer, k and v [L, pages, Hkv, page_size, D], how many hold each page, and which
-    are free."""
+    are free.  A cache and its forks have one pool, whose work is in one order whichever streams they are used
+    from: a page that one gives back, or memory that one's growth replaces, is another's in the same call."""
 
     def __init__(self, layers, pages, heads, page_size, head_dim, dtype, device):
         shape = (layers, pages, heads, page_size, head_dim)
@@ -39,6 +53,19 @@ class _Pool:
         self.holders = [0] * pages
         self.free = list(range(pages - 1, -1, -1))
         self._views()
+        self.device, self.raw = self.k.device, _stream_of(self.k.device)  # the stream that was used last
+        self.stream = torch.cuda.current_stream(self.device) if self.k.is_cuda else None
+
+    def enter(self) -> None:
+        """The current stream goes on after all that the pool's caches have queued on another one.  (Not within a
+        capture, which may not wait for work outside of it, and begins with a synchronization.)"""
+        raw = _stream_of(self.device)
+        if raw == self.raw or torch.cuda.is_current_stream_capturing():
+            return
+        now = torch.cuda.current_stream(self.device)
+        now.wait_stream(self.stream)
+        _keep((self.k, self.v), now)
+        self.raw, self.stream = raw, now
 
     def _views(self):
         n = len(self.holders)
@@ -46,7 +73,7 @@ class _Pool:
 
     def grow(self, pages):
         """To ``pages`` pages, contents kept.  Where memory for v is short after k has its own, k stays the larger
-        one and all else as it was.  The memory before may be read on another stream than this one."""
+        one and all else as it was."""
         old = len(self.holders)
         for name in ("k", "v"):
             t = getattr(self, name)
@@ -54,8 +81,6 @@ class _Pool:
                 continue
             new = torch.empty((t.shape[0], pages, *t.shape[2:]), dtype=t.dtype, device=t.device)
             new[:, :old] = t[:, :old]
-            if t.is_cuda:
-                t.record_stream(torch.cuda.current_stream(t.device))
             setattr(self, name, new)
             self._views()
         self.holders += [0] * (pages - old)
@@ -87,8 +112,9 @@ class PagedCache(_CacheBase):
 
     Every layer has the same tokens in the same pages.  A step brings n tokens a sequence to each layer in
     turn: ``append`` (keys rotated on the way) then ``attend``.  A call that is refused changes nothing.
-    A step's batch lies in tensors that the next step changes in place, on the stream that is current
-    then: use a cache from one stream at a time.
+    A step's batch lies in tensors that the next step changes in place.  Calls may come from different
+    streams: those of a cache and of its forks, which share its pages, run in the order in which they
+    were made.  They have to come from one thread at a time.
     """
 
     def __init__(self, config, batch_size, dtype=torch.bfloat16, page_size: int = 16, num_pages: Optional[int] = None,
@@ -110,6 +136,7 @@ class PagedCache(_CacheBase):
             self._pool = _Pool(self.num_layers, max(1, pages), self.n_kv_heads, self.page_size, self.head_dim, dtype,
                                self.device)
         else:
+            _of._enter()
             for name in ("head_dim", "n_kv_heads", "num_layers", "page_size", "_pool"):
                 setattr(self, name, getattr(_of, name))
             self.prefix_length = _of._total
@@ -126,8 +153,17 @@ class PagedCache(_CacheBase):
         self._seen = [0] * self.num_layers          # those of each layer
         self._batch = self._prefix = None           # of the step in progress
         self._cu = {}
+        self._raw = self._pool.raw                  # the stream that was used last
 
     # ---- pages ----
+
+    def _enter(self) -> None:
+        """Before every use of the pages and of the cache's own tensors on the current stream."""
+        self._pool.enter()
+        if self._raw != self._pool.raw:
+            more = () if self._common is None else (self._prefix_table, self._prefix_lengths)
+            _keep((self._table, self._lengths, self._start, *more, *self._cu.values()), self._pool.stream)
+            self._raw = self._pool.raw
 
     def _starts(self, rows: int, n: int) -> torch.Tensor:
         """0, n, 2 n, .. for ``rows`` entries."""
@@ -234,6 +270,7 @@ class PagedCache(_CacheBase):
                 raise ValueError(f"cos {list(cos.shape)} {cos.dtype} and sin {list(sin.shape)} {sin.dtype} differ")
             if cos.stride() != sin.stride() or cos.stride(1) != 1:
                 cos, sin = cos.contiguous(), sin.contiguous()
+        self._enter()
         before = self._step()
         try:
             self._begin(layer_idx, n)
@@ -263,6 +300,7 @@ class PagedCache(_CacheBase):
         n = self._batch.max_seqlen
         if query.dim() != 3 or query.shape[0] != self.bsz * n:
             raise ValueError(f"query must hold the step's {n} tokens of {self.bsz} sequences, got {list(query.shape)}")
+        self._enter()
         kv = self._pool.layers[layer_idx]
         if self._prefix is None:
             out = paged.paged_attention(query, kv, self._batch, scale=scaling)

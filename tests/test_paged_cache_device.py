@@ -12,7 +12,7 @@ def test_device_of_a_cache(monkeypatch):
     from deltaattention_amd import paged_cache
     made = []
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
-    monkeypatch.setattr(paged_cache, "_Pool", lambda *a: made.append(a[-1]))
+    monkeypatch.setattr(paged_cache, "_Pool", lambda *a: made.append(a[-1]) or types.SimpleNamespace(raw=0, drop=len))
     monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **k: made.append(device))
     config = types.SimpleNamespace(head_dim=64, num_key_value_heads=2, num_hidden_layers=1, hidden_size=256,
                                    num_attention_heads=4)
@@ -20,7 +20,6 @@ def test_device_of_a_cache(monkeypatch):
         made.clear()
         cache = paged_cache.PagedCache(config, 2, device=given)
         assert cache.device == torch.device("cuda", want) and made == [torch.device("cuda", want)] * 3
-        del cache._pool
 
 
 @pytest.mark.gpu
