@@ -248,8 +248,8 @@ extern "C" int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const 
   if (D <= 0 || D > 128 || (D & 7))
     return set_error(DA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [8, 128] (got %lld)", who, (long long)D);
   DA_REQUIRE(k && v && (!q || q_out), "%s: null pointer", who);
-  DA_REQUIRE(T > 0 && T < (1ll << 28) && Hkv > 0 && Hkv < (1 << 16) && (!q || (Hq > 0 && Hq < (1 << 16))), "%s: empty shape",
-             who);
+  DA_REQUIRE(T > 0 && Hkv > 0 && Hkv < (1 << 16) && (!q || (Hq > 0 && Hq < (1 << 16))), "%s: empty shape", who);
+  DA_REQUIRE(T < (1ll << 26), "%s: more than 2^26 tokens", who);  // a launch has less than 2^32 threads, 64 a token
   DA_REQUIRE(rot >= 0 && rot <= D && (rot & 3) == 0, "%s: the rotated dims must be a multiple of 4 up to head_dim (got %lld)",
              who, (long long)rot);
   if (rot) {

@@ -60,6 +60,7 @@ typedef struct DaPagedBatch {
  * fp32, rounded once; dims from rot on stay.  cos, sin [rows, rot / 2] fp32 or of the pages' type
  * (rot_dtype), rows s_rot apart (0: one row for all); row p is for position p, or with per_token for
  * token p (rows >= T).  A position outside the rows takes the nearest row.  rot = 0: no rotation.
+ * T is less than 2^26.
  * Two tokens meant for one place (tables with a page in common) leave either of them there.
  */
 int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_t, int64_t sv_h,
