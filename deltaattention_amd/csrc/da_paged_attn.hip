@@ -169,7 +169,8 @@ static PagedPlan plan(PagedAttnArgs& a, int dtype) {
     shape_rows(a, i, p.wide[i], paired_rows(p, i), dtype);
     if (a.splits[i] > 1 || a.prefix.B) parts |= 1 << i;
   }
-  a.whole = stream_whole((int64_t)E * a.Hkv, keys);
+  // a workgroup an item needs a launch of less than 2^32 threads
+  a.whole = stream_whole((int64_t)E * a.Hkv, keys) && (int64_t)E * a.Hkv < (1ll << 24);
   a.workers = a.whole ? E * a.Hkv : 2 * cu_count();
   a.slot_rows = (int)slot_rows;
   const bool cut = p.stream && !a.whole;
