@@ -119,11 +119,11 @@ def _paged_attention(self, cache, query_states, key_states, value_states, cos, s
         # PATH 1 selects among the rotated keys of the whole prompt, which go to the pages as they are
         from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
         query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
-        cache.append(key_states, value_states, self.layer_idx)
         out, view = _out_view(query_states)
         _timed(lambda: attention.delta_prefill_attention(
             query_states, key_states, value_states, layer_idx=self.layer_idx, scaling=self.scaling,
             track_sparsity=_track_sparsity(), out=view), query_states.is_cuda)
+        cache.append(key_states, value_states, self.layer_idx)  # after what may refuse the prompt
         return out
     query = cache.append(key_states, value_states, self.layer_idx, query_states, cos, sin)
     if N == 1:
