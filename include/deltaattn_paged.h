@@ -76,8 +76,9 @@ int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, in
  * group g also sees all prefix->lengths[g] keys in the pages prefix->table[g], as if they stood
  * before its own (prefix->start is not read, prefix->max_seqlen is the most tokens of a group).
  * q, out [T, Hq, D] (strides *_t, *_h; rows 16-byte aligned) of the pages' type; query head h reads
- * KV head h / (Hq / Hkv).  A query that sees no key gives zeros.  Scores, maxima, sums and partial
- * results are fp32.  Deterministic.  T is less than 2^24.  What batch and prefix point to must not
+ * KV head h / (Hq / Hkv).  A query that sees no key gives zeros.  A key that it does not see has
+ * weight 0: an infinity or a NaN in the values of a call's own later tokens can reach earlier ones.
+ * Scores, maxima, sums and partial results are fp32.  Deterministic.  T is less than 2^24.  What batch and prefix point to must not
  * change while the call runs.  workspace: da_paged_attention_workspace_size() bytes of the same
  * arguments (none, and null, where it returns 0), 256-byte aligned.
  */
