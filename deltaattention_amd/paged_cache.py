@@ -29,9 +29,9 @@ def _indexed(device) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
 
 
-def _stream_of(device: torch.device) -> int:
-    """The handle of the device's current stream."""
-    return _raw_stream(device.index) if device.type == "cuda" else 0
+def _stream_of(index: Optional[int]) -> int:
+    """The handle of the current stream of GPU ``index`` (None: the CPU)."""
+    return 0 if index is None else _raw_stream(index)
 
 
 def _keep(tensors, stream) -> None:
@@ -53,13 +53,14 @@ class _Pool:
         self.holders = [0] * pages
         self.free = list(range(pages - 1, -1, -1))
         self._views()
-        self.device, self.raw = self.k.device, _stream_of(self.k.device)  # the stream that was used last
+        self.device, self.index = self.k.device, self.k.device.index
+        self.raw = _stream_of(self.index)           # the stream that was used last
         self.stream = torch.cuda.current_stream(self.device) if self.k.is_cuda else None
 
     def enter(self) -> None:
         """The current stream goes on after all that the pool's caches have queued on another one.  (Not within a
         capture, which may not wait for work outside of it, and begins with a synchronization.)"""
-        raw = _stream_of(self.device)
+        raw = _stream_of(self.index)
         if raw == self.raw or torch.cuda.is_current_stream_capturing():
             return
         now = torch.cuda.current_stream(self.device)
@@ -159,11 +160,13 @@ class PagedCache(_CacheBase):
 
     def _enter(self) -> None:
         """Before every use of the pages and of the cache's own tensors on the current stream."""
-        self._pool.enter()
-        if self._raw != self._pool.raw:
+        pool = self._pool
+        if _stream_of(pool.index) != pool.raw:
+            pool.enter()
+        if self._raw != pool.raw:
             more = () if self._common is None else (self._prefix_table, self._prefix_lengths)
-            _keep((self._table, self._lengths, self._start, *more, *self._cu.values()), self._pool.stream)
-            self._raw = self._pool.raw
+            _keep((self._table, self._lengths, self._start, *more, *self._cu.values()), pool.stream)
+            self._raw = pool.raw
 
     def _starts(self, rows: int, n: int) -> torch.Tensor:
         """0, n, 2 n, .. for ``rows`` entries."""
@@ -265,10 +268,8 @@ class PagedCache(_CacheBase):
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin come together")
         if cos is not None:
-            cos, sin = (self._rows(t, n) for t in (cos, sin))
-            if cos.shape != sin.shape or cos.dtype != sin.dtype:
-                raise ValueError(f"cos {list(cos.shape)} {cos.dtype} and sin {list(sin.shape)} {sin.dtype} differ")
-            if cos.stride() != sin.stride() or cos.stride(1) != 1:
+            cos, sin = self._rows(cos, n), self._rows(sin, n)
+            if cos.stride() != sin.stride():
                 cos, sin = cos.contiguous(), sin.contiguous()
         self._enter()
         before = self._step()
