@@ -71,10 +71,10 @@ int da_paged_append(const void* k, int64_t sk_t, int64_t sk_h, const void* v, in
 
 /*
  * Attention of the new tokens, which are in their pages already: query token t of sequence b over
- * the keys 0 .. lengths[b] - cu[b + 1] + t of its sequence that its table holds.  With `prefix`, the batch's tokens are cut
- * into prefix->B groups (prefix->cu, in tokens; each sequence inside one group), and every query of
- * group g also sees all prefix->lengths[g] keys in the pages prefix->table[g], as if they stood
- * before its own (prefix->start is not read, prefix->max_seqlen is the most tokens of a group).
+ * the keys 0 .. lengths[b] - cu[b + 1] + t of its sequence that its table holds.  With `prefix`, the
+ * batch's tokens are cut into prefix->B groups (prefix->cu, in tokens; each sequence inside one group),
+ * and every query of group g also sees all prefix->lengths[g] keys in the pages prefix->table[g], as if
+ * they stood before its own (prefix->start is not read, prefix->max_seqlen is the most tokens of a group).
  * q, out [T, Hq, D] (strides *_t, *_h; rows 16-byte aligned) of the pages' type; query head h reads
  * KV head h / (Hq / Hkv).  A query that sees no key gives zeros.  A key that it does not see has
  * weight 0: an infinity or a NaN in the values of a call's own later tokens can reach earlier ones.
