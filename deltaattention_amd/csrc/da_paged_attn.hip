@@ -31,10 +31,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     const int e = entry[list];
     if (e < 0) continue;
     const int tokens = s.tokens(e), i = t - s.first(e);
-    if (i >= tokens) {
-      if (list) return;
-      continue;
-    }
+    if (i >= tokens) return;  // past max_seqlen: left as it is
     const float* state;
     int64_t step = 0;
     int n = 1;

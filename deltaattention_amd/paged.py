@@ -225,7 +225,8 @@ def shared_prefix_attention(q: torch.Tensor, kv: PagedKV, batch: PagedBatch, pre
     """``paged_attention`` where groups of sequences have their first tokens in common: ``prefix``
     holds a row of ``table`` and ``lengths`` for every group, and ``cu_seqlens`` over q's tokens
     says which are the group's (whole sequences, in order; ``max_seqlen`` the most tokens of a group).
-    Every query of a group sees all of its prefix and then its own sequence as in ``paged_attention``.
+    Every query of a group sees all of its prefix and then its own sequence as in ``paged_attention``;
+    tokens past the group's ``max_seqlen`` are left as ``out`` has them.
     The prefix's keys and values are read once for the group, not once for each sequence."""
     if prefix.cu is None:
         raise ValueError("prefix needs cu_seqlens: which of q's tokens belong to which group")

@@ -41,8 +41,8 @@ typedef struct DaPagedKV {
  * [0, num_pages) is never touched (its tokens' keys and values count as zeros, a token meant for
  * it is not written).  A token whose place j is not in the table (before row 0, as in a sequence that
  * is shorter than what it brings, or from width * page_size on) is not written, and attends to the
- * places before its own that are there.  Attention leaves the tokens of a sequence past max_seqlen as they
- * are.  With a cu that does not rise no row outside the batch is touched.
+ * places before its own that are there.  Attention leaves the tokens past max_seqlen of a sequence, or of
+ * a prefix's group, as they are.  With a cu that does not rise no row outside the batch is touched.
  */
 typedef struct DaPagedBatch {
   const int32_t* table; /* [B, width], rows table_stride apart */
